@@ -1,0 +1,379 @@
+// What a served batch needs beside its forward pass: the plan of a ragged batch before it, the processing of its logits after it.
+//
+//   process_logits   biases, penalties for repeated tokens and a grammar's mask on [B, V] logits, one pass, one rounding
+//   count_tokens     the occurrences that the penalties go by
+//   plan_batch       positions, KV slots and block tables of a ragged batch from the lengths of its requests
+//
+// The reference applies penalties from a count tensor in front of its sampler (mfq/kernels/cuda/sampling.cu) and plans batches on the
+// host (cpp_runtime/engine/include/continuous_batch.h).
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace mfq {
+
+// ----- logits -----
+// For row b with tables' row r and vocabulary id v:
+//   l = logit + sum of the row's biases for v;   word = counts[r][v]: 15 bits of occurrences n, the top bit: the prompt has v
+//   word != 0:  l = l > 0 ? l / repetition : l * repetition;   n > 0:  l -= presence + frequency * n
+//   out = allowed[r] bit v ? round(l) : fill     (chosen, not added: a masked NaN or infinity is gone)
+// All of it in fp32, rounded once to the logits' type.
+
+struct LogitRecord {  // the 32 bytes a row's sampler reads
+  float temperature;
+  int top_k;
+  float top_p, presence, frequency, repetition;
+  unsigned long long seed;
+};
+
+struct LogitArgs {
+  const void* logits;
+  void* out;
+  const LogitRecord* records;
+  const unsigned short* counts;  // [R, >= V], null: no penalties
+  const int* bias_ids;           // [R, K] vocabulary ids (null: no biases)
+  const float* bias_values;
+  const unsigned* allowed;       // [R, words], null: all allowed
+  const int* rows;               // [B] row of the tables (null: b); outside 0 .. R - 1: the logits pass through
+  int V, R, K, words, first;     // first: vocabulary id of column 0
+  long long in_stride, out_stride, counts_stride;
+  float fill;
+};
+
+constexpr int kLogitThreads = 256, kLogitVec = 8, kLogitChunk = kLogitThreads * kLogitVec, kMaxBias = 1024;
+
+template <typename T> __device__ __forceinline__ float logit_to_f32(T v);
+template <> __device__ __forceinline__ float logit_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float logit_to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float logit_to_f32(float v) { return v; }
+template <typename T> __device__ __forceinline__ T logit_from_f32(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 logit_from_f32(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half logit_from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float logit_from_f32(float v) { return v; }
+
+template <typename T>
+struct alignas(16) LogitVec {
+  T v[kLogitVec];
+};
+
+// A thread has eight values: eight neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16 bytes), else eight that
+// lie a block apart, so that a warp's accesses are whole lines at any alignment.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kLogitThreads)
+process_logits_kernel(const LogitArgs a) {
+  pdl_trigger();
+  __shared__ float s_bias[kLogitChunk];
+  __shared__ int s_hit[kMaxBias];
+  __shared__ int s_hits;
+  pdl_wait();
+  const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kLogitChunk, hi = min(a.V, lo + kLogitChunk);
+  const int r = a.rows ? a.rows[b] : b;
+  const bool known = r >= 0 && r < a.R;
+  const T* in = static_cast<const T*>(a.logits) + b * a.in_stride;
+  T* out = static_cast<T*>(a.out) + b * a.out_stride;
+  const auto column = [&](int j) { return kVec ? lo + tid * kLogitVec + j : lo + tid + j * kLogitThreads; };
+  const bool whole = kVec && column(kLogitVec - 1) < hi;
+
+  LogitVec<T> x;
+  if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
+  else {
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j)
+      if (column(j) < hi) x.v[j] = in[column(j)];
+  }
+  if (!known) {
+    if (in == out) return;
+    if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = x;
+    else {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j)
+        if (column(j) < hi) out[column(j)] = x.v[j];
+    }
+    return;
+  }
+  unsigned allow = 0xffu;  // bit j: value j
+  if (a.allowed) {
+    const unsigned* words = a.allowed + size_t(r) * a.words;
+    if (whole && a.first % 8 == 0) {
+      allow = reinterpret_cast<const unsigned char*>(words)[(a.first + column(0)) >> 3];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j) {
+        const int id = a.first + column(j);
+        if (column(j) < hi && !(words[id >> 5] >> (id & 31) & 1u)) allow &= ~(1u << j);
+      }
+    }
+  }
+  float presence = 0.f, frequency = 0.f, repetition = 1.f;
+  if (a.counts) {
+    presence = a.records[r].presence;
+    frequency = a.records[r].frequency;
+    repetition = a.records[r].repetition;
+  }
+  unsigned short c[kLogitVec] = {};
+  if (presence != 0.f || frequency != 0.f || repetition != 1.f) {
+    const unsigned short* row = a.counts + r * a.counts_stride;
+    if (whole) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(row + column(0));
+      const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j) c[j] = static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j)
+        if (column(j) < hi) c[j] = row[column(j)];
+    }
+  }
+  // biases: those of this block's columns are gathered, then each id's are summed by one thread in the order of the row
+  if (a.bias_ids) {
+    if (tid == 0) s_hits = 0;
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j) s_bias[tid + j * kLogitThreads] = 0.f;
+    __syncthreads();
+    const int* ids = a.bias_ids + size_t(r) * a.K;
+    const float* values = a.bias_values + size_t(r) * a.K;
+    for (int j = tid; j < a.K; j += kLogitThreads) {
+      const int v = ids[j] - a.first;
+      if (ids[j] >= 0 && v >= lo && v < hi) s_hit[atomicAdd(&s_hits, 1)] = j;
+    }
+    __syncthreads();
+    const int hits = s_hits;
+    for (int h = tid; h < hits; h += kLogitThreads) {
+      const int id = ids[s_hit[h]];
+      float sum = 0.f;
+      int last = -1;
+      bool mine = true;
+      while (mine) {  // the next place of the same id
+        int next = a.K;
+        for (int i = 0; i < hits; ++i) {
+          const int j = s_hit[i];
+          if (j > last && j < next && ids[j] == id) next = j;
+        }
+        if (next == a.K) break;
+        if (last < 0) mine = next == s_hit[h];
+        sum += values[next];
+        last = next;
+      }
+      if (mine) s_bias[id - a.first - lo] = sum;
+    }
+    __syncthreads();
+  }
+  LogitVec<T> y;
+#pragma unroll
+  for (int j = 0; j < kLogitVec; ++j) {
+    float l = logit_to_f32(x.v[j]);
+    if (a.bias_ids && column(j) < hi) l += s_bias[column(j) - lo];
+    const unsigned n = c[j] & 0x7fffu;
+    if (c[j]) l = l > 0.f ? l / repetition : l * repetition;
+    if (n) l -= presence + frequency * float(n);
+    y.v[j] = allow >> j & 1u ? logit_from_f32<T>(l) : logit_from_f32<T>(a.fill);
+  }
+  if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
+  else {
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j)
+      if (column(j) < hi) out[column(j)] = y.v[j];
+  }
+}
+
+// counts[row][token] of every (row, token): its top bit is set (prompt) or its lower 15 go up by one and stay at their largest value.
+// Pairs with a token or row outside the table are left out.  The lanes of a warp that have the same pair add together.
+__global__ void __launch_bounds__(256)
+count_tokens_kernel(unsigned short* __restrict__ counts, long long stride, int R, int V, const int* __restrict__ tokens, const int* __restrict__ rows, int T,
+                    int prompt) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int token = i < T ? tokens[i] : -1, row = i < T ? rows[i] : -1;
+  const bool in = token >= 0 && token < V && row >= 0 && row < R;
+  const unsigned live = __ballot_sync(0xffffffffu, in);
+  if (!in) return;
+  unsigned short* at = counts + row * stride + token;
+  const unsigned same = __match_any_sync(live, reinterpret_cast<unsigned long long>(at));
+  if ((threadIdx.x & 31) != __ffs(same) - 1) return;
+  unsigned old = *reinterpret_cast<volatile unsigned short*>(at);
+  for (;;) {  // a failed exchange means that another one succeeded
+    const unsigned now = prompt ? old | 0x8000u : (old & 0x8000u) | min((old & 0x7fffu) + unsigned(__popc(same)), 0x7fffu);
+    if (now == old) return;
+    const unsigned seen = atomicCAS(at, static_cast<unsigned short>(old), static_cast<unsigned short>(now));
+    if (seen == old) return;
+    old = seen;
+  }
+}
+
+// ----- plan of a ragged batch -----
+// Request i has past_i tokens in the pages of table row rows_i and brings counts_i more.  With s_i the sum of the counts before it, token
+// t of s_i <= t < s_{i+1} is at position past_i + t - s_i, in slot page * size + offset.  With a list of free pages, request i takes
+// ceil((past_i + counts_i) / size) - ceil(past_i / size) of them, in the order of the requests, behind the pages of its past.
+// Every block sums the lengths for itself (at most kPlanRequests, so that no block waits for another) and takes its share of tokens and table entries.
+constexpr int kPlanThreads = 256, kPlanRequests = 1024, kPlanPer = kPlanRequests / kPlanThreads, kPlanRows = 1 << 16;
+enum : int { kPlanBadRequest = 1, kPlanNoRoom = 2, kPlanNoPages = 3 };
+
+struct PlanArgs {
+  int* table;  // [R, P]; written where pages are handed out
+  const int *rows, *past, *counts, *pages;
+  int *positions, *slots, *tok_seq, *q_starts, *seq_lens, *out_table, *info;
+  int R, P, b, T, page_size, free_pages;  // free_pages < 0: none are handed out
+};
+
+__global__ void __launch_bounds__(kPlanThreads)
+plan_batch_kernel(const PlanArgs a) {
+  pdl_trigger();
+  __shared__ int s_start[kPlanRequests + 1], s_past[kPlanRequests], s_row[kPlanRequests], s_have[kPlanRequests], s_first[kPlanRequests];
+  __shared__ long long s_sum[2][kPlanThreads / 32];
+  __shared__ int s_bad;
+  __shared__ unsigned s_seen[kPlanRows / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ps = a.page_size;
+  if (tid == 0) s_bad = 0;
+  const bool hand = a.free_pages >= 0;
+  if (hand)
+    for (int i = tid; i < (a.R + 31) / 32; i += kPlanThreads) s_seen[i] = 0u;
+  __syncthreads();
+  pdl_wait();
+  // neighbouring requests per thread, so that one scan over the threads orders them
+  long long tokens = 0, need = 0;
+  int mine[kPlanPer], want[kPlanPer], bad = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int i = tid * kPlanPer + k;
+    mine[k] = want[k] = 0;
+    if (i >= a.b) continue;
+    const int row = a.rows[i], past = a.past[i], count = a.counts[i];
+    const long long len = static_cast<long long>(past) + count;
+    if (row < 0 || row >= a.R || past < 0 || count < 0) bad = max(bad, int(kPlanBadRequest));
+    else if (len > static_cast<long long>(a.P) * ps) bad = max(bad, int(kPlanNoRoom));
+    else {
+      const int have = (past + ps - 1) / ps;
+      if (hand) {
+        want[k] = int((len + ps - 1) / ps) - have;
+        if (atomicOr(&s_seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u) bad = max(bad, int(kPlanBadRequest));  // two requests would take pages for one row
+      }
+      mine[k] = count;
+      s_row[i] = row;
+      s_past[i] = past;
+      s_have[i] = have;
+    }
+    tokens += mine[k];
+    need += want[k];
+  }
+  if (bad) atomicMax(&s_bad, bad);
+  long long before_t = tokens, before_n = need;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, before_t, o), n = __shfl_up_sync(0xffffffffu, before_n, o);
+    if (lane >= o) { before_t += t; before_n += n; }
+  }
+  if (lane == 31) { s_sum[0][warp] = before_t; s_sum[1][warp] = before_n; }
+  __syncthreads();
+  long long total = 0, taken = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) { before_t += s_sum[0][w]; before_n += s_sum[1][w]; }
+    total += s_sum[0][w];
+    taken += s_sum[1][w];
+  }
+  int refused = s_bad;
+  if (!refused && total > a.T) refused = kPlanNoRoom;
+  if (!refused && hand && taken > a.free_pages) refused = kPlanNoPages;
+  if (blockIdx.x == 0 && tid == 0) {
+    a.info[0] = refused ? -refused : int(total);
+    a.info[1] = refused ? 0 : int(taken);
+  }
+  if (refused) total = 0;
+  before_t -= tokens;
+  before_n -= need;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int i = tid * kPlanPer + k;
+    if (i < a.b) {
+      s_start[i] = refused ? 0 : int(before_t);
+      s_first[i] = refused ? 0 : int(before_n);
+      if (blockIdx.x == 0) {
+        a.q_starts[i] = s_start[i];
+        a.seq_lens[i] = refused ? 0 : s_past[i] + mine[k];
+      }
+    }
+    before_t += mine[k];
+    before_n += want[k];
+  }
+  if (tid == 0) {
+    s_start[a.b] = int(total);
+    if (blockIdx.x == 0) a.q_starts[a.b] = int(total);
+  }
+  __syncthreads();
+  const auto page_of = [&](int i, int j) {  // entry j of request i's row, its new pages included
+    if (hand && j >= s_have[i]) return a.pages[s_first[i] + j - s_have[i]];
+    return a.table[size_t(s_row[i]) * a.P + j];
+  };
+  const int step = gridDim.x * kPlanThreads;
+  for (int t = blockIdx.x * kPlanThreads + tid; t < a.T; t += step) {
+    int pos = 0, slot = -1, seq = -1;
+    if (t < total) {
+      int lo = 0, hi = a.b;  // the last request that starts at t or before
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_start[mid] <= t) lo = mid; else hi = mid;
+      }
+      seq = lo;
+      pos = s_past[lo] + t - s_start[lo];
+      slot = page_of(lo, pos / ps) * ps + pos % ps;
+    }
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+    a.tok_seq[t] = seq;
+  }
+  const long long entries = static_cast<long long>(a.b) * a.P;
+  for (long long e = static_cast<long long>(blockIdx.x) * kPlanThreads + tid; e < entries; e += step) {
+    const int i = int(e / a.P), j = int(e - static_cast<long long>(i) * a.P);
+    int page = 0;
+    if (!refused && j < (s_past[i] + s_start[i + 1] - s_start[i] + ps - 1) / ps) {
+      page = page_of(i, j);
+      if (hand && j >= s_have[i]) a.table[size_t(s_row[i]) * a.P + j] = page;
+    }
+    a.out_table[e] = page;
+  }
+}
+
+template <typename T>
+static int launch_logits(const LogitArgs& a, int B, bool vec, cudaStream_t stream) {
+  const dim3 grid((a.V + kLogitChunk - 1) / kLogitChunk, B);
+  launch_kernel(vec ? process_logits_kernel<T, true> : process_logits_kernel<T, false>, grid, dim3(kLogitThreads), 0, stream, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -7;
+}
+
+}  // namespace mfq
+
+// dtype: 0 bf16, 1 fp16, 2 fp32.  Strides count values.  What may be null, and what the tables hold: see LogitArgs.
+extern "C" int mfq_process_logits(const void* logits, void* out, int dtype, int B, int V, long long in_stride, long long out_stride, const void* records, int R,
+                                  const void* counts, long long counts_stride, const int* bias_ids, const float* bias_values, int K, const void* allowed,
+                                  int words, const int* rows, int first, float fill, cudaStream_t stream) {
+  using namespace mfq;
+  if (B <= 0 || B > 65535 || V <= 0 || R <= 0 || first < 0 || K < 0 || K > kMaxBias || dtype < 0 || dtype > 2) return -1;
+  if (first > INT32_MAX - V || (allowed && (first + V + 31) / 32 > words)) return -1;
+  const LogitArgs a{logits, out, static_cast<const LogitRecord*>(records), static_cast<const unsigned short*>(counts), K ? bias_ids : nullptr, bias_values,
+                    static_cast<const unsigned*>(allowed), rows, V, R, K, words, first, in_stride, out_stride, counts_stride, fill};
+  const int size = dtype == 2 ? 4 : 2;
+  const auto even = [](const void* p, long long stride, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * bytes % 16 == 0; };
+  const bool vec = even(logits, in_stride, size) && even(out, out_stride, size) && (!counts || even(counts, counts_stride, 2));
+  return dtype == 0 ? launch_logits<__nv_bfloat16>(a, B, vec, stream) : dtype == 1 ? launch_logits<__half>(a, B, vec, stream) : launch_logits<float>(a, B, vec, stream);
+}
+
+extern "C" int mfq_count_tokens(void* counts, long long stride, int R, int V, const int* tokens, const int* rows, int T, int prompt, cudaStream_t stream) {
+  if (R <= 0 || V <= 0 || T < 0) return -1;
+  if (T == 0) return 0;
+  mfq::launch_kernel(mfq::count_tokens_kernel, dim3((T + 255) / 256), dim3(256), 0, stream, static_cast<unsigned short*>(counts), stride, R, V, tokens, rows, T, prompt);
+  return cudaGetLastError() == cudaSuccess ? 0 : -7;
+}
+
+// table [R, P] int32; rows / past / counts [b]; pages [free_pages], or free_pages < 0; positions / slots / tok_seq [T], q_starts [b + 1], seq_lens [b], out_table [b, P],
+// info [2]: tokens and pages taken, or minus the reason of a refusal and 0.
+extern "C" int mfq_plan_batch(int* table, int R, int P, const int* rows, const int* past, const int* counts, int b, const int* pages, int free_pages, int* positions,
+                              int* slots, int* tok_seq, int T, int* q_starts, int* seq_lens, int* out_table, int* info, int page_size, cudaStream_t stream) {
+  using namespace mfq;
+  if (R <= 0 || P <= 0 || b <= 0 || b > kPlanRequests || T < 0 || page_size <= 0 || (free_pages >= 0 && R > kPlanRows)) return -1;
+  if (static_cast<long long>(P) * page_size > INT32_MAX) return -1;
+  const PlanArgs a{table, rows, past, counts, pages, positions, slots, tok_seq, q_starts, seq_lens, out_table, info, R, P, b, T, page_size, free_pages};
+  const long long work = T + static_cast<long long>(b) * P, per = 4 * kPlanThreads;
+  const int blocks = int(work / per < 1 ? 1 : work / per > 148 ? 148 : (work + per - 1) / per);
+  launch_kernel(plan_batch_kernel, dim3(blocks), dim3(kPlanThreads), 0, stream, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -7;
+}

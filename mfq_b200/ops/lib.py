@@ -8,6 +8,7 @@ reused by every call on that device's current stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from functools import lru_cache
 
@@ -15,7 +16,7 @@ import torch
 
 from .build import DENSE_LIB_PATH, LIB_PATH
 
-_vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_vp, _i, _f, _sz, _ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
 
 _SIGNATURES = {
     "mfq_fp8_gemm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp],
@@ -41,6 +42,9 @@ _SIGNATURES = {
     "mfq_paged_attn_decode_mma": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _vp],
     "mfq_argmax": [_vp, _vp, _i, _i, _i, _vp],
     "mfq_argmax_f32": [_vp, _vp, _i, _i, _i, _vp],
+    "mfq_process_logits": [_vp, _vp, _i, _i, _i, _ll, _ll, _vp, _i, _vp, _ll, _vp, _vp, _i, _vp, _i, _vp, _i, _f, _vp],
+    "mfq_count_tokens": [_vp, _ll, _i, _i, _vp, _vp, _i, _i, _vp],
+    "mfq_plan_batch": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
     "mfq_embed": [_vp, _vp, _vp, _i, _i, _vp],
     "mfq_decode_advance": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp],
     "mfq_mtp_prepare": [_vp] * 9 + [_i, _i, _i, _i, _vp],
@@ -133,6 +137,16 @@ def stream_ptr() -> int:
     if _raw_stream is None or _device_index is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_device_index())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def current_device(device: torch.device):
+    """Context in which ``device`` is the current one (nothing to do when it is): kernels are launched on the stream that the tensors'
+    own device has as its current one."""
+    index = torch.cuda.current_device() if _device_index is None else _device_index()
+    return _HERE if index == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -139,3 +139,85 @@ def write_kv(kv, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     kv.v[pages, :, :, vslot] = vq
     kv.k_scale[pages, :, off] = ks
     kv.v_scale[pages, :, off] = vs
+
+
+def process_logits(logits, records, counts=None, bias=None, allowed=None, rows=None, first: int = 0, fill: float = float("-inf")) -> torch.Tensor:
+    b, v = logits.shape
+    rows = torch.arange(b, device=logits.device) if rows is None else rows.long()
+    known = (rows >= 0) & (rows < records.shape[0])
+    rows = torch.where(known, rows, 0)
+    l = logits.float()
+    if bias is not None and bias[0].shape[1]:
+        ids, values = bias[0][rows].long() - first, bias[1][rows]
+        ok = (bias[0][rows] >= 0) & (ids >= 0) & (ids < v)
+        l = l + torch.zeros_like(l).scatter_add_(1, ids.clamp(0, v - 1), torch.where(ok, values, torch.zeros_like(values)))
+    if counts is not None:
+        presence, frequency, repetition = (records[rows, i].view(torch.float32)[:, None] for i in (3, 4, 5))
+        on = (presence != 0) | (frequency != 0) | (repetition != 1)
+        word = counts[rows].int() & 0xFFFF
+        n = (word & 0x7FFF).float()
+        l = torch.where(on & (word != 0), torch.where(l > 0, l / repetition, l * repetition), l)
+        l = torch.where(on & (n > 0), l - (presence + frequency * n), l)
+    if allowed is not None:
+        ids = torch.arange(first, first + v, device=logits.device)
+        l = torch.where((allowed[rows][:, ids // 32] >> (ids % 32).int()) & 1 != 0, l, torch.full_like(l, fill))
+    return torch.where(known[:, None], l.to(logits.dtype), logits)
+
+
+def count_tokens(counts, tokens, rows, prompt: bool = False) -> None:
+    ok = (tokens >= 0) & (tokens < counts.shape[1]) & (rows >= 0) & (rows < counts.shape[0])
+    t, r = tokens[ok].long(), rows[ok].long()
+    word = counts[r, t].int() & 0xFFFF
+    if prompt:
+        word = word | 0x8000
+    else:
+        pair, times = torch.unique(r * counts.shape[1] + t, return_counts=True)
+        r, t = pair // counts.shape[1], pair % counts.shape[1]
+        word = counts[r, t].int() & 0xFFFF
+        word = (word & 0x8000) | ((word & 0x7FFF) + times.int()).clamp(max=0x7FFF)
+    counts[r, t] = torch.where(word >= 0x8000, word - 0x10000, word).to(torch.int16)
+
+
+def plan_batch(plan, block_table, rows, past, counts, tokens: int, page_size: int, pages=None) -> None:
+    for t, empty in ((plan.positions, 0), (plan.slots, -1), (plan.tok_seq, -1), (plan.q_starts, 0), (plan.seq_lens, 0), (plan.block_table, 0)):
+        t.fill_(empty)
+    r, n, c = (t.tolist() for t in (rows, past, counts))
+    table_rows, width = block_table.shape
+
+    def whole(x: int) -> int:
+        return -(-x // page_size)
+
+    def code() -> int:  # of a refusal: the latest rule that a request breaks, then the sums
+        bad = [0]
+        for i, (row, a, m) in enumerate(zip(r, n, c)):
+            if not 0 <= row < table_rows or a < 0 or m < 0:
+                bad.append(1)
+            elif a + m > width * page_size:
+                bad.append(2)
+            elif pages is not None and row in [q for q, x, y in zip(r[:i], n, c) if x >= 0 and y >= 0 and x + y <= width * page_size]:
+                bad.append(1)
+        if not max(bad) and sum(c) > tokens:
+            return 2
+        if not max(bad) and pages is not None and sum(whole(a + m) - whole(a) for a, m in zip(n, c)) > pages.numel():
+            return 3
+        return max(bad)
+
+    refused = code()
+    plan.info[0], plan.info[1] = -refused, 0
+    if refused:
+        return
+    at = taken = 0
+    for i, (row, a, m) in enumerate(zip(r, n, c)):
+        have, need = whole(a), whole(a + m)
+        if pages is not None:
+            block_table[row, have:need] = pages[taken : taken + max(0, need - have)]
+            taken += need - have
+        mine = block_table[row, :need]
+        pos = torch.arange(a, a + m, dtype=torch.int32)
+        plan.positions[at : at + m] = pos
+        plan.slots[at : at + m] = mine[(pos // page_size).long()] * page_size + pos % page_size
+        plan.tok_seq[at : at + m] = i
+        at += m
+        plan.q_starts[i + 1], plan.seq_lens[i] = at, a + m
+        plan.block_table[i, :need] = mine
+    plan.info[0], plan.info[1] = at, taken
