@@ -42,6 +42,7 @@ _SIGNATURES = {
     "mfq_paged_attn_decode_mma": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _vp],
     "mfq_argmax": [_vp, _vp, _i, _i, _i, _vp],
     "mfq_argmax_f32": [_vp, _vp, _i, _i, _i, _vp],
+    "mfq_paged_attn_decode_shared": [_vp] * 13 + [_i] * 11 + [_f, _vp, _vp],
     "mfq_process_logits": [_vp, _vp, _i, _i, _i, _ll, _ll, _vp, _i, _vp, _ll, _vp, _vp, _i, _vp, _i, _vp, _i, _f, _vp],
     "mfq_count_tokens": [_vp, _ll, _i, _i, _vp, _vp, _i, _i, _vp],
     "mfq_plan_batch": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],

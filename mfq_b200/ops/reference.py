@@ -126,6 +126,26 @@ def paged_attn_decode(q, kv, block_table, seq_lens, sm_scale, q_len: int = 1):
     return torch.cat(outs, 0)
 
 
+def paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale, members, q_len: int, out) -> None:
+    starts, width = group_starts.tolist(), block_table.shape[1]
+    order = list(range(seq_lens.numel())) if members is None else members.tolist()
+    for g, prefix in enumerate(prefix_lens.tolist()):
+        rows = order[starts[g] : starts[g + 1]]
+        front = min(max(0, prefix) // kv.page_size, width)
+        for r in rows:
+            table = torch.cat([block_table[rows[0], :front], block_table[r, front:]])
+            n = min(int(seq_lens[r]), width * kv.page_size)
+            at = slice(r * q_len, (r + 1) * q_len)
+            if n <= 0:
+                out[at] = 0
+                continue
+            k, v = gather_paged(kv, table, n)
+            o = attention(q[at], k, v, sm_scale, causal_offset=n - q_len)
+            if n < q_len:  # a window's queries in front of the sequence's first token see nothing
+                o[: q_len - n] = 0
+            out[at] = o
+
+
 def write_kv(kv, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     from ..engine.kv_cache import V_SLOT_OF_TOKEN
     kq, ks = quant_kv(k)

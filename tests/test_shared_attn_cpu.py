@@ -1,0 +1,52 @@
+"""``ops.paged_attn_decode_shared`` on CPU tensors, and what it refuses."""
+
+import pytest
+import torch
+
+from mfq_b200 import ops
+from shared_attn_cases import BATCHES, assert_attends, batch, call, exact
+
+
+@pytest.mark.parametrize("groups,how", BATCHES)
+def test_against_the_definition(groups, how):
+    s = batch(len(groups), groups, **how)
+    out = torch.full_like(s.q, 3.0)
+    assert call(ops, s, out=out) is out
+    assert_attends(s, out, exact(s))
+    rest = [r * s.q_len + i for r in range(s.seq_lens.numel()) if r not in s.grouped for i in range(s.q_len)]
+    assert (out[rest] == 3).all()
+
+
+def test_refusals():
+    s = batch(1, [(16, [20, 30])])
+    long = lambda t: t.long()  # noqa: E731
+    for name, make in (("q", lambda t: t.float()), ("q", lambda t: t[:, :7]), ("q", lambda t: t[:, :, :96].contiguous()), ("q", lambda t: t.transpose(0, 1)),
+                       ("table", long), ("table", lambda t: t[:1]), ("table", lambda t: t[:, ::2]), ("seq_lens", long), ("seq_lens", lambda t: t[:1]), ("starts", long),
+                       ("starts", lambda t: t[:1]), ("prefixes", long), ("members", long), ("members", lambda t: t[:1])):
+        held = getattr(s, name)
+        setattr(s, name, make(held))
+        with pytest.raises(ValueError):
+            call(ops, s)
+        setattr(s, name, held)
+    with pytest.raises(ValueError, match="16 query rows"):
+        call(ops, batch(1, [(16, [20, 30])], hq=24, hk=1))
+    s.q_len = 3
+    with pytest.raises(ValueError):
+        call(ops, s)
+    s.q_len = 1
+    with pytest.raises(ValueError, match="out"):
+        call(ops, s, out=torch.zeros_like(s.q, dtype=torch.float32))
+    s.kv.page_size = 32
+    with pytest.raises(ValueError, match="16 tokens"):
+        call(ops, s)
+    s.kv.page_size = 16
+    s.starts, s.prefixes = torch.tensor([0, 1, 2, 2], dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="3 groups of 2 rows"):
+        call(ops, s)
+
+
+def test_no_groups():
+    s = batch(1, [(16, [20, 30])])
+    s.starts, s.prefixes = s.starts[:1].contiguous(), s.prefixes[:0].contiguous()
+    out = torch.full_like(s.q, 3.0)
+    assert (call(ops, s, out=out) == 3).all()
