@@ -20,6 +20,14 @@ def _pick_splits(units: int, pages: int, per_sm: int, least: int, most: int = 32
     return max(1, min(SMS * per_sm // max(1, units), pages // least, most))
 
 
+def _pick_tile(rows: int, d: int) -> int:
+    """Query rows of a prefix CTA for groups of ``rows`` query rows a KV head: 16, 32, 64 on mma.sync, 128 and 256 on tcgen05."""
+    for tile in (16, 32, 64):
+        if rows <= tile:
+            return tile
+    return 64 if d > 128 else 128 if rows <= 128 else 256
+
+
 def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, group_starts: torch.Tensor,
                              prefix_lens: torch.Tensor, *, sm_scale: float, members: torch.Tensor | None = None, q_len: int = 1,
                              max_group: int | None = None, max_prefix: int | None = None, max_tail: int | None = None,
@@ -65,15 +73,15 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
     tail = width if max_tail is None else min(width, max(0, max_tail) // 16 + 1)
     rows = max_group * (hq // hk) * q_len
-    tile = 16 if rows <= 16 else 32 if rows <= 32 else 64
-    prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 3 if d <= 128 else 1, 16)
+    tile = _pick_tile(rows, d)
+    prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 1 if tile >= 128 or d > 128 else 3, 16)
     tail_splits = _pick_splits(b * hk, tail, 3 if d <= 128 else 1, 16)
-    slots = prefix_splits + tail_splits
+    slots = prefix_splits * (2 if tile == 128 else 1) + tail_splits
     with current_device(dev):
         scratch = torch.empty(n * hq * slots * (d + 2), dtype=torch.float32, device=dev)  # of this call: a workspace would tie streams and graphs together
         split = n * hq * slots * d
         check(lib().mfq_paged_attn_decode_shared(
             ptr(q), ptr(kv.k), ptr(kv.v), ptr(kv.k_scale), ptr(kv.v_scale), ptr(block_table), ptr(seq_lens), ptr(group_starts), ptr(prefix_lens), ptr(members),
-            ptr(out), ptr(scratch), scratch.data_ptr() + 4 * split, b, hq, hk, d, width, pages, groups, q_len, max_group, prefix_splits, tail_splits,
+            ptr(out), ptr(scratch), scratch.data_ptr() + 4 * split, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
             float(sm_scale), ptr(Workspace.get(dev).status), stream_ptr()), "paged_attn_decode_shared", 3)
     return out
