@@ -351,7 +351,7 @@ int launch_shared_prefix_tc(const SharedAttnArgs& a, int dim, bool two_tiles, cu
 
 template <int D>
 static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream) {
-  const dim3 grid(a.B * (a.Hq / a.Hk) * a.q_len / tile + a.groups, a.Hk, a.prefix_splits);
+  const dim3 grid(tiles_at_most(a, tile), a.Hk, a.prefix_splits);
   const int rc = tile == 16   ? launch_shared_units<D, 1, true>(a, grid, stream)
                  : tile == 32 ? launch_shared_units<D, 2, true>(a, grid, stream)
                  : tile == 64 ? launch_shared_units<D, 4, true>(a, grid, stream)

@@ -46,8 +46,7 @@ __device__ __forceinline__ float power_to(float x, int at) {
   const int e = int(__float_as_uint(x) >> 23 & 0xff);
   return e == 0 || e == 255 ? 1.f : __uint_as_float(uint32_t(min(max(254 + at - e, 1), 254)) << 23);
 }
-// The x-th of the groups' tiles of `per_tile` query rows, all groups in order (whole warp): its group and number, false behind the last one.  n rows in
-// g groups have at most n / per_tile + g tiles, whatever the groups are.
+// The x-th of the groups' tiles of `per_tile` query rows, all groups in order (whole warp): its group and number, false behind the last one.
 __device__ __forceinline__ bool find_tile(const SharedAttnArgs& a, int x, int per_tile, int per_seq, int& group, int& tile) {
   int before = 0;
   for (int g = 0; g < a.groups; g += 32) {
@@ -88,5 +87,11 @@ __device__ __forceinline__ int member_row(const SharedAttnArgs& a, int place) { 
   return row >= 0 && row < a.B ? row : -1;
 }
 
+
+// A group of n rows has (n - 1) / per_tile + 1 tiles, so that g groups of n in all have at most this, whatever the groups are.
+inline int tiles_at_most(const SharedAttnArgs& a, int per_tile) {
+  const int rows = a.B * (a.Hq / a.Hk) * a.q_len;
+  return (rows - a.groups) / per_tile + a.groups;
+}
 
 }  // namespace mfq
