@@ -13,6 +13,7 @@
 // two, kept for the rows of a warp, that brings the multipliers near 2^4 and is raised, the sums with it, where a page has larger ones.
 // The reference reads shared prefixes once per row (mfq/kernels/cuda/paged_kv.cu).
 #include "attn_shared.cuh"
+#include "pair.cuh"
 
 namespace mfq {
 
@@ -26,10 +27,10 @@ struct SharedTile {
   static_assert(kRing >= 4 * (16 * D + 32) * 4, "the ring is the merge's scratch too");
 };
 
-// kPrefix: blockIdx.x = one of the groups' tiles of 16 WR rows; else blockIdx.x = place.  blockIdx.z = split.
-template <int D, int WR, bool kPrefix>
+// The prefixes of groups with few query rows: blockIdx.x = one of the groups' tiles of 16 WR rows, blockIdx.z = split.
+template <int D, int WR>
 __global__ void __launch_bounds__(128, D <= 128 ? 3 : 1)
-shared_attn_kernel(const SharedAttnArgs a) {
+shared_prefix_kernel(const SharedAttnArgs a) {
   using L = SharedTile<D, WR>;
   constexpr int KSTEPS = D / 16, NBD = D / 8, kStages = L::kStages, kLanes = L::kLanes;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -39,7 +40,6 @@ shared_attn_kernel(const SharedAttnArgs a) {
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + page_lane * kStages;
   uint64_t* empty = reinterpret_cast<uint64_t*>(smem + L::kRing) + (kLanes + page_lane) * kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + 2 * kLanes * kStages * 8);
-  pdl_trigger();
   if (threadIdx.x == 0) *abort_flag = 0;
   if (lane == 0 && tile16 == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], WR); }
@@ -47,39 +47,21 @@ shared_attn_kernel(const SharedAttnArgs a) {
   }
   __syncthreads();
   pdl_wait();
+  pdl_trigger();  // behind the wait: the tails, which may start now, read what this kernel's predecessors wrote
 
-  const int kvh = blockIdx.y, G = a.Hq / a.Hk, per_seq = G * a.q_len;
-  const int splits = kPrefix ? a.prefix_splits : a.tail_splits, split = blockIdx.z;
-  int first, count, slot, tile = 0;  // places of the unit, where its partial goes
-  int page_lo, page_hi;
-  if constexpr (kPrefix) {
-    int g;
-    if (!find_tile(a, blockIdx.x, 16 * WR, per_seq, g, tile)) return;
-    first = min(max(a.group_starts[g], 0), a.B);
-    count = min(max(a.group_starts[g + 1], first), a.B) - first;
-    page_lo = 0;
-    page_hi = min(max(a.prefix_lens[g], 0) >> 4, a.max_pages);
-    slot = split;
-  } else {
-    first = blockIdx.x;
-    const int g = group_of(a, first);
-    count = g < a.groups && first >= a.group_starts[0] ? 1 : 0;
-    const int row = count ? member_row(a, first) : -1;
-    page_lo = count ? min(max(a.prefix_lens[g], 0) >> 4, a.max_pages) : 0;
-    page_hi = row >= 0 ? min((max(a.seq_lens[row], 0) + 15) >> 4, a.max_pages) : 0;
-    slot = a.slots - a.tail_splits + split;
-  }
-  if (count == 0) return;
+  const int kvh = blockIdx.y, G = a.Hq / a.Hk, per_seq = G * a.q_len, split = blockIdx.z;
+  int group, tile;
+  if (!find_tile(a, blockIdx.x, 16 * WR, per_seq, group, tile)) return;
+  const int first = min(max(a.group_starts[group], 0), a.B), rows = (min(max(a.group_starts[group + 1], first), a.B) - first) * per_seq;
   const int table_row = member_row(a, first);
-  if (table_row < 0) { page_hi = page_lo; }
-  {
-    const int n = max(page_hi - page_lo, 0), per = (n + splits - 1) / splits;
-    page_lo += split * per;
-    page_hi = min(page_hi, page_lo + per);
+  int page_lo = 0, page_hi = 0;
+  if (table_row >= 0) {
+    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
+    page_lo = min(split * per, n);
+    page_hi = min(n, page_lo + per);
   }
   const int my_pages = page_hi > page_lo + page_lane ? (page_hi - page_lo - page_lane + kLanes - 1) / kLanes : 0;
   const int* bt = a.table + size_t(max(table_row, 0)) * a.max_pages;
-  const int rows = count * per_seq;
   bool ok = true;
 
   auto issue = [&](int i) {  // one thread of the lane: start the copies of its i-th page
@@ -289,61 +271,423 @@ shared_attn_kernel(const SharedAttnArgs a) {
       ll += wo[16 * D + 2 * r + 1] * cw;
       acc += wo[r * D + d] * cw;
     }
-    const size_t part = ((size_t(row) * a.q_len + in / G) * a.Hq + kvh * G + in % G) * a.slots + slot;
+    const size_t part = ((size_t(row) * a.q_len + in / G) * a.Hq + kvh * G + in % G) * a.slots + split;
     a.part_o[part * D + d] = acc;
     if (d == 0) { a.part_ml[2 * part] = mm; a.part_ml[2 * part + 1] = ll; }
   }
 }
 
-// A warp per query row and head: o = sum of the partials' o 2^(m - max) / sum of their l 2^(m - max).
-template <int D>
-__global__ void __launch_bounds__(256)
-shared_attn_merge_kernel(const SharedAttnArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int item = blockIdx.x * 8 + warp, per_seq = a.q_len * a.Hq, place = item / per_seq;
-  if (place >= a.B || place < a.group_starts[0] || place >= a.group_starts[a.groups]) return;
-  const int row = member_row(a, place);
-  if (row < 0) return;
-  const size_t hq = size_t(row) * per_seq + item % per_seq;
-  const float* ml = a.part_ml + hq * a.slots * 2;
-  const float* po = a.part_o + hq * a.slots * D;
-  float mm = kSharedNeg;
-  for (int s = lane; s < a.slots; s += 32) mm = fmaxf(mm, ml[2 * s + 1] > 0.f || isnan(ml[2 * s + 1]) ? ml[2 * s] : kSharedNeg);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  float ll = 0.f, acc[D / 32] = {};
-  for (int s = 0; s < a.slots; ++s) {
-    const float l = ml[2 * s + 1];
-    if (l == 0.f) continue;  // nothing seen there
-    const float w = exp2f(ml[2 * s] - mm);
-    ll += l * w;
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const float2 x = *reinterpret_cast<const float2*>(po + s * D + 64 * j + 2 * lane);
-      acc[2 * j] += x.x * w;
-      acc[2 * j + 1] += x.y * w;
-    }
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll
-  for (int j = 0; j < D / 64; ++j)
-    *reinterpret_cast<__nv_bfloat162*>(a.out + hq * D + 64 * j + 2 * lane) = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+__device__ __forceinline__ uint32_t transposed_pairs(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float4 load_peer(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 load_peer2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
 }
 
-template <int D, int WR, bool kPrefix>
-static int launch_shared_units(const SharedAttnArgs& a, dim3 grid, cudaStream_t stream) {
-  using L = SharedTile<D, WR>;
-  auto kernel = &shared_attn_kernel<D, WR, kPrefix>;
-  static bool attr[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
-  if (!attr[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return -6;
-    attr[dev] = true;
+// What a warp has of a tail: the running maximum and sum of its rows and their outputs, in one of two forms.
+//   wide   (up to 16 query rows): rows are the rows of the products, lane parts (g8, c) of m16n8k16 fragments
+//   narrow (up to 8): the page's 16 tokens are the rows and the query rows the columns, S^T = K Q^T and O^T += V^T P, which halves the
+//          products and the softmax (attn_decode.cu); a lane has the columns 2c and 2c + 1, of tokens (dims) g8 and g8 + 8
+template <int D, bool kNarrow>
+struct TailRows {
+  static constexpr int kSteps = D / 16, kOut = kNarrow ? D / 16 : D / 8, kQ = kNarrow ? 2 : 4;
+  uint32_t q[kSteps][kQ];
+  float o[kOut][4], m[2], l[2], to_log2[2], v_up;
+  int len[2], low, most;
+
+  // a row of the unit as this lane loads it: r = g8 (narrow), g8 + 8 half (wide)
+  __device__ __forceinline__ void load(const SharedAttnArgs& a, int row, int kvh, int G, int rows, int seq_len, int g8, int c) {
+    float up[2];
+#pragma unroll
+    for (int half = 0; half < (kNarrow ? 1 : 2); ++half) {
+      const int r = g8 + 8 * half;
+      const __nv_bfloat16* qp = a.q + ((size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G) * D;
+      uint2 raw[kSteps];
+      float top = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        raw[s] = make_uint2(0, 0);
+        if (r < rows) raw[s] = *reinterpret_cast<const uint2*>(qp + 64 * (s >> 2) + 16 * c + 4 * (s & 3));
+        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[s]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(__bfloat162float(b[e])));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      up[half] = power_to(top, 13);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[s]);
+        q[s][half] = half_pair(__bfloat162float(b[0]) * up[half], __bfloat162float(b[1]) * up[half]);
+        q[s][kNarrow ? 1 : 2 + half] = half_pair(__bfloat162float(b[2]) * up[half], __bfloat162float(b[3]) * up[half]);
+      }
+    }
+    int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = kNarrow ? 2 * c + e : g8 + 8 * e;
+      const float of = kNarrow ? __shfl_sync(0xffffffffu, up[0], r * 4) : up[e];
+      to_log2[e] = a.scale_log2 / of;
+      // a row that is not there has a zero query and is never stored: unmasked, it leaves `whole` below to the others
+      len[e] = r < rows ? seq_len - (a.q_len - 1 - r / G) : 0x7fffffff;
+      lo = min(lo, len[e]);
+      hi = max(hi, r < rows ? len[e] : 0);
+      m[e] = kSharedNeg;
+      l[e] = 0.f;
+    }
+    low = __reduce_min_sync(0xffffffffu, lo);
+    most = __reduce_max_sync(0xffffffffu, hi);
+    v_up = 0.f;  // power of two on the V multipliers; 0: none chosen yet
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   }
-  launch_kernel(kernel, grid, dim3(128), L::kSmem, stream, a);
+
+  // the V multipliers of this lane's tokens, near 2^4 or less after a power of two that the warp keeps; what nobody sees may hold anything
+  __device__ __forceinline__ bool raises(float a, float b) const {
+    const float big = fmaxf(fabsf(a), fabsf(b));
+    return big * v_up > 1024.f || (v_up == 0.f && big > 0.f);
+  }
+  __device__ __forceinline__ void raise(float big, float (&o_corr)[2]) {
+    const float up = power_to(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))), 4);
+    if (v_up != 0.f) { o_corr[0] *= up / v_up; o_corr[1] *= up / v_up; }
+    v_up = up;
+  }
+
+  __device__ __forceinline__ void page(const uint8_t* sK, int tok0, int g8, int c) {
+    const uint8_t* sV = sK + 16 * D;
+    const float *sKs = reinterpret_cast<const float*>(sV + 16 * D), *sVs = sKs + 16;
+    const bool whole = tok0 + 16 <= low;  // all rows see all of the page
+    uint32_t keep = 0xffffffffu;  // codes of tokens that no row sees are left out: 0 times a NaN would be one
+    if (!whole) {
+      keep = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (tok0 + 2 * c + (e & 1) + 8 * (e >> 1) < most) keep |= 0xffu << (8 * e);
+    }
+    if constexpr (kNarrow) {
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ch = 0; ch < D / 64; ++ch) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(sK + ch * 1024 + g8 * 64 + c * 16);
+        const uint4 k1 = *reinterpret_cast<const uint4*>(sK + ch * 1024 + (8 + g8) * 64 + c * 16);
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) {
+          const uint32_t f[4] = {e4m3_pair(w0[sub]), e4m3_pair(w1[sub]), e4m3_pair(w0[sub] >> 16), e4m3_pair(w1[sub] >> 16)};
+          mma_half(sc, f, q[ch * 4 + sub][0], q[ch * 4 + sub][1]);
+        }
+      }
+      const float ks0 = sKs[g8], ks1 = sKs[g8 + 8];
+      float vs0 = sVs[g8], vs1 = sVs[g8 + 8];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sc[x] *= (x < 2 ? ks0 : ks1) * to_log2[x & 1];
+      if (!whole) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (tok0 + g8 + 8 * (x >> 1) >= len[x & 1]) sc[x] = kSharedNeg;
+        if (tok0 + g8 >= most) vs0 = 0.f;
+        if (tok0 + g8 + 8 >= most) vs1 = 0.f;
+      }
+      float corr[2], o_corr[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(sc[e], sc[2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[e], mx);
+        o_corr[e] = corr[e] = exp2f(m[e] - mn);
+        m[e] = mn;
+      }
+      if (__any_sync(0xffffffffu, raises(vs0, vs1))) raise(fmaxf(fabsf(vs0), fabsf(vs1)), o_corr);
+      float p[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int e = x & 1;
+        // a masked score is kSharedNeg: exp2 gives 0 unless the whole row is still empty, hence the test (true for NaN)
+        const float pe = !(sc[x] <= 0.5f * kSharedNeg) ? exp2f(sc[x] - m[e]) : 0.f;
+        l[e] = (x < 2 ? l[e] * corr[e] : l[e]) + pe;
+        p[x] = pe * ((x < 2 ? vs0 : vs1) * v_up);
+      }
+      const uint32_t pb0 = transposed_pairs(half_pair(p[0], p[1])), pb1 = transposed_pairs(half_pair(p[2], p[3]));
+      if (__any_sync(0xffffffffu, o_corr[0] != 1.f || o_corr[1] != 1.f)) {
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) { o[j][0] *= o_corr[0]; o[j][1] *= o_corr[1]; o[j][2] *= o_corr[0]; o[j][3] *= o_corr[1]; }
+      }
+#pragma unroll
+      for (int j = 0; j < kOut; ++j) {
+        const uint32_t v0 = *reinterpret_cast<const uint32_t*>(sV + (16 * j + g8) * 16 + 4 * c) & keep;
+        const uint32_t v1 = *reinterpret_cast<const uint32_t*>(sV + (16 * j + 8 + g8) * 16 + 4 * c) & keep;
+        const uint32_t f[4] = {e4m3_pair(v0), e4m3_pair(v1), e4m3_pair(v0 >> 16), e4m3_pair(v1 >> 16)};
+        mma_half(o[j], f, pb0, pb1);
+      }
+    } else {
+      float sc[2][4], mx[2] = {kSharedNeg, kSharedNeg};
+      float2 vs[2];
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < D / 64; ++ch) {
+          const uint4 kw = *reinterpret_cast<const uint4*>(sK + ch * 1024 + (nb * 8 + g8) * 64 + c * 16);
+          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+          for (int sub = 0; sub < 4; ++sub) mma_half(sc[nb], q[ch * 4 + sub], e4m3_pair(w[sub]), e4m3_pair(w[sub] >> 16));
+        }
+      }
+      bool up = false;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        const int tk = nb * 8 + 2 * c;
+        const float2 ks = *reinterpret_cast<const float2*>(sKs + tk);
+        vs[nb] = *reinterpret_cast<const float2*>(sVs + tk);
+        if (!whole) {
+          if (tok0 + tk >= most) vs[nb].x = 0.f;
+          if (tok0 + tk + 1 >= most) vs[nb].y = 0.f;
+        }
+        up |= raises(vs[nb].x, vs[nb].y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int half = e >> 1;
+          sc[nb][e] *= ((e & 1) ? ks.y : ks.x) * to_log2[half];
+          if (!whole && tok0 + tk + (e & 1) >= len[half]) sc[nb][e] = kSharedNeg;
+          mx[half] = fmaxf(mx[half], sc[nb][e]);
+        }
+      }
+      float corr[2], o_corr[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+        const float mn = fmaxf(m[half], mx[half]);
+        o_corr[half] = corr[half] = exp2f(m[half] - mn);
+        m[half] = mn;
+      }
+      if (__any_sync(0xffffffffu, up)) raise(fmaxf(fmaxf(fabsf(vs[0].x), fabsf(vs[0].y)), fmaxf(fabsf(vs[1].x), fabsf(vs[1].y))), o_corr);
+      float psum[2] = {0.f, 0.f}, p[2][4];
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int half = e >> 1;
+          const float pe = !(sc[nb][e] <= 0.5f * kSharedNeg) ? exp2f(sc[nb][e] - m[half]) : 0.f;
+          psum[half] += pe;
+          p[nb][e] = pe * (((e & 1) ? vs[nb].y : vs[nb].x) * v_up);
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) l[half] = l[half] * corr[half] + psum[half];
+      const uint32_t pa[4] = {half_pair(p[0][0], p[0][1]), half_pair(p[0][2], p[0][3]), half_pair(p[1][0], p[1][1]), half_pair(p[1][2], p[1][3])};
+      if (__any_sync(0xffffffffu, o_corr[0] != 1.f || o_corr[1] != 1.f)) {
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) { o[j][0] *= o_corr[0]; o[j][1] *= o_corr[0]; o[j][2] *= o_corr[1]; o[j][3] *= o_corr[1]; }
+      }
+#pragma unroll
+      for (int j = 0; j < kOut; ++j) {
+        const uint32_t vw = *reinterpret_cast<const uint32_t*>(sV + (8 * j + g8) * 16 + 4 * c) & keep;
+        mma_half(o[j], pa, e4m3_pair(vw), e4m3_pair(vw >> 16));
+      }
+    }
+  }
+
+  // [rows][D] outputs, then (m, l) of each row
+  __device__ __forceinline__ void put(float* to, int g8, int c) {
+    const float down = v_up != 0.f ? 1.f / v_up : 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = kNarrow ? 2 * c + e : g8 + 8 * e;
+      if constexpr (kNarrow) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) {
+          to[r * D + 16 * j + g8] = o[j][e] * down;
+          to[r * D + 16 * j + 8 + g8] = o[j][2 + e] * down;
+        }
+      } else {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) *reinterpret_cast<float2*>(to + r * D + 8 * j + 2 * c) = make_float2(o[j][2 * e] * down, o[j][2 * e + 1] * down);
+      }
+      if ((kNarrow ? g8 : c) == 0) *reinterpret_cast<float2*>(to + 16 * D + 2 * r) = make_float2(m[e], l[e]);
+    }
+  }
+};
+
+constexpr int kMostSlots = 64, kMostRanks = 8;
+
+// The tails, and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
+// are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own part done.
+template <int D, bool kNarrow>
+__global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
+shared_tail_kernel(const SharedAttnArgs a) {
+  using L = SharedTile<D, 1>;
+  constexpr int kStages = L::kStages, kPart = 16 * D + 32;  // floats of a partial
+  static_assert(L::kRing >= (5 * kPart + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the ring is the merge's scratch too");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * kStages * L::kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + warp * kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + 2 * L::kLanes * kStages * 8);
+  pdl_trigger();
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  const int place = blockIdx.x, kvh = blockIdx.y, ranks = gridDim.z, rank = blockIdx.z;
+  const int G = a.Hq / a.Hk, rows = G * a.q_len;
+  const int group = group_of(a, place);
+  const int row = group < a.groups && place >= a.group_starts[0] ? member_row(a, place) : -1;
+  if (row < 0) {  // the whole cluster alike
+    pdl_wait();  // this grid ends behind the prefixes' in any case
+    return;
+  }
+  const int front = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), seq_len = a.seq_lens[row];
+  const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
+  const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
+  const int my_pages = page_hi > page_lo + warp ? (page_hi - page_lo - warp + 3) / 4 : 0;
+  const int* bt = a.table + size_t(row) * a.max_pages;
+  int next = lane == 0 && my_pages > 0 ? bt[page_lo + warp] : 0;
+  const auto issue = [&](int i) {  // lane 0: start the copies of this warp's i-th page; its id was fetched a page ahead
+    const int s = i % kStages;
+    int page = next;
+    if (i + 1 < my_pages) next = bt[page_lo + warp + 4 * (i + 1)];
+    if (page < 0 || page >= a.pages) {
+      atomicCAS(a.status, 0, kStatusBadArgument);
+      page = 0;
+    }
+    const size_t ph = size_t(page) * a.Hk + kvh;
+    uint8_t* st = ring + s * L::kStage;
+    mbar_expect_tx(&full[s], L::kStage);
+    shared_bulk_load(st, a.k + ph * L::kPage, L::kPage, &full[s]);
+    shared_bulk_load(st + L::kPage, a.v + ph * L::kPage, L::kPage, &full[s]);
+    shared_bulk_load(st + 2 * L::kPage, a.k_scale + ph * 16, 64, &full[s]);
+    shared_bulk_load(st + 2 * L::kPage + 64, a.v_scale + ph * 16, 64, &full[s]);
+  };
+  if (lane == 0)
+    for (int i = 0; i < min(my_pages, kStages); ++i) issue(i);
+  TailRows<D, kNarrow> t;
+  t.load(a, row, kvh, G, rows, seq_len, g8, c);
+  for (int i = 0; i < my_pages; ++i) {
+    const int s = i % kStages;
+    if (!mbar_wait_warp(&full[s], (i / kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) break;
+    t.page(ring + s * L::kStage, (page_lo + warp + 4 * i) << 4, g8, c);
+    __syncwarp();
+    if (lane == 0 && i + kStages < my_pages) issue(i + kStages);
+  }
+  // ---- the warps' parts to one, in shared memory ----
+  float* parts = reinterpret_cast<float*>(smem);
+  float *mine = parts + 4 * kPart, *weights = mine + kPart, *inverse = weights + 16 * (kMostSlots + kMostRanks);
+  __syncthreads();
+  t.put(parts + warp * kPart, g8, c);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float mm = kSharedNeg, ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, parts[w * kPart + 16 * D + 2 * r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = exp2f(parts[w * kPart + 16 * D + 2 * r] - mm);
+      const float4 v = *reinterpret_cast<const float4*>(parts + w * kPart + r * D + d);
+      ll += parts[w * kPart + 16 * D + 2 * r + 1] * by;
+      acc.x += v.x * by; acc.y += v.y * by; acc.z += v.z * by; acc.w += v.w * by;
+    }
+    *reinterpret_cast<float4*>(mine + r * D + d) = acc;
+    if (d == 0) *reinterpret_cast<float2*>(mine + 16 * D + 2 * r) = make_float2(mm, ll);
+  }
+  if (ranks > 1) cluster_sync_all();
+  else __syncthreads();
+  pdl_wait();  // the prefixes' partials
+  // ---- weights of the ranks' parts and of the prefix's, a warp to a row ----
+  const int entries = ranks + a.slots;
+  for (int r = warp; r < rows; r += 4) {
+    const size_t hq = (size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G;
+    float2 ml[(kMostSlots + kMostRanks + 31) / 32];
+    float mm = kSharedNeg, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < (kMostSlots + kMostRanks + 31) / 32; ++x) {
+      const int e = x * 32 + lane;
+      ml[x] = make_float2(kSharedNeg, 0.f);
+      if (e < ranks) ml[x] = load_peer2(map_to_cta(mine + 16 * D + 2 * r, e));
+      else if (e < entries) ml[x] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (hq * a.slots + e - ranks));
+      if (ml[x].y != 0.f) mm = fmaxf(mm, ml[x].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+#pragma unroll
+    for (int x = 0; x < (kMostSlots + kMostRanks + 31) / 32; ++x) {
+      const int e = x * 32 + lane;
+      const float by = ml[x].y != 0.f ? exp2f(ml[x].x - mm) : 0.f;  // a part that saw nothing may hold anything
+      sum += ml[x].y * by;
+      if (e < entries) weights[r * (kMostSlots + kMostRanks) + e] = by;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) inverse[r] = sum != 0.f ? 1.f / sum : 0.f;
+  }
+  __syncthreads();
+  for (int i = rank * 128 + threadIdx.x; i < rows * (D / 4); i += ranks * 128) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    const size_t hq = (size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G;
+    const float* by = weights + r * (kMostSlots + kMostRanks);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](const float4& v, float w) {
+      if (w != 0.f) { acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w; }
+    };
+    for (int e = 0; e < ranks; ++e) add(load_peer(map_to_cta(mine + r * D + d, e)), by[e]);
+    const float4* src = reinterpret_cast<const float4*>(a.part_o + hq * a.slots * D + d);
+    int e = 0;
+    for (; e + 8 <= a.slots; e += 8) {  // all requested before the first is used
+      float4 v[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = __ldcg(src + (e + x) * (D / 4));
+#pragma unroll
+      for (int x = 0; x < 8; ++x) add(v[x], by[ranks + e + x]);
+    }
+    for (; e < a.slots; ++e) add(__ldcg(src + e * (D / 4)), by[ranks + e]);
+    const float n = inverse[r];
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * n, acc.y * n), __floats2bfloat162_rn(acc.z * n, acc.w * n)};
+    *reinterpret_cast<uint2*>(a.out + hq * D + d) = *reinterpret_cast<const uint2*>(h);
+  }
+  if (ranks > 1) cluster_sync_all();  // parts are read until here
+}
+
+template <typename K>
+static bool set_smem(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!done[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  return done[dev] = true;
+}
+template <int D, int WR>
+static int launch_shared_prefix(const SharedAttnArgs& a, cudaStream_t stream) {
+  static bool done[64] = {};
+  if (!set_smem(shared_prefix_kernel<D, WR>, SharedTile<D, WR>::kSmem, done)) return -6;
+  launch_kernel(shared_prefix_kernel<D, WR>, dim3(tiles_at_most(a, 16 * WR), a.Hk, a.prefix_splits), dim3(128), SharedTile<D, WR>::kSmem, stream, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -7;
+}
+template <int D, bool kNarrow>
+static int launch_shared_tail(const SharedAttnArgs& a, cudaStream_t stream) {
+  static bool done[64] = {};
+  if (!set_smem(shared_tail_kernel<D, kNarrow>, SharedTile<D, 1>::kSmem, done)) return -6;
+  const dim3 grid(a.B, a.Hk, a.tail_splits);
+  if (a.tail_splits > 1) launch_kernel_clustered(shared_tail_kernel<D, kNarrow>, grid, dim3(128), dim3(1, 1, a.tail_splits), SharedTile<D, 1>::kSmem, stream, a);
+  else launch_kernel(shared_tail_kernel<D, kNarrow>, grid, dim3(128), SharedTile<D, 1>::kSmem, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 
@@ -351,32 +695,30 @@ int launch_shared_prefix_tc(const SharedAttnArgs& a, int dim, bool two_tiles, cu
 
 template <int D>
 static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream) {
-  const dim3 grid(tiles_at_most(a, tile), a.Hk, a.prefix_splits);
-  const int rc = tile == 16   ? launch_shared_units<D, 1, true>(a, grid, stream)
-                 : tile == 32 ? launch_shared_units<D, 2, true>(a, grid, stream)
-                 : tile == 64 ? launch_shared_units<D, 4, true>(a, grid, stream)
+  const int rc = tile == 16   ? launch_shared_prefix<D, 1>(a, stream)
+                 : tile == 32 ? launch_shared_prefix<D, 2>(a, stream)
+                 : tile == 64 ? launch_shared_prefix<D, 4>(a, stream)
                               : launch_shared_prefix_tc(a, D, tile == 256, stream);
   if (rc) return rc;
-  if (const int rc = launch_shared_units<D, 1, false>(a, dim3(a.B, a.Hk, a.tail_splits), stream)) return rc;
-  launch_kernel(shared_attn_merge_kernel<D>, dim3((a.B * a.q_len * a.Hq + 7) / 8), dim3(256), 0, stream, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -7;
+  return (a.Hq / a.Hk) * a.q_len <= 8 ? launch_shared_tail<D, true>(a, stream) : launch_shared_tail<D, false>(a, stream);
 }
 
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16; pages of the FP8 pool, `pages` of them; group_starts [groups + 1], prefix_lens [groups], members [B] or null; tile: query rows of a
-// prefix CTA, 16, 32, 64 or for heads of 64 and 128 also 128, 256; partials [B * q_len * Hq * (prefix_splits (twice for a tile of 128) + tail_splits)] x D and x 2 floats.  (Hq / Hk) * q_len <= 16.  Rows in no group are not written.
+// prefix CTA, 16, 32, 64 or for heads of 64 and 128 also 128, 256; partials [B * q_len * Hq * prefix_splits (twice
+// that for a tile of 128; 64 at most)] x D and x 2 floats; tail_splits: 8 at most.  (Hq / Hk) * q_len <= 16.  Rows in no group are not written.
 extern "C" int mfq_paged_attn_decode_shared(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* table,
                                             const int* seq_lens, const int* group_starts, const int* prefix_lens, const int* members, void* out,
                                             float* part_o, float* part_ml, int B, int Hq, int Hk, int D, int max_pages, int pages, int groups, int q_len,
                                             int tile, int prefix_splits, int tail_splits, float sm_scale, int* status, cudaStream_t stream) {
   using namespace mfq;
   if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (tile != 16 && tile != 32 && tile != 64 && (D > 128 || (tile != 128 && tile != 256))) || prefix_splits < 1 ||
-      tail_splits < 1 || pages < 1 || max_pages < 1 || Hk > 65535 || prefix_splits > 65535 || tail_splits > 65535)
+      tail_splits < 1 || pages < 1 || max_pages < 1 || Hk > 65535 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits > kMostRanks)
     return -1;
   const SharedAttnArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_scale, v_scale, table, seq_lens,
                          group_starts, prefix_lens, members, part_o, part_ml, static_cast<__nv_bfloat16*>(out), status, B, Hq, Hk, max_pages, pages, groups,
-                         q_len, prefix_splits * (tile == 128 ? 2 : 1) + tail_splits, prefix_splits, tail_splits, sm_scale * 1.4426950408889634f};
+                         q_len, prefix_splits * (tile == 128 ? 2 : 1), prefix_splits, tail_splits, sm_scale * 1.4426950408889634f};
   if (D == 128) return launch_shared<128>(a, tile, stream);
   if (D == 256) return launch_shared<256>(a, tile, stream);
   if (D == 64) return launch_shared<64>(a, tile, stream);

@@ -15,10 +15,10 @@ struct SharedAttnArgs {
   const float *k_scale, *v_scale;
   const int *table, *seq_lens;         // [B, max_pages], [B]
   const int *group_starts, *prefix_lens, *members;  // [groups + 1] places, [groups], [B] batch row of each place (null: its number)
-  float *part_o, *part_ml;             // [B * q_len * Hq, slots, D], [.., slots, 2]
+  float *part_o, *part_ml;             // of the prefixes: [B * q_len * Hq, slots, D], [.., slots, 2]
   __nv_bfloat16* out;
   int* status;
-  int B, Hq, Hk, max_pages, pages, groups, q_len, slots, prefix_splits, tail_splits;  // slots: partials of a query row and head, the tail's behind the prefix's
+  int B, Hq, Hk, max_pages, pages, groups, q_len, slots, prefix_splits, tail_splits;  // slots: partials of a query row and head over its prefix
   float scale_log2;
 };
 

@@ -75,13 +75,13 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     rows = max_group * (hq // hk) * q_len
     tile = _pick_tile(rows, d)
     prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 1 if tile >= 128 or d > 128 else 3, 16)
-    tail_splits = _pick_splits(b * hk, tail, 3 if d <= 128 else 1, 16)
-    slots = prefix_splits * (2 if tile == 128 else 1) + tail_splits
+    tail_splits = _pick_splits(b * hk, tail, 4 if d <= 128 else 2, 4, 8)
+    slots = prefix_splits * (2 if tile == 128 else 1)
     with current_device(dev):
         scratch = torch.empty(n * hq * slots * (d + 2), dtype=torch.float32, device=dev)  # of this call: a workspace would tie streams and graphs together
         split = n * hq * slots * d
         check(lib().mfq_paged_attn_decode_shared(
             ptr(q), ptr(kv.k), ptr(kv.v), ptr(kv.k_scale), ptr(kv.v_scale), ptr(block_table), ptr(seq_lens), ptr(group_starts), ptr(prefix_lens), ptr(members),
             ptr(out), ptr(scratch), scratch.data_ptr() + 4 * split, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
-            float(sm_scale), ptr(Workspace.get(dev).status), stream_ptr()), "paged_attn_decode_shared", 3)
+            float(sm_scale), ptr(Workspace.get(dev).status), stream_ptr()), "paged_attn_decode_shared", 2)
     return out
