@@ -651,15 +651,13 @@ shared_tail_kernel(const SharedAttnArgs a) {
     };
     for (int e = 0; e < ranks; ++e) add(load_peer(map_to_cta(mine + r * D + d, e)), by[e]);
     const float4* src = reinterpret_cast<const float4*>(a.part_o + hq * a.slots * D + d);
-    int e = 0;
-    for (; e + 8 <= a.slots; e += 8) {  // all requested before the first is used
+    for (int e = 0; e < a.slots; e += 8) {  // eight requested before the first is used; behind the last one the last again, for nothing
       float4 v[8];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = __ldcg(src + (e + x) * (D / 4));
+      for (int x = 0; x < 8; ++x) v[x] = __ldcg(src + min(e + x, a.slots - 1) * (D / 4));
 #pragma unroll
-      for (int x = 0; x < 8; ++x) add(v[x], by[ranks + e + x]);
+      for (int x = 0; x < 8; ++x) add(v[x], e + x < a.slots ? by[ranks + e + x] : 0.f);
     }
-    for (; e < a.slots; ++e) add(__ldcg(src + e * (D / 4)), by[ranks + e]);
     const float n = inverse[r];
     __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * n, acc.y * n), __floats2bfloat162_rn(acc.z * n, acc.w * n)};
     *reinterpret_cast<uint2*>(a.out + hq * D + d) = *reinterpret_cast<const uint2*>(h);

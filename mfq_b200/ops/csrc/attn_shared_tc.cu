@@ -101,7 +101,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 3); mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8); mbar_init(&o_full[i], 1);
     }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 16);
     for (int i = 0; i < 8; ++i) mbar_init(&x_bar[i], 2);
     *abort_flag = 0;
     *s_low = 0x7fffffff;
@@ -301,33 +301,36 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
   } else {
     // ----- softmax: warps 8 - 15 stream 0, 16 - 23 stream 1; a warp has 32 rows and 64 of a block's keys, a lane parts of four rows -----
     const int t = (warp - 8) >> 3, half = (warp - 8) >> 2 & 1, quarter = warp & 3, c = lane & 3;
-    uint8_t* tile_q = sQ + t * kTile;
-    if (half == 0) {  // this thread's row of Q to fp16: as it is where its largest value is between 2^-4 and 2^15 (exact down to 2^-21 of that), else scaled to 2^13
-      const int r = quarter * 32 + lane, hq = s_hq[t * 128 + r];
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + size_t(max(hq, 0)) * D);
-      float top = 0.f;
-      if (hq >= 0) {
-#pragma unroll 8
-        for (int n = 0; n < D / 8; ++n) {
-          const uint4 v = src[n];
-          const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
+    {  // 16 rows of Q to fp16, D / 8 lanes to a row: as they are where the largest value is between 2^-4 and 2^15 (exact down to 2^-21 of that), else scaled to 2^13
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+      const int row16 = (warp - 8) * 16 + lane / kLanes, piece = lane % kLanes;
+      uint4 v[16 / kAtOnce];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(__bfloat162float(b[e])));
-        }
+      for (int n = 0; n < 16 / kAtOnce; ++n) {
+        const int hq = s_hq[row16 + n * kAtOnce];
+        v[n] = *reinterpret_cast<const uint4*>(a.q + size_t(max(hq, 0)) * D + piece * 8);
+        if (hq < 0) v[n] = make_uint4(0, 0, 0, 0);
       }
-      const float up = top == 0.f || (top >= 0.0625f && top < 32768.f) ? 1.f : power_to(top, 13);
-      s_rowc[t * 128 + r] = 1.f / up;
-      if (up != 1.f) atomicOr(s_scaled, 1);
-#pragma unroll 4
-      for (int n = 0; n < D / 8; ++n) {  // read again, from the cache: a row does not fit beside what else the thread holds
-        const uint4 v = hq >= 0 ? src[n] : make_uint4(0, 0, 0, 0);
-        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+      for (int n = 0; n < 16 / kAtOnce; ++n) {
+        const int r = row16 + n * kAtOnce;
+        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v[n]);
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(__bfloat162float(b[e])));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float up = top == 0.f || (top >= 0.0625f && top < 32768.f) ? 1.f : power_to(top, 13);
+        if (piece == 0) {
+          s_rowc[r] = 1.f / up;
+          if (up != 1.f) atomicOr(s_scaled, 1);
+        }
         uint4 h;
         h.x = half_pair(__bfloat162float(b[0]) * up, __bfloat162float(b[1]) * up);
         h.y = half_pair(__bfloat162float(b[2]) * up, __bfloat162float(b[3]) * up);
         h.z = half_pair(__bfloat162float(b[4]) * up, __bfloat162float(b[5]) * up);
         h.w = half_pair(__bfloat162float(b[6]) * up, __bfloat162float(b[7]) * up);
-        *reinterpret_cast<uint4*>(tile_q + (n >> 3) * (kTcBlock * 128) + r * 128 + (((n & 7) ^ (r & 7)) << 4)) = h;
+        *reinterpret_cast<uint4*>(sQ + t * kTile + (piece >> 3) * (kTcBlock * 128) + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4)) = h;
       }
       fence_proxy_async_smem();
       __syncwarp();

@@ -71,11 +71,10 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
         return out
     max_group = b if max_group is None else max(1, min(b, max_group))
     whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
-    tail = width if max_tail is None else min(width, max(0, max_tail) // 16 + 1)
     rows = max_group * (hq // hk) * q_len
     tile = _pick_tile(rows, d)
-    prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 1 if tile >= 128 or d > 128 else 3, 16)
-    tail_splits = _pick_splits(b * hk, tail, 4 if d <= 128 else 2, 4, 8)
+    prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 1 if tile >= 128 or d > 128 else 3, 8 if tile >= 128 else 4)
+    tail_splits = _pick_splits(b * hk, 8, 4 if d <= 128 else 2, 1, 8)
     slots = prefix_splits * (2 if tile == 128 else 1)
     with current_device(dev):
         scratch = torch.empty(n * hq * slots * (d + 2), dtype=torch.float32, device=dev)  # of this call: a workspace would tie streams and graphs together
