@@ -10,7 +10,8 @@
 // A warp takes tensor memory as matrix fragments: four lanes share a row and a lane has two columns of each eight, so that what belongs to
 // columns is read from shared memory once for 16 rows.  It goes over S twice, 16 columns at a time, and two warps share the keys of a block: registers for a whole block spilled, and the code of
 // all roles together has to stay within the instruction cache (unrolled, a step took 9000 cycles, a third of them without an instruction).
-// Seven warps hold the codes of the next block in registers while the tensor core has the two in shared memory, and put them down as fp16 (exact).
+// Seven warps put down codes as fp16 (exact) from rings of pages that bulk copies fill: loads to registers have to pass the few KB of L1 that such a CTA leaves,
+// and took 4000 cycles a block.
 //
 // Per block of 128 x 128 the tensor core and the exponentials both need 1024 cycles of an SM, shared memory (operands, codes) some 1250.
 #include "attn_shared.cuh"
@@ -22,16 +23,24 @@ constexpr int kTcThreads = 24 * 32;  // warps 0 - 3 bring K, 4 - 6 V, 7 issues p
 constexpr float kTcRoom = 4.f, kTcGrowth = 15.f;  // P begins at most at 2^4, where fp16 reaches 2^-28 of it, and may grow to 2^15
 constexpr float kTcFloor = -5e29f, kTcMasked = -1e30f;  // below every score; what masked keys have (2^(kTcMasked - kTcFloor) = 0)
 
+template <bool kYes>
+struct Special {
+  static constexpr bool value = kYes;
+};
+
 template <int D>
 struct SharedTc {
   static constexpr int kTile = kTcBlock * D * 2;  // Q or K: D / 64 slices of [128 rows][128 bytes]; V: two slices of [D dims][64 keys]
-  static constexpr int kConst = 6 * kTile;        // behind two Q and two stages of K and V
-  static constexpr int kRowAt = kConst + 2 * (64 * 16 + 64 * 8);
+  static constexpr int kVPage = 16 * D, kKPage = kVPage + 128;  // a page's V, its K and both multipliers, as they lie in the pool
+  static constexpr int kKDepth = 3, kVDepth = 4;  // pages that a loading warp has under way
+  static constexpr int kKRing = 5 * kTile;        // behind two Q, K and two stages of V: a ring for each of four warps, then of three
+  static constexpr int kVRing = kKRing + 4 * kKDepth * kKPage;
+  static constexpr int kConst = kVRing + 3 * kVDepth * kVPage, kConsts = 4;  // what belongs to columns: of four blocks
+  static constexpr int kRowAt = kConst + kConsts * (64 * 16 + 64 * 8);
   static constexpr int kBarsAt = kRowAt + 7 * 256 * 4;
-  static constexpr int kSmem = kBarsAt + 256 + 1024;
-  static constexpr int kPieces = D / 16;           // 16-byte pieces of a block's K per loading thread, 128 / D pages apart
-  static constexpr int kChunks = (D / 4 + 2) / 3;  // ... of its V, by chunks of 32 dims of a page
-  static_assert(kSmem <= 227 * 1024 && (kTile & 1023) == 0);
+  static constexpr int kBars = 28 + 4 * kKDepth + 3 * kVDepth;
+  static constexpr int kSmem = kBarsAt + kBars * 8 + 64 + 1024;
+  static_assert(kSmem <= 227 * 1024 && kTile % 1024 == 0 && kConst % 16 == 0);
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -56,15 +65,6 @@ __device__ __forceinline__ void umma_p_v(uint32_t d, uint32_t a_tmem, uint64_t b
 }
 __device__ __forceinline__ float u2f(uint32_t v) { return __uint_as_float(v); }
 
-// Loads under a predicate: as a branch, each load was waited for before the next (a block's took 4000 cycles instead of 500)
-__device__ __forceinline__ void load_if(bool there, const void* from, uint4& to) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-               : "+r"(to.x), "+r"(to.y), "+r"(to.z), "+r"(to.w)
-               : "l"(from), "r"(int(there)));
-}
-__device__ __forceinline__ void load_if(bool there, const float* from, float& to) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.cg.f32 %0, [%1];\n\t}" : "+f"(to) : "l"(from), "r"(int(there)));
-}
 // 16 codes as fp16 in the order given: 32 bytes at two 16-byte places
 __device__ __forceinline__ void put_halves(uint8_t* lo, uint8_t* hi, const uint32_t (&h)[8]) {
   *reinterpret_cast<uint4*>(lo) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -78,18 +78,20 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
   constexpr int kTile = L::kTile, kSlices = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = base, *sK = base + 2 * kTile, *sV = base + 4 * kTile;
-  float4* s_col = reinterpret_cast<float4*>(base + L::kConst);          // [2 stages][64 column pairs]: ks, ks, lv, lv
-  float2* s_inv = reinterpret_cast<float2*>(base + L::kConst + 2048);   // [2][64]: 1 / V multiplier
+  uint8_t *sQ = base, *sK = base + 2 * kTile, *sV = base + 3 * kTile;
+  float4* s_col = reinterpret_cast<float4*>(base + L::kConst);          // [block % 4][64 column pairs]: ks, ks, lv, lv
+  float2* s_inv = reinterpret_cast<float2*>(s_col + L::kConsts * 64);   // [block % 4][64]: 1 / V multiplier
   float* s_rowc = reinterpret_cast<float*>(base + L::kRowAt);           // [256] power of two that the row's q was divided by
   int* s_len = reinterpret_cast<int*>(s_rowc + 256);                    // [256] keys that the row sees
   int* s_hq = s_len + 256;                                              // [256] row of the outputs, -1: none
   float* s_max = reinterpret_cast<float*>(s_hq + 256);                  // [2][2 halves][256] maxima of even and odd blocks, at last the sums
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::kBarsAt);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;  // [2 stages]; with V comes what belongs to the columns
-  uint64_t *s_full = bars + 8, *p_full = bars + 10, *o_full = bars + 12;                  // [2 streams]
-  uint64_t *q_full = bars + 14, *x_bar = bars + 15;  // x_bar: [2 streams][4 quarters] two warps have put down their maxima
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 4, *q_full = bars + 6;  // v: [2 stages]
+  uint64_t *c_full = bars + 8;                                             // [block % 4] what belongs to the columns
+  uint64_t *s_full = bars + 12, *p_full = bars + 14, *o_full = bars + 16;  // [2 streams]
+  uint64_t* x_bar = bars + 18;                                             // [2 streams][4 quarters] two warps have put down their maxima
+  uint64_t* ring_full = bars + 28;                                         // [4][kKDepth], [3][kVDepth]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_low = reinterpret_cast<int*>(tmem_slot + 2);  // fewest and most keys that a row of the CTA sees
   int* s_most = s_low + 1;
@@ -97,12 +99,13 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
 
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    mbar_init(k_full, 4); mbar_init(k_empty, 1); mbar_init(q_full, 16);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 3); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8); mbar_init(&o_full[i], 1);
+      mbar_init(&v_full[i], 3); mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8); mbar_init(&o_full[i], 1);
     }
-    mbar_init(q_full, 16);
+    for (int i = 0; i < L::kConsts; ++i) mbar_init(&c_full[i], 4);
     for (int i = 0; i < 8; ++i) mbar_init(&x_bar[i], 2);
+    for (int i = 0; i < 4 * L::kKDepth + 3 * L::kVDepth; ++i) mbar_init(&ring_full[i], 1);
     *abort_flag = 0;
     *s_low = 0x7fffffff;
     *s_most = 0;
@@ -127,52 +130,37 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
     page_lo = min(split * per, n);
     page_hi = min(n, page_lo + per);
   }
-  // ----- what the loaders hold.  K: thread i has piece i % D of pages i / D, i / D + 128 / D, ... of a block.  V: warp w of three has the chunks w, w + 3, ...,
-  // D / 32 of them a page, and the multipliers of keys 32 w + lane, its first one's also those of keys 96 + lane -----
-  const int i = threadIdx.x & 127, in = i % D, w = warp - 4;
-  uint4 raw[L::kChunks];  // of which K has kPieces
-  float ks[2], vs[2];
-  int ids = -1;  // lanes 0 - 7: pages of the next block
-  bool bad = false;
+  // ----- the loaders: four warps take K of every fourth page, three V of every third, through rings of their own -----
+  const bool of_k = warp < 4;
+  const int lanes = of_k ? 4 : 3, w = of_k ? warp : warp - 4, depth = of_k ? L::kKDepth : L::kVDepth, page_bytes = of_k ? L::kKPage : L::kVPage;
+  uint8_t* ring = base + (of_k ? L::kKRing + w * L::kKDepth * L::kKPage : L::kVRing + w * L::kVDepth * L::kVPage);
+  uint64_t* ring_bar = ring_full + (of_k ? w * L::kKDepth : 4 * L::kKDepth + w * L::kVDepth);
+  const int own_pages = max(0, (page_hi - page_lo - w + lanes - 1) / lanes);
   const int* bt = a.table + size_t(max(table_row, 0)) * a.max_pages;
-  const auto look_up = [&](int step) {
-    const int at = page_lo + step * 8 + lane;
-    ids = lane < 8 && at < page_hi ? bt[at] : 0;
-  };
-  const auto fetch = [&](int step) {  // whole warp; zeros behind the last page
-    const int have = page_hi - page_lo - step * 8;
-    bad |= lane < have && (ids < 0 || ids >= a.pages);
-    const int page = lane >= have ? -1 : ids < 0 || ids >= a.pages ? 0 : ids;
-    const size_t stride = size_t(a.Hk) * (16 * D);
-    const uint8_t* src = (warp < 4 ? a.k + in * 16 : a.v + lane * 16) + size_t(kvh) * (16 * D);
-    if (warp < 4) {
-#pragma unroll
-      for (int n = 0; n < L::kPieces; ++n) {
-        const int p = __shfl_sync(0xffffffffu, page, n * (128 / D) + i / D);
-        raw[n] = make_uint4(0, 0, 0, 0);
-        load_if(p >= 0, src + p * stride, raw[n]);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < L::kChunks; ++n) {
-        const int chunk = w + 3 * n, of = __shfl_sync(0xffffffffu, page, chunk / (D / 32) & 7), p = chunk < D / 4 ? of : -1;
-        raw[n] = make_uint4(0, 0, 0, 0);
-        load_if(p >= 0, src + p * stride + chunk % (D / 32) * 512, raw[n]);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = (e ? 96 : w * 32) + lane, p = __shfl_sync(0xffffffffu, page, key >> 4);
-        const size_t at = (size_t(max(p, 0)) * a.Hk + kvh) * 16 + (key & 15);
-        ks[e] = vs[e] = 0.f;
-        load_if(p >= 0, a.k_scale + at, ks[e]);
-        load_if(p >= 0, a.v_scale + at, vs[e]);
-      }
+  int next_id = 0, asked = 0;  // one lane: the page that is requested next, and how many were
+  const auto request = [&](int slot) {  // one lane: copies of the warp's next page; its id was fetched a page ahead
+    int id = next_id;
+    if (++asked < own_pages) next_id = bt[page_lo + w + lanes * asked];
+    if (id < 0 || id >= a.pages) {
+      atomicCAS(a.status, 0, kStatusBadArgument);
+      id = 0;
     }
-    look_up(step + 1);
+    const size_t ph = size_t(id) * a.Hk + kvh;
+    uint8_t* to = ring + slot * page_bytes;
+    uint64_t* bar = &ring_bar[slot];
+    mbar_expect_tx(bar, page_bytes);
+    shared_bulk_load(to, (of_k ? a.k : a.v) + ph * (16 * D), 16 * D, bar);
+    if (of_k) {
+      shared_bulk_load(to + 16 * D, a.k_scale + ph * 16, 64, bar);
+      shared_bulk_load(to + 16 * D + 64, a.v_scale + ph * 16, 64, bar);
+    }
   };
   if (warp < 7) {
-    look_up(0);
-    fetch(0);  // ahead of what the rows see
+    if (lane == 0 && own_pages > 0) {  // ahead of what the rows see
+      next_id = bt[page_lo + w];
+      for (int n = 0; n < min(own_pages, depth); ++n) request(n);
+    }
+    asked = __shfl_sync(0xffffffffu, asked, 0);
   } else if (warp >= 8 && !((warp - 8) & 4)) {
     const int x = ((warp - 8) >> 3) * 128 + (warp & 3) * 32 + lane, r = tile * (kTwoTiles ? 256 : 128) + (kTwoTiles ? x : x & 127);
     int hq = -1, len = 0x7fffffff;
@@ -197,69 +185,129 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
   const int steps = key_hi > key_lo ? (key_hi - key_lo + kTcBlock - 1) / kTcBlock : 0;
   const int turns = kTwoTiles ? 2 * steps : steps;  // turn u: stream u & 1
 
+  int slot = 0, taken = 0;  // the warp's next page: its place in the ring, its number
+  uint32_t round = 0;
+  const auto ring_wait = [&] { return mbar_wait_warp(&ring_bar[slot], round, abort_flag, a.status, kStatusTimeoutProducer); };
+  const auto ring_next = [&] {  // (counted along: a division by the depth, which the roles do not share, took longer than the page)
+    ++taken;
+    if (++slot == depth) { slot = 0; round ^= 1; }
+  };
+  const auto drain = [&] {  // pages that were requested and that no row sees: their copies end before the CTA does
+    while (taken < asked) {
+      ring_wait();
+      ring_next();
+    }
+  };
   if (warp < 4) {
-    const int tok = in >> 2 & 15, c = in & 3, page0 = i / D;
-    const uint32_t lo = ((2 * c) ^ (tok & 7)) << 4, hi = ((2 * c + 1) ^ (tok & 7)) << 4;
+    const int tok = lane >> 2, c = lane & 3;  // of the first 8 tokens; the others are 8 on
+    const uint32_t lo = ((2 * c) ^ tok) << 4, hi = ((2 * c + 1) ^ tok) << 4;
+    bool ok = true;
     for (int step = 0; step < steps; ++step) {
-      const int s = step & 1, left = key_hi - key_lo - step * kTcBlock - page0 * 16 - tok;  // of the block's keys, from this thread's first on
-      if (!mbar_wait_warp(&k_empty[s], ((step >> 1) & 1) ^ 1, abort_flag, a.status, kStatusTimeoutProducer)) break;
-      uint8_t* at = sK + s * kTile + (in >> 6) * (kTcBlock * 128) + (page0 * 16 + tok) * 128;
+      // what the next Q K^T waits for comes first: the codes of the block's two pages; then their multipliers, then the requests that follow them
+      const int left = key_hi - key_lo - step * kTcBlock;  // keys of the block
+      const int held = (left > w * 16) + (left > w * 16 + 64);
+      const uint8_t* raw[2];
+      int slots[2];
 #pragma unroll
-      for (int n = 0; n < L::kPieces; ++n) {
-        const bool there = n * (128 / D) * 16 < left;
-        const uint32_t x[4] = {there ? raw[n].x : 0u, there ? raw[n].y : 0u, there ? raw[n].z : 0u, there ? raw[n].w : 0u};
-        const uint32_t h[8] = {e4m3_pair(x[0]), e4m3_pair(x[0] >> 16), e4m3_pair(x[1]), e4m3_pair(x[1] >> 16),
-                               e4m3_pair(x[2]), e4m3_pair(x[2] >> 16), e4m3_pair(x[3]), e4m3_pair(x[3] >> 16)};
-        put_halves(at + n * (128 / D) * 2048 + lo, at + n * (128 / D) * 2048 + hi, h);
+      for (int y = 0; y < 2; ++y) {
+        raw[y] = ring + slot * L::kKPage;
+        slots[y] = slot;
+        if (y < held) {
+          ok = ok && ring_wait();
+          ring_next();
+        }
+      }
+      ok = ok && mbar_wait_warp(k_empty, (step & 1) ^ 1, abort_flag, a.status, kStatusTimeoutProducer);
+      if (!ok) break;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        uint4 v[D / 32];
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) v[x] = *reinterpret_cast<const uint4*>(raw[y] + lane * 16 + x * 512);
+        uint8_t* at = sK + ((w + 4 * y) * 16 + tok) * 128;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          if ((w + 4 * y) * 16 + tok + 8 * (x & 1) >= left) v[x] = make_uint4(0, 0, 0, 0);
+          const uint32_t h[8] = {e4m3_pair(v[x].x), e4m3_pair(v[x].x >> 16), e4m3_pair(v[x].y), e4m3_pair(v[x].y >> 16),
+                                 e4m3_pair(v[x].z), e4m3_pair(v[x].z >> 16), e4m3_pair(v[x].w), e4m3_pair(v[x].w >> 16)};
+          uint8_t* to = at + (x >> 1) * (kTcBlock * 128) + (x & 1) * 1024;
+          put_halves(to + lo, to + hi, h);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[s]);
-      if (step + 1 < steps) fetch(step + 1);
-    }
-  } else if (warp < 7) {
-    for (int step = 0; step < steps; ++step) {
-      const int s = step & 1, left = key_hi - key_lo - step * kTcBlock;  // keys of the block
-      if (!mbar_wait_warp(&v_empty[s], ((step >> 1) & 1) ^ 1, abort_flag, a.status, kStatusTimeoutProducer)) break;
-      uint8_t* at = sV + s * kTile + lane * 128;
-#pragma unroll
-      for (int n = 0; n < L::kChunks; ++n) {
-        const int chunk = w + 3 * n, page = chunk / (D / 32), c = 2 * (page & 3);
-        const uint32_t h[8] = {e4m3_pair(raw[n].x), e4m3_pair(raw[n].y), e4m3_pair(raw[n].z), e4m3_pair(raw[n].w),
-                               e4m3_pair(raw[n].x >> 16), e4m3_pair(raw[n].y >> 16), e4m3_pair(raw[n].z >> 16), e4m3_pair(raw[n].w >> 16)};
-        uint8_t* row = at + (page >> 2) * (D * 128) + chunk % (D / 32) * (32 * 128);
-        if (chunk < D / 4) put_halves(row + ((c ^ (lane & 7)) << 4), row + (((c + 1) ^ (lane & 7)) << 4), h);
-      }
-      if (left < kTcBlock && left % 16) {  // no row sees all of the last page: zeros behind what they see, by the lane that wrote them
-        const int page = left >> 4;
-#pragma unroll 1
-        for (int chunk = page * (D / 32); chunk < (page + 1) * (D / 32); ++chunk) {
-          if (chunk % 3 != w) continue;
-#pragma unroll 1
-          for (int key = left & 15; key < 16; ++key) {
-            uint8_t* row = at + (page >> 2) * (D * 128) + chunk % (D / 32) * (32 * 128);
-            *reinterpret_cast<uint16_t*>(row + (((2 * (page & 3) + (key >> 3)) ^ (lane & 7)) << 4) + (key & 7) * 2) = 0;
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {  // column `key`: pair (key / 8, key % 8 / 2); a key that is not there has P = 0
-        const int key = (e ? 96 : w * 32) + lane, pair = s * 64 + (key >> 3) * 4 + ((key & 7) >> 1);
-        const bool there = key < left;
+      if (lane == 0) mbar_arrive(k_full);
+      {  // a lane to a column; the softmax of four blocks before is over: products behind its P V are
+        const int y = lane >> 4, key = (w + 4 * y) * 16 + (lane & 15), pair = (step & 3) * 64 + (key >> 3) * 4 + ((key & 7) >> 1);
+        const float* scales = reinterpret_cast<const float*>((y ? raw[1] : raw[0]) + 16 * D) + (lane & 15);
+        const bool there = key < left;  // a key that is not there has P = 0
+        const float vs = scales[16];
         // V multipliers under 2^-100 count as that: one of zero gives values of zero, and a finite quotient
-        const float lv = !there ? kTcMasked : isnan(vs[e]) ? vs[e] : __log2f(fmaxf(vs[e], 7.888609e-31f));
-        if (!e || w == 0) {
-          float* col = reinterpret_cast<float*>(s_col + pair) + (key & 1);
-          col[0] = there ? ks[e] * a.scale_log2 : 0.f;
-          col[2] = lv;
-          reinterpret_cast<float*>(s_inv + pair)[key & 1] = there ? exp2_fast(-lv) : 0.f;
+        const float lv = !there ? kTcMasked : isnan(vs) ? vs : __log2f(fmaxf(vs, 7.888609e-31f));
+        float* col = reinterpret_cast<float*>(s_col + pair) + (key & 1);
+        col[0] = there ? scales[0] * a.scale_log2 : 0.f;
+        col[2] = lv;
+        reinterpret_cast<float*>(s_inv + pair)[key & 1] = there ? exp2_fast(-lv) : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&c_full[step & 3]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (y < held && asked < own_pages) request(slots[y]);
+      }
+      asked = __shfl_sync(0xffffffffu, asked, 0);
+    }
+    drain();
+  } else if (warp < 7) {
+    int first_page = w;  // of the block's pages, the first of this warp
+    bool ok = true;
+    for (int step = 0; step < steps; ++step) {
+      const int s = step & 1, left = key_hi - key_lo - step * kTcBlock, slot0 = slot;  // keys of the block
+      ok = mbar_wait_warp(&v_empty[s], ((step >> 1) & 1) ^ 1, abort_flag, a.status, kStatusTimeoutProducer);
+#pragma unroll 1
+      for (int page = first_page; ok && page < 8; page += 3) {
+        const int c = 2 * (page & 3), keys = left - page * 16;  // from the page on
+        uint8_t* at = sV + s * kTile + (page >> 2) * (D * 128) + lane * 128;
+        const uint32_t lo = (c ^ (lane & 7)) << 4, hi = ((c + 1) ^ (lane & 7)) << 4;
+        const uint8_t* raw = ring + slot * L::kVPage + lane * 16;
+        if (keys > 0) {
+          ok = ring_wait();
+          ring_next();
+        }
+        uint4 v[D / 32];
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) v[x] = *reinterpret_cast<const uint4*>(raw + x * 512);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          if (keys <= 0) v[x] = make_uint4(0, 0, 0, 0);
+          const uint32_t h[8] = {e4m3_pair(v[x].x), e4m3_pair(v[x].y), e4m3_pair(v[x].z), e4m3_pair(v[x].w),
+                                 e4m3_pair(v[x].x >> 16), e4m3_pair(v[x].y >> 16), e4m3_pair(v[x].z >> 16), e4m3_pair(v[x].w >> 16)};
+          put_halves(at + x * 4096 + lo, at + x * 4096 + hi, h);
+        }
+        if (keys > 0 && keys < 16) {  // no row sees all of this page: zeros behind what they see
+#pragma unroll 1
+          for (int key = keys; key < 16; ++key)
+#pragma unroll 1
+            for (int x = 0; x < D / 32; ++x) *reinterpret_cast<uint16_t*>(at + x * 4096 + (key < 8 ? lo : hi) + (key & 7) * 2) = 0;
         }
       }
+      if (!ok) break;
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[s]);
-      if (step + 1 < steps) fetch(step + 1);
+      if (lane == 0) {
+        mbar_arrive(&v_full[s]);
+        int at = slot0;
+#pragma unroll 1
+        for (int page = first_page; page < 8 && page * 16 < left && asked < own_pages; page += 3) {
+          request(at);
+          at = at + 1 == L::kVDepth ? 0 : at + 1;
+        }
+      }
+      asked = __shfl_sync(0xffffffffu, asked, 0);
+      first_page = (first_page + 1) % 3;  // eight pages on: page p is warp p % 3's
     }
+    drain();
   } else if (warp == 7) {
     if (steps > 0) {
       constexpr uint32_t idesc_qk = umma_idesc(128, 128, 0, 0), idesc_pv = umma_idesc(128, D, 0, 0);
@@ -286,15 +334,14 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
           if (u + 2 >= turns) tc_commit_warp(&o_full[t]);
         }
         if (u + 2 < turns) {  // S takes the place of P, which the products before have read
-          const int step = step_of(u + 2), s = step & 1;
-          ok = mbar_wait_warp(&k_full[s], (step >> 1) & 1, abort_flag, a.status, kStatusTimeoutMma);
+          ok = mbar_wait_warp(k_full, step_of(u + 2) & 1, abort_flag, a.status, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t qd = q_desc + uint64_t(t) * kT, kd = k_desc + uint64_t(s) * kT;
+          const uint64_t qd = q_desc + uint64_t(t) * kT;
 #pragma unroll
-          for (int h = 0; h < kSlices; ++h) umma_f16_block(p, qd + h * kQkSlice, kd + h * kQkSlice, idesc_qk, h ? 1u : 0u);
+          for (int h = 0; h < kSlices; ++h) umma_f16_block(p, qd + h * kQkSlice, k_desc + h * kQkSlice, idesc_qk, h ? 1u : 0u);
           tc_commit_warp(&s_full[t]);
-          if (!kTwoTiles || t == 1) tc_commit_warp(&k_empty[s]);
+          if (!kTwoTiles || t == 1) tc_commit_warp(k_empty);
         }
       }
     }
@@ -349,19 +396,17 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
     const int blocks = kTwoTiles ? steps : (steps + 1 - t) >> 1;
 #pragma unroll 1
     for (int j = 0; j < blocks; ++j) {
-      const int step = kTwoTiles ? j : 2 * j + t, st = step & 1;
-      ok = ok && mbar_wait_warp(&v_full[st], (step >> 1) & 1, abort_flag, a.status, kStatusTimeoutEpilogue) &&
+      const int step = kTwoTiles ? j : 2 * j + t, st = step & 3;
+      ok = ok && mbar_wait_warp(&c_full[st], (step >> 2) & 1, abort_flag, a.status, kStatusTimeoutEpilogue) &&
            mbar_wait_warp(&s_full[t], j & 1, abort_flag, a.status, kStatusTimeoutEpilogue);
       if (!ok) break;
       tc_fence_after();
       const float4* col = s_col + st * 64 + half * 32 + c;
       const float2* inv = s_inv + st * 64 + half * 32 + c;
-      // t of 16 columns: row r = 2h + e, columns 8u + 2c and one more at x[h][4u + 2e]
-      const auto scores = [&](int part, uint32_t (&x)[2][8]) {
-        tmem_ld_frag16(tS + 16 * part, x[0]);
-        tmem_ld_frag16(tS + kDown + 16 * part, x[1]);
-        tmem_wait_ld();
-        if (special) {
+      // t of 16 columns: row r = 2h + e, columns 8u + 2c and one more at x[h][4u + 2e].  kSpecial: rows of their own scale or length
+      const auto scores = [&](auto special_rows, int part, uint32_t (&x)[2][8]) {
+        constexpr bool kSpecial = decltype(special_rows)::value;
+        if (kSpecial) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float by = s_rowc[row0 + 8 * r];
@@ -385,7 +430,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
             }
           }
         }
-        if (special) {
+        if (kSpecial) {
           const int key = key_lo + step * kTcBlock + half * 64 + part * 16 + 2 * c;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -399,17 +444,59 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
         }
       };
       float mx[4] = {kTcMasked, kTcMasked, kTcMasked, kTcMasked};
-#pragma unroll 1
-      for (int part = 0; part < 4; ++part) {
-        uint32_t x[2][8];
-        scores(part, x);
+      const auto maxima = [&](auto special_rows, int part, uint32_t (&x)[2][8]) {
+        scores(special_rows, part, x);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
             mx[r] = fmaxf(fmaxf(mx[r], u2f(x[r >> 1][4 * u + 2 * (r & 1)])), u2f(x[r >> 1][4 * u + 2 * (r & 1) + 1]));
         }
-      }
+      };
+      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const auto exponentials = [&](auto special_rows, int part, uint32_t (&x)[2][8]) {
+        uint32_t p[2][4];
+        scores(special_rows, part, x);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float2 iv = inv[(part * 2 + u) * 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t* y = x[r >> 1] + 4 * u + 2 * (r & 1);
+            const float2 e = make_float2(exp2_fast(u2f(y[0]) - m[r]), exp2_fast(u2f(y[1]) - m[r]));
+            sum[r] = fma_f2(e, iv, sum[r]);
+            p[r >> 1][2 * u + (r & 1)] = half_pair(e.x, e.y);
+          }
+        }
+        tmem_st_pairs(tS + 8 * part, p[0]);  // over columns that have been read
+        tmem_st_pairs(tS + kDown + 8 * part, p[1]);
+      };
+      const auto parts = [&](auto&& each) {  // the next 16 columns are requested ahead of the present ones' arithmetic
+        uint32_t x[2][2][8];
+        tmem_ld_frag16(tS, x[0][0]);
+        tmem_ld_frag16(tS + kDown, x[0][1]);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          tmem_wait_ld();
+          if (part < 3) {
+            tmem_ld_frag16(tS + 16 * part + 16, x[(part + 1) & 1][0]);
+            tmem_ld_frag16(tS + kDown + 16 * part + 16, x[(part + 1) & 1][1]);
+          }
+          each(part, x[part & 1]);
+        }
+      };
+      const auto one_by_one = [&](auto&& each) {
+#pragma unroll 1
+        for (int part = 0; part < 4; ++part) {
+          uint32_t x[2][8];
+          tmem_ld_frag16(tS + 16 * part, x[0]);
+          tmem_ld_frag16(tS + kDown + 16 * part, x[1]);
+          tmem_wait_ld();
+          each(part, x);
+        }
+      };
+      if (special) one_by_one([&](int part, uint32_t (&x)[2][8]) { maxima(Special<true>(), part, x); });
+      else parts([&](int part, uint32_t (&x)[2][8]) { maxima(Special<false>(), part, x); });
       float* theirs = s_max + (j & 1) * 512;  // the other half's of two blocks before have been read: it was at the exchange since
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -450,25 +537,8 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
           }
         }
       }
-      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-      for (int part = 0; part < 4; ++part) {
-        uint32_t x[2][8], p[2][4];
-        scores(part, x);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float2 iv = inv[(part * 2 + u) * 4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t* y = x[r >> 1] + 4 * u + 2 * (r & 1);
-            const float2 e = make_float2(exp2_fast(u2f(y[0]) - m[r]), exp2_fast(u2f(y[1]) - m[r]));
-            sum[r] = fma_f2(e, iv, sum[r]);
-            p[r >> 1][2 * u + (r & 1)] = half_pair(e.x, e.y);
-          }
-        }
-        tmem_st_pairs(tS + 8 * part, p[0]);  // over columns that have been read
-        tmem_st_pairs(tS + kDown + 8 * part, p[1]);
-      }
+      if (special) one_by_one([&](int part, uint32_t (&x)[2][8]) { exponentials(Special<true>(), part, x); });
+      else parts([&](int part, uint32_t (&x)[2][8]) { exponentials(Special<false>(), part, x); });
 #pragma unroll
       for (int r = 0; r < 4; ++r) l[r] += sum[r].x + sum[r].y;
       tmem_wait_st();
@@ -516,7 +586,6 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       }
     }
   }
-  if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
