@@ -10,8 +10,8 @@ from dataclasses import dataclass
 import torch
 
 from . import reference
-from .lib import check, current_device, lib, ptr, stream_ptr
-from .logits import _index
+from .lib import check, elsewhere, lib, ptr, stream_ptr
+from .logits import _index, _refuse
 
 MAX_REQUESTS = 1024  # of a batch; kPlanRequests of the kernel
 MAX_TABLE_ROWS = 1 << 16  # of a table whose pages are handed out; kPlanRows
@@ -50,34 +50,33 @@ def plan_batch(block_table: torch.Tensor, rows: torch.Tensor, past: torch.Tensor
 
     Lengths that do not fit are found on the device: the plan then is that of a batch without tokens, nothing is written into
     ``block_table``, and :meth:`BatchPlan.check` says why."""
-    dev = block_table.device
-    if block_table.dtype != torch.int32 or block_table.ndim != 2 or not block_table.is_contiguous() or block_table.numel() == 0:
-        raise ValueError(f"block_table: contiguous int32 [R, P] is wanted, got {block_table.dtype} {tuple(block_table.shape)}")
-    b, (r, p) = rows.numel(), block_table.shape
-    for name, t in (("rows", rows), ("past", past), ("counts", counts)):
-        _index(name, t, b, dev)
+    if block_table.dtype is not torch.int32 or block_table.ndim != 2 or not block_table.is_contiguous() or not block_table.numel():
+        _refuse("block_table", "contiguous int32 [R, P] is", block_table)
+    b, (r, p), index = rows.numel(), block_table.shape, block_table.get_device()
+    _index("rows", rows, None, index)
+    _index("past", past, b, index)
+    _index("counts", counts, b, index)
     if not 1 <= b <= MAX_REQUESTS:
         raise ValueError(f"a plan takes 1 to {MAX_REQUESTS} requests, got {b}")
     if tokens < 0 or page_size < 1 or p * page_size > 2 ** 31 - 1:
         raise ValueError(f"{tokens} tokens, rows of {p} pages of {page_size}")
     if pages is not None:
-        _index("pages", pages, None, dev)
+        _index("pages", pages, None, index)
         if r > MAX_TABLE_ROWS:
             raise ValueError(f"pages are handed out to tables of at most {MAX_TABLE_ROWS} rows, got {r}")
-    flat = torch.empty(3 * tokens + 2 * b + 3 + b * p, dtype=torch.int32, device=dev)  # one allocation; a part's beginning needs no alignment
-    at = 0
-
-    def part(n: int) -> torch.Tensor:
-        nonlocal at
-        at += n
-        return flat[at - n : at]
-
-    plan = BatchPlan(part(tokens), part(tokens), part(tokens), part(b + 1), part(b), part(b * p).view(b, p), part(2))
-    if not block_table.is_cuda:
+    if index >= 0 and elsewhere(index):
+        with torch.cuda.device(index):
+            return plan_batch(block_table, rows, past, counts, tokens=tokens, page_size=page_size, pages=pages)
+    sizes = [tokens, tokens, tokens, b + 1, b, b * p, 2]
+    whole = block_table.new_empty(sum(sizes))  # one allocation; a part's beginning needs no alignment
+    parts = list(torch.split_with_sizes(whole, sizes))
+    parts[5] = parts[5].view(b, p)
+    plan = BatchPlan(*parts)
+    if index < 0:
         reference.plan_batch(plan, block_table, rows, past, counts, tokens, page_size, pages)
         return plan
-    with current_device(dev):
-        check(lib().mfq_plan_batch(ptr(block_table), r, p, ptr(rows), ptr(past), ptr(counts), b, ptr(pages), pages.numel() if pages is not None else -1,
-                                   ptr(plan.positions), ptr(plan.slots), ptr(plan.tok_seq), tokens, ptr(plan.q_starts), ptr(plan.seq_lens),
-                                   ptr(plan.block_table), ptr(plan.info), page_size, stream_ptr()), "plan_batch")
+    at = whole.data_ptr()  # (an empty part has no address)
+    check(lib().mfq_plan_batch(block_table.data_ptr(), r, p, rows.data_ptr(), past.data_ptr(), counts.data_ptr(), b, ptr(pages), -1 if pages is None else pages.numel(),
+                               at, at + 4 * tokens, at + 8 * tokens, tokens, at + 12 * tokens, at + 12 * tokens + 4 * (b + 1), at + 12 * tokens + 8 * b + 4,
+                               at + 12 * tokens + 8 * b + 4 + 4 * b * p, page_size, stream_ptr()), "plan_batch")
     return plan

@@ -126,7 +126,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
   const int table_row = member_row(a, first);
   int page_lo = 0, page_hi = 0;
   if (table_row >= 0) {
-    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
+    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = ((n + 7) / 8 + a.prefix_splits - 1) / a.prefix_splits * 8;  // whole blocks
     page_lo = min(split * per, n);
     page_hi = min(n, page_lo + per);
   }

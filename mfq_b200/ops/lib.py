@@ -8,7 +8,6 @@ reused by every call on that device's current stream.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from functools import lru_cache
 
@@ -140,14 +139,10 @@ def stream_ptr() -> int:
     return _raw_stream(_device_index())
 
 
-_HERE = contextlib.nullcontext()
-
-
-def current_device(device: torch.device):
-    """Context in which ``device`` is the current one (nothing to do when it is): kernels are launched on the stream that the tensors'
-    own device has as its current one."""
-    index = torch.cuda.current_device() if _device_index is None else _device_index()
-    return _HERE if index == device.index else torch.cuda.device(device)
+def elsewhere(index: int) -> bool:
+    """Whether the tensors' device ``index`` is not the current one: a call then makes it so (``torch.cuda.device``) and begins again, so that kernels
+    are launched on the stream that the tensors' own device has as its current one."""
+    return index != (torch.cuda.current_device() if _device_index is None else _device_index())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

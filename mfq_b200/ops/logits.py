@@ -13,21 +13,20 @@ from __future__ import annotations
 import torch
 
 from . import reference
-from .lib import check, current_device, lib, ptr, stream_ptr
+from .lib import check, elsewhere, lib, ptr, stream_ptr
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_BIASES = 1024  # places per row; kMaxBias of the kernel
 RECORD_WORDS = 8  # a sampling record: temperature f32, top_k i32, top_p f32, presence f32, frequency f32, repetition f32, seed u64
 
 
-def _table(name: str, t: torch.Tensor, dtype: torch.dtype, device, rows: int | None = None) -> None:
-    if t.dtype != dtype or t.ndim != 2 or t.device != device or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name}: a {dtype} table [{'rows' if rows is None else rows}, ...] on {device} is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _refuse(name: str, wanted: str, t: torch.Tensor) -> None:
+    raise ValueError(f"{name}: {wanted} wanted, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}")
 
 
-def _index(name: str, t: torch.Tensor, count: int | None, device) -> None:
-    if t.dtype != torch.int32 or t.ndim != 1 or t.device != device or not t.is_contiguous() or (count is not None and t.numel() != count):
-        raise ValueError(f"{name}: contiguous int32 [{'n' if count is None else count}] on {device} is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _index(name: str, t: torch.Tensor, count: int | None, index: int) -> None:
+    if t.dtype is not torch.int32 or t.ndim != 1 or t.get_device() != index or not t.is_contiguous() or (count is not None and t.numel() != count):
+        _refuse(name, f"contiguous int32 [{'n' if count is None else count}] on the device of the others are", t)
 
 
 def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch.Tensor | None = None,
@@ -45,50 +44,48 @@ def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch
     * ``rows [B]`` int32: the tables' row of each row of logits (default: its own number); a row outside the tables passes through;
     * ``first``: vocabulary id of column 0, for a shard of the vocabulary (biases and masks go by ids, ``counts`` by columns)."""
     if logits.ndim != 2 or logits.dtype not in _DTYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError(f"logits: bf16, fp16 or fp32 [B, V] with neighbouring columns are wanted, got {logits.dtype} {tuple(logits.shape)} strides {logits.stride()}")
+        _refuse("logits", "bf16, fp16 or fp32 [B, V] with neighbouring columns are", logits)
     b, v = logits.shape
-    dev = logits.device
-    _table("records", records, torch.int32, dev)
+    index = logits.get_device()
+    if records.dtype is not torch.int32 or records.ndim != 2 or records.shape[1] != RECORD_WORDS or records.get_device() != index or \
+            not records.is_contiguous() or not records.numel():
+        _refuse("records", f"contiguous int32 [R, {RECORD_WORDS}] on the logits' device are", records)
     r = records.shape[0]
-    if records.shape[1] != RECORD_WORDS or not records.is_contiguous() or r == 0:
-        raise ValueError(f"records: contiguous [R, {RECORD_WORDS}] are wanted, got {tuple(records.shape)}")
-    if rows is None:
-        if b > r:
-            raise ValueError(f"{b} rows of logits, but {r} records")
-    else:
-        _index("rows", rows, b, dev)
-    if first < 0:
+    if rows is not None:
+        _index("rows", rows, b, index)
+    elif b > r:
+        raise ValueError(f"{b} rows of logits, but {r} records")
+    if not 0 <= first <= 2 ** 31 - 1 - v:
         raise ValueError(f"first: {first}")
-    if counts is not None:
-        _table("counts", counts, torch.int16, dev, r)
-        if counts.shape[1] != v or (v > 1 and counts.stride(1) != 1):
-            raise ValueError(f"counts: [R, {v}] with neighbouring columns are wanted, got {tuple(counts.shape)}")
+    if counts is not None and (counts.dtype is not torch.int16 or counts.shape != (r, v) or counts.get_device() != index or (v > 1 and counts.stride(1) != 1)):
+        _refuse("counts", f"int16 [{r}, {v}] with neighbouring columns on the logits' device are", counts)
     ids = values = None
     k = 0
     if bias is not None:
         ids, values = bias
-        _table("bias ids", ids, torch.int32, dev, r)
-        _table("bias values", values, torch.float32, dev, r)
+        if ids.dtype is not torch.int32 or ids.ndim != 2 or ids.shape[0] != r or ids.get_device() != index or not ids.is_contiguous() or ids.shape[1] > MAX_BIASES:
+            _refuse("bias ids", f"contiguous int32 [{r}, at most {MAX_BIASES}] on the logits' device are", ids)
+        if values.dtype is not torch.float32 or values.shape != ids.shape or values.get_device() != index or not values.is_contiguous():
+            _refuse("bias values", f"contiguous fp32 {tuple(ids.shape)} on the logits' device are", values)
         k = ids.shape[1]
-        if values.shape != ids.shape or k > MAX_BIASES or not (ids.is_contiguous() and values.is_contiguous()):
-            raise ValueError(f"bias: contiguous ids and values of one shape [R, at most {MAX_BIASES}] are wanted, got {tuple(ids.shape)} and {tuple(values.shape)}")
-    if allowed is not None:
-        _table("allowed", allowed, torch.int32, dev, r)
-        if allowed.shape[1] * 32 < first + v or not allowed.is_contiguous():
-            raise ValueError(f"allowed: contiguous [R, at least {(first + v + 31) // 32}] are wanted, got {tuple(allowed.shape)}")
+    if allowed is not None and (allowed.dtype is not torch.int32 or allowed.ndim != 2 or allowed.shape[0] != r or allowed.shape[1] * 32 < first + v or
+                                allowed.get_device() != index or not allowed.is_contiguous()):
+        _refuse("allowed", f"contiguous int32 [{r}, at least {(first + v + 31) // 32}] on the logits' device are", allowed)
     if out is None:
-        out = torch.empty((b, v), dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v):
-        raise ValueError(f"out: {logits.dtype} {tuple(logits.shape)} on {dev} with neighbouring columns is wanted, got {out.dtype} {tuple(out.shape)} on {out.device}")
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((b, v))
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != index or (v > 1 and out.stride(1) != 1) or (b > 1 and out.stride(0) < v):
+        _refuse("out", f"{logits.dtype} {tuple(logits.shape)} with neighbouring columns on the logits' device is", out)
     if b == 0 or v == 0:
         return out
-    if not logits.is_cuda:
+    if index < 0:
         out.copy_(reference.process_logits(logits, records, counts, bias, allowed, rows, first, fill))
         return out
-    with current_device(dev):
-        check(lib().mfq_process_logits(ptr(logits), ptr(out), _DTYPES[logits.dtype], b, v, logits.stride(0), out.stride(0), ptr(records), r, ptr(counts),
-                                       counts.stride(0) if counts is not None else 0, ptr(ids), ptr(values), k, ptr(allowed),
-                                       allowed.shape[1] if allowed is not None else 0, ptr(rows), first, fill, stream_ptr()), "process_logits")
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return process_logits(logits, records, counts=counts, bias=bias, allowed=allowed, rows=rows, first=first, fill=fill, out=out)
+    check(lib().mfq_process_logits(logits.data_ptr(), out.data_ptr(), _DTYPES[logits.dtype], b, v, logits.stride(0), out.stride(0), records.data_ptr(), r, ptr(counts),
+                                   0 if counts is None else counts.stride(0), ptr(ids), ptr(values), k, ptr(allowed), 0 if allowed is None else allowed.shape[1],
+                                   ptr(rows), first, fill, stream_ptr()), "process_logits")
     return out
 
 
@@ -96,15 +93,18 @@ def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, rows: torch.Tensor,
     """Count ``tokens [n]`` int32 in ``counts[rows [n], token]`` (int16 words ``[R, V]``, see the top of this module): as tokens of an
     answer, whose counts stay at 32767 once there, or with ``prompt`` as tokens that the prompt has.  A pair outside the table is left
     out, so a batch may be padded with negative rows."""
-    if counts.dtype != torch.int16 or counts.ndim != 2 or (counts.shape[1] > 1 and counts.stride(1) != 1):
-        raise ValueError(f"counts: int16 [R, V] with neighbouring columns are wanted, got {counts.dtype} {tuple(counts.shape)}")
-    _index("tokens", tokens, None, counts.device)
-    _index("rows", rows, tokens.numel(), counts.device)
+    if counts.dtype is not torch.int16 or counts.ndim != 2 or (counts.shape[1] > 1 and counts.stride(1) != 1):
+        _refuse("counts", "int16 [R, V] with neighbouring columns are", counts)
+    index = counts.get_device()
+    _index("tokens", tokens, None, index)
+    _index("rows", rows, tokens.numel(), index)
     if counts.numel() == 0 or tokens.numel() == 0:
         return
-    if not counts.is_cuda:
+    if index < 0:
         reference.count_tokens(counts, tokens, rows, prompt)
         return
-    with current_device(counts.device):
-        check(lib().mfq_count_tokens(ptr(counts), counts.stride(0), counts.shape[0], counts.shape[1], ptr(tokens), ptr(rows), tokens.numel(), int(prompt),
-                                     stream_ptr()), "count_tokens")
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return count_tokens(counts, tokens, rows, prompt=prompt)
+    check(lib().mfq_count_tokens(counts.data_ptr(), counts.stride(0), counts.shape[0], counts.shape[1], tokens.data_ptr(), rows.data_ptr(), tokens.numel(), int(prompt),
+                                 stream_ptr()), "count_tokens")

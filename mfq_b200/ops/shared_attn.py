@@ -6,18 +6,16 @@ restatement in :mod:`mfq_b200.ops.reference`.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import reference
-from .lib import Workspace, check, current_device, lib, ptr, stream_ptr
+from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
+from .logits import _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
 SMS = 148
-
-
-def _pick_splits(units: int, pages: int, per_sm: int, least: int, most: int = 32) -> int:
-    """Splits of ``pages`` for a grid of ``units`` CTAs a split: as many as fit one wave of ``per_sm`` CTAs an SM, each of at least ``least`` pages."""
-    return max(1, min(SMS * per_sm // max(1, units), pages // least, most))
 
 
 def _pick_tile(rows: int, d: int) -> int:
@@ -26,6 +24,25 @@ def _pick_tile(rows: int, d: int) -> int:
         if rows <= tile:
             return tile
     return 64 if d > 128 else 128 if rows <= 128 else 256
+
+
+@lru_cache(maxsize=4096)
+def _shape(b: int, per_seq: int, hk: int, d: int, groups: int, width: int, max_group: int | None, max_prefix: int | None, max_tail: int | None) -> tuple[int, int, int]:
+    """(query rows of a prefix CTA, splits of a prefix, splits of a tail) for ``b`` sequences of ``per_seq`` query rows a KV head."""
+    max_group = b if max_group is None else max(1, min(b, max_group))
+    whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
+    tail = width if max_tail is None else min(width, max(0, max_tail) // 16 + 1)
+    tile = _pick_tile(max_group * per_seq, d)
+    units = -(-max_group * per_seq // tile) * hk * groups
+    if tile >= 128:  # one CTA an SM, blocks of eight pages: no more splits than give each of them whole blocks
+        blocks = max(1, -(-whole // 8))
+        most = max(1, min(SMS // units, blocks, 32))
+        prefix = -(-blocks // -(-blocks // most))
+    else:
+        prefix = max(1, min(SMS * (3 if d <= 128 else 1) // units, whole // 4, 32))
+    # a tail's splits share its pages and the reading of the prefix's partials
+    tails = max(1, min(SMS * (4 if d <= 128 else 2) // (b * hk), -(-(tail + prefix) // 8), 8))
+    return tile, prefix, tails
 
 
 def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, group_starts: torch.Tensor,
@@ -43,44 +60,48 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
 
     All of that may change on the device between replays of a graph.  ``max_group`` (rows of a group), ``max_prefix`` and ``max_tail`` (tokens):
     what the host knows of them; they choose the shape of the launches, a wrong one costs time."""
-    if q.ndim != 3 or q.dtype != torch.bfloat16 or not q.is_contiguous() or q.shape[2] not in HEAD_DIMS or q_len < 1 or q.shape[0] % q_len:
-        raise ValueError(f"q: contiguous bf16 [B * {q_len}, Hq, 64 | 128 | 256] is wanted, got {q.dtype} {tuple(q.shape)}")
+    if q.ndim != 3 or q.dtype is not torch.bfloat16 or not q.is_contiguous() or q.shape[2] not in HEAD_DIMS or q_len < 1 or q.shape[0] % q_len:
+        _refuse("q", f"contiguous bf16 [B * {q_len}, Hq, 64 | 128 | 256] are", q)
     n, hq, d = q.shape
-    b, dev = n // q_len, q.device
-    pages, hk = kv.k.shape[:2]
-    if kv.page_size != 16 or kv.k.dtype != torch.float8_e4m3fn or kv.k.shape != (pages, hk, d // 64, 16, 64) or kv.v.shape != (pages, hk, d, 16) or \
-            any(not t.is_contiguous() or t.device != dev for t in (kv.k, kv.v, kv.k_scale, kv.v_scale)):
-        raise ValueError(f"kv: contiguous FP8 pages of 16 tokens and {d}-wide heads on {dev} are wanted, got {kv.k.dtype} {tuple(kv.k.shape)} on {kv.k.device}")
+    b, index = n // q_len, q.get_device()
+    k, v = kv.k, kv.v
+    pages, hk = k.shape[:2]
+    if kv.page_size != 16 or k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn or k.shape != (pages, hk, d // 64, 16, 64) or v.shape != (pages, hk, d, 16):
+        _refuse("kv", f"FP8 pages of 16 tokens and {d}-wide heads are", k)
+    for t in (k, v, kv.k_scale, kv.v_scale):
+        if t.get_device() != index or not t.is_contiguous():
+            _refuse("kv", "contiguous pages on the device of q are", t)
     if hq % hk or hq // hk * q_len > 16:
         raise ValueError(f"{hq} query heads on {hk} KV heads in windows of {q_len}: at most 16 query rows a KV head are taken")
-    for name, t, shape in (("block_table", block_table, (b, block_table.shape[-1])), ("seq_lens", seq_lens, (b,)), ("group_starts", group_starts, (prefix_lens.numel() + 1,)),
-                           ("prefix_lens", prefix_lens, (prefix_lens.numel(),))) + ((("members", members, (b,)),) if members is not None else ()):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous int32 {shape} on {dev} is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous():
+        _refuse("block_table", f"contiguous int32 [{b}, P] on the device of q is", block_table)
     groups, width = prefix_lens.numel(), block_table.shape[1]
+    _index("seq_lens", seq_lens, b, index)
+    _index("group_starts", group_starts, groups + 1, index)
+    _index("prefix_lens", prefix_lens, groups, index)
+    if members is not None:
+        _index("members", members, b, index)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out: contiguous bf16 {tuple(q.shape)} on {dev} is wanted, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
+        _refuse("out", f"contiguous bf16 {tuple(q.shape)} on the device of q is", out)
     if b == 0 or groups == 0:
         return out
     if groups > b:
         raise ValueError(f"{groups} groups of {b} rows")
-    if not q.is_cuda:
+    if index < 0:
         reference.paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale, members, q_len, out)
         return out
-    max_group = b if max_group is None else max(1, min(b, max_group))
-    whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
-    rows = max_group * (hq // hk) * q_len
-    tile = _pick_tile(rows, d)
-    prefix_splits = _pick_splits(-(-rows // tile) * hk * groups, whole, 1 if tile >= 128 or d > 128 else 3, 8 if tile >= 128 else 4)
-    tail_splits = _pick_splits(b * hk, 8, 4 if d <= 128 else 2, 1, 8)
-    slots = prefix_splits * (2 if tile == 128 else 1)
-    with current_device(dev):
-        scratch = torch.empty(n * hq * slots * (d + 2), dtype=torch.float32, device=dev)  # of this call: a workspace would tie streams and graphs together
-        split = n * hq * slots * d
-        check(lib().mfq_paged_attn_decode_shared(
-            ptr(q), ptr(kv.k), ptr(kv.v), ptr(kv.k_scale), ptr(kv.v_scale), ptr(block_table), ptr(seq_lens), ptr(group_starts), ptr(prefix_lens), ptr(members),
-            ptr(out), ptr(scratch), scratch.data_ptr() + 4 * split, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
-            float(sm_scale), ptr(Workspace.get(dev).status), stream_ptr()), "paged_attn_decode_shared", 2)
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale=sm_scale, members=members, q_len=q_len,
+                                            max_group=max_group, max_prefix=max_prefix, max_tail=max_tail, out=out)
+    tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
+    parts = n * hq * prefix_splits * (2 if tile == 128 else 1)
+    scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)  # of this call: a workspace would tie streams and graphs together
+    at = scratch.data_ptr()
+    check(lib().mfq_paged_attn_decode_shared(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), group_starts.data_ptr(),
+        prefix_lens.data_ptr(), ptr(members), out.data_ptr(), at, at + 4 * parts * d, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
+        sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_shared", 2)
     return out
