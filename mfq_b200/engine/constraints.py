@@ -2,9 +2,9 @@
 
 ``response_format = {"type": "json_object"}`` (or ``json_schema``, which is held to "a JSON object") makes the engine
 keep a grammar state per row.  Before every step the state's allowed-token mask (computed natively over a byte trie of
-the vocabulary, ``native/src/json_constraint.cpp``) becomes an additive bias row -- 0 for allowed tokens, a large
-negative number for the others -- that is added to the row's logits ahead of the sampler, inside the captured graph of
-the constrained variant of the step; after the step the sampled token advances the state.  The end-of-sequence tokens
+the vocabulary, ``native/src/json_constraint.cpp``) becomes a row of bit words; where its bit is not set, a logit turns into a large
+negative number ahead of the sampler, inside the captured graph of the step's processed variant, beside biases and penalties
+(:class:`LogitTables`, ``ops.process_logits``); after the step the sampled token advances the state.  The end-of-sequence tokens
 are allowed exactly when the document is complete, so a constrained request stops by itself on valid JSON.
 
 Reference: engine token constraints + the tokenizer's grammar (``cpp_runtime/engine/include``: token constraints;
@@ -16,6 +16,8 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+
+from .. import ops
 
 NEG = -1.0e30  # representable in bf16; exp() of it is 0 and an arg-max never picks it
 
@@ -34,19 +36,22 @@ class JsonTokenConstraint:
             mask[list(self.stop_ids)] = True
         return mask
 
-    def bias(self, width: int) -> torch.Tensor:
-        """bf16 ``[width]``: 0 where a token may come next, a large negative number elsewhere (ids past the
-        vocabulary, e.g. padding columns of the output projection, are never allowed)."""
-        cache = self.vocabulary.__dict__.setdefault("_bias_cache", {})
+    def biases(self) -> dict:
+        return {}
+
+    def words(self, width: int) -> torch.Tensor:
+        """Bit words ``[ceil(width / 32)]`` int32: set where a token may come next (ids past the vocabulary, e.g. padding columns
+        of the output projection, are never allowed)."""
+        cache = self.vocabulary.__dict__.setdefault("_words_cache", {})
         key = (self.state.key, self.state.complete, self.stop_ids, width)
         hit = cache.get(key)
-        if hit is not None:  # e.g. every step inside a string value: same state, same 256 KB row
+        if hit is not None:  # e.g. every step inside a string value: same state, same row
             return hit
-        out = np.full(width, NEG, dtype=np.float32)
+        out = np.zeros((width + 31) // 32 * 32, dtype=np.uint8)
         mask = self.allowed()
         n = min(width, mask.size)
-        out[:n][mask[:n]] = 0.0
-        row = torch.from_numpy(out).to(torch.bfloat16)
+        out[:n] = mask[:n]
+        row = torch.from_numpy(np.packbits(out, bitorder="little").view(np.int32).copy())
         if len(cache) >= 128:
             cache.pop(next(iter(cache)))
         cache[key] = row
@@ -68,12 +73,11 @@ class LogitBias:
         self.inner = inner
         self.finished = False
 
-    def bias(self, width: int) -> torch.Tensor:
-        out = self.inner.bias(width).float() if self.inner is not None else torch.zeros(width)
-        for t, v in self.table.items():
-            if 0 <= t < width:
-                out[t] += v
-        return out.to(torch.bfloat16)
+    def biases(self) -> dict:
+        return self.table
+
+    def words(self, width: int) -> torch.Tensor | None:
+        return self.inner.words(width) if self.inner is not None else None
 
     def advance(self, token: int) -> None:
         if self.inner is not None:
@@ -89,3 +93,50 @@ def make_constraint(response_format, vocabulary, stop_ids):
     if kind in ("json_object", "json_schema", "json"):
         return JsonTokenConstraint(vocabulary, stop_ids, need_object=True)
     return None
+
+
+def penalized(params) -> bool:
+    """Whether a request penalizes tokens that it has already."""
+    return params is not None and (params.presence_penalty != 0.0 or params.frequency_penalty != 0.0 or params.repetition_penalty != 1.0)
+
+
+class LogitTables:
+    """What ``ops.process_logits`` reads beside the sampling records, a row per batch row: token counts, biases and allowed tokens."""
+
+    def __init__(self, rows: int, width: int, device: torch.device) -> None:
+        self.width = width
+        self.counts = torch.zeros((rows, width), dtype=torch.int16, device=device)
+        self.counted = torch.full((rows,), -1, dtype=torch.int32, device=device)  # the rows whose token a step counts
+        self.allowed = torch.full((rows, (width + 31) // 32), -1, dtype=torch.int32, device=device)
+        self._held: dict[int, tuple] = {}  # row -> the host's words and biases that its rows hold (None: no limit)
+        self.make_places(8)
+
+    def make_places(self, places: int) -> None:
+        """Room for ``places`` biases a row; the biases are written again by the next :meth:`limit`."""
+        most = 8
+        while most < places:
+            most *= 2
+        if most > ops.MAX_BIASES:
+            raise ValueError(f"a request may have at most {ops.MAX_BIASES} biases, got {places}")
+        rows, dev = self.counts.shape[0], self.counts.device
+        self.bias_ids = torch.full((rows, most), -1, dtype=torch.int32, device=dev)
+        self.bias_values = torch.zeros((rows, most), dtype=torch.float32, device=dev)
+        self._held = {r: (w, None) for r, (w, _) in self._held.items()}
+
+    def limit(self, row: int, constraint) -> None:
+        """Bring row ``row`` in line with a constraint (None: no limits)."""
+        words, table = (None, {}) if constraint is None else (constraint.words(self.width), constraint.biases())
+        held_words, held_table = self._held.get(row, (None, {}))
+        if words is not held_words:  # the words of a grammar state are one tensor: within a string, say, the device has them already
+            if words is None:
+                self.allowed[row].fill_(-1)
+            else:
+                self.allowed[row].copy_(words, non_blocking=True)
+        if table is not held_table and not (held_table == {} and not table):
+            self.bias_ids[row].fill_(-1)
+            if table:
+                n = len(table)
+                self.bias_ids[row, :n] = torch.tensor(list(table), dtype=torch.int32).to(self.bias_ids.device)
+                # held as the bf16 numbers that logits had added before there was a kernel for it
+                self.bias_values[row, :n] = torch.tensor(list(table.values())).to(torch.bfloat16).float().to(self.bias_values.device)
+        self._held[row] = (words, table)

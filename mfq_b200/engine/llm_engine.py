@@ -22,6 +22,7 @@ import torch
 from .. import ops
 from ..models.llama import LlamaModel, StepBuffers
 from ..utils.profiler import scope
+from .constraints import NEG, LogitTables, penalized
 from .kv_cache import PAGE_SIZE, PagedKVCache
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
@@ -123,7 +124,8 @@ class LLMEngine:
         self.row_stochastic: dict[int, bool] = {}
         self.row_prompt: dict[int, PendingPrompt] = {}  # rows whose prompt is still being read (mixed batches)
         self.row_constraint: dict[int, object] = {}  # row -> grammar state of a structured-output request
-        self.logit_bias: torch.Tensor | None = None  # [max_batch, vocabulary] bf16, allocated by the first such request
+        self.logit_tables: LogitTables | None = None  # what rows' logits are processed by, allocated by the first such request
+        self.row_penalized: set[int] = set()  # rows whose request has penalties for repeated tokens
         self._token_bytes, self._constraint_vocab, self._constraint_stop = None, None, ()
         self._next_seq_id = 0
         # models with recurrent (linear-attention) state keep it per batch row
@@ -178,30 +180,38 @@ class LLMEngine:
         stops = tuple(getattr(params, "stop_token_ids", ()) or ()) or self._constraint_stop
         return make_constraint(fmt, self._constraint_vocab, stops)
 
-    def _bias_rows(self, logits: torch.Tensor, b: int) -> torch.Tensor:
-        """The persistent ``[max_batch, vocabulary]`` bias, cut to this rank's vocabulary shard of ``logits``."""
-        v = logits.shape[1]
-        tp = self.model.tp
-        if self.logit_bias is None or self.logit_bias.shape[1] != v * tp:
-            self.logit_bias = torch.zeros((self.max_batch, v * tp), dtype=torch.bfloat16, device=self.device)
-        lo = self.model.w.tp_rank * v if tp > 1 else 0
-        return self.logit_bias[:b, lo : lo + v]
+    def _tables(self, width: int) -> LogitTables:
+        """The tables of the rows' biases, masks and token counts for a vocabulary of ``width``."""
+        t = self.logit_tables
+        if t is None or t.width != width:
+            self._drop_processed_graphs()
+            t = self.logit_tables = LogitTables(self.max_batch, width, self.device)
+        return t
 
-    def _write_bias(self, rows) -> None:
-        """Refresh the bias rows of ``rows`` from their grammar states (zero for rows without one)."""
-        if self.logit_bias is None:
-            return
-        held = self.__dict__.setdefault("_bias_held", {})  # row -> the host row its device copy came from (None: zeros)
+    def _drop_processed_graphs(self) -> None:
+        """Forget the graphs of the steps that process logits: they hold the tables' addresses."""
+        self.graphs = {k: g for k, g in self.graphs.items() if True not in k[3:]}
+
+    def _is_processed(self, row: int) -> bool:
+        return row in self.row_constraint or row in self.row_penalized
+
+    def _write_limits(self, rows, width: int) -> None:
+        """Refresh the tables' rows ``rows`` from their constraints (no limits for rows without one)."""
+        t = self._tables(width)
+        places = max((len(c.biases()) for c in self.row_constraint.values()), default=0)
+        if places > t.bias_ids.shape[1]:
+            self._drop_processed_graphs()
+            t.make_places(places)
         for r in rows:
-            c = self.row_constraint.get(r)
-            src = None if c is None else c.bias(self.logit_bias.shape[1])
-            if r in held and held[r] is src:
-                continue  # same grammar state as last step (e.g. inside a string): the device row is already right
-            if src is None:
-                self.logit_bias[r].zero_()
-            else:
-                self.logit_bias[r].copy_(src, non_blocking=True)
-            held[r] = src
+            t.limit(r, self.row_constraint.get(r))
+
+    def _process(self, logits: torch.Tensor, rows: torch.Tensor | None = None) -> torch.Tensor:
+        """Biases, penalties and masks on ``logits``, in place; row ``i`` by the tables' row ``rows[i]`` (default ``i``)."""
+        v, tp = logits.shape[1], self.model.tp
+        t = self._tables(v * tp)
+        lo = self.model.w.tp_rank * v if tp > 1 else 0
+        return ops.process_logits(logits, self.sample_rows, counts=t.counts[:, lo : lo + v], bias=(t.bias_ids, t.bias_values), allowed=t.allowed, rows=rows,
+                                  first=lo, fill=NEG, out=logits)
 
     # -- capacity (scheduler backend protocol) ------------------------------------------------------------------
     def free_tokens(self) -> int:
@@ -230,6 +240,7 @@ class LLMEngine:
         self.row_prompt.pop(row, None)
         self.row_stochastic.pop(row, None)
         self.row_constraint.pop(row, None)
+        self.row_penalized.discard(row)
 
     # -- sampling ---------------------------------------------------------------------------------------------------
     def set_sampling(self, row: int, params) -> None:
@@ -246,6 +257,9 @@ class LLMEngine:
             rec[5] = torch.tensor([1.0]).view(torch.int32)[0]
         self.sample_rows[row] = rec.to(self.device)
         self.row_stochastic[row] = stochastic
+        self.row_penalized.discard(row)
+        if penalized(params):
+            self.row_penalized.add(row)
 
     def _sample(self, logits: torch.Tensor, b: int, stochastic: bool) -> None:
         if not stochastic:
@@ -271,10 +285,9 @@ class LLMEngine:
         and draw counters (``seq_lens``); the tokens also become the rows' ``sampled``."""
         n, dev = len(rows), self.device
         idx = torch.tensor(rows, dtype=torch.long).to(dev)
-        if any(r in self.row_constraint for r in rows):
-            bias = self._bias_rows(logits, self.max_batch)
-            self._write_bias(rows)
-            logits = logits + bias.index_select(0, idx)
+        if any(self._is_processed(r) for r in rows):
+            self._write_limits(rows, logits.shape[1] * self.model.tp)
+            logits = self._process(logits, idx.to(torch.int32))
         if not any(self.row_stochastic.get(r, False) for r in rows):
             toks = self.model.sample_greedy(logits)
         else:
@@ -327,11 +340,10 @@ class LLMEngine:
             state_slots = self.row_ids[row : row + 1]
         last = torch.tensor([n - 1], dtype=torch.int32, device=dev)
         logits, hidden = self._prefill_span(row, seq_id, ids, start, n, state_slots)
-        constraint = self._prompt_read(row, ids, start, keys, params, generated)
-        if constraint is not None:
-            bias = self._bias_rows(logits, self.max_batch)[row : row + 1]
-            self._write_bias([row])
-            logits = logits + bias
+        constraint = self._prompt_read(row, ids, start, keys, params, generated, logits.shape[1] * self.model.tp)
+        if self._is_processed(row):
+            self._write_limits([row], logits.shape[1] * self.model.tp)
+            logits = self._process(logits, self.row_ids[row : row + 1])
         if self.row_stochastic[row]:
             # sample row 0 of the one-row logits with this row's record
             saved_rows, saved_len = self.sample_rows[0].clone(), self.seq_lens[0].clone()
@@ -377,12 +389,19 @@ class LLMEngine:
             start, keys = self._restore_prefix(seq_id, token_ids, n)
         return ids, start, keys
 
-    def _prompt_read(self, row: int, ids, start: int, keys, params, generated: int):
-        """Bookkeeping once every prompt token is in the cache; returns the row's token constraint (or None)."""
+    def _prompt_read(self, row: int, ids, start: int, keys, params, generated: int, width: int):
+        """Bookkeeping once every prompt token is in the cache (``width``: columns of the logits over all ranks); returns the row's token
+        constraint (or None)."""
         n = int(ids.numel())
         self._store_prefix(self.row_seq[row], keys, start)
         self.seq_lens[row] = n
         self.row_len[row] = n
+        if row in self.row_penalized:
+            table = self._tables(width).counts
+            table[row].zero_()
+            of = self.row_ids[row : row + 1].repeat(n)
+            ops.count_tokens(table, ids[: n - generated], of[: n - generated], prompt=True)
+            ops.count_tokens(table, ids[n - generated :], of[n - generated :])
         constraint = self._constraint_for(params)
         if constraint is not None:
             for t in (ids[n - generated :].tolist() if generated else ()):
@@ -411,29 +430,24 @@ class LLMEngine:
 
     def _ragged_step(self, portions, ids: torch.Tensor) -> StepBuffers:
         """Step of a ragged batch.  ``portions``: ``(row, first position, tokens)``, single tokens first; ``ids`` (device): their
-        tokens one after the other.  Everything the host knows travels in one copy."""
+        tokens one after the other.  The host sends the lengths in one copy, the rest follows from them on the device."""
         rows = [r for r, _, _ in portions]
         counts = [m for _, _, m in portions]
         total, b = sum(counts), len(portions)
         starts = [0]
         for m in counts:
             starts.append(starts[-1] + m)
-        host = torch.cat([
-            torch.cat([torch.arange(c, c + m, dtype=torch.int32) for _, c, m in portions]),
-            torch.cat([self.cache.slots(self.row_seq[r], c, m) for r, c, m in portions]),
-            torch.repeat_interleave(torch.arange(b, dtype=torch.int32), torch.tensor(counts)),
-            torch.tensor(starts, dtype=torch.int32), torch.tensor([c + m for _, c, m in portions], dtype=torch.int32),
-            torch.tensor(rows, dtype=torch.int32)])
+        host = torch.tensor([rows, [c for _, c, _ in portions], counts], dtype=torch.int32)
         if self.device.type == "cuda":
             host = host.pin_memory()
-        positions, slots, tok_seq, q_starts, seq_lens, row_ids = host.to(self.device, non_blocking=True).split(
-            [total, total, total, b + 1, b, b])
+        row_ids, past, new = host.to(self.device, non_blocking=True)
+        plan = ops.plan_batch(self.cache.block_table, row_ids, past, new, tokens=total, page_size=self.cache.page_size)
         singles = next((i for i, m in enumerate(counts) if m != 1), b)
         if hasattr(self.model, "decode_splits"):
             self.model.attn_splits = self.model.decode_splits(max(1, singles), max(c + m for _, c, m in portions))
-        return StepBuffers(input_ids=ids, positions=positions, slots=slots, block_table=self.cache.block_table.index_select(0, row_ids.long()),
-                           seq_lens=seq_lens, state_slots=row_ids if self.rec_state is not None else None, cu_seqlens=starts,
-                           q_starts=q_starts, tok_seq=tok_seq, max_q=max(counts), num_decode=singles,
+        return StepBuffers(input_ids=ids, positions=plan.positions, slots=plan.slots, block_table=plan.block_table,
+                           seq_lens=plan.seq_lens, state_slots=row_ids if self.rec_state is not None else None, cu_seqlens=starts,
+                           q_starts=plan.q_starts, tok_seq=plan.tok_seq, max_q=max(counts), num_decode=singles,
                            portions=[(c, m) for _, c, m in portions])
 
     def extend(self, portions, wanted=None) -> torch.Tensor | None:
@@ -491,6 +505,10 @@ class LLMEngine:
                 answer.append(r)
                 places.append(end - 1)
         logits = self._forward_ragged(step, torch.tensor(places or [0], dtype=torch.int32).to(self.device))
+        counted = [r for r in decode_rows if r in self.row_penalized]
+        if counted:  # what was fed is a token of the answer by now
+            of = torch.tensor(counted, dtype=torch.int32).to(self.device)
+            ops.count_tokens(self.logit_tables.counts, self.sampled.index_select(0, of.long()), of)
         self.seq_lens.index_copy_(0, torch.tensor([r for r, _, _ in spans]).to(self.device), step.seq_lens)
         for r, a, m in spans:
             self.row_len[r] = a + m
@@ -498,7 +516,7 @@ class LLMEngine:
             p = self.row_prompt[r]
             p.done = a + m
             if p.done == p.total:
-                self._prompt_read(r, p.ids, p.start, p.keys, p.params, p.generated)
+                self._prompt_read(r, p.ids, p.start, p.keys, p.params, p.generated, logits.shape[1] * self.model.tp)
                 del self.row_prompt[r]
         if not answer:
             return {}
@@ -691,7 +709,10 @@ class LLMEngine:
         else:
             logits = self.model.forward(step, self.cache, prefill=False, gather_logits=False)
         if constrained:
-            logits += self._bias_rows(logits, b)
+            t = self._tables(logits.shape[1] * self.model.tp)
+            torch.where(self.active[:b] > 0, self.row_ids[:b], torch.full_like(self.row_ids[:b], -1), out=t.counted[:b])
+            ops.count_tokens(t.counts, self.input_ids[:b], t.counted[:b])
+            self._process(logits)
         self._sample(logits, b, stochastic)
         if keep_head:
             # parked speculation: the head still reads every position (its hidden state paired with the token that
@@ -728,7 +749,7 @@ class LLMEngine:
 
     def decode_step(self, b: int, stochastic: bool = False, constrained: bool = False, keep_head: bool = False) -> None:
         """Advance the active rows among ``[0, b)`` by one token (result in ``self.sampled[:b]``, on the device).
-        ``constrained``: add the rows' token-constraint bias to the logits before sampling (a graph variant of its own)."""
+        ``constrained``: process the logits by the rows' constraints and penalties before sampling (a graph variant of its own)."""
         if getattr(self, "moe_miss_count", None) is None:
             self._decode_step_once(b, stochastic, constrained, keep_head)
             return
@@ -738,11 +759,14 @@ class LLMEngine:
         # few the step runs in waves instead, which also leaves its experts resident.
         res = self.model.residencies()
         snap = (self.seq_lens.clone(), self.sampled.clone())
+        counts = self.logit_tables.counts.clone() if constrained and self.logit_tables is not None else None
         self.residency_stats["steps"] += 1
 
         def restore():
             self.seq_lens.copy_(snap[0])
             self.sampled.copy_(snap[1])  # the sampler's counter is the row length: a replay draws the same token
+            if counts is not None:
+                self.logit_tables.counts.copy_(counts)
 
         for r in res:
             r.optimistic = True
@@ -781,6 +805,7 @@ class LLMEngine:
             saved = (self.seq_lens.clone(), self.sampled.clone())
             saved_draft = self.draft.clone() if keep_head else None
             saved_rec = self.rec_state.save() if self.rec_state is not None else None
+            saved_counts = self.logit_tables.counts.clone() if constrained else None
             with torch.cuda.stream(side):
                 for _ in range(2):
                     self._decode_body(b, stochastic, constrained, keep_head)
@@ -797,6 +822,8 @@ class LLMEngine:
             self.sampled.copy_(saved[1])
             if saved_draft is not None:
                 self.draft.copy_(saved_draft)
+            if saved_counts is not None:
+                self.logit_tables.counts.copy_(saved_counts)
             if saved_rec is not None:  # the recurrent state cannot be "rewritten later" like KV rows: put it back
                 self.rec_state.load(saved_rec)
             self.graphs[key] = g
@@ -995,9 +1022,9 @@ class LLMEngine:
         mask = torch.zeros(self.max_batch, dtype=torch.int32)
         mask[rows] = 1
         self.active.copy_(mask.to(self.device), non_blocking=True)
-        constrained = any(r in self.row_constraint for r in rows)
+        constrained = any(self._is_processed(r) for r in rows)
         if constrained:
-            self._write_bias(range(b))
+            self._write_limits(range(b), self.logit_tables.width)  # there since the rows' prompts were read
         stochastic = any(self.row_stochastic.get(r, False) for r in rows)
         if self.mtp_k and not constrained:
             ctl = self.mtp_controller

@@ -30,6 +30,7 @@ from dataclasses import dataclass, field
 from typing import Callable, Protocol
 
 from ..config import trace
+from .constraints import penalized
 
 INITIAL_NEW_TOKEN_RATIO = 0.7
 MIN_NEW_TOKEN_RATIO = 0.098
@@ -303,8 +304,9 @@ class ContinuousBatchScheduler:
                 extra = {}
                 if req.session is not None and hasattr(self.backend, "save_session"):
                     extra["session"] = req.session
-                if req.generated and (req.params.response_format or req.params.logit_bias):  # replay after a retraction: the grammar has to
-                    extra["generated"] = len(req.generated)       # re-read what was generated before
+                # replay after a retraction: the grammar has to re-read what was generated before, penalties count it as the answer's
+                if req.generated and (req.params.response_format or req.params.logit_bias or penalized(req.params)):
+                    extra["generated"] = len(req.generated)
                 tok = start(req, extra)
             except MemoryError:
                 self.running.pop(row, None)

@@ -40,7 +40,7 @@ struct LogitArgs {
   float fill;
 };
 
-constexpr int kLogitThreads = 256, kLogitVec = 8, kLogitChunk = kLogitThreads * kLogitVec, kMaxBias = 1024;
+constexpr int kLogitThreads = 256, kLogitVec = 8, kLogitChunk = kLogitThreads * kLogitVec, kMaxBias = 1 << 16;
 
 template <typename T> __device__ __forceinline__ float logit_to_f32(T v);
 template <> __device__ __forceinline__ float logit_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kLogitThreads)
 process_logits_kernel(const LogitArgs a) {
   pdl_trigger();
   __shared__ float s_bias[kLogitChunk];
-  __shared__ int s_hit[kMaxBias];
+  __shared__ int s_hit[kLogitChunk];
   __shared__ int s_hits;
   pdl_wait();
   const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kLogitChunk, hi = min(a.V, lo + kLogitChunk);
@@ -134,10 +134,22 @@ process_logits_kernel(const LogitArgs a) {
     const float* values = a.bias_values + size_t(r) * a.K;
     for (int j = tid; j < a.K; j += kLogitThreads) {
       const int v = ids[j] - a.first;
-      if (ids[j] >= 0 && v >= lo && v < hi) s_hit[atomicAdd(&s_hits, 1)] = j;
+      if (ids[j] >= 0 && v >= lo && v < hi) {
+        const int at = atomicAdd(&s_hits, 1);
+        if (at < kLogitChunk) s_hit[at] = j;
+      }
     }
     __syncthreads();
     const int hits = s_hits;
+    if (hits > kLogitChunk) {  // ids many times over: each column goes through the whole row
+#pragma unroll 1
+      for (int n = tid; n < hi - lo; n += kLogitThreads) {
+        float sum = 0.f;
+        for (int j = 0; j < a.K; ++j)
+          if (ids[j] == a.first + lo + n) sum += values[j];
+        s_bias[n] = sum;
+      }
+    } else
     for (int h = tid; h < hits; h += kLogitThreads) {
       const int id = ids[s_hit[h]];
       float sum = 0.f;

@@ -16,7 +16,7 @@ from . import reference
 from .lib import check, elsewhere, lib, ptr, stream_ptr
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-MAX_BIASES = 1024  # places per row; kMaxBias of the kernel
+MAX_BIASES = 1 << 16  # places per row; kMaxBias of the kernel
 RECORD_WORDS = 8  # a sampling record: temperature f32, top_k i32, top_p f32, presence f32, frequency f32, repetition f32, seed u64
 
 

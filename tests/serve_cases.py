@@ -116,7 +116,7 @@ def logits_case(seed, b, r, v, dtype, *, first=0, k=0, mask=False, counted=True,
 LOGITS = [  # b, r, v, what else
     (1, 1, 1, {}), (1, 1, 7, {"mask": True}), (2, 2, 8, {"k": 1}), (3, 5, 2047, {"mask": True, "k": 9, "mapped": True}), (2, 2, 2048, {"mask": True, "k": 300}),
     (4, 4, 2049, {"odd": True, "mask": True, "k": 40}), (5, 3, 6000, {"mask": True, "k": 1024, "mapped": True}), (2, 2, 4104, {"first": 40, "mask": True, "k": 30}),
-    (2, 3, 1001, {"first": 333, "mask": True, "k": 60, "odd": True}), (3, 3, 5000, {"counted": False, "mask": True}), (2, 2, 128256, {"k": 5})]
+    (2, 3, 1001, {"first": 333, "mask": True, "k": 60, "odd": True}), (3, 3, 5000, {"counted": False, "mask": True}), (2, 2, 9, {"k": 3000}), (2, 2, 7000, {"k": 2500}), (2, 2, 128256, {"k": 5})]
 
 
 def plan_case(seed, b, most, past, rows=None, ps=16, pages=False, wide=None, device="cpu"):

@@ -97,7 +97,7 @@ def test_refusals():
                 dict(records=rec[:, :6]), dict(records=rec[:1]), dict(records=rec[:0], rows=torch.zeros(2, dtype=i32)), dict(rows=torch.zeros(3, dtype=i32)), dict(rows=torch.zeros(2)),
                 dict(counts=torch.zeros(2, 40)), dict(counts=torch.zeros((2, 39), dtype=torch.int16)), dict(counts=torch.zeros((1, 40), dtype=torch.int16)),
                 dict(bias=(torch.zeros((2, 3), dtype=i32), torch.zeros(2, 4))), dict(bias=(torch.zeros((2, 3)), torch.zeros(2, 3))),
-                dict(bias=(torch.zeros((2, 1025), dtype=i32), torch.zeros(2, 1025))), dict(allowed=torch.zeros((2, 1), dtype=i32)), dict(allowed=torch.zeros((2, 2))),
+                dict(bias=(torch.zeros((2, 65537), dtype=i32), torch.zeros(2, 65537))), dict(allowed=torch.zeros((2, 1), dtype=i32)), dict(allowed=torch.zeros((2, 2))),
                 dict(first=-1), dict(first=25, allowed=torch.zeros((2, 2), dtype=i32)), dict(out=torch.zeros(2, 41)), dict(out=torch.zeros(2, 40, dtype=torch.bfloat16)),
                 dict(out=torch.zeros(1, 40).expand(2, 40))):
         with pytest.raises(ValueError):
