@@ -40,7 +40,7 @@ struct LogitArgs {
   float fill;
 };
 
-constexpr int kLogitThreads = 256, kLogitVec = 8, kLogitChunk = kLogitThreads * kLogitVec, kMaxBias = 1 << 16;
+constexpr int kLogitThreads = 256, kLogitVec = 8, kMaxBias = 1 << 16;
 
 template <typename T> __device__ __forceinline__ float logit_to_f32(T v);
 template <> __device__ __forceinline__ float logit_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -56,22 +56,27 @@ struct alignas(16) LogitVec {
   T v[kLogitVec];
 };
 
-// A thread has eight values: eight neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16 bytes), else eight that
-// lie a block apart, so that a warp's accesses are whole lines at any alignment.
+// A thread has eight values: eight neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16 bytes), else eight that lie a block
+// apart, so that a warp's accesses are whole lines at any alignment.  Logits, counts and mask are requested together, ahead of the record that says
+// whether the row needs the counts.  Where none of a thread's eight tokens has a count or a bias their bits stay as they are, and only the mask chooses:
+// with the arithmetic (a division among it) for all of them, 64 x 128256 bf16 with all three on a B200 took 18.9 us, bound by instructions, now KKK; four
+// sets of eight a thread took as long as one.
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kLogitThreads)
+__global__ void __launch_bounds__(kLogitThreads, 5)
 process_logits_kernel(const LogitArgs a) {
+  constexpr int kChunk = kLogitThreads * kLogitVec;
   pdl_trigger();
-  __shared__ float s_bias[kLogitChunk];
-  __shared__ int s_hit[kLogitChunk];
+  __shared__ float s_bias[kChunk];
+  __shared__ int s_hit[kChunk], s_id[kChunk];  // places of the row whose ids are in the chunk, and those
+  __shared__ unsigned s_biased[kChunk / 32];  // bit: whether the column has a bias
   __shared__ int s_hits;
   pdl_wait();
-  const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kLogitChunk, hi = min(a.V, lo + kLogitChunk);
+  const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kChunk, hi = min(a.V, lo + kChunk);
   const int r = a.rows ? a.rows[b] : b;
   const bool known = r >= 0 && r < a.R;
   const T* in = static_cast<const T*>(a.logits) + b * a.in_stride;
   T* out = static_cast<T*>(a.out) + b * a.out_stride;
-  const auto column = [&](int j) { return kVec ? lo + tid * kLogitVec + j : lo + tid + j * kLogitThreads; };
+  const auto column = [&](int j) { return lo + (kVec ? tid * kLogitVec + j : tid + j * kLogitThreads); };
   const bool whole = kVec && column(kLogitVec - 1) < hi;
 
   LogitVec<T> x;
@@ -81,15 +86,28 @@ process_logits_kernel(const LogitArgs a) {
     for (int j = 0; j < kLogitVec; ++j)
       if (column(j) < hi) x.v[j] = in[column(j)];
   }
-  if (!known) {
-    if (in == out) return;
-    if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = x;
+  const auto store = [&](const LogitVec<T>& y) {
+    if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
     else {
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) out[column(j)] = x.v[j];
+        if (column(j) < hi) out[column(j)] = y.v[j];
     }
+  };
+  if (!known) {
+    if (in != out) store(x);
     return;
+  }
+  unsigned w[kLogitVec / 2] = {};  // eight words of counts
+  if (a.counts) {
+    const unsigned short* row = a.counts + r * a.counts_stride;
+    if (whole) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(row + column(0));
+      w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j) w[j >> 1] |= (column(j) < hi ? unsigned(row[column(j)]) : 0u) << (16 * (j & 1));
+    }
   }
   unsigned allow = 0xffu;  // bit j: value j
   if (a.allowed) {
@@ -104,112 +122,144 @@ process_logits_kernel(const LogitArgs a) {
       }
     }
   }
-  float presence = 0.f, frequency = 0.f, repetition = 1.f;
-  if (a.counts) {
-    presence = a.records[r].presence;
-    frequency = a.records[r].frequency;
-    repetition = a.records[r].repetition;
-  }
-  unsigned short c[kLogitVec] = {};
-  if (presence != 0.f || frequency != 0.f || repetition != 1.f) {
-    const unsigned short* row = a.counts + r * a.counts_stride;
-    if (whole) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(row + column(0));
-      const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int j = 0; j < kLogitVec; ++j) c[j] = static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) c[j] = row[column(j)];
-    }
-  }
+  const float presence = a.records[r].presence, frequency = a.records[r].frequency, repetition = a.records[r].repetition;
+  const bool penalties = presence != 0.f || frequency != 0.f || repetition != 1.f;
+  unsigned biased = 0;  // bit j: value j
   // biases: those of this block's columns are gathered, then each id's are summed by one thread in the order of the row
   if (a.bias_ids) {
     if (tid == 0) s_hits = 0;
-#pragma unroll
-    for (int j = 0; j < kLogitVec; ++j) s_bias[tid + j * kLogitThreads] = 0.f;
+    if (tid < kChunk / 32) s_biased[tid] = 0u;
     __syncthreads();
     const int* ids = a.bias_ids + size_t(r) * a.K;
     const float* values = a.bias_values + size_t(r) * a.K;
     for (int j = tid; j < a.K; j += kLogitThreads) {
-      const int v = ids[j] - a.first;
-      if (ids[j] >= 0 && v >= lo && v < hi) {
+      const int id = ids[j], v = id - a.first;
+      if (id >= 0 && v >= lo && v < hi) {
         const int at = atomicAdd(&s_hits, 1);
-        if (at < kLogitChunk) s_hit[at] = j;
+        if (at < kChunk) { s_hit[at] = j; s_id[at] = id; }
       }
     }
     __syncthreads();
     const int hits = s_hits;
-    if (hits > kLogitChunk) {  // ids many times over: each column goes through the whole row
+    if (hits > kChunk) {  // ids many times over: each column goes through the whole row
 #pragma unroll 1
       for (int n = tid; n < hi - lo; n += kLogitThreads) {
         float sum = 0.f;
         for (int j = 0; j < a.K; ++j)
           if (ids[j] == a.first + lo + n) sum += values[j];
         s_bias[n] = sum;
+        atomicOr(&s_biased[n >> 5], 1u << (n & 31));
       }
-    } else
-    for (int h = tid; h < hits; h += kLogitThreads) {
-      const int id = ids[s_hit[h]];
-      float sum = 0.f;
-      int last = -1;
-      bool mine = true;
-      while (mine) {  // the next place of the same id
-        int next = a.K;
-        for (int i = 0; i < hits; ++i) {
-          const int j = s_hit[i];
-          if (j > last && j < next && ids[j] == id) next = j;
+    } else {
+      for (int h = tid; h < hits; h += kLogitThreads) {
+        const int id = s_id[h], n = id - a.first - lo;
+        int same = 0, first = a.K;
+        for (int i = 0; i < hits; ++i)
+          if (s_id[i] == id) {
+            ++same;
+            first = min(first, s_hit[i]);
+          }
+        const bool mine = first == s_hit[h];
+        float sum = values[s_hit[h]];
+        for (int last = first; mine && same > 1; --same) {  // the next place of the same id
+          int next = a.K;
+          for (int i = 0; i < hits; ++i)
+            if (s_id[i] == id && s_hit[i] > last) next = min(next, s_hit[i]);
+          sum += values[next];
+          last = next;
         }
-        if (next == a.K) break;
-        if (last < 0) mine = next == s_hit[h];
-        sum += values[next];
-        last = next;
+        if (mine) {
+          s_bias[n] = sum;
+          atomicOr(&s_biased[n >> 5], 1u << (n & 31));
+        }
       }
-      if (mine) s_bias[id - a.first - lo] = sum;
     }
-    __syncthreads();
-  }
-  LogitVec<T> y;
+    if (hits) {
+      __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kLogitVec; ++j) {
-    float l = logit_to_f32(x.v[j]);
-    if (a.bias_ids && column(j) < hi) l += s_bias[column(j) - lo];
-    const unsigned n = c[j] & 0x7fffu;
-    if (c[j]) l = l > 0.f ? l / repetition : l * repetition;
-    if (n) l -= presence + frequency * float(n);
-    y.v[j] = allow >> j & 1u ? logit_from_f32<T>(l) : logit_from_f32<T>(a.fill);
+      for (int j = 0; j < kLogitVec; ++j)
+        if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
+    }
   }
-  if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
-  else {
+  LogitVec<T> y = x;
+  if ((penalties && (w[0] | w[1] | w[2] | w[3])) || biased) {
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j) {
+      float l = logit_to_f32(x.v[j]);
+      if (biased >> j & 1u) l += s_bias[column(j) - lo];
+      const unsigned word = w[j >> 1] >> (16 * (j & 1)) & 0xffffu, n = word & 0x7fffu;
+      if (penalties && word) l = l > 0.f ? l / repetition : l * repetition;
+      if (penalties && n) l -= presence + frequency * float(n);
+      y.v[j] = logit_from_f32<T>(l);
+    }
+  }
+  if (allow != 0xffu) {
+    const T fill = logit_from_f32<T>(a.fill);
 #pragma unroll
     for (int j = 0; j < kLogitVec; ++j)
-      if (column(j) < hi) out[column(j)] = y.v[j];
+      if (!(allow >> j & 1u)) y.v[j] = fill;
   }
+  store(y);
 }
 
 // counts[row][token] of every (row, token): its top bit is set (prompt) or its lower 15 go up by one and stay at their largest value.
-// Pairs with a token or row outside the table are left out.  The lanes of a warp that have the same pair add together.
+// Pairs with a token or row outside the table are left out.
+__device__ __forceinline__ void count_up(unsigned short* at, unsigned times, bool prompt) {
+  unsigned old = *reinterpret_cast<volatile unsigned short*>(at);
+  for (;;) {  // a failed exchange means that another one succeeded
+    const unsigned now = prompt ? old | 0x8000u : (old & 0x8000u) | min((old & 0x7fffu) + times, 0x7fffu);
+    if (now == old) return;
+    const unsigned seen = atomicCAS(at, static_cast<unsigned short>(old), static_cast<unsigned short>(now));
+    if (seen == old) return;
+    old = seen;
+  }
+}
+// Few pairs, or a bit to set (whoever finds it set is done): the lanes of a warp that have the same pair add together.
 __global__ void __launch_bounds__(256)
 count_tokens_kernel(unsigned short* __restrict__ counts, long long stride, int R, int V, const int* __restrict__ tokens, const int* __restrict__ rows, int T,
                     int prompt) {
   pdl_trigger();
   pdl_wait();
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int token = i < T ? tokens[i] : -1, row = i < T ? rows[i] : -1;
   const bool in = token >= 0 && token < V && row >= 0 && row < R;
   const unsigned live = __ballot_sync(0xffffffffu, in);
   if (!in) return;
   unsigned short* at = counts + row * stride + token;
   const unsigned same = __match_any_sync(live, reinterpret_cast<unsigned long long>(at));
-  if ((threadIdx.x & 31) != __ffs(same) - 1) return;
-  unsigned old = *reinterpret_cast<volatile unsigned short*>(at);
-  for (;;) {  // a failed exchange means that another one succeeded
-    const unsigned now = prompt ? old | 0x8000u : (old & 0x8000u) | min((old & 0x7fffu) + unsigned(__popc(same)), 0x7fffu);
-    if (now == old) return;
-    const unsigned seen = atomicCAS(at, static_cast<unsigned short>(old), static_cast<unsigned short>(now));
-    if (seen == old) return;
-    old = seen;
+  if ((threadIdx.x & 31) == __ffs(same) - 1) count_up(at, __popc(same), prompt);
+}
+// Many: the pairs of a block are added up in shared memory first (open addressing; twice as many places as pairs, so that one is always free), and
+// every different one goes to the table once.  The common tokens of a text then meet in a few blocks instead of in every warp: 32000 tokens of 24
+// rows took 32 us by warps on a B200, KKK by blocks.
+constexpr int kCountThreads = 512, kCountPer = 2, kCountPlaces = 2 * kCountThreads * kCountPer;
+__global__ void __launch_bounds__(kCountThreads)
+count_many_kernel(unsigned short* __restrict__ counts, long long stride, int R, int V, const int* __restrict__ tokens, const int* __restrict__ rows, int T) {
+  pdl_trigger();
+  __shared__ unsigned long long s_key[kCountPlaces];  // row and token; all ones: free
+  __shared__ unsigned s_times[kCountPlaces];
+  for (int i = threadIdx.x; i < kCountPlaces; i += kCountThreads) { s_key[i] = ~0ull; s_times[i] = 0u; }
+  __syncthreads();
+  pdl_wait();
+#pragma unroll
+  for (int n = 0; n < kCountPer; ++n) {
+    const long long i = (static_cast<long long>(blockIdx.x) * kCountPer + n) * kCountThreads + threadIdx.x;
+    if (i >= T) break;
+    const int token = tokens[i], row = rows[i];
+    if (token < 0 || token >= V || row < 0 || row >= R) continue;
+    const unsigned long long key = static_cast<unsigned long long>(row) << 32 | unsigned(token);
+    unsigned at = (unsigned(token) * 2654435761u ^ unsigned(row) * 2246822519u) % kCountPlaces;  // odd multipliers spread neighbours
+    for (;;) {
+      const unsigned long long held = atomicCAS(&s_key[at], ~0ull, key);
+      if (held == ~0ull || held == key) break;
+      at = (at + 1) % kCountPlaces;
+    }
+    atomicAdd(&s_times[at], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kCountPlaces; i += kCountThreads) {
+    if (s_times[i] == 0u) continue;
+    count_up(counts + (s_key[i] >> 32) * stride + unsigned(s_key[i]), s_times[i], false);
   }
 }
 
@@ -347,8 +397,8 @@ plan_batch_kernel(const PlanArgs a) {
 
 template <typename T>
 static int launch_logits(const LogitArgs& a, int B, bool vec, cudaStream_t stream) {
-  const dim3 grid((a.V + kLogitChunk - 1) / kLogitChunk, B);
-  launch_kernel(vec ? process_logits_kernel<T, true> : process_logits_kernel<T, false>, grid, dim3(kLogitThreads), 0, stream, a);
+  constexpr int kChunk = kLogitThreads * kLogitVec;
+  launch_kernel(vec ? process_logits_kernel<T, true> : process_logits_kernel<T, false>, dim3((a.V + kChunk - 1) / kChunk, B), dim3(kLogitThreads), 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 
@@ -372,7 +422,11 @@ extern "C" int mfq_process_logits(const void* logits, void* out, int dtype, int 
 extern "C" int mfq_count_tokens(void* counts, long long stride, int R, int V, const int* tokens, const int* rows, int T, int prompt, cudaStream_t stream) {
   if (R <= 0 || V <= 0 || T < 0) return -1;
   if (T == 0) return 0;
-  mfq::launch_kernel(mfq::count_tokens_kernel, dim3((T + 255) / 256), dim3(256), 0, stream, static_cast<unsigned short*>(counts), stride, R, V, tokens, rows, T, prompt);
+  constexpr int many = mfq::kCountThreads * mfq::kCountPer;
+  if (prompt || T <= many)
+    mfq::launch_kernel(mfq::count_tokens_kernel, dim3((T - 1) / 256 + 1), dim3(256), 0, stream, static_cast<unsigned short*>(counts), stride, R, V, tokens, rows, T, prompt);
+  else
+    mfq::launch_kernel(mfq::count_many_kernel, dim3((T - 1) / many + 1), dim3(mfq::kCountThreads), 0, stream, static_cast<unsigned short*>(counts), stride, R, V, tokens, rows, T);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 
