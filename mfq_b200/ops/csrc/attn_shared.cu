@@ -19,17 +19,18 @@ namespace mfq {
 
 template <int D, int WR>
 struct SharedTile {
-  static constexpr int kLanes = 4 / WR;  // groups of warps that take alternate pages
+  static constexpr int kLanes = D == 256 && WR == 4 ? 2 : 4 / WR;  // groups of warps that take alternate pages
+  static constexpr int kThreads = 32 * WR * kLanes;
   static constexpr int kStages = WR == 1 ? 3 : WR == 2 ? 4 : 8;
   static constexpr int kPage = 16 * D, kStage = 2 * kPage + 128;
   static constexpr int kRing = kLanes * kStages * kStage;
   static constexpr int kSmem = kRing + 2 * kLanes * kStages * 8 + 16;
-  static_assert(kRing >= 4 * (16 * D + 32) * 4, "the ring is the merge's scratch too");
+  static_assert(kRing >= WR * kLanes * (16 * D + 32) * 4, "the ring is the merge's scratch too");
 };
 
 // The prefixes of groups with few query rows: blockIdx.x = one of the groups' tiles of 16 WR rows, blockIdx.z = split.
 template <int D, int WR>
-__global__ void __launch_bounds__(128, D <= 128 ? 3 : 1)
+__global__ void __launch_bounds__(SharedTile<D, WR>::kThreads, D <= 128 ? 3 : 1)
 shared_prefix_kernel(const SharedAttnArgs a) {
   using L = SharedTile<D, WR>;
   constexpr int KSTEPS = D / 16, NBD = D / 8, kStages = L::kStages, kLanes = L::kLanes;
@@ -254,7 +255,7 @@ shared_prefix_kernel(const SharedAttnArgs a) {
   }
   __syncthreads();
   if (!ok || *abort_flag) return;
-  for (int idx = threadIdx.x; idx < 16 * WR * D; idx += 128) {
+  for (int idx = threadIdx.x; idx < 16 * WR * D; idx += L::kThreads) {
     const int t = idx / (16 * D), r = idx / D % 16, d = idx % D;
     const int global = (tile * WR + t) * 16 + r;
     if (global >= rows) continue;
@@ -527,7 +528,7 @@ struct TailRows {
 
 constexpr int kMostSlots = 64, kMostRanks = 8;
 
-// The tails, and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
+// The tails (without prefix splits: whole sequences, each through its own table), and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
 // are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own part done.
 template <int D, bool kNarrow>
 __global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
@@ -547,6 +548,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
     mbar_fence_init();
   }
   __syncthreads();
+  if (a.prefix_splits == 0) pdl_wait();  // no prefixes' kernel has waited for what is read here
   const int place = blockIdx.x, kvh = blockIdx.y, ranks = gridDim.z, rank = blockIdx.z;
   const int G = a.Hq / a.Hk, rows = G * a.q_len;
   const int group = group_of(a, place);
@@ -555,7 +557,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
     pdl_wait();  // this grid ends behind the prefixes' in any case
     return;
   }
-  const int front = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), seq_len = a.seq_lens[row];
+  const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0, seq_len = a.seq_lens[row];
   const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
   const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
   const int my_pages = page_hi > page_lo + warp ? (page_hi - page_lo - warp + 3) / 4 : 0;
@@ -650,7 +652,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
       if (w != 0.f) { acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w; }
     };
     for (int e = 0; e < ranks; ++e) add(load_peer(map_to_cta(mine + r * D + d, e)), by[e]);
-    const float4* src = reinterpret_cast<const float4*>(a.part_o + hq * a.slots * D + d);
+    const float4* src = reinterpret_cast<const float4*>(a.part_o + hq * a.slots * D + d);  // (no slots: not read)
     for (int e = 0; e < a.slots; e += 8) {  // eight requested before the first is used; behind the last one the last again, for nothing
       float4 v[8];
 #pragma unroll
@@ -676,7 +678,7 @@ template <int D, int WR>
 static int launch_shared_prefix(const SharedAttnArgs& a, cudaStream_t stream) {
   static bool done[64] = {};
   if (!set_smem(shared_prefix_kernel<D, WR>, SharedTile<D, WR>::kSmem, done)) return -6;
-  launch_kernel(shared_prefix_kernel<D, WR>, dim3(tiles_at_most(a, 16 * WR), a.Hk, a.prefix_splits), dim3(128), SharedTile<D, WR>::kSmem, stream, a);
+  launch_kernel(shared_prefix_kernel<D, WR>, dim3(tiles_at_most(a, 16 * WR), a.Hk, a.prefix_splits), dim3(SharedTile<D, WR>::kThreads), SharedTile<D, WR>::kSmem, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 template <int D, bool kNarrow>
@@ -693,7 +695,8 @@ int launch_shared_prefix_tc(const SharedAttnArgs& a, int dim, bool two_tiles, cu
 
 template <int D>
 static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream) {
-  const int rc = tile == 16   ? launch_shared_prefix<D, 1>(a, stream)
+  const int rc = !a.prefix_splits ? 0
+                 : tile == 16   ? launch_shared_prefix<D, 1>(a, stream)
                  : tile == 32 ? launch_shared_prefix<D, 2>(a, stream)
                  : tile == 64 ? launch_shared_prefix<D, 4>(a, stream)
                               : launch_shared_prefix_tc(a, D, tile == 256, stream);
@@ -711,7 +714,7 @@ extern "C" int mfq_paged_attn_decode_shared(const void* q, const void* k, const 
                                             float* part_o, float* part_ml, int B, int Hq, int Hk, int D, int max_pages, int pages, int groups, int q_len,
                                             int tile, int prefix_splits, int tail_splits, float sm_scale, int* status, cudaStream_t stream) {
   using namespace mfq;
-  if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (tile != 16 && tile != 32 && tile != 64 && (D > 128 || (tile != 128 && tile != 256))) || prefix_splits < 1 ||
+  if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (tile != 16 && tile != 32 && tile != 64 && (D > 128 || (tile != 128 && tile != 256))) || prefix_splits < 0 ||
       tail_splits < 1 || pages < 1 || max_pages < 1 || Hk > 65535 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits > kMostRanks)
     return -1;
   const SharedAttnArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_scale, v_scale, table, seq_lens,

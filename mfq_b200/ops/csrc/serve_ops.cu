@@ -40,7 +40,7 @@ struct LogitArgs {
   float fill;
 };
 
-constexpr int kLogitThreads = 256, kLogitVec = 8, kMaxBias = 1 << 16;
+constexpr int kLogitThreads = 256, kLogitVec = 8, kMaxBias = 1 << 16, kMostHits = 1024;
 
 template <typename T> __device__ __forceinline__ float logit_to_f32(T v);
 template <> __device__ __forceinline__ float logit_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -67,9 +67,11 @@ process_logits_kernel(const LogitArgs a) {
   constexpr int kChunk = kLogitThreads * kLogitVec;
   pdl_trigger();
   __shared__ float s_bias[kChunk];
-  __shared__ int s_hit[kChunk], s_id[kChunk];  // places of the row whose ids are in the chunk, and those
-  __shared__ unsigned s_biased[kChunk / 32];  // bit: whether the column has a bias
+  __shared__ int s_hit[kMostHits], s_id[kMostHits];  // places of the row whose ids are in the chunk, and those
+  __shared__ unsigned s_biased[kChunk / 32];   // bit: whether the column has a bias
   __shared__ int s_hits;
+  if (threadIdx.x == 0) s_hits = 0;
+  if (threadIdx.x < kChunk / 32) s_biased[threadIdx.x] = 0u;
   pdl_wait();
   const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kChunk, hi = min(a.V, lo + kChunk);
   const int r = a.rows ? a.rows[b] : b;
@@ -80,11 +82,13 @@ process_logits_kernel(const LogitArgs a) {
   const bool whole = kVec && column(kLogitVec - 1) < hi;
 
   LogitVec<T> x;
-  if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
-  else {
+  {
+    if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
+    else {
 #pragma unroll
-    for (int j = 0; j < kLogitVec; ++j)
-      if (column(j) < hi) x.v[j] = in[column(j)];
+      for (int j = 0; j < kLogitVec; ++j)
+        if (column(j) < hi) x.v[j] = in[column(j)];
+    }
   }
   const auto store = [&](const LogitVec<T>& y) {
     if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
@@ -95,13 +99,20 @@ process_logits_kernel(const LogitArgs a) {
     }
   };
   if (!known) {
-    if (in != out) store(x);
+    if (in == out) return;
+    store(x);
     return;
   }
-  unsigned w[kLogitVec / 2] = {};  // eight words of counts
-  if (a.counts) {
+  const int* ids = a.bias_ids + size_t(r) * a.K;  // (K is zero where there are none)
+  const float* values = a.bias_values + size_t(r) * a.K;
+  int id = tid < a.K ? ids[tid] : -1;  // this thread's first place, requested with the rest
+  unsigned w[kLogitVec / 2];  // eight words of counts
+  {
+#pragma unroll
+    for (int j = 0; j < kLogitVec / 2; ++j) w[j] = 0;
     const unsigned short* row = a.counts + r * a.counts_stride;
-    if (whole) {
+    if (!a.counts) {
+    } else if (whole) {
       const uint4 raw = *reinterpret_cast<const uint4*>(row + column(0));
       w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
     } else {
@@ -109,39 +120,38 @@ process_logits_kernel(const LogitArgs a) {
       for (int j = 0; j < kLogitVec; ++j) w[j >> 1] |= (column(j) < hi ? unsigned(row[column(j)]) : 0u) << (16 * (j & 1));
     }
   }
-  unsigned allow = 0xffu;  // bit j: value j
-  if (a.allowed) {
+  unsigned allow;  // bit j: value j
+  {
+    allow = 0xffu;
     const unsigned* words = a.allowed + size_t(r) * a.words;
-    if (whole && a.first % 8 == 0) {
+    if (!a.allowed) {
+    } else if (whole && a.first % 8 == 0) {
       allow = reinterpret_cast<const unsigned char*>(words)[(a.first + column(0)) >> 3];
     } else {
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j) {
-        const int id = a.first + column(j);
-        if (column(j) < hi && !(words[id >> 5] >> (id & 31) & 1u)) allow &= ~(1u << j);
+        const int of = a.first + column(j);
+        if (column(j) < hi && !(words[of >> 5] >> (of & 31) & 1u)) allow &= ~(1u << j);
       }
     }
   }
   const float presence = a.records[r].presence, frequency = a.records[r].frequency, repetition = a.records[r].repetition;
   const bool penalties = presence != 0.f || frequency != 0.f || repetition != 1.f;
-  unsigned biased = 0;  // bit j: value j
+  int hits = 0;
   // biases: those of this block's columns are gathered, then each id's are summed by one thread in the order of the row
-  if (a.bias_ids) {
-    if (tid == 0) s_hits = 0;
-    if (tid < kChunk / 32) s_biased[tid] = 0u;
+  if (a.K) {
     __syncthreads();
-    const int* ids = a.bias_ids + size_t(r) * a.K;
-    const float* values = a.bias_values + size_t(r) * a.K;
     for (int j = tid; j < a.K; j += kLogitThreads) {
-      const int id = ids[j], v = id - a.first;
+      if (j != tid) id = ids[j];
+      const int v = id - a.first;
       if (id >= 0 && v >= lo && v < hi) {
         const int at = atomicAdd(&s_hits, 1);
-        if (at < kChunk) { s_hit[at] = j; s_id[at] = id; }
+        if (at < kMostHits) { s_hit[at] = j; s_id[at] = id; }
       }
     }
     __syncthreads();
-    const int hits = s_hits;
-    if (hits > kChunk) {  // ids many times over: each column goes through the whole row
+    hits = s_hits;
+    if (hits > kMostHits) {  // each column goes through the whole row
 #pragma unroll 1
       for (int n = tid; n < hi - lo; n += kLogitThreads) {
         float sum = 0.f;
@@ -152,10 +162,10 @@ process_logits_kernel(const LogitArgs a) {
       }
     } else {
       for (int h = tid; h < hits; h += kLogitThreads) {
-        const int id = s_id[h], n = id - a.first - lo;
+        const int of = s_id[h], n = of - a.first - lo;
         int same = 0, first = a.K;
         for (int i = 0; i < hits; ++i)
-          if (s_id[i] == id) {
+          if (s_id[i] == of) {
             ++same;
             first = min(first, s_hit[i]);
           }
@@ -164,7 +174,7 @@ process_logits_kernel(const LogitArgs a) {
         for (int last = first; mine && same > 1; --same) {  // the next place of the same id
           int next = a.K;
           for (int i = 0; i < hits; ++i)
-            if (s_id[i] == id && s_hit[i] > last) next = min(next, s_hit[i]);
+            if (s_id[i] == of && s_hit[i] > last) next = min(next, s_hit[i]);
           sum += values[next];
           last = next;
         }
@@ -174,32 +184,46 @@ process_logits_kernel(const LogitArgs a) {
         }
       }
     }
+    if (hits) __syncthreads();
+  }
+  {
+    unsigned touched = 0, biased = 0;  // bit j: value j
     if (hits) {
-      __syncthreads();
+      if (kVec) {
+        if (column(0) < hi) biased = reinterpret_cast<const unsigned char*>(s_biased)[(column(0) - lo) >> 3];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLogitVec; ++j)
+          if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
+      }
+    }
+    if (penalties) {
+#pragma unroll
+      for (int j = 0; j < kLogitVec / 2; ++j) touched |= (w[j] & 0xffffu ? 1u << 2 * j : 0u) | (w[j] >> 16 ? 2u << 2 * j : 0u);
+    }
+    LogitVec<T> y = x;
+    if (touched | biased) {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j) {
+        if (!((touched | biased) >> j & 1u)) continue;  // value by value: few of a warp's 256 are touched
+        float l = logit_to_f32(x.v[j]);
+        if (biased >> j & 1u) l += s_bias[column(j) - lo];
+        if (touched >> j & 1u) {
+          const unsigned n = w[j >> 1] >> (16 * (j & 1)) & 0x7fffu;
+          l = l > 0.f ? l / repetition : l * repetition;
+          if (n) l -= presence + frequency * float(n);
+        }
+        y.v[j] = logit_from_f32<T>(l);
+      }
+    }
+    if (allow != 0xffu) {
+      const T fill = logit_from_f32<T>(a.fill);
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
+        if (!(allow >> j & 1u)) y.v[j] = fill;
     }
+    store(y);
   }
-  LogitVec<T> y = x;
-  if ((penalties && (w[0] | w[1] | w[2] | w[3])) || biased) {
-#pragma unroll
-    for (int j = 0; j < kLogitVec; ++j) {
-      float l = logit_to_f32(x.v[j]);
-      if (biased >> j & 1u) l += s_bias[column(j) - lo];
-      const unsigned word = w[j >> 1] >> (16 * (j & 1)) & 0xffffu, n = word & 0x7fffu;
-      if (penalties && word) l = l > 0.f ? l / repetition : l * repetition;
-      if (penalties && n) l -= presence + frequency * float(n);
-      y.v[j] = logit_from_f32<T>(l);
-    }
-  }
-  if (allow != 0xffu) {
-    const T fill = logit_from_f32<T>(a.fill);
-#pragma unroll
-    for (int j = 0; j < kLogitVec; ++j)
-      if (!(allow >> j & 1u)) y.v[j] = fill;
-  }
-  store(y);
 }
 
 // counts[row][token] of every (row, token): its top bit is set (prompt) or its lower 15 go up by one and stay at their largest value.
@@ -411,7 +435,7 @@ extern "C" int mfq_process_logits(const void* logits, void* out, int dtype, int 
   using namespace mfq;
   if (B <= 0 || B > 65535 || V <= 0 || R <= 0 || first < 0 || K < 0 || K > kMaxBias || dtype < 0 || dtype > 2) return -1;
   if (first > INT32_MAX - V || (allowed && (first + V + 31) / 32 > words)) return -1;
-  const LogitArgs a{logits, out, static_cast<const LogitRecord*>(records), static_cast<const unsigned short*>(counts), K ? bias_ids : nullptr, bias_values,
+  const LogitArgs a{logits, out, static_cast<const LogitRecord*>(records), static_cast<const unsigned short*>(counts), bias_ids, bias_values,
                     static_cast<const unsigned*>(allowed), rows, V, R, K, words, first, in_stride, out_stride, counts_stride, fill};
   const int size = dtype == 2 ? 4 : 2;
   const auto even = [](const void* p, long long stride, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * bytes % 16 == 0; };

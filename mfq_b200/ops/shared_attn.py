@@ -15,6 +15,7 @@ from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
 from .logits import _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
+_FORCED = None
 SMS = 148
 
 
@@ -96,12 +97,12 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
         with torch.cuda.device(index):
             return paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale=sm_scale, members=members, q_len=q_len,
                                             max_group=max_group, max_prefix=max_prefix, max_tail=max_tail, out=out)
-    tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
+    tile, prefix_splits, tail_splits = _FORCED or _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
     parts = n * hq * prefix_splits * (2 if tile == 128 else 1)
     scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)  # of this call: a workspace would tie streams and graphs together
     at = scratch.data_ptr()
     check(lib().mfq_paged_attn_decode_shared(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), group_starts.data_ptr(),
         prefix_lens.data_ptr(), ptr(members), out.data_ptr(), at, at + 4 * parts * d, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
-        sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_shared", 2)
+        sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_shared", 2 if prefix_splits else 1)
     return out
