@@ -17,266 +17,12 @@
 
 namespace mfq {
 
-template <int D, int WR>
-struct SharedTile {
-  static constexpr int kLanes = D == 256 && WR == 4 ? 2 : 4 / WR;  // groups of warps that take alternate pages
-  static constexpr int kThreads = 32 * WR * kLanes;
-  static constexpr int kStages = WR == 1 ? 3 : WR == 2 ? 4 : 8;
-  static constexpr int kPage = 16 * D, kStage = 2 * kPage + 128;
-  static constexpr int kRing = kLanes * kStages * kStage;
-  static constexpr int kSmem = kRing + 2 * kLanes * kStages * 8 + 16;
-  static_assert(kRing >= WR * kLanes * (16 * D + 32) * 4, "the ring is the merge's scratch too");
+template <int D>
+struct SharedRing {  // four warps take alternate pages, each through a ring of its own
+  static constexpr int kStages = 3, kPage = 16 * D, kStage = 2 * kPage + 128, kRing = 4 * kStages * kStage;
+  static constexpr int kSmem = kRing + 4 * kStages * 8 + 16;
+  static constexpr int kPart = 16 * D + 32;  // floats of a partial: [16 rows][D], then (m, l) of each row
 };
-
-// The prefixes of groups with few query rows: blockIdx.x = one of the groups' tiles of 16 WR rows, blockIdx.z = split.
-template <int D, int WR>
-__global__ void __launch_bounds__(SharedTile<D, WR>::kThreads, D <= 128 ? 3 : 1)
-shared_prefix_kernel(const SharedAttnArgs a) {
-  using L = SharedTile<D, WR>;
-  constexpr int KSTEPS = D / 16, NBD = D / 8, kStages = L::kStages, kLanes = L::kLanes;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
-  const int tile16 = warp % WR, page_lane = warp / WR;
-  uint8_t* ring = smem + page_lane * kStages * L::kStage;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + page_lane * kStages;
-  uint64_t* empty = reinterpret_cast<uint64_t*>(smem + L::kRing) + (kLanes + page_lane) * kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + 2 * kLanes * kStages * 8);
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0 && tile16 == 0) {
-    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], WR); }
-    mbar_fence_init();
-  }
-  __syncthreads();
-  pdl_wait();
-  pdl_trigger();  // behind the wait: the tails, which may start now, read what this kernel's predecessors wrote
-
-  const int kvh = blockIdx.y, G = a.Hq / a.Hk, per_seq = G * a.q_len, split = blockIdx.z;
-  int group, tile;
-  if (!find_tile(a, blockIdx.x, 16 * WR, per_seq, group, tile)) return;
-  const int first = min(max(a.group_starts[group], 0), a.B), rows = (min(max(a.group_starts[group + 1], first), a.B) - first) * per_seq;
-  const int table_row = member_row(a, first);
-  int page_lo = 0, page_hi = 0;
-  if (table_row >= 0) {
-    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
-    page_lo = min(split * per, n);
-    page_hi = min(n, page_lo + per);
-  }
-  const int my_pages = page_hi > page_lo + page_lane ? (page_hi - page_lo - page_lane + kLanes - 1) / kLanes : 0;
-  const int* bt = a.table + size_t(max(table_row, 0)) * a.max_pages;
-  bool ok = true;
-
-  auto issue = [&](int i) {  // one thread of the lane: start the copies of its i-th page
-    const int s = i % kStages;
-    int page = bt[page_lo + page_lane + kLanes * i];
-    if (page < 0 || page >= a.pages) {
-      atomicCAS(a.status, 0, kStatusBadArgument);
-      page = 0;
-    }
-    const size_t ph = size_t(page) * a.Hk + kvh;
-    uint8_t* st = ring + s * L::kStage;
-    mbar_expect_tx(&full[s], L::kStage);
-    shared_bulk_load(st, a.k + ph * L::kPage, L::kPage, &full[s]);
-    shared_bulk_load(st + L::kPage, a.v + ph * L::kPage, L::kPage, &full[s]);
-    shared_bulk_load(st + 2 * L::kPage, a.k_scale + ph * 16, 64, &full[s]);
-    shared_bulk_load(st + 2 * L::kPage + 64, a.v_scale + ph * 16, 64, &full[s]);
-  };
-  if (lane == 0 && tile16 == 0)
-    for (int i = 0; i < min(my_pages, kStages); ++i) issue(i);
-
-  // ---- this thread's two rows: their place, causal length and part of q ----
-  uint32_t qa[KSTEPS][4];
-  int row_len[2];
-  size_t hq[2];
-  bool live[2];
-  float to_log2[2];
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = (tile * WR + tile16) * 16 + g8 + 8 * half;
-    const int place = first + r / per_seq, in = r % per_seq, qr = in / G;
-    const int row = r < rows ? member_row(a, place) : -1;
-    live[half] = row >= 0;
-    hq[half] = live[half] ? (size_t(row) * a.q_len + qr) * a.Hq + kvh * G + in % G : 0;
-    // a row that is not there has a zero query and is never stored: unmasked, it leaves `whole` below to the others
-    row_len[half] = live[half] ? a.seq_lens[row] - (a.q_len - 1 - qr) : 0x7fffffff;
-    const __nv_bfloat16* qp = a.q + hq[half] * D;
-    float x[KSTEPS][4], top = 0.f;
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      const int d0 = 64 * (s >> 2) + 16 * c + 4 * (s & 3);
-      uint2 raw = make_uint2(0, 0);
-      if (live[half]) raw = *reinterpret_cast<const uint2*>(qp + d0);
-      const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[s][e] = __bfloat162float(b[e]);
-        top = fmaxf(top, fabsf(x[s][e]));
-      }
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float up = power_to(top, 13);
-    to_log2[half] = a.scale_log2 / up;
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      qa[s][half] = half_pair(x[s][0] * up, x[s][1] * up);
-      qa[s][2 + half] = half_pair(x[s][2] * up, x[s][3] * up);
-    }
-  }
-  const int low = __reduce_min_sync(0xffffffffu, min(row_len[0], row_len[1]));
-  int most = max(live[0] ? row_len[0] : 0, live[1] ? row_len[1] : 0);
-  most = __reduce_max_sync(0xffffffffu, most);
-
-  float o[NBD][4];
-#pragma unroll
-  for (int j = 0; j < NBD; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m_run[2] = {kSharedNeg, kSharedNeg}, l_run[2] = {0.f, 0.f};
-  float v_up = 0.f;  // power of two on the V multipliers; 0: none chosen yet
-
-  for (int i = 0; i < my_pages; ++i) {
-    const int s = i % kStages;
-    ok = mbar_wait(&full[s], (i / kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    const uint8_t *sK = ring + s * L::kStage, *sV = sK + L::kPage;
-    const float* sKs = reinterpret_cast<const float*>(sV + L::kPage);
-    const float* sVs = sKs + 16;
-    const int tok0 = (page_lo + page_lane + kLanes * i) << 4;
-    float sc[2][4];
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-#pragma unroll
-      for (int ch = 0; ch < D / 64; ++ch) {
-        const uint4 kw = *reinterpret_cast<const uint4*>(sK + ch * 1024 + (nb * 8 + g8) * 64 + c * 16);
-        const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
-#pragma unroll
-        for (int sub = 0; sub < 4; ++sub) mma_half(sc[nb], qa[ch * 4 + sub], e4m3_pair(w[sub]), e4m3_pair(w[sub] >> 16));
-      }
-    }
-    const bool whole = tok0 + 16 <= low;  // all rows see all of the page
-    float mx[2] = {kSharedNeg, kSharedNeg};
-    float2 vs[2];
-    bool raise = false;
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int tk = nb * 8 + 2 * c;
-      const float2 ks = *reinterpret_cast<const float2*>(sKs + tk);
-      vs[nb] = *reinterpret_cast<const float2*>(sVs + tk);
-      if (!whole) {  // what nobody sees may hold anything
-        if (tok0 + tk >= most) vs[nb].x = 0.f;
-        if (tok0 + tk + 1 >= most) vs[nb].y = 0.f;
-      }
-      const float big = fmaxf(fabsf(vs[nb].x), fabsf(vs[nb].y));
-      raise |= big * v_up > 1024.f || (v_up == 0.f && big > 0.f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int half = e >> 1;
-        sc[nb][e] *= ((e & 1) ? ks.y : ks.x) * to_log2[half];
-        if (!whole && tok0 + tk + (e & 1) >= row_len[half]) sc[nb][e] = kSharedNeg;
-        mx[half] = fmaxf(mx[half], sc[nb][e]);
-      }
-    }
-    float corr[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-      mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-      const float mn = fmaxf(m_run[half], mx[half]);
-      corr[half] = exp2f(m_run[half] - mn);
-      m_run[half] = mn;
-    }
-    float o_corr[2] = {corr[0], corr[1]};
-    if (__any_sync(0xffffffffu, raise)) {
-      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(vs[0].x), fabsf(vs[0].y)), fmaxf(fabsf(vs[1].x), fabsf(vs[1].y))))));
-      const float up = power_to(top, 4);
-      if (v_up != 0.f) { o_corr[0] *= up / v_up; o_corr[1] *= up / v_up; }
-      v_up = up;
-    }
-    float psum[2] = {0.f, 0.f}, p[2][4];
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int half = e >> 1;
-        // a masked score is kSharedNeg: exp2 gives 0 unless the whole row is still empty, hence the test (true for NaN)
-        const float pe = !(sc[nb][e] <= 0.5f * kSharedNeg) ? exp2f(sc[nb][e] - m_run[half]) : 0.f;
-        psum[half] += pe;
-        p[nb][e] = pe * (((e & 1) ? vs[nb].y : vs[nb].x) * v_up);
-      }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) l_run[half] = l_run[half] * corr[half] + psum[half];
-    const uint32_t pa[4] = {half_pair(p[0][0], p[0][1]), half_pair(p[0][2], p[0][3]), half_pair(p[1][0], p[1][1]), half_pair(p[1][2], p[1][3])};
-    if (__any_sync(0xffffffffu, o_corr[0] != 1.f || o_corr[1] != 1.f)) {
-#pragma unroll
-      for (int j = 0; j < NBD; ++j) { o[j][0] *= o_corr[0]; o[j][1] *= o_corr[0]; o[j][2] *= o_corr[1]; o[j][3] *= o_corr[1]; }
-    }
-    // codes of tokens that no row sees are left out: 0 times a NaN would be one
-    uint32_t keep = 0xffffffffu;
-    if (!whole) {
-      keep = 0u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (tok0 + 2 * c + (e & 1) + 8 * (e >> 1) < most) keep |= 0xffu << (8 * e);
-    }
-#pragma unroll
-    for (int j = 0; j < NBD; ++j) {
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(sV + (8 * j + g8) * 16 + 4 * c) & keep;
-      mma_half(o[j], pa, e4m3_pair(vw), e4m3_pair(vw >> 16));
-    }
-    __syncwarp();
-    if constexpr (WR == 1) {
-      if (lane == 0 && i + kStages < my_pages) issue(i + kStages);
-    } else {
-      if (lane == 0) mbar_arrive(&empty[s]);
-      if (tile16 == 0 && lane == 0 && i >= 1 && i - 1 + kStages < my_pages) {  // the stage of the page before: its other readers are done by now, or nearly
-        const int e = (i - 1) % kStages;
-        if (mbar_wait(&empty[e], ((i - 1) / kStages) & 1, abort_flag, a.status, kStatusTimeoutProducer)) issue(i - 1 + kStages);
-      }
-      __syncwarp();
-    }
-  }
-  // ---- merge: the lanes of a row, then the warps that took other pages of it ----
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    l_run[half] += __shfl_xor_sync(0xffffffffu, l_run[half], 1);
-    l_run[half] += __shfl_xor_sync(0xffffffffu, l_run[half], 2);
-  }
-  __syncthreads();
-  float* w_o = reinterpret_cast<float*>(smem) + warp * (16 * D + 32);  // [16][D], then (m, l) of each row
-  const float down = v_up != 0.f ? 1.f / v_up : 0.f;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = g8 + 8 * half;
-#pragma unroll
-    for (int j = 0; j < NBD; ++j)
-      *reinterpret_cast<float2*>(w_o + r * D + 8 * j + 2 * c) = make_float2(o[j][2 * half] * down, o[j][2 * half + 1] * down);
-    if (c == 0) { w_o[16 * D + 2 * r] = m_run[half]; w_o[16 * D + 2 * r + 1] = l_run[half]; }
-  }
-  __syncthreads();
-  if (!ok || *abort_flag) return;
-  for (int idx = threadIdx.x; idx < 16 * WR * D; idx += L::kThreads) {
-    const int t = idx / (16 * D), r = idx / D % 16, d = idx % D;
-    const int global = (tile * WR + t) * 16 + r;
-    if (global >= rows) continue;
-    const int row = member_row(a, first + global / per_seq), in = global % per_seq;
-    if (row < 0) continue;
-    const float* base = reinterpret_cast<const float*>(smem) + t * (16 * D + 32);
-    float mm = kSharedNeg, ll = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kLanes; ++w) mm = fmaxf(mm, base[w * WR * (16 * D + 32) + 16 * D + 2 * r]);
-#pragma unroll
-    for (int w = 0; w < kLanes; ++w) {
-      const float* wo = base + w * WR * (16 * D + 32);
-      const float cw = exp2f(wo[16 * D + 2 * r] - mm);
-      ll += wo[16 * D + 2 * r + 1] * cw;
-      acc += wo[r * D + d] * cw;
-    }
-    const size_t part = ((size_t(row) * a.q_len + in / G) * a.Hq + kvh * G + in % G) * a.slots + split;
-    a.part_o[part * D + d] = acc;
-    if (d == 0) { a.part_ml[2 * part] = mm; a.part_ml[2 * part + 1] = ll; }
-  }
-}
 
 __device__ __forceinline__ uint32_t transposed_pairs(uint32_t v) {
   uint32_t r;
@@ -294,30 +40,31 @@ __device__ __forceinline__ float2 load_peer2(uint32_t addr) {
   return v;
 }
 
-// What a warp has of a tail: the running maximum and sum of its rows and their outputs, in one of two forms.
+// What a warp has of a unit: the running maximum and sum of its rows and their outputs, in one of two forms.
 //   wide   (up to 16 query rows): rows are the rows of the products, lane parts (g8, c) of m16n8k16 fragments
 //   narrow (up to 8): the page's 16 tokens are the rows and the query rows the columns, S^T = K Q^T and O^T += V^T P, which halves the
 //          products and the softmax (attn_decode.cu); a lane has the columns 2c and 2c + 1, of tokens (dims) g8 and g8 + 8
 template <int D, bool kNarrow>
-struct TailRows {
+struct UnitRows {
   static constexpr int kSteps = D / 16, kOut = kNarrow ? D / 16 : D / 8, kQ = kNarrow ? 2 : 4;
   uint32_t q[kSteps][kQ];
   float o[kOut][4], m[2], l[2], to_log2[2], v_up;
   int len[2], low, most;
 
-  // a row of the unit as this lane loads it: r = g8 (narrow), g8 + 8 half (wide)
-  __device__ __forceinline__ void load(const SharedAttnArgs& a, int row, int kvh, int G, int rows, int seq_len, int g8, int c) {
+  // row_of(r): where row r's q is, in rows of D (negative: there is none); len_of(r): the keys that it sees
+  template <typename RowOf, typename LenOf>
+  __device__ __forceinline__ void load(const SharedAttnArgs& a, RowOf row_of, LenOf len_of, int g8, int c) {
     float up[2];
 #pragma unroll
     for (int half = 0; half < (kNarrow ? 1 : 2); ++half) {
-      const int r = g8 + 8 * half;
-      const __nv_bfloat16* qp = a.q + ((size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G) * D;
+      const long long row = row_of(g8 + 8 * half);
+      const __nv_bfloat16* qp = a.q + row * D;
       uint2 raw[kSteps];
       float top = 0.f;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         raw[s] = make_uint2(0, 0);
-        if (r < rows) raw[s] = *reinterpret_cast<const uint2*>(qp + 64 * (s >> 2) + 16 * c + 4 * (s & 3));
+        if (row >= 0) raw[s] = *reinterpret_cast<const uint2*>(qp + 64 * (s >> 2) + 16 * c + 4 * (s & 3));
         const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[s]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(__bfloat162float(b[e])));
@@ -337,11 +84,12 @@ struct TailRows {
     for (int e = 0; e < 2; ++e) {
       const int r = kNarrow ? 2 * c + e : g8 + 8 * e;
       const float of = kNarrow ? __shfl_sync(0xffffffffu, up[0], r * 4) : up[e];
+      const bool there = row_of(r) >= 0;
       to_log2[e] = a.scale_log2 / of;
       // a row that is not there has a zero query and is never stored: unmasked, it leaves `whole` below to the others
-      len[e] = r < rows ? seq_len - (a.q_len - 1 - r / G) : 0x7fffffff;
+      len[e] = there ? len_of(r) : 0x7fffffff;
       lo = min(lo, len[e]);
-      hi = max(hi, r < rows ? len[e] : 0);
+      hi = max(hi, there ? len[e] : 0);
       m[e] = kSharedNeg;
       l[e] = 0.f;
     }
@@ -526,42 +274,17 @@ struct TailRows {
   }
 };
 
-constexpr int kMostSlots = 64, kMostRanks = 8;
-
-// The tails (without prefix splits: whole sequences, each through its own table), and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
-// are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own part done.
-template <int D, bool kNarrow>
-__global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
-shared_tail_kernel(const SharedAttnArgs a) {
-  using L = SharedTile<D, 1>;
-  constexpr int kStages = L::kStages, kPart = 16 * D + 32;  // floats of a partial
-  static_assert(L::kRing >= (5 * kPart + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the ring is the merge's scratch too");
-  extern __shared__ __align__(128) uint8_t smem[];
+// The pages page_lo .. page_hi - 1 of a table row by four warps in turn, through their rings (barriers initialised), into one part at `mine`
+// (shared memory; all of it behind a block barrier).  `load` fills a UnitRows; what it reads is requested behind the first pages.
+template <int D, bool kNarrow, typename Load>
+__device__ __forceinline__ void unit_part(const SharedAttnArgs& a, uint8_t* smem, const int* bt, int kvh, int page_lo, int page_hi, int rows, float* mine, Load load) {
+  using L = SharedRing<D>;
+  constexpr int kStages = L::kStages, kPart = L::kPart;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * kStages * L::kStage;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + warp * kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + 2 * L::kLanes * kStages * 8);
-  pdl_trigger();
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
-    mbar_fence_init();
-  }
-  __syncthreads();
-  if (a.prefix_splits == 0) pdl_wait();  // no prefixes' kernel has waited for what is read here
-  const int place = blockIdx.x, kvh = blockIdx.y, ranks = gridDim.z, rank = blockIdx.z;
-  const int G = a.Hq / a.Hk, rows = G * a.q_len;
-  const int group = group_of(a, place);
-  const int row = group < a.groups && place >= a.group_starts[0] ? member_row(a, place) : -1;
-  if (row < 0) {  // the whole cluster alike
-    pdl_wait();  // this grid ends behind the prefixes' in any case
-    return;
-  }
-  const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0, seq_len = a.seq_lens[row];
-  const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
-  const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + 4 * kStages * 8);
   const int my_pages = page_hi > page_lo + warp ? (page_hi - page_lo - warp + 3) / 4 : 0;
-  const int* bt = a.table + size_t(row) * a.max_pages;
   int next = lane == 0 && my_pages > 0 ? bt[page_lo + warp] : 0;
   const auto issue = [&](int i) {  // lane 0: start the copies of this warp's i-th page; its id was fetched a page ahead
     const int s = i % kStages;
@@ -581,8 +304,8 @@ shared_tail_kernel(const SharedAttnArgs a) {
   };
   if (lane == 0)
     for (int i = 0; i < min(my_pages, kStages); ++i) issue(i);
-  TailRows<D, kNarrow> t;
-  t.load(a, row, kvh, G, rows, seq_len, g8, c);
+  UnitRows<D, kNarrow> t;
+  load(t, g8, c);
   for (int i = 0; i < my_pages; ++i) {
     const int s = i % kStages;
     if (!mbar_wait_warp(&full[s], (i / kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) break;
@@ -590,9 +313,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
     __syncwarp();
     if (lane == 0 && i + kStages < my_pages) issue(i + kStages);
   }
-  // ---- the warps' parts to one, in shared memory ----
-  float* parts = reinterpret_cast<float*>(smem);
-  float *mine = parts + 4 * kPart, *weights = mine + kPart, *inverse = weights + 16 * (kMostSlots + kMostRanks);
+  float* parts = reinterpret_cast<float*>(smem);  // the rings have been read
   __syncthreads();
   t.put(parts + warp * kPart, g8, c);
   __syncthreads();
@@ -612,13 +333,101 @@ shared_tail_kernel(const SharedAttnArgs a) {
     *reinterpret_cast<float4*>(mine + r * D + d) = acc;
     if (d == 0) *reinterpret_cast<float2*>(mine + 16 * D + 2 * r) = make_float2(mm, ll);
   }
+}
+template <int D>
+__device__ __forceinline__ void unit_barriers(uint8_t* smem) {
+  using L = SharedRing<D>;
+  if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(smem + L::kRing + 4 * L::kStages * 8) = 0;
+  if ((threadIdx.x & 31) == 0) {
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + (threadIdx.x >> 5) * L::kStages;
+    for (int s = 0; s < L::kStages; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+}
+
+// The prefixes of groups with few query rows: blockIdx.x = one of the groups' tiles of 16 query rows (8, narrow), blockIdx.z = split.
+template <int D, bool kNarrow>
+__global__ void __launch_bounds__(128, kNarrow ? 4 : 3)
+shared_prefix_kernel(const SharedAttnArgs a) {
+  using L = SharedRing<D>;
+  constexpr int kTile = kNarrow ? 8 : 16;
+  static_assert(L::kRing >= 5 * L::kPart * 4, "the rings are the merge's scratch too");
+  extern __shared__ __align__(128) uint8_t smem[];
+  unit_barriers<D>(smem);
+  pdl_wait();
+  pdl_trigger();  // behind the wait: the tails, which may start now, read what this kernel's predecessors wrote
+  const int kvh = blockIdx.y, G = a.Hq / a.Hk, per_seq = G * a.q_len, split = blockIdx.z;
+  int group, tile;
+  if (!find_tile(a, blockIdx.x, kTile, per_seq, group, tile)) return;
+  const int first = min(max(a.group_starts[group], 0), a.B), rows = (min(max(a.group_starts[group + 1], first), a.B) - first) * per_seq;
+  const int table_row = member_row(a, first);
+  int page_lo = 0, page_hi = 0;
+  if (table_row >= 0) {
+    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
+    page_lo = min(split * per, n);
+    page_hi = min(n, page_lo + per);
+  }
+  const auto row_of = [&](int r) -> long long {
+    const int i = tile * kTile + r, in = i % per_seq;
+    const int row = r < kTile && i < rows ? member_row(a, first + i / per_seq) : -1;
+    return row < 0 ? -1 : (static_cast<long long>(row) * a.q_len + in / G) * a.Hq + kvh * G + in % G;
+  };
+  const auto len_of = [&](int r) {
+    const int i = tile * kTile + r;
+    return a.seq_lens[member_row(a, first + i / per_seq)] - (a.q_len - 1 - i % per_seq / G);
+  };
+  float* mine = reinterpret_cast<float*>(smem) + 4 * L::kPart;
+  unit_part<D, kNarrow>(a, smem, a.table + size_t(max(table_row, 0)) * a.max_pages, kvh, page_lo, page_hi, kTile, mine,
+                        [&](UnitRows<D, kNarrow>& t, int g8, int c) { t.load(a, row_of, len_of, g8, c); });
+  __syncthreads();
+  for (int i = threadIdx.x; i < kTile * (D / 4); i += 128) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    const long long row = row_of(r);
+    if (row < 0) continue;
+    const size_t part = row * a.slots + split;
+    *reinterpret_cast<float4*>(a.part_o + part * D + d) = *reinterpret_cast<const float4*>(mine + r * D + d);
+    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = *reinterpret_cast<const float2*>(mine + 16 * D + 2 * r);
+  }
+}
+
+constexpr int kMostSlots = 64, kMostRanks = 8;
+
+// The tails (without prefix splits: whole sequences, each through its own table), and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
+// are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own part done.
+template <int D, bool kNarrow>
+__global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
+shared_tail_kernel(const SharedAttnArgs a) {
+  using L = SharedRing<D>;
+  static_assert(L::kRing >= (5 * L::kPart + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the rings are the merge's scratch too");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  unit_barriers<D>(smem);
+  if (a.prefix_splits == 0) pdl_wait();  // no prefixes' kernel has waited for what is read here
+  const int place = blockIdx.x, kvh = blockIdx.y, ranks = gridDim.z, rank = blockIdx.z;
+  const int G = a.Hq / a.Hk, rows = G * a.q_len;
+  const int group = group_of(a, place);
+  const int row = group < a.groups && place >= a.group_starts[0] ? member_row(a, place) : -1;
+  if (row < 0) {  // the whole cluster alike
+    pdl_wait();  // this grid ends behind the prefixes' in any case
+    return;
+  }
+  const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0, seq_len = a.seq_lens[row];
+  const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
+  const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
+  float *mine = reinterpret_cast<float*>(smem) + 4 * L::kPart, *weights = mine + L::kPart, *inverse = weights + 16 * (kMostSlots + kMostRanks);
+  const auto row_of = [&](int r) -> long long { return r < rows ? (static_cast<long long>(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G : -1; };
+  const auto len_of = [&](int r) { return seq_len - (a.q_len - 1 - r / G); };
+  unit_part<D, kNarrow>(a, smem, a.table + size_t(row) * a.max_pages, kvh, page_lo, page_hi, rows, mine,
+                        [&](UnitRows<D, kNarrow>& t, int g8, int c) { t.load(a, row_of, len_of, g8, c); });
   if (ranks > 1) cluster_sync_all();
   else __syncthreads();
   pdl_wait();  // the prefixes' partials
   // ---- weights of the ranks' parts and of the prefix's, a warp to a row ----
   const int entries = ranks + a.slots;
   for (int r = warp; r < rows; r += 4) {
-    const size_t hq = (size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G;
+    const size_t hq = row_of(r);
     float2 ml[(kMostSlots + kMostRanks + 31) / 32];
     float mm = kSharedNeg, sum = 0.f;
 #pragma unroll
@@ -645,7 +454,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
   __syncthreads();
   for (int i = rank * 128 + threadIdx.x; i < rows * (D / 4); i += ranks * 128) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
-    const size_t hq = (size_t(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G;
+    const size_t hq = row_of(r);
     const float* by = weights + r * (kMostSlots + kMostRanks);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const auto add = [&](const float4& v, float w) {
@@ -674,20 +483,20 @@ static bool set_smem(K kernel, int bytes, bool (&done)[64]) {
   if (!done[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
   return done[dev] = true;
 }
-template <int D, int WR>
+template <int D, bool kNarrow>
 static int launch_shared_prefix(const SharedAttnArgs& a, cudaStream_t stream) {
   static bool done[64] = {};
-  if (!set_smem(shared_prefix_kernel<D, WR>, SharedTile<D, WR>::kSmem, done)) return -6;
-  launch_kernel(shared_prefix_kernel<D, WR>, dim3(tiles_at_most(a, 16 * WR), a.Hk, a.prefix_splits), dim3(SharedTile<D, WR>::kThreads), SharedTile<D, WR>::kSmem, stream, a);
+  if (!set_smem(shared_prefix_kernel<D, kNarrow>, SharedRing<D>::kSmem, done)) return -6;
+  launch_kernel(shared_prefix_kernel<D, kNarrow>, dim3(tiles_at_most(a, kNarrow ? 8 : 16), a.Hk, a.prefix_splits), dim3(128), SharedRing<D>::kSmem, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 template <int D, bool kNarrow>
 static int launch_shared_tail(const SharedAttnArgs& a, cudaStream_t stream) {
   static bool done[64] = {};
-  if (!set_smem(shared_tail_kernel<D, kNarrow>, SharedTile<D, 1>::kSmem, done)) return -6;
+  if (!set_smem(shared_tail_kernel<D, kNarrow>, SharedRing<D>::kSmem, done)) return -6;
   const dim3 grid(a.B, a.Hk, a.tail_splits);
-  if (a.tail_splits > 1) launch_kernel_clustered(shared_tail_kernel<D, kNarrow>, grid, dim3(128), dim3(1, 1, a.tail_splits), SharedTile<D, 1>::kSmem, stream, a);
-  else launch_kernel(shared_tail_kernel<D, kNarrow>, grid, dim3(128), SharedTile<D, 1>::kSmem, stream, a);
+  if (a.tail_splits > 1) launch_kernel_clustered(shared_tail_kernel<D, kNarrow>, grid, dim3(128), dim3(1, 1, a.tail_splits), SharedRing<D>::kSmem, stream, a);
+  else launch_kernel(shared_tail_kernel<D, kNarrow>, grid, dim3(128), SharedRing<D>::kSmem, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 
@@ -695,11 +504,11 @@ int launch_shared_prefix_tc(const SharedAttnArgs& a, int dim, bool two_tiles, cu
 
 template <int D>
 static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream) {
-  const int rc = !a.prefix_splits ? 0
-                 : tile == 16   ? launch_shared_prefix<D, 1>(a, stream)
-                 : tile == 32 ? launch_shared_prefix<D, 2>(a, stream)
-                 : tile == 64 ? launch_shared_prefix<D, 4>(a, stream)
-                              : launch_shared_prefix_tc(a, D, tile == 256, stream);
+  int rc = 0;
+  if constexpr (D <= 128) {
+    if (a.prefix_splits)
+      rc = tile == 8 ? launch_shared_prefix<D, true>(a, stream) : tile == 16 ? launch_shared_prefix<D, false>(a, stream) : launch_shared_prefix_tc(a, D, tile == 256, stream);
+  }
   if (rc) return rc;
   return (a.Hq / a.Hk) * a.q_len <= 8 ? launch_shared_tail<D, true>(a, stream) : launch_shared_tail<D, false>(a, stream);
 }
@@ -707,14 +516,15 @@ static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream)
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16; pages of the FP8 pool, `pages` of them; group_starts [groups + 1], prefix_lens [groups], members [B] or null; tile: query rows of a
-// prefix CTA, 16, 32, 64 or for heads of 64 and 128 also 128, 256; partials [B * q_len * Hq * prefix_splits (twice
-// that for a tile of 128; 64 at most)] x D and x 2 floats; tail_splits: 8 at most.  (Hq / Hk) * q_len <= 16.  Rows in no group are not written.
+// prefix CTA, 8, 16, 128 or 256; partials [B * q_len * Hq * prefix_splits (twice
+// that for a tile of 128; 64 at most)] x D and x 2 floats; prefix_splits: 0 has every
+// sequence read whole through its own table (heads of 256: always); tail_splits: 8 at most.  (Hq / Hk) * q_len <= 16.  Rows in no group are not written.
 extern "C" int mfq_paged_attn_decode_shared(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* table,
                                             const int* seq_lens, const int* group_starts, const int* prefix_lens, const int* members, void* out,
                                             float* part_o, float* part_ml, int B, int Hq, int Hk, int D, int max_pages, int pages, int groups, int q_len,
                                             int tile, int prefix_splits, int tail_splits, float sm_scale, int* status, cudaStream_t stream) {
   using namespace mfq;
-  if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (tile != 16 && tile != 32 && tile != 64 && (D > 128 || (tile != 128 && tile != 256))) || prefix_splits < 0 ||
+  if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (prefix_splits && (D > 128 || (tile != 8 && tile != 16 && tile != 128 && tile != 256))) || prefix_splits < 0 ||
       tail_splits < 1 || pages < 1 || max_pages < 1 || Hk > 65535 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits > kMostRanks)
     return -1;
   const SharedAttnArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_scale, v_scale, table, seq_lens,

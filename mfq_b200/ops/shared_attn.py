@@ -15,35 +15,49 @@ from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
 from .logits import _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
-_FORCED = None
 SMS = 148
-
-
-def _pick_tile(rows: int, d: int) -> int:
-    """Query rows of a prefix CTA for groups of ``rows`` query rows a KV head: 16, 32, 64 on mma.sync, 128 and 256 on tcgen05."""
-    for tile in (16, 32, 64):
-        if rows <= tile:
-            return tile
-    return 64 if d > 128 else 128 if rows <= 128 else 256
 
 
 @lru_cache(maxsize=4096)
 def _shape(b: int, per_seq: int, hk: int, d: int, groups: int, width: int, max_group: int | None, max_prefix: int | None, max_tail: int | None) -> tuple[int, int, int]:
-    """(query rows of a prefix CTA, splits of a prefix, splits of a tail) for ``b`` sequences of ``per_seq`` query rows a KV head."""
-    max_group = b if max_group is None else max(1, min(b, max_group))
+    """(query rows of a prefix CTA, splits of a prefix, splits of a sequence's own pages) for ``b`` sequences of ``per_seq`` query rows a KV head: the form
+    that a few numbers fitted to sweeps on a B200 (1 and 4 groups of 2 to 64 rows, prefixes of 256 to 32768 tokens, heads of 64 and 128) say is
+    fastest, in microseconds.  0 splits of a prefix: every sequence is read whole, which is one kernel, and all that heads of 256 have."""
+    group = b if max_group is None else max(1, min(b, max_group))
     whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
     tail = width if max_tail is None else min(width, max(0, max_tail) // 16 + 1)
-    tile = _pick_tile(max_group * per_seq, d)
-    units = -(-max_group * per_seq // tile) * hk * groups
-    if tile >= 128:  # one CTA an SM, blocks of eight pages: no more splits than give each of them whole blocks
-        blocks = max(1, -(-whole // 8))
-        most = max(1, min(SMS // units, blocks, 32))
-        prefix = -(-blocks // -(-blocks // most))
-    else:
-        prefix = max(1, min(SMS * (3 if d <= 128 else 1) // units, whole // 4, 32))
-    # a tail's splits share its pages and the reading of the prefix's partials
-    tails = max(1, min(SMS * (4 if d <= 128 else 2) // (b * hk), -(-(tail + prefix) // 8), 8))
-    return tile, prefix, tails
+    rows, per_sm = group * per_seq, 4 if d <= 128 else 2
+    slow = (1.0 if per_seq <= 8 else 1.6) * (1.0 if d <= 128 else 2.0)  # a page, by one warp
+    bandwidth = 6.0e6 / (16 * (2 * d + 8))  # pages of a head, from memory
+
+    def ranks(pages: int, least: int) -> int:  # CTAs that share a sequence: a power of two, which fills the grid better than others
+        n = 1
+        while n < 8 and 2 * n * b * hk <= SMS * per_sm and n * least < pages:
+            n *= 2
+        return n
+
+    def own_pages(pages: int, r: int) -> float:
+        return max(pages / (4 * r) * slow * (1.4 if b * hk * r > SMS else 1.0), b * hk * pages / bandwidth)
+
+    r = ranks(whole + tail, 8)
+    best = (5 + own_pages(whole + tail, r), 16, 0, r)
+    if d > 128 or whole == 0 or group == 1:
+        return best[1:]
+    for tile in ((8 if rows <= 8 else 16,) if rows <= 32 else ()) + (((128,) if rows <= 128 else (256,)) if rows > 8 else ()):
+        units = -(-rows // tile) * hk * groups
+        if tile >= 128:  # one CTA an SM, blocks of eight pages: no more splits than give each of them whole blocks
+            blocks = -(-whole // 8)
+            splits = -(-blocks // -(-blocks // max(1, min(SMS // units, blocks, 32))))
+            each = (2.4 if tile == 128 else 3.6) * -(-blocks // splits) + 7
+            t = each * max(1.0, units * splits / SMS)
+        else:
+            splits = max(1, min(SMS * 3 // units, -(-whole // 8), 32))
+            t = (5 if tile == 8 else 8) + max(-(-whole // (4 * splits)) * (1.0 if tile == 8 else 1.4), units * whole / bandwidth) * max(1.0, units * splits / (SMS * 3))
+        slots = splits * (2 if tile == 128 else 1)
+        r = max(ranks(tail, 32), ranks(-(-per_seq * d // 512) * -(-slots // 8), 8))  # pages of its own, and rounds of reading partials
+        t += 3 + own_pages(tail, r) + b * per_seq * hk * slots * d / 1.0e6 + 0.4 * -(-slots // 8)
+        best = min(best, (t, tile, splits, r))
+    return best[1:]
 
 
 def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, group_starts: torch.Tensor,
@@ -56,8 +70,9 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     * ``members [B]`` int32: batch rows in the order of the groups (default ``0 .. B - 1``);
     * ``group_starts [n + 1]`` int32, ascending: group ``g`` has the rows ``members[group_starts[g] : group_starts[g + 1]]``; rows behind
       the last group are left as ``out`` has them;
-    * ``prefix_lens [n]`` int32: the leading tokens whose pages the group's rows share.  Whole pages of them are read through the first
-      row's table, the rest through each row's own; 0 shares nothing.
+    * ``prefix_lens [n]`` int32: the leading tokens whose pages the group's rows share: their tables name the same pages for them.  Whole pages of
+      them are read through the table of the group's first row, or through each row's own where sharing would take longer, the rest through each row's
+      own; 0 shares nothing.
 
     All of that may change on the device between replays of a graph.  ``max_group`` (rows of a group), ``max_prefix`` and ``max_tail`` (tokens):
     what the host knows of them; they choose the shape of the launches, a wrong one costs time."""
@@ -97,7 +112,7 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
         with torch.cuda.device(index):
             return paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale=sm_scale, members=members, q_len=q_len,
                                             max_group=max_group, max_prefix=max_prefix, max_tail=max_tail, out=out)
-    tile, prefix_splits, tail_splits = _FORCED or _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
+    tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
     parts = n * hq * prefix_splits * (2 if tile == 128 else 1)
     scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)  # of this call: a workspace would tie streams and graphs together
     at = scratch.data_ptr()
