@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from mfq_b200 import ops
+from mfq_b200.ops import shared_attn
 from gpu_common import assert_close, check_status, require_gpu_lib
 from shared_attn_cases import BATCHES, assert_attends, batch, call, exact
 
@@ -29,6 +30,36 @@ def test_against_the_definition(groups, how):
     assert torch.equal(one, run(s, want)), "the same inputs, the same bits"
     run(s, want, max_group=1, max_prefix=10 ** 6, max_tail=10 ** 6)  # wrong in each direction: only slower
     run(s, want, max_group=max(len(n) for _, n in groups), max_prefix=max(p for p, _ in groups), max_tail=0)
+
+
+FORMS = [(16, 0, 1), (16, 0, 8), (8, 1, 2), (8, 5, 1), (16, 1, 1), (16, 7, 4), (128, 1, 1), (128, 3, 2), (128, 32, 8), (256, 1, 4), (256, 5, 1), (256, 64, 3)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("groups,how", [x for x in BATCHES if x[1].get("d", 128) <= 128])
+def test_every_form_takes_every_batch(groups, how, form, monkeypatch):
+    """The forms (query rows of a prefix CTA, splits of a prefix, CTAs of a tail) differ in time alone."""
+    require_gpu_lib()
+    monkeypatch.setattr(shared_attn, "_shape", lambda *a: form)
+    s = batch(len(groups), groups, device="cuda", **how)
+    want = exact(s)
+    one = run(s, want)
+    assert torch.equal(one, run(s, want)), "the same inputs, the same bits"
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_every_form_with_large_and_small_rows(form, monkeypatch):
+    """Rows of q from 2^-60 to 2^4, scores that differ by thousands, multipliers of V from 2^-30 to 2^30."""
+    require_gpu_lib()
+    monkeypatch.setattr(shared_attn, "_shape", lambda *a: form)
+    s = batch(3, [(600, [700, 640, 620, 900, 610, 601])], device="cuda")
+    s.q *= torch.exp2(torch.linspace(-60, 4, s.q.shape[0] * s.q.shape[1], device="cuda").round()).view(*s.q.shape[:2], 1).to(torch.bfloat16)
+    run(s, exact(s))
+    s = batch(4, [(1200, [1300, 1240, 1220, 1500])], v_spread=2.0 ** 30, device="cuda")
+    run(s, exact(s))
+    s = batch(5, [(600, [700, 640, 620, 900])], q_std=2.0 ** 60, device="cuda")
+    s.scale *= 2.0 ** -60
+    run(s, exact(s))
 
 
 @pytest.mark.parametrize("hq,hk,d,q_len", [(32, 8, 128, 1), (16, 8, 64, 1), (32, 8, 128, 4), (16, 2, 256, 2), (8, 8, 128, 1), (16, 1, 128, 1), (40, 8, 128, 1), (14, 2, 64, 2)])
