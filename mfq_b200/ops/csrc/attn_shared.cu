@@ -15,6 +15,8 @@
 #include "attn_shared.cuh"
 #include "pair.cuh"
 
+#include <initializer_list>
+
 namespace mfq {
 
 template <int D>
@@ -393,8 +395,9 @@ shared_prefix_kernel(const SharedAttnArgs a) {
 
 constexpr int kMostSlots = 64, kMostRanks = 8;
 
-// The tails (without prefix splits: whole sequences, each through its own table), and what comes of them and of the prefixes' partials: blockIdx.x = place, blockIdx.z = split of its pages; the splits of a place
-// are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own part done.
+// The tails (without prefix splits: whole sequences, each through its own table), and what comes of them and of the prefixes' partials: blockIdx.x = place,
+// blockIdx.z = split of its pages; the splits of a place are one cluster.  Starts beside the prefixes (behind their wait) and waits for them with its own
+// part done.
 template <int D, bool kNarrow>
 __global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
 shared_tail_kernel(const SharedAttnArgs a) {
@@ -410,6 +413,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
   const int group = group_of(a, place);
   const int row = group < a.groups && place >= a.group_starts[0] ? member_row(a, place) : -1;
   if (row < 0) {  // the whole cluster alike
+    if (group < a.groups && place >= a.group_starts[0] && threadIdx.x == 0) atomicCAS(a.status, 0, kStatusBadArgument);  // a member that is no row
     pdl_wait();  // this grid ends behind the prefixes' in any case
     return;
   }
@@ -516,17 +520,20 @@ static int launch_shared(const SharedAttnArgs& a, int tile, cudaStream_t stream)
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16; pages of the FP8 pool, `pages` of them; group_starts [groups + 1], prefix_lens [groups], members [B] or null; tile: query rows of a
-// prefix CTA, 8, 16, 128 or 256; partials [B * q_len * Hq * prefix_splits (twice
-// that for a tile of 128; 64 at most)] x D and x 2 floats; prefix_splits: 0 has every
-// sequence read whole through its own table (heads of 256: always); tail_splits: 8 at most.  (Hq / Hk) * q_len <= 16.  Rows in no group are not written.
+// prefix CTA, 8, 16, 128 or 256; partials [B * q_len * Hq * slots] x D and x 2 floats, slots = prefix_splits (twice that for a tile of 128), 64 at most;
+// prefix_splits: 0 has every sequence read whole through its own table (heads of 256: always); tail_splits: 8 at most.  (Hq / Hk) * q_len <= 16.
+// q, out, pages and multipliers lie on 16 bytes.  Rows in no group are not written.
 extern "C" int mfq_paged_attn_decode_shared(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* table,
                                             const int* seq_lens, const int* group_starts, const int* prefix_lens, const int* members, void* out,
                                             float* part_o, float* part_ml, int B, int Hq, int Hk, int D, int max_pages, int pages, int groups, int q_len,
                                             int tile, int prefix_splits, int tail_splits, float sm_scale, int* status, cudaStream_t stream) {
   using namespace mfq;
-  if (B <= 0 || B > 65535 || Hk <= 0 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || (prefix_splits && (D > 128 || (tile != 8 && tile != 16 && tile != 128 && tile != 256))) || prefix_splits < 0 ||
-      tail_splits < 1 || pages < 1 || max_pages < 1 || Hk > 65535 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits > kMostRanks)
+  if (B <= 0 || B > 65535 || Hk <= 0 || Hk > 65535 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || pages < 1 || max_pages < 1)
     return -1;
+  if (prefix_splits < 0 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits < 1 || tail_splits > kMostRanks) return -1;
+  if (prefix_splits && (D > 128 || (tile != 8 && tile != 16 && tile != 128 && tile != 256))) return -1;
+  for (const void* p : {q, k, v, static_cast<const void*>(k_scale), static_cast<const void*>(v_scale), static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return -1;
   const SharedAttnArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_scale, v_scale, table, seq_lens,
                          group_starts, prefix_lens, members, part_o, part_ml, static_cast<__nv_bfloat16*>(out), status, B, Hq, Hk, max_pages, pages, groups,
                          q_len, prefix_splits * (tile == 128 ? 2 : 1), prefix_splits, tail_splits, sm_scale * 1.4426950408889634f};

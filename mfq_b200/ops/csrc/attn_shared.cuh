@@ -86,8 +86,6 @@ __device__ __forceinline__ int member_row(const SharedAttnArgs& a, int place) { 
   const int row = a.members ? a.members[place] : place;
   return row >= 0 && row < a.B ? row : -1;
 }
-
-
 // A group of n rows has (n - 1) / per_tile + 1 tiles, so that g groups of n in all have at most this, whatever the groups are.
 inline int tiles_at_most(const SharedAttnArgs& a, int per_tile) {
   const int rows = a.B * (a.Hq / a.Hk) * a.q_len;

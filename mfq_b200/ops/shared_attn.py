@@ -67,14 +67,17 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     """``q [B * q_len, Hq, D]`` (bf16) against the paged FP8 cache ``kv`` (a :class:`LayerKV`), ``D`` 64, 128 or 256 and at most 16 query heads
     times ``q_len`` to a KV head; ``block_table [B, P]`` and ``seq_lens [B]`` int32 as for ``paged_attn_decode`` (the lengths count the query tokens too).
 
-    * ``members [B]`` int32: batch rows in the order of the groups (default ``0 .. B - 1``);
+    * ``members [B]`` int32: batch rows in the order of the groups, each once (default ``0 .. B - 1``);
     * ``group_starts [n + 1]`` int32, ascending: group ``g`` has the rows ``members[group_starts[g] : group_starts[g + 1]]``; rows behind
       the last group are left as ``out`` has them;
     * ``prefix_lens [n]`` int32: the leading tokens whose pages the group's rows share: their tables name the same pages for them.  Whole pages of
       them are read through the table of the group's first row, or through each row's own where sharing would take longer, the rest through each row's
       own; 0 shares nothing.
 
-    All of that may change on the device between replays of a graph.  ``max_group`` (rows of a group), ``max_prefix`` and ``max_tail`` (tokens):
+    Multipliers of the pages are not negative; ``q``, ``out``, the pages and their multipliers begin on 16 bytes.  A page or a member out of range
+    is reported by ``Workspace.check``.
+
+    All of the indices may change on the device between replays of a graph.  ``max_group`` (rows of a group), ``max_prefix`` and ``max_tail`` (tokens):
     what the host knows of them; they choose the shape of the launches, a wrong one costs time."""
     if q.ndim != 3 or q.dtype is not torch.bfloat16 or not q.is_contiguous() or q.shape[2] not in HEAD_DIMS or q_len < 1 or q.shape[0] % q_len:
         _refuse("q", f"contiguous bf16 [B * {q_len}, Hq, 64 | 128 | 256] are", q)
@@ -101,6 +104,9 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
         _refuse("out", f"contiguous bf16 {tuple(q.shape)} on the device of q is", out)
+    wide = [t.data_ptr() for t in (q, k, v, kv.k_scale, kv.v_scale, out)]
+    if (wide[0] | wide[1] | wide[2] | wide[3] | wide[4] | wide[5]) & 15:
+        raise ValueError("q, out, the pages and their multipliers have to begin on 16 bytes")
     if b == 0 or groups == 0:
         return out
     if groups > b:
@@ -117,7 +123,6 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)  # of this call: a workspace would tie streams and graphs together
     at = scratch.data_ptr()
     check(lib().mfq_paged_attn_decode_shared(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), group_starts.data_ptr(),
-        prefix_lens.data_ptr(), ptr(members), out.data_ptr(), at, at + 4 * parts * d, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
+        *wide[:5], block_table.data_ptr(), seq_lens.data_ptr(), group_starts.data_ptr(), prefix_lens.data_ptr(), ptr(members), wide[5], at, at + 4 * parts * d, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
         sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_shared", 2 if prefix_splits else 1)
     return out

@@ -148,6 +148,19 @@ def test_a_page_outside_the_pool_is_reported():
         check_status()
 
 
+@pytest.mark.parametrize("form", [(16, 0, 1), (8, 1, 2), (128, 1, 1), (256, 1, 1)])
+def test_a_member_that_is_no_row_is_reported(form, monkeypatch):
+    """Kernels leave such a place out (and read nothing through it)."""
+    require_gpu_lib()
+    monkeypatch.setattr(shared_attn, "_shape", lambda *a: form)
+    for bad in (-1, 3):
+        s = batch(2, [(64, [80, 90, 70])], device="cuda")
+        s.members[1] = bad
+        call(ops, s)
+        with pytest.raises(RuntimeError, match="status code 5"):
+            check_status()
+
+
 def test_equals_the_attention_of_unshared_rows():
     require_gpu_lib()
     s = batch(9, [(1000, [1100 + 9 * i for i in range(20)])], hq=32, hk=8, device="cuda")

@@ -50,3 +50,23 @@ def test_no_groups():
     s.starts, s.prefixes = s.starts[:1].contiguous(), s.prefixes[:0].contiguous()
     out = torch.full_like(s.q, 3.0)
     assert (call(ops, s, out=out) == 3).all()
+
+
+@pytest.mark.parametrize("name", ["q", "out", "k", "v", "k_scale", "v_scale"])
+def test_tensors_that_begin_between_16_bytes_are_refused(name):
+    """The kernels read and write them 16 bytes at a time; a slice of a buffer may begin anywhere."""
+    s = batch(1, [(16, [20, 30])])
+    out = torch.zeros_like(s.q)
+
+    def shifted(t):
+        buffer = torch.zeros(t.numel() + 16, dtype=t.dtype)
+        part = buffer[4 // t.element_size():][:t.numel()].view(t.shape)
+        assert part.data_ptr() % 16 == 4
+        return part.copy_(t)
+
+    if name == "q":
+        s.q = shifted(s.q)
+    elif name != "out":
+        setattr(s.kv, name, shifted(getattr(s.kv, name)))
+    with pytest.raises(ValueError, match="16 bytes"):
+        call(ops, s, out=shifted(out) if name == "out" else out)
