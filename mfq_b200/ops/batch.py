@@ -58,7 +58,7 @@ def plan_batch(block_table: torch.Tensor, rows: torch.Tensor, past: torch.Tensor
     _index("counts", counts, b, index)
     if not 1 <= b <= MAX_REQUESTS:
         raise ValueError(f"a plan takes 1 to {MAX_REQUESTS} requests, got {b}")
-    if tokens < 0 or page_size < 1 or p * page_size > 2 ** 31 - 1:
+    if not 0 <= tokens <= 1 << 30 or page_size < 1 or p * page_size > 2 ** 31 - 1:
         raise ValueError(f"{tokens} tokens, rows of {p} pages of {page_size}")
     if pages is not None:
         _index("pages", pages, None, index)

@@ -19,11 +19,11 @@ namespace mfq {
 //   out = allowed[r] bit v ? round(l) : fill     (chosen, not added: a masked NaN or infinity is gone)
 // All of it in fp32, rounded once to the logits' type.
 
-struct LogitRecord {  // the 32 bytes a row's sampler reads
+struct LogitRecord {  // the 32 bytes a row's sampler reads; on 4 bytes, whatever the sampler wants
   float temperature;
   int top_k;
   float top_p, presence, frequency, repetition;
-  unsigned long long seed;
+  unsigned seed[2];
 };
 
 struct LogitArgs {
@@ -59,8 +59,8 @@ struct alignas(16) LogitVec {
 // A thread has eight values: eight neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16 bytes), else eight that lie a block
 // apart, so that a warp's accesses are whole lines at any alignment.  Logits, counts and mask are requested together, ahead of the record that says
 // whether the row needs the counts.  Where none of a thread's eight tokens has a count or a bias their bits stay as they are, and only the mask chooses:
-// with the arithmetic (a division among it) for all of them, 64 x 128256 bf16 with all three on a B200 took 18.9 us, bound by instructions, now KKK; four
-// sets of eight a thread took as long as one.
+// with the arithmetic (a division among it) for all of them, 64 x 128256 bf16 with all three on a B200 took 18.9 us, bound by instructions, and takes 14.4
+// (7.7 for its bytes at the rate of a copy); four sets of eight a thread took as long as one.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kLogitThreads, 5)
 process_logits_kernel(const LogitArgs a) {
@@ -82,13 +82,11 @@ process_logits_kernel(const LogitArgs a) {
   const bool whole = kVec && column(kLogitVec - 1) < hi;
 
   LogitVec<T> x;
-  {
-    if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
-    else {
+  if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
+  else {
 #pragma unroll
-      for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) x.v[j] = in[column(j)];
-    }
+    for (int j = 0; j < kLogitVec; ++j)
+      if (column(j) < hi) x.v[j] = in[column(j)];
   }
   const auto store = [&](const LogitVec<T>& y) {
     if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
@@ -107,32 +105,27 @@ process_logits_kernel(const LogitArgs a) {
   const float* values = a.bias_values + size_t(r) * a.K;
   int id = tid < a.K ? ids[tid] : -1;  // this thread's first place, requested with the rest
   unsigned w[kLogitVec / 2];  // eight words of counts
-  {
 #pragma unroll
-    for (int j = 0; j < kLogitVec / 2; ++j) w[j] = 0;
-    const unsigned short* row = a.counts + r * a.counts_stride;
-    if (!a.counts) {
-    } else if (whole) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(row + column(0));
-      w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
-    } else {
+  for (int j = 0; j < kLogitVec / 2; ++j) w[j] = 0;
+  const unsigned short* count_row = a.counts + r * a.counts_stride;
+  if (!a.counts) {
+  } else if (whole) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(count_row + column(0));
+    w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
+  } else {
 #pragma unroll
-      for (int j = 0; j < kLogitVec; ++j) w[j >> 1] |= (column(j) < hi ? unsigned(row[column(j)]) : 0u) << (16 * (j & 1));
-    }
+    for (int j = 0; j < kLogitVec; ++j) w[j >> 1] |= (column(j) < hi ? unsigned(count_row[column(j)]) : 0u) << (16 * (j & 1));
   }
-  unsigned allow;  // bit j: value j
-  {
-    allow = 0xffu;
-    const unsigned* words = a.allowed + size_t(r) * a.words;
-    if (!a.allowed) {
-    } else if (whole && a.first % 8 == 0) {
-      allow = reinterpret_cast<const unsigned char*>(words)[(a.first + column(0)) >> 3];
-    } else {
+  unsigned allow = 0xffu;  // bit j: value j
+  const unsigned* words = a.allowed + size_t(r) * a.words;
+  if (!a.allowed) {
+  } else if (whole && a.first % 8 == 0) {
+    allow = reinterpret_cast<const unsigned char*>(words)[(a.first + column(0)) >> 3];
+  } else {
 #pragma unroll
-      for (int j = 0; j < kLogitVec; ++j) {
-        const int of = a.first + column(j);
-        if (column(j) < hi && !(words[of >> 5] >> (of & 31) & 1u)) allow &= ~(1u << j);
-      }
+    for (int j = 0; j < kLogitVec; ++j) {
+      const int of = a.first + column(j);
+      if (column(j) < hi && !(words[of >> 5] >> (of & 31) & 1u)) allow &= ~(1u << j);
     }
   }
   const float presence = a.records[r].presence, frequency = a.records[r].frequency, repetition = a.records[r].repetition;
@@ -186,44 +179,42 @@ process_logits_kernel(const LogitArgs a) {
     }
     if (hits) __syncthreads();
   }
-  {
-    unsigned touched = 0, biased = 0;  // bit j: value j
-    if (hits) {
-      if (kVec) {
-        if (column(0) < hi) biased = reinterpret_cast<const unsigned char*>(s_biased)[(column(0) - lo) >> 3];
-      } else {
-#pragma unroll
-        for (int j = 0; j < kLogitVec; ++j)
-          if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
-      }
-    }
-    if (penalties) {
-#pragma unroll
-      for (int j = 0; j < kLogitVec / 2; ++j) touched |= (w[j] & 0xffffu ? 1u << 2 * j : 0u) | (w[j] >> 16 ? 2u << 2 * j : 0u);
-    }
-    LogitVec<T> y = x;
-    if (touched | biased) {
-#pragma unroll
-      for (int j = 0; j < kLogitVec; ++j) {
-        if (!((touched | biased) >> j & 1u)) continue;  // value by value: few of a warp's 256 are touched
-        float l = logit_to_f32(x.v[j]);
-        if (biased >> j & 1u) l += s_bias[column(j) - lo];
-        if (touched >> j & 1u) {
-          const unsigned n = w[j >> 1] >> (16 * (j & 1)) & 0x7fffu;
-          l = l > 0.f ? l / repetition : l * repetition;
-          if (n) l -= presence + frequency * float(n);
-        }
-        y.v[j] = logit_from_f32<T>(l);
-      }
-    }
-    if (allow != 0xffu) {
-      const T fill = logit_from_f32<T>(a.fill);
+  unsigned touched = 0, biased = 0;  // bit j: value j
+  if (hits) {
+    if (kVec) {
+      if (column(0) < hi) biased = reinterpret_cast<const unsigned char*>(s_biased)[(column(0) - lo) >> 3];
+    } else {
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j)
-        if (!(allow >> j & 1u)) y.v[j] = fill;
+        if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
     }
-    store(y);
   }
+  if (penalties) {
+#pragma unroll
+    for (int j = 0; j < kLogitVec / 2; ++j) touched |= (w[j] & 0xffffu ? 1u << 2 * j : 0u) | (w[j] >> 16 ? 2u << 2 * j : 0u);
+  }
+  LogitVec<T> y = x;
+  if (touched | biased) {
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j) {
+      if (!((touched | biased) >> j & 1u)) continue;  // value by value: few of a warp's 256 are touched
+      float l = logit_to_f32(x.v[j]);
+      if (biased >> j & 1u) l += s_bias[column(j) - lo];
+      if (touched >> j & 1u) {
+        const unsigned n = w[j >> 1] >> (16 * (j & 1)) & 0x7fffu;
+        l = l > 0.f ? l / repetition : l * repetition;
+        if (n) l -= presence + frequency * float(n);
+      }
+      y.v[j] = logit_from_f32<T>(l);
+    }
+  }
+  if (allow != 0xffu) {
+    const T fill = logit_from_f32<T>(a.fill);
+#pragma unroll
+    for (int j = 0; j < kLogitVec; ++j)
+      if (!(allow >> j & 1u)) y.v[j] = fill;
+  }
+  store(y);
 }
 
 // counts[row][token] of every (row, token): its top bit is set (prompt) or its lower 15 go up by one and stay at their largest value.
@@ -255,7 +246,7 @@ count_tokens_kernel(unsigned short* __restrict__ counts, long long stride, int R
 }
 // Many: the pairs of a block are added up in shared memory first (open addressing; twice as many places as pairs, so that one is always free), and
 // every different one goes to the table once.  The common tokens of a text then meet in a few blocks instead of in every warp: 32000 tokens of 24
-// rows took 32 us by warps on a B200, KKK by blocks.
+// rows and the processing of their logits took 42.6 us by warps on a B200, 25.5 by blocks.  Up to a block's worth, one block would be slower than warps on several SMs.
 constexpr int kCountThreads = 512, kCountPer = 2, kCountPlaces = 2 * kCountThreads * kCountPer;
 __global__ void __launch_bounds__(kCountThreads)
 count_many_kernel(unsigned short* __restrict__ counts, long long stride, int R, int V, const int* __restrict__ tokens, const int* __restrict__ rows, int T) {
@@ -434,7 +425,7 @@ extern "C" int mfq_process_logits(const void* logits, void* out, int dtype, int 
                                   int words, const int* rows, int first, float fill, cudaStream_t stream) {
   using namespace mfq;
   if (B <= 0 || B > 65535 || V <= 0 || R <= 0 || first < 0 || K < 0 || K > kMaxBias || dtype < 0 || dtype > 2) return -1;
-  if (first > INT32_MAX - V || (allowed && (first + V + 31) / 32 > words)) return -1;
+  if (V > 1 << 30 || first > INT32_MAX - V || (allowed && (first + V + 31) / 32 > words)) return -1;
   const LogitArgs a{logits, out, static_cast<const LogitRecord*>(records), static_cast<const unsigned short*>(counts), bias_ids, bias_values,
                     static_cast<const unsigned*>(allowed), rows, V, R, K, words, first, in_stride, out_stride, counts_stride, fill};
   const int size = dtype == 2 ? 4 : 2;
@@ -459,7 +450,7 @@ extern "C" int mfq_count_tokens(void* counts, long long stride, int R, int V, co
 extern "C" int mfq_plan_batch(int* table, int R, int P, const int* rows, const int* past, const int* counts, int b, const int* pages, int free_pages, int* positions,
                               int* slots, int* tok_seq, int T, int* q_starts, int* seq_lens, int* out_table, int* info, int page_size, cudaStream_t stream) {
   using namespace mfq;
-  if (R <= 0 || P <= 0 || b <= 0 || b > kPlanRequests || T < 0 || page_size <= 0 || (free_pages >= 0 && R > kPlanRows)) return -1;
+  if (R <= 0 || P <= 0 || b <= 0 || b > kPlanRequests || T < 0 || T > 1 << 30 || page_size <= 0 || (free_pages >= 0 && R > kPlanRows)) return -1;
   if (static_cast<long long>(P) * page_size > INT32_MAX) return -1;
   const PlanArgs a{table, rows, past, counts, pages, positions, slots, tok_seq, q_starts, seq_lens, out_table, info, R, P, b, T, page_size, free_pages};
   const long long work = T + static_cast<long long>(b) * P, per = 4 * kPlanThreads;

@@ -25,7 +25,8 @@ def _refuse(name: str, wanted: str, t: torch.Tensor) -> None:
 
 
 def _index(name: str, t: torch.Tensor, count: int | None, index: int) -> None:
-    if t.dtype is not torch.int32 or t.ndim != 1 or t.get_device() != index or not t.is_contiguous() or (count is not None and t.numel() != count):
+    n = t.numel()
+    if t.dtype is not torch.int32 or t.ndim != 1 or t.get_device() != index or not t.is_contiguous() or n != (min(n, 1 << 30) if count is None else count):
         _refuse(name, f"contiguous int32 [{'n' if count is None else count}] on the device of the others are", t)
 
 
@@ -55,8 +56,8 @@ def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch
         _index("rows", rows, b, index)
     elif b > r:
         raise ValueError(f"{b} rows of logits, but {r} records")
-    if not 0 <= first <= 2 ** 31 - 1 - v:
-        raise ValueError(f"first: {first}")
+    if v > 1 << 30 or not 0 <= first <= 2 ** 31 - 1 - v:
+        raise ValueError(f"{v} columns from token {first}")
     if counts is not None and (counts.dtype is not torch.int16 or counts.shape != (r, v) or counts.get_device() != index or (v > 1 and counts.stride(1) != 1)):
         _refuse("counts", f"int16 [{r}, {v}] with neighbouring columns on the logits' device are", counts)
     ids = values = None

@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from mfq_b200 import ops
-from gpu_common import require_gpu_lib
+from gpu_common import check_status, require_gpu_lib
 from serve_cases import LOGITS, PLANS, assert_logits, exact_counts, exact_logits, exact_plan, logits_case, plan_case, plan_parts, records, words
+from served_batch import serve
 from test_serve_ops_cpu import BAD_PLANS, spoilt_plan
 
 pytestmark = pytest.mark.gpu
@@ -41,6 +42,16 @@ def test_rows_of_nothing_and_unusual_values():
         want = exact_logits(logits, rec, counts, bias, mask, None, 0, -np.inf)
         assert_logits(got, *want, float("-inf"))
         assert (got[0] == -float("inf")).all()
+
+
+def test_records_that_begin_on_4_bytes():
+    require_gpu_lib()
+    args, table = logits_case(11, 3, 3, 5000, torch.bfloat16, mask=True, device="cuda")
+    buffer = torch.zeros(3 * 8 + 1, dtype=torch.int32, device="cuda")
+    part = buffer[1:].view(3, 8)
+    part.copy_(args["records"])
+    args["records"] = part
+    assert_logits(ops.process_logits(**args), *exact_logits(args["logits"], part, args["counts"], None, table, None, 0, -np.inf), float("-inf"))
 
 
 def test_process_logits_by_another_stream_in_a_graph_and_in_bands():
@@ -127,3 +138,9 @@ def test_plan_batch_in_a_graph():
         want, _ = exact_plan(table, rows, pasts, counts, **kw)
         for got, w in zip(plan_parts(plan), want):
             assert got.tolist() == w
+
+
+def test_a_served_batch_and_its_captured_step():
+    require_gpu_lib()
+    assert serve("cuda") == serve("cuda", graphed=True), "the same kernels on the same inputs"
+    check_status()

@@ -6,6 +6,7 @@ import torch
 
 from mfq_b200 import ops
 from serve_cases import LOGITS, PLANS, assert_logits, exact_counts, exact_logits, exact_plan, logits_case, plan_case, plan_parts, records, words
+from served_batch import serve
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -124,3 +125,14 @@ def test_empty_calls():
     assert not counts.any()
     plan = ops.plan_batch(torch.ones((1, 1), dtype=torch.int32), *[torch.zeros(1, dtype=torch.int32)] * 3, tokens=0)
     assert plan.check() == (0, 0) and not plan.block_table.any()
+
+
+def test_plans_of_too_many_places_are_refused():
+    """Places are counted in 32 bits on the device."""
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.plan_batch(torch.ones((1, 4), dtype=torch.int32), one, one, one, tokens=(1 << 30) + 1)
+
+
+def test_a_served_batch():
+    serve("cpu")
