@@ -23,7 +23,12 @@ template <int D>
 struct SharedRing {  // four warps take alternate pages, each through a ring of its own
   static constexpr int kStages = 3, kPage = 16 * D, kStage = 2 * kPage + 128, kRing = 4 * kStages * kStage;
   static constexpr int kSmem = kRing + 4 * kStages * 8 + 16;
-  static constexpr int kPart = 16 * D + 32;  // floats of a partial: [16 rows][D], then (m, l) of each row
+};
+// What the four warps of a unit have, in floats where the rings were: parts [16 rows][kStride], then (m, l) of each row.  The columns behind D bring the rows
+// of a fragment to different banks.  The first part becomes the unit's; its (m, l) are behind the four.
+template <int D, bool kNarrow>
+struct UnitParts {
+  static constexpr int kStride = D + (kNarrow ? 4 : 8), kPart = 16 * kStride + 32, kMl = 4 * kPart, kEnd = kMl + 32;
 };
 
 __device__ __forceinline__ uint32_t transposed_pairs(uint32_t v) {
@@ -56,18 +61,33 @@ struct UnitRows {
   // row_of(r): where row r's q is, in rows of D (negative: there is none); len_of(r): the keys that it sees
   template <typename RowOf, typename LenOf>
   __device__ __forceinline__ void load(const SharedAttnArgs& a, RowOf row_of, LenOf len_of, int g8, int c) {
-    float up[2];
+    constexpr int kHalves = kNarrow ? 1 : 2;
+    float up[kHalves];
+    uint2 raw[kHalves][kSteps];
 #pragma unroll
-    for (int half = 0; half < (kNarrow ? 1 : 2); ++half) {
+    for (int half = 0; half < kHalves; ++half) {  // all requested before the first is used
       const long long row = row_of(g8 + 8 * half);
       const __nv_bfloat16* qp = a.q + row * D;
-      uint2 raw[kSteps];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        raw[half][s] = make_uint2(0, 0);
+        if (row >= 0) raw[half][s] = *reinterpret_cast<const uint2*>(qp + 64 * (s >> 2) + 16 * c + 4 * (s & 3));
+      }
+    }
+    bool there[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = kNarrow ? 2 * c + e : g8 + 8 * e;
+      there[e] = row_of(r) >= 0;
+      // a row that is not there has a zero query and is never stored: unmasked, it leaves `whole` below to the others
+      len[e] = there[e] ? len_of(r) : 0x7fffffff;
+    }
+#pragma unroll
+    for (int half = 0; half < kHalves; ++half) {
       float top = 0.f;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        raw[s] = make_uint2(0, 0);
-        if (row >= 0) raw[s] = *reinterpret_cast<const uint2*>(qp + 64 * (s >> 2) + 16 * c + 4 * (s & 3));
-        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[s]);
+        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[half][s]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(__bfloat162float(b[e])));
       }
@@ -76,7 +96,7 @@ struct UnitRows {
       up[half] = power_to(top, 13);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[s]);
+        const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&raw[half][s]);
         q[s][half] = half_pair(__bfloat162float(b[0]) * up[half], __bfloat162float(b[1]) * up[half]);
         q[s][kNarrow ? 1 : 2 + half] = half_pair(__bfloat162float(b[2]) * up[half], __bfloat162float(b[3]) * up[half]);
       }
@@ -84,14 +104,10 @@ struct UnitRows {
     int lo = 0x7fffffff, hi = 0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = kNarrow ? 2 * c + e : g8 + 8 * e;
-      const float of = kNarrow ? __shfl_sync(0xffffffffu, up[0], r * 4) : up[e];
-      const bool there = row_of(r) >= 0;
+      const float of = kNarrow ? __shfl_sync(0xffffffffu, up[0], (2 * c + e) * 4) : up[e % kHalves];
       to_log2[e] = a.scale_log2 / of;
-      // a row that is not there has a zero query and is never stored: unmasked, it leaves `whole` below to the others
-      len[e] = there ? len_of(r) : 0x7fffffff;
       lo = min(lo, len[e]);
-      hi = max(hi, there ? len[e] : 0);
+      hi = max(hi, there[e] ? len[e] : 0);
       m[e] = kSharedNeg;
       l[e] = 0.f;
     }
@@ -250,8 +266,8 @@ struct UnitRows {
     }
   }
 
-  // [rows][D] outputs, then (m, l) of each row
   __device__ __forceinline__ void put(float* to, int g8, int c) {
+    constexpr int kStride = UnitParts<D, kNarrow>::kStride;
     const float down = v_up != 0.f ? 1.f / v_up : 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -262,26 +278,27 @@ struct UnitRows {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
 #pragma unroll
         for (int j = 0; j < kOut; ++j) {
-          to[r * D + 16 * j + g8] = o[j][e] * down;
-          to[r * D + 16 * j + 8 + g8] = o[j][2 + e] * down;
+          to[r * kStride + 16 * j + g8] = o[j][e] * down;
+          to[r * kStride + 16 * j + 8 + g8] = o[j][2 + e] * down;
         }
       } else {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
 #pragma unroll
-        for (int j = 0; j < kOut; ++j) *reinterpret_cast<float2*>(to + r * D + 8 * j + 2 * c) = make_float2(o[j][2 * e] * down, o[j][2 * e + 1] * down);
+        for (int j = 0; j < kOut; ++j) *reinterpret_cast<float2*>(to + r * kStride + 8 * j + 2 * c) = make_float2(o[j][2 * e] * down, o[j][2 * e + 1] * down);
       }
-      if ((kNarrow ? g8 : c) == 0) *reinterpret_cast<float2*>(to + 16 * D + 2 * r) = make_float2(m[e], l[e]);
+      if ((kNarrow ? g8 : c) == 0) *reinterpret_cast<float2*>(to + 16 * kStride + 2 * r) = make_float2(m[e], l[e]);
     }
   }
 };
 
-// The pages page_lo .. page_hi - 1 of a table row by four warps in turn, through their rings (barriers initialised), into one part at `mine`
-// (shared memory; all of it behind a block barrier).  `load` fills a UnitRows; what it reads is requested behind the first pages.
+// The pages page_lo .. page_hi - 1 of a table row by four warps in turn, through their rings (barriers initialised), into one part (UnitParts;
+// all of it behind a block barrier).  `load` fills a UnitRows; what it reads is requested behind the first pages.
 template <int D, bool kNarrow, typename Load>
-__device__ __forceinline__ void unit_part(const SharedAttnArgs& a, uint8_t* smem, const int* bt, int kvh, int page_lo, int page_hi, int rows, float* mine, Load load) {
+__device__ __forceinline__ void unit_part(const SharedAttnArgs& a, uint8_t* smem, const int* bt, int kvh, int page_lo, int page_hi, int rows, Load load) {
   using L = SharedRing<D>;
-  constexpr int kStages = L::kStages, kPart = L::kPart;
+  using P = UnitParts<D, kNarrow>;
+  constexpr int kStages = L::kStages, kPart = P::kPart;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * kStages * L::kStage;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing) + warp * kStages;
@@ -319,21 +336,26 @@ __device__ __forceinline__ void unit_part(const SharedAttnArgs& a, uint8_t* smem
   __syncthreads();
   t.put(parts + warp * kPart, g8, c);
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float mm = kSharedNeg, ll = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, parts[w * kPart + 16 * D + 2 * r]);
+  const int d = threadIdx.x % (D / 4) * 4;
+#pragma unroll 4
+  for (int r = threadIdx.x / (D / 4); r < rows; r += 512 / D) {
+    float2 ml[4];
+    float4 v[4], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float by = exp2f(parts[w * kPart + 16 * D + 2 * r] - mm);
-      const float4 v = *reinterpret_cast<const float4*>(parts + w * kPart + r * D + d);
-      ll += parts[w * kPart + 16 * D + 2 * r + 1] * by;
-      acc.x += v.x * by; acc.y += v.y * by; acc.z += v.z * by; acc.w += v.w * by;
+      ml[w] = *reinterpret_cast<const float2*>(parts + w * kPart + 16 * P::kStride + 2 * r);
+      v[w] = *reinterpret_cast<const float4*>(parts + w * kPart + r * P::kStride + d);
     }
-    *reinterpret_cast<float4*>(mine + r * D + d) = acc;
-    if (d == 0) *reinterpret_cast<float2*>(mine + 16 * D + 2 * r) = make_float2(mm, ll);
+    const float mm = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+    float ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = exp2f(ml[w].x - mm);
+      ll += ml[w].y * by;
+      acc.x += v[w].x * by; acc.y += v[w].y * by; acc.z += v[w].z * by; acc.w += v[w].w * by;
+    }
+    *reinterpret_cast<float4*>(parts + r * P::kStride + d) = acc;
+    if (d == 0) *reinterpret_cast<float2*>(parts + P::kMl + 2 * r) = make_float2(mm, ll);
   }
 }
 template <int D>
@@ -354,7 +376,8 @@ __global__ void __launch_bounds__(128, kNarrow ? 4 : 3)
 shared_prefix_kernel(const SharedAttnArgs a) {
   using L = SharedRing<D>;
   constexpr int kTile = kNarrow ? 8 : 16;
-  static_assert(L::kRing >= 5 * L::kPart * 4, "the rings are the merge's scratch too");
+  using P = UnitParts<D, kNarrow>;
+  static_assert(L::kRing >= P::kEnd * 4, "the rings are the merge's scratch too");
   extern __shared__ __align__(128) uint8_t smem[];
   unit_barriers<D>(smem);
   pdl_wait();
@@ -363,10 +386,10 @@ shared_prefix_kernel(const SharedAttnArgs a) {
   int group, tile;
   if (!find_tile(a, blockIdx.x, kTile, per_seq, group, tile)) return;
   const int first = min(max(a.group_starts[group], 0), a.B), rows = (min(max(a.group_starts[group + 1], first), a.B) - first) * per_seq;
-  const int table_row = member_row(a, first);
+  const int prefix = a.prefix_lens[group], table_row = member_row(a, first);  // (a group with a tile has a first row)
   int page_lo = 0, page_hi = 0;
   if (table_row >= 0) {
-    const int n = min(max(a.prefix_lens[group], 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
+    const int n = min(max(prefix, 0) >> 4, a.max_pages), per = (n + a.prefix_splits - 1) / a.prefix_splits;
     page_lo = min(split * per, n);
     page_hi = min(n, page_lo + per);
   }
@@ -379,8 +402,8 @@ shared_prefix_kernel(const SharedAttnArgs a) {
     const int i = tile * kTile + r;
     return a.seq_lens[member_row(a, first + i / per_seq)] - (a.q_len - 1 - i % per_seq / G);
   };
-  float* mine = reinterpret_cast<float*>(smem) + 4 * L::kPart;
-  unit_part<D, kNarrow>(a, smem, a.table + size_t(max(table_row, 0)) * a.max_pages, kvh, page_lo, page_hi, kTile, mine,
+  const float* mine = reinterpret_cast<const float*>(smem);
+  unit_part<D, kNarrow>(a, smem, a.table + size_t(max(table_row, 0)) * a.max_pages, kvh, page_lo, page_hi, kTile,
                         [&](UnitRows<D, kNarrow>& t, int g8, int c) { t.load(a, row_of, len_of, g8, c); });
   __syncthreads();
   for (int i = threadIdx.x; i < kTile * (D / 4); i += 128) {
@@ -388,8 +411,8 @@ shared_prefix_kernel(const SharedAttnArgs a) {
     const long long row = row_of(r);
     if (row < 0) continue;
     const size_t part = row * a.slots + split;
-    *reinterpret_cast<float4*>(a.part_o + part * D + d) = *reinterpret_cast<const float4*>(mine + r * D + d);
-    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = *reinterpret_cast<const float2*>(mine + 16 * D + 2 * r);
+    *reinterpret_cast<float4*>(a.part_o + part * D + d) = *reinterpret_cast<const float4*>(mine + r * P::kStride + d);
+    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = *reinterpret_cast<const float2*>(mine + P::kMl + 2 * r);
   }
 }
 
@@ -402,7 +425,8 @@ template <int D, bool kNarrow>
 __global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ? 2 : 1))
 shared_tail_kernel(const SharedAttnArgs a) {
   using L = SharedRing<D>;
-  static_assert(L::kRing >= (5 * L::kPart + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the rings are the merge's scratch too");
+  using P = UnitParts<D, kNarrow>;
+  static_assert(L::kRing >= (P::kEnd + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the rings are the merge's scratch too");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -410,50 +434,60 @@ shared_tail_kernel(const SharedAttnArgs a) {
   if (a.prefix_splits == 0) pdl_wait();  // no prefixes' kernel has waited for what is read here
   const int place = blockIdx.x, kvh = blockIdx.y, ranks = gridDim.z, rank = blockIdx.z;
   const int G = a.Hq / a.Hk, rows = G * a.q_len;
-  const int group = group_of(a, place);
-  const int row = group < a.groups && place >= a.group_starts[0] ? member_row(a, place) : -1;
-  if (row < 0) {  // the whole cluster alike
-    if (group < a.groups && place >= a.group_starts[0] && threadIdx.x == 0) atomicCAS(a.status, 0, kStatusBadArgument);  // a member that is no row
+  // requested side by side: the row and its length, the group and its prefix
+  const int row = member_row(a, place), seq_len = a.seq_lens[max(row, 0)], group = group_of(a, place), grouped_from = a.group_starts[0];
+  const bool grouped = group < a.groups && place >= grouped_from;
+  if (row < 0 || !grouped) {  // the whole cluster alike
+    if (grouped && threadIdx.x == 0) atomicCAS(a.status, 0, kStatusBadArgument);  // a member that is no row
     pdl_wait();  // this grid ends behind the prefixes' in any case
     return;
   }
-  const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0, seq_len = a.seq_lens[row];
+  const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0;
   const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
   const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
-  float *mine = reinterpret_cast<float*>(smem) + 4 * L::kPart, *weights = mine + L::kPart, *inverse = weights + 16 * (kMostSlots + kMostRanks);
+  float *mine = reinterpret_cast<float*>(smem), *weights = mine + P::kEnd, *inverse = weights + 16 * (kMostSlots + kMostRanks);
   const auto row_of = [&](int r) -> long long { return r < rows ? (static_cast<long long>(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G : -1; };
   const auto len_of = [&](int r) { return seq_len - (a.q_len - 1 - r / G); };
-  unit_part<D, kNarrow>(a, smem, a.table + size_t(row) * a.max_pages, kvh, page_lo, page_hi, rows, mine,
+  unit_part<D, kNarrow>(a, smem, a.table + size_t(row) * a.max_pages, kvh, page_lo, page_hi, rows,
                         [&](UnitRows<D, kNarrow>& t, int g8, int c) { t.load(a, row_of, len_of, g8, c); });
   if (ranks > 1) cluster_sync_all();
   else __syncthreads();
   pdl_wait();  // the prefixes' partials
   // ---- weights of the ranks' parts and of the prefix's, a warp to a row ----
   const int entries = ranks + a.slots;
-  for (int r = warp; r < rows; r += 4) {
-    const size_t hq = row_of(r);
-    float2 ml[(kMostSlots + kMostRanks + 31) / 32];
+  constexpr int kEntries = (kMostSlots + kMostRanks + 31) / 32, kRows = kNarrow ? 2 : 4;  // of a lane, of a warp: all requested before the first is used
+  float2 ml[kRows][kEntries];
+#pragma unroll
+  for (int y = 0; y < kRows; ++y) {
+    const int r = warp + 4 * y;
+#pragma unroll
+    for (int x = 0; x < kEntries; ++x) {
+      const int e = x * 32 + lane;
+      ml[y][x] = make_float2(kSharedNeg, 0.f);
+      if (r >= rows) {
+      } else if (e < ranks) ml[y][x] = load_peer2(map_to_cta(mine + P::kMl + 2 * r, e));
+      else if (e < entries) ml[y][x] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (size_t(row_of(r)) * a.slots + e - ranks));
+    }
+  }
+#pragma unroll
+  for (int y = 0; y < kRows; ++y) {
+    const int r = warp + 4 * y;
     float mm = kSharedNeg, sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < (kMostSlots + kMostRanks + 31) / 32; ++x) {
-      const int e = x * 32 + lane;
-      ml[x] = make_float2(kSharedNeg, 0.f);
-      if (e < ranks) ml[x] = load_peer2(map_to_cta(mine + 16 * D + 2 * r, e));
-      else if (e < entries) ml[x] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (hq * a.slots + e - ranks));
-      if (ml[x].y != 0.f) mm = fmaxf(mm, ml[x].x);
-    }
+    for (int x = 0; x < kEntries; ++x)
+      if (ml[y][x].y != 0.f) mm = fmaxf(mm, ml[y][x].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
 #pragma unroll
-    for (int x = 0; x < (kMostSlots + kMostRanks + 31) / 32; ++x) {
+    for (int x = 0; x < kEntries; ++x) {
       const int e = x * 32 + lane;
-      const float by = ml[x].y != 0.f ? exp2f(ml[x].x - mm) : 0.f;  // a part that saw nothing may hold anything
-      sum += ml[x].y * by;
-      if (e < entries) weights[r * (kMostSlots + kMostRanks) + e] = by;
+      const float by = ml[y][x].y != 0.f ? exp2f(ml[y][x].x - mm) : 0.f;  // a part that saw nothing may hold anything
+      sum += ml[y][x].y * by;
+      if (r < rows && e < entries) weights[r * (kMostSlots + kMostRanks) + e] = by;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) inverse[r] = sum != 0.f ? 1.f / sum : 0.f;
+    if (r < rows && lane == 0) inverse[r] = sum != 0.f ? 1.f / sum : 0.f;
   }
   __syncthreads();
   for (int i = rank * 128 + threadIdx.x; i < rows * (D / 4); i += ranks * 128) {
@@ -464,7 +498,13 @@ shared_tail_kernel(const SharedAttnArgs a) {
     const auto add = [&](const float4& v, float w) {
       if (w != 0.f) { acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w; }
     };
-    for (int e = 0; e < ranks; ++e) add(load_peer(map_to_cta(mine + r * D + d, e)), by[e]);
+    float4 theirs[kMostRanks];
+#pragma unroll
+    for (int e = 0; e < kMostRanks; ++e)
+      if (e < ranks) theirs[e] = load_peer(map_to_cta(mine + r * P::kStride + d, e));
+#pragma unroll
+    for (int e = 0; e < kMostRanks; ++e)
+      if (e < ranks) add(theirs[e], by[e]);
     const float4* src = reinterpret_cast<const float4*>(a.part_o + hq * a.slots * D + d);  // (no slots: not read)
     for (int e = 0; e < a.slots; e += 8) {  // eight requested before the first is used; behind the last one the last again, for nothing
       float4 v[8];
