@@ -426,9 +426,8 @@ __global__ void __launch_bounds__(128, D <= 128 ? (kNarrow ? 4 : 3) : (kNarrow ?
 shared_tail_kernel(const SharedAttnArgs a) {
   using L = SharedRing<D>;
   using P = UnitParts<D, kNarrow>;
-  static_assert(L::kRing >= (P::kEnd + 16 * (kMostSlots + kMostRanks) + 16) * 4, "the rings are the merge's scratch too");
+  static_assert(L::kRing >= (P::kEnd + 16 * (kMostRanks + kMostSlots) + 16) * 4, "the rings are the merge's scratch too");
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   unit_barriers<D>(smem);
   if (a.prefix_splits == 0) pdl_wait();  // no prefixes' kernel has waited for what is read here
@@ -445,7 +444,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
   const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0;
   const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
   const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
-  float *mine = reinterpret_cast<float*>(smem), *weights = mine + P::kEnd, *inverse = weights + 16 * (kMostSlots + kMostRanks);
+  float *mine = reinterpret_cast<float*>(smem), *weights = mine + P::kEnd, *inverse = weights + 16 * (kMostRanks + kMostSlots);
   const auto row_of = [&](int r) -> long long { return r < rows ? (static_cast<long long>(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G : -1; };
   const auto len_of = [&](int r) { return seq_len - (a.q_len - 1 - r / G); };
   unit_part<D, kNarrow>(a, smem, a.table + size_t(row) * a.max_pages, kvh, page_lo, page_hi, rows,
@@ -453,47 +452,41 @@ shared_tail_kernel(const SharedAttnArgs a) {
   if (ranks > 1) cluster_sync_all();
   else __syncthreads();
   pdl_wait();  // the prefixes' partials
-  // ---- weights of the ranks' parts and of the prefix's, a warp to a row ----
-  const int entries = ranks + a.slots;
-  constexpr int kEntries = (kMostSlots + kMostRanks + 31) / 32, kRows = kNarrow ? 2 : 4;  // of a lane, of a warp: all requested before the first is used
-  float2 ml[kRows][kEntries];
+  {  // weights of the ranks' parts and of the prefix's: eight threads to a row, all of its (m, l) requested before the first is used
+    const int r = threadIdx.x >> 3, e8 = threadIdx.x & 7;
+    constexpr int kEntries = 1 + kMostSlots / 8;  // a rank's, then slots'
+    static_assert(kMostRanks == 8 && kMostSlots % 8 == 0);
+    float2 ml[kEntries];
 #pragma unroll
-  for (int y = 0; y < kRows; ++y) {
-    const int r = warp + 4 * y;
+    for (int x = 0; x < kEntries; ++x) ml[x] = make_float2(kSharedNeg, 0.f);
+    if (r < rows) {
+      const float* prefix_ml = a.part_ml + 2 * (size_t(row_of(r)) * a.slots + e8);
+      if (e8 < ranks) ml[0] = load_peer2(map_to_cta(mine + P::kMl + 2 * r, e8));
 #pragma unroll
-    for (int x = 0; x < kEntries; ++x) {
-      const int e = x * 32 + lane;
-      ml[y][x] = make_float2(kSharedNeg, 0.f);
-      if (r >= rows) {
-      } else if (e < ranks) ml[y][x] = load_peer2(map_to_cta(mine + P::kMl + 2 * r, e));
-      else if (e < entries) ml[y][x] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (size_t(row_of(r)) * a.slots + e - ranks));
+      for (int x = 1; x < kEntries; ++x)
+        if (8 * (x - 1) + e8 < a.slots) ml[x] = *reinterpret_cast<const float2*>(prefix_ml + 16 * (x - 1));
     }
-  }
-#pragma unroll
-  for (int y = 0; y < kRows; ++y) {
-    const int r = warp + 4 * y;
     float mm = kSharedNeg, sum = 0.f;
 #pragma unroll
     for (int x = 0; x < kEntries; ++x)
-      if (ml[y][x].y != 0.f) mm = fmaxf(mm, ml[y][x].x);
+      if (ml[x].y != 0.f) mm = fmaxf(mm, ml[x].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    for (int o = 1; o < 8; o <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
 #pragma unroll
     for (int x = 0; x < kEntries; ++x) {
-      const int e = x * 32 + lane;
-      const float by = ml[y][x].y != 0.f ? exp2f(ml[y][x].x - mm) : 0.f;  // a part that saw nothing may hold anything
-      sum += ml[y][x].y * by;
-      if (r < rows && e < entries) weights[r * (kMostSlots + kMostRanks) + e] = by;
+      const float by = ml[x].y != 0.f ? exp2f(ml[x].x - mm) : 0.f;  // a part that saw nothing may hold anything
+      sum += ml[x].y * by;
+      if (r < rows && (x == 0 || 8 * (x - 1) + e8 < a.slots)) weights[r * (kMostRanks + kMostSlots) + 8 * x + e8] = by;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (r < rows && lane == 0) inverse[r] = sum != 0.f ? 1.f / sum : 0.f;
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (r < rows && e8 == 0) inverse[r] = sum != 0.f ? 1.f / sum : 0.f;
   }
   __syncthreads();
   for (int i = rank * 128 + threadIdx.x; i < rows * (D / 4); i += ranks * 128) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     const size_t hq = row_of(r);
-    const float* by = weights + r * (kMostSlots + kMostRanks);
+    const float* by = weights + r * (kMostRanks + kMostSlots);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const auto add = [&](const float4& v, float w) {
       if (w != 0.f) { acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w; }
@@ -511,7 +504,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
 #pragma unroll
       for (int x = 0; x < 8; ++x) v[x] = __ldcg(src + min(e + x, a.slots - 1) * (D / 4));
 #pragma unroll
-      for (int x = 0; x < 8; ++x) add(v[x], e + x < a.slots ? by[ranks + e + x] : 0.f);
+      for (int x = 0; x < 8; ++x) add(v[x], e + x < a.slots ? by[kMostRanks + e + x] : 0.f);
     }
     const float n = inverse[r];
     __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * n, acc.y * n), __floats2bfloat162_rn(acc.z * n, acc.w * n)};

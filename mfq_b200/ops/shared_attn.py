@@ -120,8 +120,8 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
                                             max_group=max_group, max_prefix=max_prefix, max_tail=max_tail, out=out)
     tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
     parts = n * hq * prefix_splits * (2 if tile == 128 else 1)
-    scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)  # of this call: a workspace would tie streams and graphs together
-    at = scratch.data_ptr()
+    scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device) if parts else None  # of this call: a workspace would tie streams and graphs together
+    at = scratch.data_ptr() if parts else 0
     check(lib().mfq_paged_attn_decode_shared(
         *wide[:5], block_table.data_ptr(), seq_lens.data_ptr(), group_starts.data_ptr(), prefix_lens.data_ptr(), ptr(members), wide[5], at, at + 4 * parts * d, b, hq, hk, d, width, pages, groups, q_len, tile, prefix_splits, tail_splits,
         sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_shared", 2 if prefix_splits else 1)
