@@ -40,7 +40,7 @@ struct LogitArgs {
   float fill;
 };
 
-constexpr int kLogitThreads = 256, kLogitVec = 8, kMaxBias = 1 << 16, kMostHits = 1024;
+constexpr int kLogitThreads = 256, kLogitVec = 8, kMaxBias = 1 << 16;
 
 template <typename T> __device__ __forceinline__ float logit_to_f32(T v);
 template <> __device__ __forceinline__ float logit_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -55,166 +55,160 @@ template <typename T>
 struct alignas(16) LogitVec {
   T v[kLogitVec];
 };
-
-// A thread has eight values: eight neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16 bytes), else eight that lie a block
-// apart, so that a warp's accesses are whole lines at any alignment.  Logits, counts and mask are requested together, ahead of the record that says
-// whether the row needs the counts.  Where none of a thread's eight tokens has a count or a bias their bits stay as they are, and only the mask chooses:
-// with the arithmetic (a division among it) for all of them, 64 x 128256 bf16 with all three on a B200 took 18.9 us, bound by instructions, and takes 14.4
-// (7.7 for its bytes at the rate of a copy); four sets of eight a thread took as long as one.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kLogitThreads, 5)
+// A warp has kSets times 256 neighbouring columns, a thread eight of each 256: neighbours in 16-byte accesses (kVec: every row of every tensor starts on 16
+// bytes), else eight that lie 32 apart, so that a warp's accesses are whole lines at any alignment.  Logits, counts, mask and the first ids of the biases
+// are requested together, ahead of the record that says whether the row needs the counts.  A warp goes over the row's biases by itself, in their order
+// (nothing waits for another warp): few are its own.  Where none of a thread's eight tokens has a count or a bias their bits stay as they are, and
+// only the mask chooses; few of a warp's 256 are others, and a warp passes over the arithmetic of the places where it has none.  Logits of 16 bits are
+// multiplied by the penalty's reciprocal, taken once: 2^-24 more of an error beside their own rounding of 2^-8 or 2^-11, for a division a value (1 x 32000: 2.4 us
+// with, 2.0 without).
+// 64 x 128256 bf16 with all three on a B200: 18.9 us with the arithmetic and a division for all values, 14.4 value by value behind block barriers that the
+// gathering of the biases needed, 11.4 now (7.7 for its bytes at the rate of a copy; without any of the three 5.1, from L2).  Choosing registers by the number of a touched
+// value, instead of passing over eight places, took 14.0.
+template <typename T, bool kVec, int kSets>
+__global__ void __launch_bounds__(kLogitThreads, kSets == 1 ? 5 : 4)
 process_logits_kernel(const LogitArgs a) {
-  constexpr int kChunk = kLogitThreads * kLogitVec;
+  constexpr int kMine = 256 * kSets, kAhead = 4;  // columns of a warp; ids of a lane that are requested together
   pdl_trigger();
-  __shared__ float s_bias[kChunk];
-  __shared__ int s_hit[kMostHits], s_id[kMostHits];  // places of the row whose ids are in the chunk, and those
-  __shared__ unsigned s_biased[kChunk / 32];   // bit: whether the column has a bias
-  __shared__ int s_hits;
-  if (threadIdx.x == 0) s_hits = 0;
-  if (threadIdx.x < kChunk / 32) s_biased[threadIdx.x] = 0u;
+  __shared__ float s_bias[kLogitThreads / 32][kMine];
+  __shared__ unsigned s_biased[kLogitThreads / 32][kMine / 32];  // bit: whether the column has a bias
+  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lo = (blockIdx.x * (kLogitThreads / 32) + warp) * kMine;
   pdl_wait();
-  const int b = blockIdx.y, tid = threadIdx.x, lo = blockIdx.x * kChunk, hi = min(a.V, lo + kChunk);
+  if (lo >= a.V) return;
   const int r = a.rows ? a.rows[b] : b;
   const bool known = r >= 0 && r < a.R;
   const T* in = static_cast<const T*>(a.logits) + b * a.in_stride;
   T* out = static_cast<T*>(a.out) + b * a.out_stride;
-  const auto column = [&](int j) { return lo + (kVec ? tid * kLogitVec + j : tid + j * kLogitThreads); };
-  const bool whole = kVec && column(kLogitVec - 1) < hi;
-
-  LogitVec<T> x;
-  if (whole) x = *reinterpret_cast<const LogitVec<T>*>(in + column(0));
-  else {
+  const auto column = [&](int s, int j) { return lo + s * 256 + (kVec ? lane * kLogitVec + j : lane + j * 32); };
+  const auto whole = [&](int s) { return kVec && column(s, kLogitVec - 1) < a.V; };
+  const bool inside = lo + kMine <= a.V;  // a warp's accesses value by value need no comparison
+  const auto each = [&](int s, auto&& f) {
+    if (inside) {
 #pragma unroll
-    for (int j = 0; j < kLogitVec; ++j)
-      if (column(j) < hi) x.v[j] = in[column(j)];
-  }
-  const auto store = [&](const LogitVec<T>& y) {
-    if (whole) *reinterpret_cast<LogitVec<T>*>(out + column(0)) = y;
-    else {
+      for (int j = 0; j < kLogitVec; ++j) f(j);
+    } else {
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) out[column(j)] = y.v[j];
+        if (column(s, j) < a.V) f(j);
     }
+  };
+
+  LogitVec<T> x[kSets];
+#pragma unroll
+  for (int s = 0; s < kSets; ++s) {
+    if (whole(s)) x[s] = *reinterpret_cast<const LogitVec<T>*>(in + column(s, 0));
+    else each(s, [&](int j) { x[s].v[j] = in[column(s, j)]; });
+  }
+  const auto store = [&](int s) {
+    if (whole(s)) *reinterpret_cast<LogitVec<T>*>(out + column(s, 0)) = x[s];
+    else each(s, [&](int j) { out[column(s, j)] = x[s].v[j]; });
   };
   if (!known) {
     if (in == out) return;
-    store(x);
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) store(s);
     return;
   }
   const int* ids = a.bias_ids + size_t(r) * a.K;  // (K is zero where there are none)
   const float* values = a.bias_values + size_t(r) * a.K;
-  int id = tid < a.K ? ids[tid] : -1;  // this thread's first place, requested with the rest
-  unsigned w[kLogitVec / 2];  // eight words of counts
+  int id[kAhead];
 #pragma unroll
-  for (int j = 0; j < kLogitVec / 2; ++j) w[j] = 0;
+  for (int q = 0; q < kAhead; ++q) id[q] = q * 32 + lane < a.K ? ids[q * 32 + lane] : -1;
+  unsigned w[kSets][kLogitVec / 2];  // eight words of counts
   const unsigned short* count_row = a.counts + r * a.counts_stride;
-  if (!a.counts) {
-  } else if (whole) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(count_row + column(0));
-    w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
-  } else {
 #pragma unroll
-    for (int j = 0; j < kLogitVec; ++j) w[j >> 1] |= (column(j) < hi ? unsigned(count_row[column(j)]) : 0u) << (16 * (j & 1));
+  for (int s = 0; s < kSets; ++s) {
+#pragma unroll
+    for (int j = 0; j < kLogitVec / 2; ++j) w[s][j] = 0;
+    if (!a.counts) {
+    } else if (whole(s)) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(count_row + column(s, 0));
+      w[s][0] = raw.x; w[s][1] = raw.y; w[s][2] = raw.z; w[s][3] = raw.w;
+    } else each(s, [&](int j) { w[s][j >> 1] |= unsigned(count_row[column(s, j)]) << (16 * (j & 1)); });
   }
-  unsigned allow = 0xffu;  // bit j: value j
+  unsigned allow[kSets];  // bit j: value j
   const unsigned* words = a.allowed + size_t(r) * a.words;
-  if (!a.allowed) {
-  } else if (whole && a.first % 8 == 0) {
-    allow = reinterpret_cast<const unsigned char*>(words)[(a.first + column(0)) >> 3];
-  } else {
 #pragma unroll
-    for (int j = 0; j < kLogitVec; ++j) {
-      const int of = a.first + column(j);
-      if (column(j) < hi && !(words[of >> 5] >> (of & 31) & 1u)) allow &= ~(1u << j);
-    }
+  for (int s = 0; s < kSets; ++s) {
+    allow[s] = 0xffu;
+    if (!a.allowed) {
+    } else if (whole(s) && a.first % 8 == 0) {
+      allow[s] = reinterpret_cast<const unsigned char*>(words)[(a.first + column(s, 0)) >> 3];
+    } else each(s, [&](int j) {
+      const int of = a.first + column(s, j);
+      if (!(words[of >> 5] >> (of & 31) & 1u)) allow[s] &= ~(1u << j);
+    });
   }
   const float presence = a.records[r].presence, frequency = a.records[r].frequency, repetition = a.records[r].repetition;
   const bool penalties = presence != 0.f || frequency != 0.f || repetition != 1.f;
-  int hits = 0;
-  // biases: those of this block's columns are gathered, then each id's are summed by one thread in the order of the row
-  if (a.K) {
-    __syncthreads();
-    for (int j = tid; j < a.K; j += kLogitThreads) {
-      if (j != tid) id = ids[j];
-      const int v = id - a.first;
-      if (id >= 0 && v >= lo && v < hi) {
-        const int at = atomicAdd(&s_hits, 1);
-        if (at < kMostHits) { s_hit[at] = j; s_id[at] = id; }
+  const float inverse = 1.f / repetition;
+  bool biases = false;  // whether a column of the warp has one
+  for (int k = 0; k < a.K; k += kAhead * 32) {
+    if (k > 0) {
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) id[q] = k + q * 32 + lane < a.K ? ids[k + q * 32 + lane] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int n = id[q] - a.first - lo;
+      const bool mine = id[q] >= 0 && n >= 0 && n < kMine;
+      unsigned left = __ballot_sync(0xffffffffu, mine);
+      if (!left) continue;
+      const float value = mine ? values[k + q * 32 + lane] : 0.f;
+      if (!biases) {
+        for (int i = lane; i < kMine / 32; i += 32) s_biased[warp][i] = 0u;
+        __syncwarp();
+        biases = true;
+      }
+      for (; left; left &= left - 1) {  // in the order of the row
+        const int from = __ffs(left) - 1;
+        if (lane == from) {
+          const unsigned had = s_biased[warp][n >> 5], bit = 1u << (n & 31);
+          s_bias[warp][n] = (had & bit ? s_bias[warp][n] : 0.f) + value;
+          s_biased[warp][n >> 5] = had | bit;
+        }
+        __syncwarp();
       }
     }
-    __syncthreads();
-    hits = s_hits;
-    if (hits > kMostHits) {  // each column goes through the whole row
-#pragma unroll 1
-      for (int n = tid; n < hi - lo; n += kLogitThreads) {
-        float sum = 0.f;
-        for (int j = 0; j < a.K; ++j)
-          if (ids[j] == a.first + lo + n) sum += values[j];
-        s_bias[n] = sum;
-        atomicOr(&s_biased[n >> 5], 1u << (n & 31));
-      }
-    } else {
-      for (int h = tid; h < hits; h += kLogitThreads) {
-        const int of = s_id[h], n = of - a.first - lo;
-        int same = 0, first = a.K;
-        for (int i = 0; i < hits; ++i)
-          if (s_id[i] == of) {
-            ++same;
-            first = min(first, s_hit[i]);
-          }
-        const bool mine = first == s_hit[h];
-        float sum = values[s_hit[h]];
-        for (int last = first; mine && same > 1; --same) {  // the next place of the same id
-          int next = a.K;
-          for (int i = 0; i < hits; ++i)
-            if (s_id[i] == of && s_hit[i] > last) next = min(next, s_hit[i]);
-          sum += values[next];
-          last = next;
-        }
-        if (mine) {
-          s_bias[n] = sum;
-          atomicOr(&s_biased[n >> 5], 1u << (n & 31));
-        }
-      }
-    }
-    if (hits) __syncthreads();
   }
-  unsigned touched = 0, biased = 0;  // bit j: value j
-  if (hits) {
-    if (kVec) {
-      if (column(0) < hi) biased = reinterpret_cast<const unsigned char*>(s_biased)[(column(0) - lo) >> 3];
-    } else {
+#pragma unroll
+  for (int s = 0; s < kSets; ++s) {
+    unsigned touched = 0, biased = 0;  // bit j: value j
+    if (biases) {
+      if (kVec) {
+        biased = reinterpret_cast<const unsigned char*>(s_biased[warp])[s * 32 + lane];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLogitVec; ++j) biased |= (s_biased[warp][s * 8 + j] >> lane & 1u) << j;
+      }
+    }
+    if (penalties && (w[s][0] | w[s][1] | w[s][2] | w[s][3])) {
+#pragma unroll
+      for (int j = 0; j < kLogitVec / 2; ++j) touched |= (w[s][j] & 0xffffu ? 1u << 2 * j : 0u) | (w[s][j] >> 16 ? 2u << 2 * j : 0u);
+    }
+    if (touched | biased) {
+#pragma unroll
+      for (int j = 0; j < kLogitVec; ++j) {
+        if (!((touched | biased) >> j & 1u)) continue;
+        float l = logit_to_f32(x[s].v[j]);
+        if (biased >> j & 1u) l += s_bias[warp][column(s, j) - lo];
+        if (touched >> j & 1u) {
+          const unsigned n = w[s][j >> 1] >> (16 * (j & 1)) & 0x7fffu;
+          if constexpr (sizeof(T) == 4) l = l > 0.f ? l / repetition : l * repetition;
+          else l *= l > 0.f ? inverse : repetition;
+          if (n) l -= presence + frequency * float(n);
+        }
+        x[s].v[j] = logit_from_f32<T>(l);
+      }
+    }
+    if (allow[s] != 0xffu) {
+      const T fill = logit_from_f32<T>(a.fill);
 #pragma unroll
       for (int j = 0; j < kLogitVec; ++j)
-        if (column(j) < hi) biased |= (s_biased[(column(j) - lo) >> 5] >> ((column(j) - lo) & 31) & 1u) << j;
+        if (!(allow[s] >> j & 1u)) x[s].v[j] = fill;
     }
+    store(s);
   }
-  if (penalties) {
-#pragma unroll
-    for (int j = 0; j < kLogitVec / 2; ++j) touched |= (w[j] & 0xffffu ? 1u << 2 * j : 0u) | (w[j] >> 16 ? 2u << 2 * j : 0u);
-  }
-  LogitVec<T> y = x;
-  if (touched | biased) {
-#pragma unroll
-    for (int j = 0; j < kLogitVec; ++j) {
-      if (!((touched | biased) >> j & 1u)) continue;  // value by value: few of a warp's 256 are touched
-      float l = logit_to_f32(x.v[j]);
-      if (biased >> j & 1u) l += s_bias[column(j) - lo];
-      if (touched >> j & 1u) {
-        const unsigned n = w[j >> 1] >> (16 * (j & 1)) & 0x7fffu;
-        l = l > 0.f ? l / repetition : l * repetition;
-        if (n) l -= presence + frequency * float(n);
-      }
-      y.v[j] = logit_from_f32<T>(l);
-    }
-  }
-  if (allow != 0xffu) {
-    const T fill = logit_from_f32<T>(a.fill);
-#pragma unroll
-    for (int j = 0; j < kLogitVec; ++j)
-      if (!(allow >> j & 1u)) y.v[j] = fill;
-  }
-  store(y);
 }
 
 // counts[row][token] of every (row, token): its top bit is set (prompt) or its lower 15 go up by one and stay at their largest value.
@@ -412,8 +406,14 @@ plan_batch_kernel(const PlanArgs a) {
 
 template <typename T>
 static int launch_logits(const LogitArgs& a, int B, bool vec, cudaStream_t stream) {
-  constexpr int kChunk = kLogitThreads * kLogitVec;
-  launch_kernel(vec ? process_logits_kernel<T, true> : process_logits_kernel<T, false>, dim3((a.V + kChunk - 1) / kChunk, B), dim3(kLogitThreads), 0, stream, a);
+  constexpr int kColumns = kLogitThreads * kLogitVec, kMany = 2;
+  // two sets for a thread where they still fill the SMs twice: 64 x 128256 bf16 took 12.2 us with one and 11.5 with two, 24 x 128256 5.7 and 6.1, 40 x 128256 8.4 with
+  // either; four spill (15.4)
+  const bool many = static_cast<long long>(B) * ((a.V + kColumns - 1) / kColumns) >= 2 * 148 * 4 * kMany;
+  const int columns = many ? kColumns * kMany : kColumns;
+  const dim3 grid((a.V + columns - 1) / columns, B);
+  if (many) launch_kernel(vec ? process_logits_kernel<T, true, kMany> : process_logits_kernel<T, false, kMany>, grid, dim3(kLogitThreads), 0, stream, a);
+  else launch_kernel(vec ? process_logits_kernel<T, true, 1> : process_logits_kernel<T, false, 1>, grid, dim3(kLogitThreads), 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -7;
 }
 
