@@ -63,7 +63,7 @@ struct alignas(16) LogitVec {
 // multiplied by the penalty's reciprocal, taken once: 2^-24 more of an error beside their own rounding of 2^-8 or 2^-11, for a division a value (1 x 32000: 2.4 us
 // with, 2.0 without).
 // 64 x 128256 bf16 with all three on a B200: 18.9 us with the arithmetic and a division for all values, 14.4 value by value behind block barriers that the
-// gathering of the biases needed, 11.4 now (7.7 for its bytes at the rate of a copy; without any of the three 5.1, from L2).  Choosing registers by the number of a touched
+// gathering of the biases needed, 10.5 now (7.7 for its bytes at the rate of a copy; without any of the three 5.8, from L2).  Choosing registers by the number of a touched
 // value, instead of passing over eight places, took 14.0.
 template <typename T, bool kVec, int kSets>
 __global__ void __launch_bounds__(kLogitThreads, kSets == 1 ? 5 : 4)
@@ -80,8 +80,7 @@ process_logits_kernel(const LogitArgs a) {
   const T* in = static_cast<const T*>(a.logits) + b * a.in_stride;
   T* out = static_cast<T*>(a.out) + b * a.out_stride;
   const auto column = [&](int s, int j) { return lo + s * 256 + (kVec ? lane * kLogitVec + j : lane + j * 32); };
-  const auto whole = [&](int s) { return kVec && column(s, kLogitVec - 1) < a.V; };
-  const bool inside = lo + kMine <= a.V;  // a warp's accesses value by value need no comparison
+  const bool inside = lo + kMine <= a.V;  // otherwise the row ends in this warp's columns
   const auto each = [&](int s, auto&& f) {
     if (inside) {
 #pragma unroll
@@ -92,15 +91,18 @@ process_logits_kernel(const LogitArgs a) {
         if (column(s, j) < a.V) f(j);
     }
   };
+  const bool wide = kVec && inside;
 
   LogitVec<T> x[kSets];
+  if (wide) {
 #pragma unroll
-  for (int s = 0; s < kSets; ++s) {
-    if (whole(s)) x[s] = *reinterpret_cast<const LogitVec<T>*>(in + column(s, 0));
-    else each(s, [&](int j) { x[s].v[j] = in[column(s, j)]; });
+    for (int s = 0; s < kSets; ++s) x[s] = *reinterpret_cast<const LogitVec<T>*>(in + column(s, 0));
+  } else {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) each(s, [&](int j) { x[s].v[j] = in[column(s, j)]; });
   }
   const auto store = [&](int s) {
-    if (whole(s)) *reinterpret_cast<LogitVec<T>*>(out + column(s, 0)) = x[s];
+    if (wide) *reinterpret_cast<LogitVec<T>*>(out + column(s, 0)) = x[s];
     else each(s, [&](int j) { out[column(s, j)] = x[s].v[j]; });
   };
   if (!known) {
@@ -114,30 +116,34 @@ process_logits_kernel(const LogitArgs a) {
   int id[kAhead];
 #pragma unroll
   for (int q = 0; q < kAhead; ++q) id[q] = q * 32 + lane < a.K ? ids[q * 32 + lane] : -1;
-  unsigned w[kSets][kLogitVec / 2];  // eight words of counts
+  unsigned w[kSets][kLogitVec / 2] = {};  // eight words of counts
   const unsigned short* count_row = a.counts + r * a.counts_stride;
+  if (!a.counts) {
+  } else if (wide) {
 #pragma unroll
-  for (int s = 0; s < kSets; ++s) {
-#pragma unroll
-    for (int j = 0; j < kLogitVec / 2; ++j) w[s][j] = 0;
-    if (!a.counts) {
-    } else if (whole(s)) {
+    for (int s = 0; s < kSets; ++s) {
       const uint4 raw = *reinterpret_cast<const uint4*>(count_row + column(s, 0));
       w[s][0] = raw.x; w[s][1] = raw.y; w[s][2] = raw.z; w[s][3] = raw.w;
-    } else each(s, [&](int j) { w[s][j >> 1] |= unsigned(count_row[column(s, j)]) << (16 * (j & 1)); });
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) each(s, [&](int j) { w[s][j >> 1] |= unsigned(count_row[column(s, j)]) << (16 * (j & 1)); });
   }
   unsigned allow[kSets];  // bit j: value j
   const unsigned* words = a.allowed + size_t(r) * a.words;
 #pragma unroll
-  for (int s = 0; s < kSets; ++s) {
-    allow[s] = 0xffu;
-    if (!a.allowed) {
-    } else if (whole(s) && a.first % 8 == 0) {
-      allow[s] = reinterpret_cast<const unsigned char*>(words)[(a.first + column(s, 0)) >> 3];
-    } else each(s, [&](int j) {
-      const int of = a.first + column(s, j);
-      if (!(words[of >> 5] >> (of & 31) & 1u)) allow[s] &= ~(1u << j);
-    });
+  for (int s = 0; s < kSets; ++s) allow[s] = 0xffu;
+  if (!a.allowed) {
+  } else if (wide && a.first % 8 == 0) {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) allow[s] = reinterpret_cast<const unsigned char*>(words)[(a.first + column(s, 0)) >> 3];
+  } else {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s)
+      each(s, [&](int j) {
+        const int of = a.first + column(s, j);
+        if (!(words[of >> 5] >> (of & 31) & 1u)) allow[s] &= ~(1u << j);
+      });
   }
   const float presence = a.records[r].presence, frequency = a.records[r].frequency, repetition = a.records[r].repetition;
   const bool penalties = presence != 0.f || frequency != 0.f || repetition != 1.f;
@@ -407,9 +413,10 @@ plan_batch_kernel(const PlanArgs a) {
 template <typename T>
 static int launch_logits(const LogitArgs& a, int B, bool vec, cudaStream_t stream) {
   constexpr int kColumns = kLogitThreads * kLogitVec, kMany = 2;
-  // two sets for a thread where they still fill the SMs twice: 64 x 128256 bf16 took 12.2 us with one and 11.5 with two, 24 x 128256 5.7 and 6.1, 40 x 128256 8.4 with
-  // either; four spill (15.4)
-  const bool many = static_cast<long long>(B) * ((a.V + kColumns - 1) / kColumns) >= 2 * 148 * 4 * kMany;
+  // two sets for a thread, which then has twice as much under way, in exchange for fewer blocks (one set and two, us): 16 bits in wide accesses gain from six blocks an
+  // SM on (16 x 128256 4.9 and 4.5, 64 x 128256 12.5 and 10.6, but 48 x 32000 4.5 and 4.9), others from some 24 on (64 x 128256 fp32 13.3 and 13.1, 40 x 128256 9.0
+  // and 9.4); four spill
+  const bool many = static_cast<long long>(B) * ((a.V + kColumns - 1) / kColumns) >= 148 * (vec && sizeof(T) == 2 ? 6 : 24);
   const int columns = many ? kColumns * kMany : kColumns;
   const dim3 grid((a.V + columns - 1) / columns, B);
   if (many) launch_kernel(vec ? process_logits_kernel<T, true, kMany> : process_logits_kernel<T, false, kMany>, grid, dim3(kLogitThreads), 0, stream, a);
