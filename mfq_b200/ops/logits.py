@@ -93,7 +93,8 @@ def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch
 def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, rows: torch.Tensor, *, prompt: bool = False) -> None:
     """Count ``tokens [n]`` int32 in ``counts[rows [n], token]`` (int16 words ``[R, V]``, see the top of this module): as tokens of an
     answer, whose counts stay at 32767 once there, or with ``prompt`` as tokens that the prompt has.  A pair outside the table is left
-    out, so a batch may be padded with negative rows."""
+    out, so a batch may be padded with negative rows.  Calls that count in the same rows follow one another: two at once could bring a count
+    past 32767 between them."""
     if counts.dtype is not torch.int16 or counts.ndim != 2 or (counts.shape[1] > 1 and counts.stride(1) != 1):
         _refuse("counts", "int16 [R, V] with neighbouring columns are", counts)
     index = counts.get_device()

@@ -26,6 +26,16 @@ def test_process_logits(b, r, v, how, dtype):
     assert_logits(ops.process_logits(**args, out=held), *want, float("-inf"))  # in place
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("b,r,v,how", [(60, 60, 30104, {"k": 40}), (240, 50, 30104, {"mapped": True}), (240, 50, 30100, {"mapped": True, "k": 9, "first": 17}), (240, 240, 30104, {"odd": True})])
+def test_process_logits_of_large_batches(b, r, v, how, dtype):
+    """Large enough for a thread to have two sets of eight, in wide accesses and value by value."""
+    require_gpu_lib()
+    args, table = logits_case(v + b, b, r, v, dtype, device="cuda", mask=True, **how)
+    want = exact_logits(args["logits"], args["records"], args["counts"], args["bias"], table, args["rows"], args["first"], -np.inf)
+    assert_logits(ops.process_logits(**args), *want, float("-inf"))
+
+
 def test_rows_of_nothing_and_unusual_values():
     require_gpu_lib()
     v = 4096
