@@ -19,45 +19,55 @@ SMS = 148
 
 
 @lru_cache(maxsize=4096)
-def _shape(b: int, per_seq: int, hk: int, d: int, groups: int, width: int, max_group: int | None, max_prefix: int | None, max_tail: int | None) -> tuple[int, int, int]:
-    """(query rows of a prefix CTA, splits of a prefix, splits of a sequence's own pages) for ``b`` sequences of ``per_seq`` query rows a KV head: the form
-    that a few numbers fitted to sweeps on a B200 (1 and 4 groups of 2 to 64 rows, prefixes of 256 to 32768 tokens, heads of 64 and 128) say is
-    fastest, in microseconds.  0 splits of a prefix: every sequence is read whole, which is one kernel, and all that heads of 256 have."""
-    group = b if max_group is None else max(1, min(b, max_group))
-    whole = width if max_prefix is None else min(width, max(0, max_prefix) // 16)
-    tail = width if max_tail is None else min(width, max(0, max_tail) // 16 + 1)
-    rows, per_sm = group * per_seq, 4 if d <= 128 else 2
-    slow = (1.0 if per_seq <= 8 else 1.6) * (1.0 if d <= 128 else 2.0)  # a page, by one warp
-    bandwidth = 6.0e6 / (16 * (2 * d + 8))  # pages of a head, from memory
+def _shape(b: int, per_seq: int, hk: int, d: int, groups: int, group: int, whole: int, tail: int) -> tuple[int, int, int]:
+    """(query rows of a prefix CTA, splits of a prefix, CTAs of a sequence's own pages) for ``b`` sequences of ``per_seq`` query rows a KV head, in groups
+    of up to ``group`` with ``whole`` pages of a prefix and ``tail`` of their own.  0 splits of a prefix: every sequence is read whole, which is one kernel, and
+    all that heads of 256 have.
 
-    def ranks(pages: int, least: int) -> int:  # CTAs that share a sequence: a power of two, which fills the grid better than others
-        n = 1
-        while n < 8 and 2 * n * b * hk <= SMS * per_sm and n * least < pages:
-            n *= 2
-        return n
+    The form that is fastest by a model of the kernels in microseconds: a few numbers fitted to 852 shapes on a B200 (1 to 5 groups of 2 to 64
+    sequences, equal and ragged, prefixes of 130 to 24000 tokens, heads of 64 and 128), some twenty forms of each measured.  What it chooses takes 3 %
+    longer than the fastest on average, and more than 12 % in 81 of them (40 % at worst)."""
+    rows, narrow = group * per_seq, per_seq <= 8
+    per_sm = 2 if d > 128 else (4 if narrow else 3) + (d == 64)  # CTAs that read pages by warps
+    slots_of_gpu = SMS * per_sm
+    bandwidth = 1.2e7 / (16 * (2 * d + 8))  # pages of a head, from memory or L2
 
-    def own_pages(pages: int, r: int) -> float:
-        return max(pages / (4 * r) * slow * (1.4 if b * hk * r > SMS else 1.0), b * hk * pages / bandwidth)
+    def waves(n: int, slots: int) -> float:
+        return 1.0 if n <= slots else 0.3 * n / slots + 0.7 * -(-n // slots)
 
-    r = ranks(whole + tail, 8)
-    best = (5 + own_pages(whole + tail, r), 16, 0, r)
-    if d > 128 or whole == 0 or group == 1:
-        return best[1:]
-    for tile in ((8 if rows <= 8 else 16,) if rows <= 32 else ()) + (((128,) if rows <= 128 else (256,)) if rows > 8 else ()):
-        units = -(-rows // tile) * hk * groups
-        if tile >= 128:  # one CTA an SM, blocks of eight pages: no more splits than give each of them whole blocks
-            blocks = -(-whole // 8)
-            splits = -(-blocks // -(-blocks // max(1, min(SMS // units, blocks, 32))))
-            each = (2.4 if tile == 128 else 3.6) * -(-blocks // splits) + 7
-            t = each * max(1.0, units * splits / SMS)
+    def pages_of(pages: int, ranks: int, n: int) -> float:  # of n CTAs, four warps each
+        each = (0.70 + 0.10 * min(n / SMS, per_sm) if narrow else 0.77 + 0.25 * min(n / SMS, per_sm)) * (1.0 if d <= 128 else 2.0)
+        return max(-(-pages // (4 * ranks)) * each * waves(n, slots_of_gpu), b * hk * pages / bandwidth)
+
+    forms = []
+    ranks = [r for r in (1, 2, 4, 8) if r == 1 or b * hk * r <= 2 * slots_of_gpu]
+    for r in ranks:
+        forms.append((4.9 + pages_of(whole + tail, r, b * hk * r) + 0.6 * (r.bit_length() - 1), 16, 0, r))
+    tiles = () if d > 128 or whole == 0 or group == 1 else ((8 if rows <= 8 else 16,) if rows <= 32 else ()) + ((128 if rows <= 128 else 256,) if rows > 8 else ())
+    for tile in tiles:
+        units, blocks = -(-rows // tile) * hk * groups, -(-whole // 8)
+        if tile >= 128:  # blocks of eight pages; as many splits as SMs, each of whole blocks, or a power of two
+            most = max(1, min(SMS // units, blocks, 32))
+            splits_to_try = {s for s in (1, 2, 4, 8, 16, 32) if s <= blocks} | {-(-blocks // -(-blocks // most))}
         else:
-            splits = max(1, min(SMS * 3 // units, -(-whole // 8), 32))
-            t = (5 if tile == 8 else 8) + max(-(-whole // (4 * splits)) * (1.0 if tile == 8 else 1.4), units * whole / bandwidth) * max(1.0, units * splits / (SMS * 3))
-        slots = splits * (2 if tile == 128 else 1)
-        r = max(ranks(tail, 32), ranks(-(-per_seq * d // 512) * -(-slots // 8), 8))  # pages of its own, and rounds of reading partials
-        t += 3 + own_pages(tail, r) + b * per_seq * hk * slots * d / 1.0e6 + 0.4 * -(-slots // 8)
-        best = min(best, (t, tile, splits, r))
-    return best[1:]
+            slots_of_tiles = SMS * ((4 if tile == 8 else 3) + (d == 64 and tile == 16))
+            splits_to_try = {s for s in (1, 2, 4, 8, 16, 32) if s <= max(1, whole // 4)} | {max(1, min(slots_of_tiles // units, whole // 4, 32))}
+        for splits in splits_to_try:
+            ctas = units * splits
+            if tile >= 128:  # one an SM, where nothing else fits beside it
+                t = 0.9 + (2.0 if tile == 128 else 3.6) * -(-blocks // splits) * max(1, -(-ctas // SMS))
+                room = max(0, SMS - ctas) * per_sm
+            else:
+                t = 2.0 + max(-(-whole // (4 * splits)) * (0.92 if tile == 8 else 1.8), units * whole / bandwidth) * waves(ctas, slots_of_tiles)
+                room = max(0, slots_of_gpu - ctas)
+            parts = splits * (2 if tile == 128 else 1)
+            for r in ranks[: 2 if tile >= 128 else 3]:
+                n = b * hk * r  # CTAs of the sequences' own pages: those with room beside the prefixes keep it until these are there, the rest come behind
+                rest = max(0, n - room)
+                whole_t = max(t, pages_of(tail, r, n - rest) if room else 0.0) + (pages_of(tail, r, rest) + 2.4 if rest else 0.0)
+                merge = 6.0 + 0.6 * (r.bit_length() - 1) + 0.64 * -(-parts // 8) * -(-per_seq * d // (512 * r)) * waves(n, slots_of_gpu) + 1.3e-6 * b * per_seq * hk * parts * d
+                forms.append((whole_t + merge, tile, splits, r))
+    return min(forms)[1:]
 
 
 def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, group_starts: torch.Tensor,
@@ -118,7 +128,9 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
         with torch.cuda.device(index):
             return paged_attn_decode_shared(q, kv, block_table, seq_lens, group_starts, prefix_lens, sm_scale=sm_scale, members=members, q_len=q_len,
                                             max_group=max_group, max_prefix=max_prefix, max_tail=max_tail, out=out)
-    tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, width, max_group, max_prefix, max_tail)
+    tile, prefix_splits, tail_splits = _shape(b, hq // hk * q_len, hk, d, groups, b if max_group is None else max(1, min(b, max_group)),
+                                              width if max_prefix is None else min(width, max(0, max_prefix) // 16),
+                                              width if max_tail is None else min(width, max(0, max_tail) // 16 + 1))
     parts = n * hq * prefix_splits * (2 if tile == 128 else 1)
     scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device) if parts else None  # of this call: a workspace would tie streams and graphs together
     at = scratch.data_ptr() if parts else 0

@@ -70,3 +70,16 @@ def test_tensors_that_begin_between_16_bytes_are_refused(name):
         setattr(s.kv, name, shifted(getattr(s.kv, name)))
     with pytest.raises(ValueError, match="16 bytes"):
         call(ops, s, out=shifted(out) if name == "out" else out)
+
+
+def test_chosen_forms_are_forms_that_the_kernels_have():
+    """Whatever the sizes: tiles, partials of a query row and CTAs of a cluster within the limits of the C entry."""
+    from mfq_b200.ops.shared_attn import _shape
+    g = torch.Generator().manual_seed(1)
+    pick = lambda *x: x[int(torch.randint(0, len(x), (1,), generator=g))]  # noqa: E731
+    for _ in range(1500):
+        b, per_seq, hk, d = pick(1, 2, 5, 31, 64, 700, 65535), pick(1, 2, 4, 7, 8, 9, 16), pick(1, 2, 8, 40), pick(64, 128, 256)
+        groups, whole, tail = min(b, pick(1, 2, 9, 300)), pick(0, 1, 3, 4, 40, 1000, 70000), pick(0, 1, 2, 30, 900, 70000)
+        tile, splits, ranks = _shape(b, per_seq, hk, d, groups, pick(1, max(1, b // groups), b), whole, tail)
+        assert tile in (8, 16, 128, 256) and ranks in (1, 2, 4, 8) and 0 <= splits * (2 if tile == 128 else 1) <= 64
+        assert splits == 0 or (d <= 128 and splits <= max(1, whole)) and (tile != 8 or per_seq <= 8)
