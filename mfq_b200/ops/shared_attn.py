@@ -97,6 +97,9 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     pages, hk = k.shape[:2]
     if kv.page_size != 16 or k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn or k.shape != (pages, hk, d // 64, 16, 64) or v.shape != (pages, hk, d, 16):
         _refuse("kv", f"FP8 pages of 16 tokens and {d}-wide heads are", k)
+    for t in (kv.k_scale, kv.v_scale):
+        if t.dtype is not torch.float32 or t.shape != (pages, hk, 16):
+            _refuse("kv multipliers", f"fp32 {(pages, hk, 16)} are", t)
     for t in (k, v, kv.k_scale, kv.v_scale):
         if t.get_device() != index or not t.is_contiguous():
             _refuse("kv", "contiguous pages on the device of q are", t)

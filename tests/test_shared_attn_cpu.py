@@ -72,6 +72,15 @@ def test_tensors_that_begin_between_16_bytes_are_refused(name):
         call(ops, s, out=shifted(out) if name == "out" else out)
 
 
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("make", [lambda t: t[:-1], lambda t: t.double(), lambda t: t[:, :, :8].contiguous()])
+def test_multipliers_of_another_pool_are_refused(name, make):
+    s = batch(1, [(16, [20, 30])])
+    setattr(s.kv, name, make(getattr(s.kv, name)))
+    with pytest.raises(ValueError, match="multipliers"):
+        call(ops, s)
+
+
 def test_chosen_forms_are_forms_that_the_kernels_have():
     """Whatever the sizes: tiles, partials of a query row and CTAs of a cluster within the limits of the C entry."""
     from mfq_b200.ops.shared_attn import _shape
