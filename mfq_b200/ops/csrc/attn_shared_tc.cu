@@ -8,12 +8,16 @@
 //   O += P V        P as fp16 pairs, those of 64 keys over the first half of their S, V codes K-major ([dim][key], what a page holds), O in tensor memory
 // m moves only where a row's maximum has grown by more than 2^11 since (O is then rescaled in place): as any m gives the same quotient, this costs no exactness.
 // A warp takes tensor memory as matrix fragments: four lanes share a row and a lane has two columns of each eight, so that what belongs to
-// columns is read from shared memory once for 16 rows.  It goes over S twice, 16 columns at a time, and two warps share the keys of a block: registers for a whole block spilled, and the code of
-// all roles together has to stay within the instruction cache (unrolled, a step took 9000 cycles, a third of them without an instruction).
+// columns is read from shared memory once for 32 rows.  It goes over S twice, 16 columns at a time, and two warps share the keys of a block and exchange
+// their maxima (16 rows and all keys a warp: no exchange, twice the reads for columns, 2 % slower): registers for a whole block spilled, and the code of all
+// roles together has to stay within the instruction cache (unrolled, a step took 9000 cycles, a third of them without an instruction).
 // Seven warps put down codes as fp16 (exact) from rings of pages that bulk copies fill: loads to registers have to pass the few KB of L1 that such a CTA leaves,
 // and took 4000 cycles a block.
 //
-// Per block of 128 x 128 the tensor core and the exponentials both need 1024 cycles of an SM, shared memory (operands, codes) some 1250.
+// Per block of 128 x 128 the tensor core and the exponentials both need 1024 cycles of an SM, shared memory (operands, codes) some 1250.  A step of two
+// tiles takes 5800 on a B200: a stream's softmax (3300 to 3900) and its products with their issue (1600) follow one another, and the two streams fill each
+// other's gaps as far as that goes.  4.8 us pass from the launch to the first scores, some 5 from the last ones to the end.  64 sequences of 32 heads on 8 behind
+// 32768 tokens: 65 us, of 21 for its operations at the measured rate; behind 8192 tokens 28.
 #include "attn_shared.cuh"
 
 namespace mfq {

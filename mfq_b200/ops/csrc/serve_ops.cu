@@ -290,6 +290,7 @@ count_tokens_kernel(unsigned short* __restrict__ counts, long long stride, int R
 // t of s_i <= t < s_{i+1} is at position past_i + t - s_i, in slot page * size + offset.  With a list of free pages, request i takes
 // ceil((past_i + counts_i) / size) - ceil(past_i / size) of them, in the order of the requests, behind the pages of its past.
 // Every block sums the lengths for itself (at most kPlanRequests, so that no block waits for another) and takes its share of tokens and table entries.
+// Bound by latency: one request of 357 tokens takes 2.9 us of a replay on a B200, 256 requests of 4500 tokens with pages from a list 5.8.
 constexpr int kPlanThreads = 256, kPlanRequests = 1024, kPlanPer = kPlanRequests / kPlanThreads, kPlanRows = 1 << 16;
 enum : int { kPlanBadRequest = 1, kPlanNoRoom = 2, kPlanNoPages = 3 };
 
