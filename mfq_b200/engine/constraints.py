@@ -14,6 +14,8 @@ Reference: engine token constraints + the tokenizer's grammar (``cpp_runtime/eng
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import torch
 
@@ -95,9 +97,19 @@ def make_constraint(response_format, vocabulary, stop_ids):
     return None
 
 
+def penalties(params) -> tuple[float, float, float]:
+    """Presence, frequency and repetition penalty of a request.  What is no number, or no factor, penalizes nothing; what fp32 would make an infinity
+    stays below it, so that no logit turns into a NaN."""
+    def held(x: float, neutral: float) -> float:
+        return neutral if math.isnan(x) else max(-1e30, min(1e30, x))
+
+    repetition = held(params.repetition_penalty, 1.0)
+    return held(params.presence_penalty, 0.0), held(params.frequency_penalty, 0.0), max(1e-30, repetition) if repetition > 0.0 else 1.0
+
+
 def penalized(params) -> bool:
     """Whether a request penalizes tokens that it has already."""
-    return params is not None and (params.presence_penalty != 0.0 or params.frequency_penalty != 0.0 or params.repetition_penalty != 1.0)
+    return params is not None and penalties(params) != (0.0, 0.0, 1.0)
 
 
 class LogitTables:

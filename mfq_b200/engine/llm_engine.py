@@ -22,7 +22,7 @@ import torch
 from .. import ops
 from ..models.llama import LlamaModel, StepBuffers
 from ..utils.profiler import scope
-from .constraints import NEG, LogitTables, penalized
+from .constraints import NEG, LogitTables, penalized, penalties
 from .kv_cache import PAGE_SIZE, PagedKVCache
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
@@ -248,8 +248,7 @@ class LLMEngine:
         rec = torch.zeros(8, dtype=torch.int32)
         stochastic = bool(params is not None and getattr(params, "temperature", 0.0) > 0.0)
         if params is not None:
-            f = torch.tensor([params.temperature, 0.0, params.top_p, params.presence_penalty, params.frequency_penalty,
-                              params.repetition_penalty], dtype=torch.float32).view(torch.int32)
+            f = torch.tensor([params.temperature, 0.0, params.top_p, *penalties(params)], dtype=torch.float32).view(torch.int32)
             rec[:6] = f
             rec[1] = int(params.top_k)
             rec[6:8] = torch.tensor([int(params.seed) & (2 ** 63 - 1)], dtype=torch.int64).view(torch.int32)
