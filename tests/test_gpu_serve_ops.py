@@ -54,6 +54,20 @@ def test_rows_of_nothing_and_unusual_values():
         assert (got[0] == -float("inf")).all()
 
 
+def test_rows_behind_4_gigabytes():
+    require_gpu_lib()
+    args, table = logits_case(12, 4, 3, 128256, torch.bfloat16, mask=True, k=30, device="cuda")
+    args["rows"] = torch.tensor([2, 0, 1, 2], dtype=torch.int32, device="cuda")
+    want = ops.process_logits(**args)
+    b = 2 ** 32 // (2 * 128256) + 20
+    logits = torch.zeros((b, 128256), dtype=torch.bfloat16, device="cuda")
+    logits[-4:].copy_(args["logits"])
+    rows = torch.full((b,), -1, dtype=torch.int32, device="cuda")
+    rows[-4:].copy_(args["rows"])
+    got = ops.process_logits(**{**args, "logits": logits, "rows": rows}, out=logits)
+    assert torch.equal(got[-4:], want) and not got[: b - 4].any()
+
+
 def test_records_that_begin_on_4_bytes():
     require_gpu_lib()
     args, table = logits_case(11, 3, 3, 5000, torch.bfloat16, mask=True, device="cuda")

@@ -139,6 +139,45 @@ def test_two_calls_at_once():
         assert all(torch.equal(got[0], x) for x in got)
 
 
+def test_two_graphs_replayed_at_once():
+    """Every captured call has partials of its own."""
+    require_gpu_lib()
+    cases = [batch(i, [(2000, [2100] * 12)], hq=32, hk=8, device="cuda") for i in (3, 4)]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in cases]
+    for s in cases:
+        call(ops, s)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(ops, s))
+    for _ in range(8):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    check_status()
+    for s, out in zip(cases, outs):
+        assert_attends(s, out, exact(s))
+
+
+@pytest.mark.parametrize("form", [(16, 0, 2), (16, 3, 1), (128, 2, 1), (256, 2, 1)])
+def test_pages_behind_4_gigabytes(form, monkeypatch):
+    require_gpu_lib()
+    monkeypatch.setattr(shared_attn, "_shape", lambda *a: form)
+    s = batch(5, [(400, [430, 410, 500, 401, 460])], hq=32, hk=8)
+    want = exact(s)
+    used, most = s.kv.k.shape[0], 2 ** 32 // (8 * 16 * 128) + 1000
+    for name in ("k", "v", "k_scale", "v_scale"):
+        small = getattr(s.kv, name).cuda()
+        large = torch.zeros((most, *small.shape[1:]), dtype=small.dtype, device="cuda")
+        large[most - used :].copy_(small)
+        setattr(s.kv, name, large)
+    for name in ("q", "table", "seq_lens", "starts", "prefixes", "members"):
+        setattr(s, name, getattr(s, name).cuda())
+    s.table += most - used
+    run(s, want)
+
+
 def test_a_page_outside_the_pool_is_reported():
     require_gpu_lib()
     s = batch(2, [(64, [80, 90])], device="cuda")
