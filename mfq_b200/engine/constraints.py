@@ -38,7 +38,7 @@ class JsonTokenConstraint:
             mask[list(self.stop_ids)] = True
         return mask
 
-    def biases(self) -> dict:
+    def biases(self, width: int) -> dict:
         return {}
 
     def words(self, width: int) -> torch.Tensor:
@@ -74,9 +74,13 @@ class LogitBias:
         self.table = {int(t): max(-100.0, min(100.0, float(v))) for t, v in bias.items()}
         self.inner = inner
         self.finished = False
+        self._inside: dict[int, dict] = {}  # columns -> the biases of tokens that there are
 
-    def biases(self) -> dict:
-        return self.table
+    def biases(self, width: int) -> dict:
+        """Token -> bias of the ids below ``width``, one dict for all steps: a request may name any id, what is no token has no logit."""
+        if width not in self._inside:
+            self._inside[width] = {t: v for t, v in self.table.items() if 0 <= t < width}
+        return self._inside[width]
 
     def words(self, width: int) -> torch.Tensor | None:
         return self.inner.words(width) if self.inner is not None else None
@@ -137,7 +141,7 @@ class LogitTables:
 
     def limit(self, row: int, constraint) -> None:
         """Bring row ``row`` in line with a constraint (None: no limits)."""
-        words, table = (None, {}) if constraint is None else (constraint.words(self.width), constraint.biases())
+        words, table = (None, {}) if constraint is None else (constraint.words(self.width), constraint.biases(self.width))
         held_words, held_table = self._held.get(row, (None, {}))
         if words is not held_words:  # the words of a grammar state are one tensor: within a string, say, the device has them already
             if words is None:

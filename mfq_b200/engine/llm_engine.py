@@ -198,7 +198,7 @@ class LLMEngine:
     def _write_limits(self, rows, width: int) -> None:
         """Refresh the tables' rows ``rows`` from their constraints (no limits for rows without one)."""
         t = self._tables(width)
-        places = max((len(c.biases()) for c in self.row_constraint.values()), default=0)
+        places = max((len(c.biases(width)) for c in self.row_constraint.values()), default=0)
         if places > t.bias_ids.shape[1]:
             self._drop_processed_graphs()
             t.make_places(places)

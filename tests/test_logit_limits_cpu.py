@@ -1,0 +1,47 @@
+"""What requests bring in biases, masks and penalties, and what neighbours and later requests see of it, on CPU engines."""
+
+import pytest
+import torch
+
+from mfq_b200.engine.llm_engine import LLMEngine
+from mfq_b200.engine.scheduler import ContinuousBatchScheduler, Request
+from mfq_b200.models.llama import LlamaConfig, LlamaModel, LlamaWeights
+from penalty_cases import PROMPTS, params
+from ragged_stub import ragged_engine
+
+
+@pytest.fixture(scope="module")
+def model():
+    cfg = LlamaConfig.tiny()
+    return LlamaModel(cfg, LlamaWeights.random_init(cfg, "cpu", seed=7))
+
+
+def serve(engine, requests, **how):
+    sched = ContinuousBatchScheduler(engine, max_queue=16, **how)
+    for r in requests:
+        sched.submit(r)
+    for _ in range(400):
+        if not sched.step() and sched.idle:
+            break
+    return sched, [list(r.generated) for r in requests]
+
+
+def both_engines(model):
+    """Engines that run a prompt at once, and that read it in portions beside other rows; with a scheduler's settings and prompts."""
+    return ((lambda: LLMEngine(model, max_batch=4, max_seq_len=160, device="cpu"), {}, PROMPTS),
+            (ragged_engine, {"mixed_tokens": 8}, [[t % 97 for t in p] for p in PROMPTS]))
+
+
+OUTSIDE = [{2 ** 31: 1.0}, {-1: 5.0, 2 ** 40: -3.0, -2 ** 33: 1.0}, {2 ** 31 - 1: 4.0, 10 ** 30: 1.0}]
+
+
+@pytest.mark.parametrize("bias", OUTSIDE)
+def test_biases_of_ids_outside_the_vocabulary_are_none(model, bias):
+    for make, how, prompts in both_engines(model):
+        _, plain = serve(make(), [Request(list(p), params()) for p in prompts], **how)
+        requests = [Request(list(p), params(logit_bias=dict(bias) if i == 1 else None)) for i, p in enumerate(prompts)]
+        sched, got = serve(make(), requests, **how)
+        assert sched.healthy and all(r.error is None for r in requests) and got == plain
+        inside = {plain[0][0]: -100}
+        one, other = (serve(make(), [Request(list(prompts[0]), params(logit_bias=b))], **how)[1][0] for b in (inside, {**bias, **inside}))
+        assert one == other and plain[0][0] not in one
