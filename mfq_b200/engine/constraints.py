@@ -127,17 +127,29 @@ class LogitTables:
         self._held: dict[int, tuple] = {}  # row -> the host's words and biases that its rows hold (None: no limit)
         self.make_places(8)
 
-    def make_places(self, places: int) -> None:
-        """Room for ``places`` biases a row; the biases are written again by the next :meth:`limit`."""
+    def make_places(self, places: int, tables: int = 1) -> None:
+        """Room for ``places`` biases a row in each of ``tables`` tables; the biases are written again by the next :meth:`limit`."""
         most = 8
         while most < places:
             most *= 2
         if most > ops.MAX_BIASES:
-            raise ValueError(f"a request may have at most {ops.MAX_BIASES} biases, got {places}")
+            raise ValueError(f"a table has at most {ops.MAX_BIASES} biases a row, got {places}")
         rows, dev = self.counts.shape[0], self.counts.device
-        self.bias_ids = torch.full((rows, most), -1, dtype=torch.int32, device=dev)
-        self.bias_values = torch.zeros((rows, most), dtype=torch.float32, device=dev)
+        self.biases = [(torch.full((rows, most), -1, dtype=torch.int32, device=dev), torch.zeros((rows, most), dtype=torch.float32, device=dev))
+                       for _ in range(tables)]
         self._held = {r: (w, None) for r, (w, _) in self._held.items()}
+
+    @property
+    def bias_ids(self) -> torch.Tensor:
+        return self.biases[0][0]
+
+    def make_room(self, places: int) -> bool:
+        """Room for ``places`` biases a row, in several tables where one is not allowed as many; whether the tables are other ones now."""
+        if places <= sum(ids.shape[1] for ids, _ in self.biases):
+            return False
+        tables = -(-places // ops.MAX_BIASES)
+        self.make_places(places if tables == 1 else ops.MAX_BIASES, tables)
+        return True
 
     def limit(self, row: int, constraint) -> None:
         """Bring row ``row`` in line with a constraint (None: no limits)."""
@@ -149,10 +161,13 @@ class LogitTables:
             else:
                 self.allowed[row].copy_(words, non_blocking=True)
         if table is not held_table and not (held_table == {} and not table):
-            self.bias_ids[row].fill_(-1)
-            if table:
-                n = len(table)
-                self.bias_ids[row, :n] = torch.tensor(list(table), dtype=torch.int32).to(self.bias_ids.device)
-                # held as the bf16 numbers that logits had added before there was a kernel for it
-                self.bias_values[row, :n] = torch.tensor(list(table.values())).to(torch.bfloat16).float().to(self.bias_values.device)
+            at = 0
+            for ids, values in self.biases:
+                part = list(table.items())[at : at + ids.shape[1]]
+                at += len(part)
+                ids[row].fill_(-1)
+                if part:
+                    ids[row, : len(part)] = torch.tensor([t for t, _ in part], dtype=torch.int32).to(ids.device)
+                    # held as the bf16 numbers that logits had added before there was a kernel for it
+                    values[row, : len(part)] = torch.tensor([v for _, v in part]).to(torch.bfloat16).float().to(values.device)
         self._held[row] = (words, table)

@@ -199,9 +199,8 @@ class LLMEngine:
         """Refresh the tables' rows ``rows`` from their constraints (no limits for rows without one)."""
         t = self._tables(width)
         places = max((len(c.biases(width)) for c in self.row_constraint.values()), default=0)
-        if places > t.bias_ids.shape[1]:
+        if t.make_room(places):
             self._drop_processed_graphs()
-            t.make_places(places)
         for r in rows:
             t.limit(r, self.row_constraint.get(r))
 
@@ -210,7 +209,9 @@ class LLMEngine:
         v, tp = logits.shape[1], self.model.tp
         t = self._tables(v * tp)
         lo = self.model.w.tp_rank * v if tp > 1 else 0
-        return ops.process_logits(logits, self.sample_rows, counts=t.counts[:, lo : lo + v], bias=(t.bias_ids, t.bias_values), allowed=t.allowed, rows=rows,
+        for bias in t.biases[1:]:  # a token has one bias, so that only its own logit is rounded once more than by the call below
+            ops.process_logits(logits, self.sample_rows, bias=bias, rows=rows, first=lo, out=logits)
+        return ops.process_logits(logits, self.sample_rows, counts=t.counts[:, lo : lo + v], bias=t.biases[0], allowed=t.allowed, rows=rows,
                                   first=lo, fill=NEG, out=logits)
 
     # -- capacity (scheduler backend protocol) ------------------------------------------------------------------

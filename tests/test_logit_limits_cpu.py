@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from mfq_b200 import ops
 from mfq_b200.engine.llm_engine import LLMEngine
 from mfq_b200.engine.scheduler import ContinuousBatchScheduler, Request
 from mfq_b200.models.llama import LlamaConfig, LlamaModel, LlamaWeights
@@ -45,3 +46,26 @@ def test_biases_of_ids_outside_the_vocabulary_are_none(model, bias):
         inside = {plain[0][0]: -100}
         one, other = (serve(make(), [Request(list(prompts[0]), params(logit_bias=b))], **how)[1][0] for b in (inside, {**bias, **inside}))
         assert one == other and plain[0][0] not in one
+
+
+def test_more_biases_than_a_table_holds():
+    """As many as there are tokens, in any engine; the last ones and the ones at the tables' edges count like the first."""
+    vocab = 2 * ops.MAX_BIASES + 500
+    left = (3, ops.MAX_BIASES - 1, ops.MAX_BIASES, 2 * ops.MAX_BIASES, vocab - 1)
+    banned = {t: -100.0 for t in range(vocab) if t not in left}
+    make = lambda: ragged_engine(vocab, max_batch=3)  # noqa: E731
+    prompts = [list(range(5, 25)), [7, 9, 7, 7, 30, 2], [11] * 20]
+    _, plain = serve(make(), [Request(list(p), params()) for p in prompts], mixed_tokens=8)
+    eng = make()
+    requests = [Request(list(prompts[0]), params(logit_bias=banned)), Request(list(prompts[1]), params()),
+                Request(list(prompts[2]), params(presence_penalty=1e4, logit_bias=banned))]
+    sched, got = serve(eng, requests, mixed_tokens=8)
+    assert sched.healthy and all(r.error is None for r in requests)
+    at = prompts[0][-1]
+    for token in got[0]:  # the arg-max of what is left
+        row = eng.model.table[at % 97]
+        assert token == max(left, key=lambda t: row[t])
+        at = token
+    assert got[1] == plain[1]
+    assert set(got[2][:5]) == set(left) and len(set(got[2])) == len(got[2])
+    assert serve(eng, [Request(list(prompts[0]), params(presence_penalty=1e-9))], mixed_tokens=8)[1][0] == plain[0]  # no biases any more
