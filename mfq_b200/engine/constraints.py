@@ -155,19 +155,23 @@ class LogitTables:
         """Bring row ``row`` in line with a constraint (None: no limits)."""
         words, table = (None, {}) if constraint is None else (constraint.words(self.width), constraint.biases(self.width))
         held_words, held_table = self._held.get(row, (None, {}))
+        parts = None
+        if table is not held_table and not (held_table == {} and not table):
+            parts, at = [], 0
+            for ids, _ in self.biases:
+                part = list(table.items())[at : at + ids.shape[1]]
+                at += len(part)
+                # held as the bf16 numbers that logits had added before there was a kernel for it
+                parts.append((torch.tensor([t for t, _ in part], dtype=torch.int32), torch.tensor([v for _, v in part], dtype=torch.float32).to(torch.bfloat16).float()))
+        self._held[row] = (self, None)  # neither is what the row holds, should a write fail
         if words is not held_words:  # the words of a grammar state are one tensor: within a string, say, the device has them already
             if words is None:
                 self.allowed[row].fill_(-1)
             else:
                 self.allowed[row].copy_(words, non_blocking=True)
-        if table is not held_table and not (held_table == {} and not table):
-            at = 0
-            for ids, values in self.biases:
-                part = list(table.items())[at : at + ids.shape[1]]
-                at += len(part)
-                ids[row].fill_(-1)
-                if part:
-                    ids[row, : len(part)] = torch.tensor([t for t, _ in part], dtype=torch.int32).to(ids.device)
-                    # held as the bf16 numbers that logits had added before there was a kernel for it
-                    values[row, : len(part)] = torch.tensor([v for _, v in part]).to(torch.bfloat16).float().to(values.device)
+        for (ids, values), (tokens, biases) in zip(self.biases, parts or ()):
+            ids[row].fill_(-1)
+            if tokens.numel():
+                ids[row, : tokens.numel()] = tokens.to(ids.device)
+                values[row, : tokens.numel()] = biases.to(values.device)
         self._held[row] = (words, table)

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from mfq_b200 import ops
+from mfq_b200.engine.constraints import LogitTables
 from mfq_b200.engine.llm_engine import LLMEngine
 from mfq_b200.engine.scheduler import ContinuousBatchScheduler, Request
 from mfq_b200.models.llama import LlamaConfig, LlamaModel, LlamaWeights
@@ -69,3 +70,33 @@ def test_more_biases_than_a_table_holds():
     assert got[1] == plain[1]
     assert set(got[2][:5]) == set(left) and len(set(got[2])) == len(got[2])
     assert serve(eng, [Request(list(prompts[0]), params(presence_penalty=1e-9))], mixed_tokens=8)[1][0] == plain[0]  # no biases any more
+
+
+class Broken:
+    """A constraint of which one half cannot be written."""
+
+    def __init__(self, words, table):
+        self.held = words, table
+
+    def words(self, width):
+        if isinstance(self.held[0], Exception):
+            raise self.held[0]
+        return self.held[0]
+
+    def biases(self, width):
+        return self.held[1]
+
+
+@pytest.mark.parametrize("words,table", [(torch.zeros(2, dtype=torch.int32), {5: 1.0, 6: "no number"}), (torch.zeros(7, dtype=torch.int32), {5: 1.0}),
+                                         (RuntimeError("no words"), {5: 1.0})])
+def test_limits_that_fail_leave_nothing_behind(words, table):
+    """The row's next request has the tables as if they were new, and a request that had the row keeps nothing of what failed."""
+    for before in (None, Broken(torch.full((2,), 12, dtype=torch.int32), {1: 2.0})):
+        t = LogitTables(3, 64, torch.device("cpu"))
+        t.limit(1, before)
+        with pytest.raises(Exception):
+            t.limit(1, Broken(words, table))
+        t.limit(1, None)
+        assert (t.allowed == -1).all() and (t.bias_ids == -1).all()
+        t.limit(1, Broken(torch.full((2,), 9, dtype=torch.int32), {7: 3.0}))
+        assert t.allowed[1].tolist() == [9, 9] and t.bias_ids[1, 0] == 7 and t.biases[0][1][1, 0] == 3.0 and (t.bias_ids[1, 1:] == -1).all()
