@@ -21,6 +21,7 @@ import torch
 
 from .. import ops
 
+PLACES_KEPT = 1024  # biases a row that tables keep room for
 NEG = -1.0e30  # representable in bf16; exp() of it is 0 and an arg-max never picks it
 
 
@@ -144,10 +145,12 @@ class LogitTables:
         return self.biases[0][0]
 
     def make_room(self, places: int) -> bool:
-        """Room for ``places`` biases a row, in several tables where one is not allowed as many; whether the tables are other ones now."""
-        if places <= sum(ids.shape[1] for ids, _ in self.biases):
+        """Room for ``places`` biases a row, in several tables where one is not allowed as many; whether the tables are other ones now.  Many places are given
+        back once a quarter is enough: the kernel goes over all of them in every row."""
+        have = sum(ids.shape[1] for ids, _ in self.biases)
+        if places <= have and (have <= PLACES_KEPT or places > have // 4):
             return False
-        tables = -(-places // ops.MAX_BIASES)
+        tables = max(1, -(-places // ops.MAX_BIASES))
         self.make_places(places if tables == 1 else ops.MAX_BIASES, tables)
         return True
 

@@ -100,3 +100,18 @@ def test_limits_that_fail_leave_nothing_behind(words, table):
         assert (t.allowed == -1).all() and (t.bias_ids == -1).all()
         t.limit(1, Broken(torch.full((2,), 9, dtype=torch.int32), {7: 3.0}))
         assert t.allowed[1].tolist() == [9, 9] and t.bias_ids[1, 0] == 7 and t.biases[0][1][1, 0] == 3.0 and (t.bias_ids[1, 1:] == -1).all()
+
+
+def test_places_of_a_large_request_go_with_it():
+    """Every row's kernel goes over all places, so that one request with very many biases must not leave them to all later ones."""
+    vocab = ops.MAX_BIASES + 4000
+    eng = ragged_engine(vocab, max_batch=3)
+    many = {t: -1.0 for t in range(vocab - 9)}
+    assert serve(eng, [Request([5, 6, 7], params(logit_bias=many))], mixed_tokens=8)[0].healthy
+    assert sum(ids.shape[1] for ids, _ in eng.logit_tables.biases) >= len(many)
+    two = {9: 100.0, 10: 99.0}
+    got = serve(eng, [Request([5, 6, 7], params(logit_bias=two, presence_penalty=3.0)), Request([8, 9], params(presence_penalty=1.0))], mixed_tokens=8)[1]
+    assert sum(ids.shape[1] for ids, _ in eng.logit_tables.biases) == 8 and set(got[0]) <= set(two)
+    t = LogitTables(2, 2000, torch.device("cpu"))
+    assert t.make_room(1500) and not t.make_room(600) and t.make_room(500)  # not back and forth between requests of like sizes
+    assert t.make_room(1000) and not t.make_room(0)  # few enough to stay
