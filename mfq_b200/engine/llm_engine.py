@@ -126,6 +126,9 @@ class LLMEngine:
         self.row_constraint: dict[int, object] = {}  # row -> grammar state of a structured-output request
         self.logit_tables: LogitTables | None = None  # what rows' logits are processed by, allocated by the first such request
         self.row_penalized: set[int] = set()  # rows whose request has penalties for repeated tokens
+        self.row_given: dict[int, list] = {}  # row -> [(tokens, whether they count as a prompt's)] that it was given
+        self.row_drawn: dict[int, list[int]] = {}  # row -> the tokens it drew in decode() and the like, the last one not fed yet
+        self.logit_width: int | None = None  # columns of the logits over all ranks, once some were computed
         self._token_bytes, self._constraint_vocab, self._constraint_stop = None, None, ()
         self._next_seq_id = 0
         # models with recurrent (linear-attention) state keep it per batch row
@@ -242,10 +245,18 @@ class LLMEngine:
         self.row_stochastic.pop(row, None)
         self.row_constraint.pop(row, None)
         self.row_penalized.discard(row)
+        self.row_given.pop(row, None)
+        self.row_drawn.pop(row, None)
 
     # -- sampling ---------------------------------------------------------------------------------------------------
     def set_sampling(self, row: int, params) -> None:
-        """Install the row's sampling record (``params``: a :class:`SamplingParams`-like object or None = greedy)."""
+        """Install the row's sampling record (``params``: a :class:`SamplingParams`-like object or None = greedy).  Penalties go by all
+        tokens of the row's sequence, those from before the call too: a row advanced by :meth:`decode_step` itself, of whose tokens the engine keeps
+        no record, cannot be given any."""
+        self.row_penalized.discard(row)
+        if penalized(params):
+            self._recount(row)
+            self.row_penalized.add(row)
         rec = torch.zeros(8, dtype=torch.int32)
         stochastic = bool(params is not None and getattr(params, "temperature", 0.0) > 0.0)
         if params is not None:
@@ -257,9 +268,39 @@ class LLMEngine:
             rec[5] = torch.tensor([1.0]).view(torch.int32)[0]
         self.sample_rows[row] = rec.to(self.device)
         self.row_stochastic[row] = stochastic
-        self.row_penalized.discard(row)
-        if penalized(params):
-            self.row_penalized.add(row)
+
+    def _count(self, row: int, tokens, prompt: bool) -> None:
+        ids = torch.as_tensor(tokens, dtype=torch.int32).to(self.device)
+        ops.count_tokens(self._tables(self.logit_width).counts, ids, self.row_ids[row : row + 1].repeat(ids.numel()), prompt=prompt)
+
+    def _recount(self, row: int) -> None:
+        """Count the tokens that the row has so far.  The one that it drew last is counted by the step that feeds it."""
+        given, drawn = self.row_given.get(row, ()), self.row_drawn.get(row, ())
+        fed = self.row_len[row] - sum(len(t) for t, _ in given) if given else 0
+        if given and (int(self.seq_lens[row]) != self.row_len[row] or not 0 <= fed <= len(drawn)):
+            raise ValueError(f"row {row}: not all of the tokens that penalties would go by are known")
+        if self.logit_width is None:
+            return  # there are no tables yet, and new ones have counted nothing
+        self._tables(self.logit_width).counts[row].zero_()
+        for tokens, prompt in given:
+            self._count(row, tokens, prompt)
+        self._count(row, drawn[:fed], False)
+
+    def _give(self, row: int, tokens, prompt: bool = True) -> None:
+        """Take down tokens (a tensor or a list) that a row was given, once they are in the cache."""
+        given = self.row_given[row]
+        if isinstance(tokens, list) and given and isinstance(given[-1][0], list):
+            given[-1][0].extend(tokens)
+        else:
+            given.append((tokens, prompt))
+        if row in self.row_penalized:
+            self._count(row, tokens, prompt)
+
+    def _drew(self, out: dict) -> dict:
+        """Take down the tokens that a step returns."""
+        for r, t in out.items():
+            self.row_drawn[r].extend(t if isinstance(t, list) else (t,))
+        return out
 
     def _sample(self, logits: torch.Tensor, b: int, stochastic: bool) -> None:
         if not stochastic:
@@ -366,7 +407,7 @@ class LLMEngine:
             self._mtp_chain(row, row + 1, mhid[n - 1 : n].contiguous(), masked=False)
         if constraint is not None:
             constraint.advance(int(tok))
-        return int(tok)
+        return self._drew({row: int(tok)})[row]
 
     def _admit(self, row: int, token_ids, params, session):
         """Give batch row ``row`` a sequence with pages for the prompt and restore what a cache holds of it.  Returns
@@ -396,12 +437,9 @@ class LLMEngine:
         self._store_prefix(self.row_seq[row], keys, start)
         self.seq_lens[row] = n
         self.row_len[row] = n
-        if row in self.row_penalized:
-            table = self._tables(width).counts
-            table[row].zero_()
-            of = self.row_ids[row : row + 1].repeat(n)
-            ops.count_tokens(table, ids[: n - generated], of[: n - generated], prompt=True)
-            ops.count_tokens(table, ids[n - generated :], of[n - generated :])
+        self.logit_width = width
+        self._give(row, ids[: n - generated])
+        self._give(row, ids[n - generated :], prompt=False)
         constraint = self._constraint_for(params)
         if constraint is not None:
             for t in (ids[n - generated :].tolist() if generated else ()):
@@ -423,6 +461,7 @@ class LLMEngine:
         self._next_seq_id += 1
         self.row_seq[row] = seq_id
         self.row_len[row] = 0
+        self.row_given[row], self.row_drawn[row] = [], []
         self.set_sampling(row, params)
         if self.rec_state is not None:
             self.rec_state.reset(row)
@@ -472,8 +511,11 @@ class LLMEngine:
         rows = [first[i] + int(w) for i in range(len(portions)) for w in wanted[i]]
         pick = torch.tensor(rows or [0], dtype=torch.int32).to(self.device)
         logits = self._forward_ragged(step, pick)
+        self.logit_width = logits.shape[1] * self.model.tp
         for row, start, m in spans:
             self.row_len[row] = start + m
+        for row, tokens in portions:
+            self._give(row, [int(t) for t in tokens])
         self.seq_lens.index_copy_(0, torch.tensor([r for r, _, _ in spans]).to(self.device), step.seq_lens)
         return logits if rows else None
 
@@ -508,7 +550,7 @@ class LLMEngine:
         counted = [r for r in decode_rows if r in self.row_penalized]
         if counted:  # what was fed is a token of the answer by now
             of = torch.tensor(counted, dtype=torch.int32).to(self.device)
-            ops.count_tokens(self.logit_tables.counts, self.sampled.index_select(0, of.long()), of)
+            ops.count_tokens(self._tables(logits.shape[1] * self.model.tp).counts, self.sampled.index_select(0, of.long()), of)
         self.seq_lens.index_copy_(0, torch.tensor([r for r, _, _ in spans]).to(self.device), step.seq_lens)
         for r, a, m in spans:
             self.row_len[r] = a + m
@@ -524,7 +566,7 @@ class LLMEngine:
         for r, t in zip(answer, toks):
             if r in self.row_constraint:
                 self.row_constraint[r].advance(int(t))
-        return {r: int(t) for r, t in zip(answer, toks)}
+        return self._drew({r: int(t) for r, t in zip(answer, toks)})
 
     def save_session(self, row: int, session: str, tokens) -> None:
         """Keep row ``row``'s KV pages (and recurrent state) as the snapshot of conversation ``session``.  ``tokens``
@@ -994,12 +1036,12 @@ class LLMEngine:
             import sys
             import time
             t0 = time.perf_counter()
-            out = self._decode_rows(rows)
+            out = self._drew(self._decode_rows(rows))
             print(f"decode_profile rows={len(rows)} tokens={sum(len(v) if isinstance(v, list) else 1 for v in out.values())} "
                   f"wall_ms={(time.perf_counter() - t0) * 1e3:.3f}", file=sys.stderr)
             return out
         with scope("decode.step", self.device):
-            return self._decode_rows(rows)
+            return self._drew(self._decode_rows(rows))
 
     def _check_pages(self, rows) -> None:
         """A row that decodes past its reserved pages would read and write the shared null page (block-table entry 0)
@@ -1024,7 +1066,9 @@ class LLMEngine:
         self.active.copy_(mask.to(self.device), non_blocking=True)
         constrained = any(self._is_processed(r) for r in rows)
         if constrained:
-            self._write_limits(range(b), self.logit_tables.width)  # there since the rows' prompts were read
+            if self.logit_width is None:
+                raise RuntimeError("penalties go by the tokens of a row, and these have none yet: read a prompt first")
+            self._write_limits(range(b), self.logit_width)
         stochastic = any(self.row_stochastic.get(r, False) for r in rows)
         if self.mtp_k and not constrained:
             ctl = self.mtp_controller

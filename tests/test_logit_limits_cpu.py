@@ -115,3 +115,101 @@ def test_places_of_a_large_request_go_with_it():
     t = LogitTables(2, 2000, torch.device("cpu"))
     assert t.make_room(1500) and not t.make_room(600) and t.make_room(500)  # not back and forth between requests of like sizes
     assert t.make_room(1000) and not t.make_room(0)  # few enough to stay
+
+
+def words_of(engine, row, prompt, answer):
+    """What the counts of a row have to be."""
+    want = torch.zeros(engine.logit_tables.width, dtype=torch.int32)
+    for t in answer:
+        want[t] += 1
+    want[torch.tensor(prompt, dtype=torch.long)] |= 0x8000
+    return torch.equal(engine.logit_tables.counts[row].int() & 0xFFFF, want)
+
+
+def decoded(engine, row, steps):
+    out = []
+    for _ in range(steps):
+        assert engine.can_grow(row)
+        t = engine.decode([row])[row]
+        out += t if isinstance(t, list) else [t]
+    return out
+
+
+def test_penalties_on_a_row_whose_prompt_was_read_without(model):
+    """They go by this sequence's tokens, whoever had the row before, from the first step on and after an interval without."""
+    strong = params(presence_penalty=1e4)
+    for occupied in (False, True):
+        eng = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu")
+        if occupied:
+            eng.prefill(0, list(range(100, 159)), strong)
+            decoded(eng, 0, 3)
+            eng.release(0)
+        prompt = PROMPTS[0]
+        answer = [eng.prefill(0, prompt)] + decoded(eng, 0, 4)
+        plain = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu")
+        assert answer == [plain.prefill(0, prompt)] + decoded(plain, 0, 4)
+        eng.set_sampling(0, strong)
+        assert words_of(eng, 0, prompt, answer[:-1])
+        more = decoded(eng, 0, 6)
+        assert not set(more) & set(answer) and len(set(more)) == len(more)
+        answer += more
+        assert words_of(eng, 0, prompt, answer[:-1])
+        eng.set_sampling(0, None)
+        answer += decoded(eng, 0, 3)
+        eng.set_sampling(0, params(repetition_penalty=1e6))
+        assert words_of(eng, 0, prompt, answer[:-1])
+        more = decoded(eng, 0, 4)
+        assert not set(more) & (set(answer) | set(prompt))
+
+
+def test_penalties_after_draft_and_verify_cycles():
+    cfg = LlamaConfig.tiny()
+    model = LlamaModel(cfg, LlamaWeights.random_init(cfg, "cpu", seed=5, std=0.05, mtp=True))
+    eng = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu", mtp_draft_tokens=2)
+    prompt = PROMPTS[0]
+    answer = [eng.prefill(0, prompt)] + decoded(eng, 0, 5)
+    eng.set_sampling(0, params(presence_penalty=1e4))
+    assert words_of(eng, 0, prompt, answer[:-1])
+    more = decoded(eng, 0, 4)
+    assert not set(more) & set(answer) and len(set(more)) == len(more)
+
+
+def test_penalties_on_rows_that_were_extended():
+    """Given tokens count as a prompt's; in mixed batches, and for a row that was opened with penalties, too."""
+    eng = ragged_engine()
+    eng.open_row(2, params(presence_penalty=1e4))
+    eng.extend([(2, [5, 6, 7])])
+    eng.extend([(2, torch.tensor([8]))], [[0]])
+    eng.sampled[2] = 30  # what the caller drew from the logits
+    eng.row_drawn[2].append(30)
+    answer = [30] + decoded(eng, 2, 5)
+    assert words_of(eng, 2, [5, 6, 7, 8], answer[:-1]) and len(set(answer)) == len(answer)
+    eng.open_row(0)
+    eng.extend([(0, [9, 9])], [[1]])
+    eng.set_sampling(0, params(presence_penalty=2.0))
+    assert words_of(eng, 0, [9], [])
+    eng.begin_prompt(1, [3, 4, 5])
+    assert eng.can_grow(2)
+    answer.append(eng.mixed_step([2], [(1, 3)])[2])
+    assert words_of(eng, 2, [5, 6, 7, 8], answer[:-1]) and len(set(answer)) == len(answer)
+    eng.set_sampling(1, params(frequency_penalty=1.0))
+    assert words_of(eng, 1, [3, 4, 5], [])
+
+
+def test_penalties_that_have_nothing_to_go_by_are_refused(model):
+    eng = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu")
+    eng.prefill(0, PROMPTS[0], params(temperature=0.5))
+    eng.grow(0, 60)
+    eng.decode_step(1)
+    kept = eng.sample_rows[0].clone()
+    with pytest.raises(ValueError, match="penalties"):
+        eng.set_sampling(0, params(presence_penalty=1.0))
+    assert torch.equal(eng.sample_rows[0], kept) and 0 not in eng.row_penalized
+    eng.set_sampling(0, params())
+    eng.prefill(0, PROMPTS[0], params(presence_penalty=1.0))  # another sequence
+    assert words_of(eng, 0, PROMPTS[0], [])
+    empty = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu")
+    empty.open_row(0, params(presence_penalty=1.0))
+    empty.grow(0, 16)
+    with pytest.raises(RuntimeError, match="penalties"):
+        empty.decode([0])
