@@ -801,14 +801,18 @@ class LLMEngine:
         # few the step runs in waves instead, which also leaves its experts resident.
         res = self.model.residencies()
         snap = (self.seq_lens.clone(), self.sampled.clone())
-        counts = self.logit_tables.counts.clone() if constrained and self.logit_tables is not None else None
+        counts = fed = words = None
+        if constrained and self.logit_width is not None:  # the step counts the tokens that it feeds: a word a row
+            counts = self._tables(self.logit_width).counts[:b]
+            fed = self.sampled[:b, None].clamp(0, counts.shape[1] - 1).long()
+            words = counts.gather(1, fed)
         self.residency_stats["steps"] += 1
 
         def restore():
             self.seq_lens.copy_(snap[0])
             self.sampled.copy_(snap[1])  # the sampler's counter is the row length: a replay draws the same token
             if counts is not None:
-                self.logit_tables.counts.copy_(counts)
+                counts.scatter_(1, fed, words)
 
         for r in res:
             r.optimistic = True

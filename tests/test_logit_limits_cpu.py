@@ -213,3 +213,52 @@ def test_penalties_that_have_nothing_to_go_by_are_refused(model):
     empty.grow(0, 16)
     with pytest.raises(RuntimeError, match="penalties"):
         empty.decode([0])
+
+
+class Misses:
+    """Stands for layers whose experts are missing in the first attempts of a step."""
+
+    optimistic = False
+
+    def __init__(self, engine, attempts):
+        self.engine, self.attempts, self.run = engine, attempts, 0
+
+    def enable_optimistic(self, count):
+        self.count = count
+
+    def settle(self):
+        return "uploaded" if self.run < 9 else "fallback"
+
+
+@pytest.mark.parametrize("attempts", [1, 2, 9])
+def test_a_step_that_is_run_again_for_its_experts_counts_once(attempts):
+    """What it had counted is taken back word by word, not by a copy of the table."""
+    eng = ragged_engine()
+    misses = Misses(eng, attempts)
+    eng.model.residencies = lambda: [misses]
+    forward = eng.model.forward
+
+    def missing(step, cache, prefill, **how):
+        if misses.optimistic:
+            misses.count.fill_(int(misses.run < attempts))
+            misses.run += 1
+        return forward(step, cache, prefill, **how)
+
+    strong = params(presence_penalty=1e4)
+    eng.model.forward = missing
+    for row, prompt in enumerate(([5, 6, 7], [9, 8])):
+        eng.begin_prompt(row, prompt, strong if row else None)
+    answer = [eng.mixed_step([], [(0, 3), (1, 2)])[1]]
+    assert eng.enable_expert_residency_graphs()
+    counts = eng.logit_tables.counts
+
+    def whole(*_):
+        raise AssertionError("a copy of all counts")
+
+    counts.clone = whole
+    for _ in range(4):
+        misses.run = 0
+        assert eng.can_grow(0) and eng.can_grow(1)
+        answer.append(eng.decode([0, 1])[1])
+        assert words_of(eng, 1, [9, 8], answer[:-1])
+    assert len(set(answer)) == len(answer) and eng.logit_tables.counts is counts
