@@ -25,6 +25,7 @@ from ..utils.profiler import scope
 from .constraints import NEG, LogitTables, penalized, penalties
 from .kv_cache import PAGE_SIZE, PagedKVCache
 
+_PLANNED = ops.batch.MAX_REQUESTS
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 from ..config import current as _config, trace
 
@@ -480,7 +481,9 @@ class LLMEngine:
         if self.device.type == "cuda":
             host = host.pin_memory()
         row_ids, past, new = host.to(self.device, non_blocking=True)
-        plan = ops.plan_batch(self.cache.block_table, row_ids, past, new, tokens=total, page_size=self.cache.page_size)
+        plans = [ops.plan_batch(self.cache.block_table, row_ids[i : i + _PLANNED], past[i : i + _PLANNED], new[i : i + _PLANNED],
+                                tokens=starts[min(b, i + _PLANNED)] - starts[i], page_size=self.cache.page_size) for i in range(0, b, _PLANNED)]
+        plan = plans[0] if len(plans) == 1 else ops.BatchPlan.joined(plans)
         singles = next((i for i, m in enumerate(counts) if m != 1), b)
         if hasattr(self.model, "decode_splits"):
             self.model.attn_splits = self.model.decode_splits(max(1, singles), max(c + m for _, c, m in portions))

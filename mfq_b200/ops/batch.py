@@ -38,6 +38,20 @@ class BatchPlan:
             raise ValueError(f"the plan was refused: {_REFUSED[-tokens]}")
         return tokens, pages
 
+    @classmethod
+    def joined(cls, plans: list["BatchPlan"]) -> "BatchPlan":
+        """The plan of the plans' batches one after the other; every one has exactly as many places as tokens, or is refused."""
+        seqs, starts, first, at = [], [], 0, 0
+        for p in plans:
+            seqs.append(p.tok_seq + first)
+            starts.append(p.q_starts[0 if not starts else 1 :] + at)
+            first, at = first + p.seq_lens.numel(), at + p.positions.numel()
+        cat = lambda name: torch.cat([getattr(p, name) for p in plans])  # noqa: E731
+        info = torch.stack([p.info for p in plans])
+        refused = info[:, 0].amin().clamp(max=0)
+        info = torch.where(refused < 0, torch.stack([refused, torch.zeros_like(refused)]), info.sum(0).to(torch.int32))
+        return cls(cat("positions"), cat("slots"), torch.cat(seqs), torch.cat(starts), cat("seq_lens"), cat("block_table"), info)
+
 
 def plan_batch(block_table: torch.Tensor, rows: torch.Tensor, past: torch.Tensor, counts: torch.Tensor, *, tokens: int, page_size: int = 16,
                pages: torch.Tensor | None = None) -> BatchPlan:

@@ -262,3 +262,44 @@ def test_a_step_that_is_run_again_for_its_experts_counts_once(attempts):
         answer.append(eng.decode([0, 1])[1])
         assert words_of(eng, 1, [9, 8], answer[:-1])
     assert len(set(answer)) == len(answer) and eng.logit_tables.counts is counts
+
+
+def test_steps_of_more_portions_than_a_plan_takes():
+    """A batch may have as many rows as the engine."""
+    rows = 2 * ops.batch.MAX_REQUESTS + 3
+    eng = ragged_engine(max_batch=rows, max_seq_len=32)
+    held = []
+    forward = eng.model.forward
+
+    def seen(step, cache, prefill, **how):
+        held.append(step)
+        return forward(step, cache, prefill, **how)
+
+    eng.model.forward = seen
+    portions = [(r, [r % 97] * (1 + r % 3)) for r in range(rows)]
+    for r in range(rows):
+        eng.open_row(r)
+    for _ in range(2):
+        before = list(eng.row_len[r] for r in range(rows))
+        got = eng.extend(portions, [[len(t) - 1] for _, t in portions])
+        assert torch.equal(got, eng.model.table[torch.arange(rows) % 97])
+        step = held.pop()
+        at = 0
+        for i, r in enumerate(sorted(range(rows), key=lambda r: len(portions[r][1]) != 1)):
+            m, past = len(portions[r][1]), before[r]
+            assert step.positions[at : at + m].tolist() == list(range(past, past + m)) and step.tok_seq[at : at + m].tolist() == [i] * m
+            assert step.slots[at : at + m].tolist() == eng.cache.slots(eng.row_seq[r], past, m).tolist()
+            assert int(step.q_starts[i]) == at and int(step.seq_lens[i]) == past + m
+            assert step.block_table[i].tolist() == eng.cache.block_table[r].tolist()
+            at += m
+        assert int(step.q_starts[rows]) == at == step.positions.numel()
+
+
+def test_joined_plans_keep_a_refusal():
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    table = torch.arange(1, 9, dtype=torch.int32).view(2, 4)
+    good, bad = ops.plan_batch(table, i32(0), i32(3), i32(20), tokens=20), ops.plan_batch(table, i32(1), i32(60), i32(5), tokens=5)
+    assert ops.BatchPlan.joined([good, good]).check() == (40, 0)
+    for plans in ([good, bad], [bad, good]):
+        with pytest.raises(ValueError, match="more pages than a row"):
+            ops.BatchPlan.joined(plans).check()
