@@ -301,6 +301,8 @@ struct PlanArgs {
   int R, P, b, T, page_size, free_pages;  // free_pages < 0: none are handed out
 };
 
+__device__ __forceinline__ int pages_for(int tokens, int page_size) { return tokens / page_size + (tokens % page_size != 0); }  // a sum of the two may pass 31 bits
+
 __global__ void __launch_bounds__(kPlanThreads)
 plan_batch_kernel(const PlanArgs a) {
   pdl_trigger();
@@ -328,7 +330,7 @@ plan_batch_kernel(const PlanArgs a) {
     if (row < 0 || row >= a.R || past < 0 || count < 0) bad = max(bad, int(kPlanBadRequest));
     else if (len > static_cast<long long>(a.P) * ps) bad = max(bad, int(kPlanNoRoom));
     else {
-      const int have = (past + ps - 1) / ps;
+      const int have = pages_for(past, ps);
       if (hand) {
         want[k] = int((len + ps - 1) / ps) - have;
         if (atomicOr(&s_seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u) bad = max(bad, int(kPlanBadRequest));  // two requests would take pages for one row
@@ -410,7 +412,7 @@ plan_batch_kernel(const PlanArgs a) {
   for (long long e = static_cast<long long>(blockIdx.x) * kPlanThreads + tid; e < entries; e += step) {
     const int i = int(e / a.P), j = int(e - static_cast<long long>(i) * a.P);
     int page = 0;
-    if (!refused && j < (s_past[i] + s_start[i + 1] - s_start[i] + ps - 1) / ps) {
+    if (!refused && j < pages_for(s_past[i] + (s_start[i + 1] - s_start[i]), ps)) {
       page = page_of(i, j);
       if (hand && j >= s_have[i]) a.table[size_t(s_row[i]) * a.P + j] = page;
     }

@@ -168,3 +168,19 @@ def test_a_served_batch_and_its_captured_step():
     require_gpu_lib()
     assert serve("cuda") == serve("cuda", graphed=True), "the same kernels on the same inputs"
     check_status()
+
+
+@pytest.mark.parametrize("ps,past,count", [(2 ** 31 - 1, 5, 3), (2 ** 31 - 1, 0, 1), (2 ** 30 + 3, 2 ** 30 + 2, 1), (2 ** 30, 1, 7)])
+def test_plans_of_pages_of_nearly_2_to_the_31_tokens(ps, past, count):
+    """Lengths and the size of a page together pass 31 bits; a page of the past is none to hand out again."""
+    require_gpu_lib()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = i32([[0], [0]]), i32([1]), i32([past]), i32([count])
+    for pages in (None, i32([0, 0])):
+        kw = dict(tokens=count + 2, page_size=ps, pages=pages)
+        want, after = exact_plan(*args, **kw)
+        mine = args[0].clone()
+        plan = ops.plan_batch(mine, *args[1:], **kw)
+        for got, w in zip(plan_parts(plan), want):
+            assert got.tolist() == w
+        assert mine.tolist() == after and plan.check() == tuple(want[-1])
