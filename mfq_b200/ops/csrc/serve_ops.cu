@@ -442,7 +442,7 @@ extern "C" int mfq_process_logits(const void* logits, void* out, int dtype, int 
                                   int words, const int* rows, int first, float fill, cudaStream_t stream) {
   using namespace mfq;
   if (B <= 0 || B > 65535 || V <= 0 || R <= 0 || first < 0 || K < 0 || K > kMaxBias || dtype < 0 || dtype > 2) return -1;
-  if (V > 1 << 30 || first > INT32_MAX - V || (allowed && (first + V + 31) / 32 > words)) return -1;
+  if (V > 1 << 30 || first > INT32_MAX - V || (allowed && (static_cast<long long>(first) + V + 31) / 32 > words)) return -1;
   const LogitArgs a{logits, out, static_cast<const LogitRecord*>(records), static_cast<const unsigned short*>(counts), bias_ids, bias_values,
                     static_cast<const unsigned*>(allowed), rows, V, R, K, words, first, in_stride, out_stride, counts_stride, fill};
   const int size = dtype == 2 ? 4 : 2;

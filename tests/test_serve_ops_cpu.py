@@ -136,3 +136,12 @@ def test_plans_of_too_many_places_are_refused():
 
 def test_a_served_batch():
     serve("cpu")
+
+
+def test_the_c_entry_refuses_short_masks_of_the_last_tokens():
+    """Ids up to 2^31 - 2: the mask's words are counted without passing 31 bits (refused before anything is launched)."""
+    from mfq_b200.ops.lib import LIB_PATH, lib
+    if not LIB_PATH.exists():
+        pytest.skip("the CUDA library is not built")
+    for first, v in ((2 ** 31 - 2, 1), (2 ** 31 - 41, 40), (64, 33)):
+        assert lib().mfq_process_logits(16, 16, 0, 1, v, v, v, 16, 1, None, 0, None, None, 0, 16, (first + v + 31) // 32 - 1, None, first, 0.0, None) == -1
