@@ -327,7 +327,10 @@ __device__ __forceinline__ void unit_part(const SharedAttnArgs& a, uint8_t* smem
   load(t, g8, c);
   for (int i = 0; i < my_pages; ++i) {
     const int s = i % kStages;
-    if (!mbar_wait_warp(&full[s], (i / kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) break;
+    if (!mbar_wait_warp(&full[s], (i / kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) {
+      let_started_work_end();
+      break;
+    }
     t.page(ring + s * L::kStage, (page_lo + warp + 4 * i) << 4, g8, c);
     __syncwarp();
     if (lane == 0 && i + kStages < my_pages) issue(i + kStages);

@@ -27,6 +27,13 @@ __device__ __forceinline__ void shared_bulk_load(void* dst, const void* src, uin
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// Behind a wait that ran out (the status says so, results are invalid): copies and products that were started may still be on their way to memory that is
+// about to be used again or given back.
+__device__ __forceinline__ void let_started_work_end() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 2000000ull) {
+  }
+}
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t v) {  // two codes to fp16
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(v)));

@@ -590,6 +590,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       }
     }
   }
+  if (*abort_flag) let_started_work_end();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

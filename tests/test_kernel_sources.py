@@ -84,3 +84,15 @@ def test_barriers_of_the_grouped_product_have_their_place():
     scope = {"kStages": stages, "kAcc": acc}
     scope["kBarBytes"] = eval(m.group(1), scope) if (m := re.search(r"kBarBytes = (.*?);", text)) else 0
     assert stages == 10 and laid_out <= eval(size, scope) - 1024
+
+
+def test_a_ring_that_was_given_up_is_not_used_or_left_at_once():
+    """Copies that were started before a wait ran out may still arrive: the kernels of shared prefixes give them time before the ring becomes the
+    scratch of the merge, and before a block that holds tensor memory gives it back and ends."""
+    units = re.sub(r"//[^\n]*", "", (CSRC / "attn_shared.cu").read_text())
+    page_loop = units[units.index("unit_part(") : units.index("parts = reinterpret_cast<float*>(smem)")]
+    (given_up,) = re.findall(r"if \(!mbar_wait_warp\([^{;]*\)(.*?)break;", page_loop, re.S)
+    assert "let_started_work_end();" in given_up
+    tc = re.sub(r"//[^\n]*", "", (CSRC / "attn_shared_tc.cu").read_text())
+    end = tc.index("tmem_dealloc(")
+    assert re.search(r"if \(\*abort_flag\) let_started_work_end\(\);\s*tc_fence_before\(\);\s*__syncthreads\(\);\s*tc_fence_after\(\);\s*if \(warp == 7\) $", tc[:end])
