@@ -21,7 +21,7 @@ import torch
 
 from .. import ops
 
-PLACES_KEPT = 1024  # biases a row that tables keep room for
+PLACES_KEPT = 1024  # biases a row that tables keep room for: 64 rows of 128256 take 7.5 us with 8 places on a B200, 16.8 with 1024, 722 with 65536
 NEG = -1.0e30  # representable in bf16; exp() of it is 0 and an arg-max never picks it
 
 

@@ -8,6 +8,7 @@ from mfq_b200.engine.constraints import LogitTables
 from mfq_b200.engine.llm_engine import LLMEngine
 from mfq_b200.engine.scheduler import ContinuousBatchScheduler, Request
 from mfq_b200.models.llama import LlamaConfig, LlamaModel, LlamaWeights
+from mfq_b200.parallel.local_collective import LocalGroup
 from penalty_cases import PROMPTS, params
 from ragged_stub import ragged_engine
 
@@ -303,3 +304,36 @@ def test_joined_plans_keep_a_refusal():
     for plans in ([good, bad], [bad, good]):
         with pytest.raises(ValueError, match="more pages than a row"):
             ops.BatchPlan.joined(plans).check()
+
+
+def test_penalties_biases_and_masks_over_vocabulary_shards():
+    """Every rank processes its columns by its slice of the counts and by vocabulary ids: the shards together are what one rank makes of all columns, and a
+    request's answer is penalized, biased and the same on all ranks."""
+    cfg = LlamaConfig.tiny()
+    g = torch.Generator().manual_seed(1)
+    whole = torch.randn((2, cfg.vocab_size), generator=g)
+    words = torch.randint(-2 ** 31, 2 ** 31, (-(-cfg.vocab_size // 32),), generator=g).to(torch.int32)
+    bias = {3: 2.0, cfg.vocab_size // 2: 30.0, cfg.vocab_size - 1: -5.0}
+    forced = cfg.vocab_size - 7
+
+    def body(rank, collective, world):
+        how = {"tp_rank": rank, "tp_size": world} if world > 1 else {}
+        weights = LlamaWeights.random_init(cfg, "cpu", seed=7, **how)
+        eng = LLMEngine(LlamaModel(cfg, weights, collective=collective) if world > 1 else LlamaModel(cfg, weights), max_batch=2, max_seq_len=160, device="cpu")
+        for row, how in enumerate((params(presence_penalty=0.4, repetition_penalty=1.5, logit_bias=bias), params(frequency_penalty=0.7))):
+            eng.prefill(row, PROMPTS[row], how)
+            eng._write_limits([row], cfg.vocab_size)
+        eng.logit_tables.allowed[1].copy_(words)
+        v = cfg.vocab_size // world
+        shard = eng._process(whole[:, rank * v : (rank + 1) * v].clone())
+        eng.logit_tables.allowed[1].fill_(-1)
+        answer = [eng.prefill(0, PROMPTS[0], params(presence_penalty=1e4, logit_bias={forced: 100.0}))] + decoded(eng, 0, 6)
+        return shard, answer, eng.logit_tables.counts[0].tolist()
+
+    shard, answer, counts = body(0, None, 1)
+    assert shard.shape == whole.shape and not torch.equal(shard, whole)
+    ranks = LocalGroup(2).run(lambda rank, collective: body(rank, collective, 2))
+    assert torch.equal(torch.cat([s for s, _, _ in ranks], 1), shard)
+    for _, a, c in ranks:
+        assert a == ranks[0][1] and c == ranks[0][2] and a[0] == forced and len(set(a)) == len(a)
+        assert sum(x & 0x7FFF for x in c) == len(a) - 1
