@@ -196,9 +196,10 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
     ++taken;
     if (++slot == depth) { slot = 0; round ^= 1; }
   };
-  const auto drain = [&] {  // pages that were requested and that no row sees: their copies end before the CTA does
+  const auto drain = [&](bool ok) {  // copies end before the CTA does: of pages that no row sees, and of what a wait that ran out has left
+    if (!ok) let_started_work_end();
     while (taken < asked) {
-      ring_wait();
+      if (!ring_wait()) let_started_work_end();
       ring_next();
     }
   };
@@ -262,7 +263,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       }
       asked = __shfl_sync(0xffffffffu, asked, 0);
     }
-    drain();
+    drain(ok);
   } else if (warp < 7) {
     int first_page = w;  // of the block's pages, the first of this warp
     bool ok = true;
@@ -311,7 +312,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       asked = __shfl_sync(0xffffffffu, asked, 0);
       first_page = (first_page + 1) % 3;  // eight pages on: page p is warp p % 3's
     }
-    drain();
+    drain(ok);
   } else if (warp == 7) {
     if (steps > 0) {
       constexpr uint32_t idesc_qk = umma_idesc(128, 128, 0, 0), idesc_pv = umma_idesc(128, D, 0, 0);
@@ -348,6 +349,7 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
           if (!kTwoTiles || t == 1) tc_commit_warp(k_empty);
         }
       }
+      if (!ok) let_started_work_end();
     }
   } else {
     // ----- softmax: warps 8 - 15 stream 0, 16 - 23 stream 1; a warp has 32 rows and 64 of a block's keys, a lane parts of four rows -----
@@ -590,7 +592,6 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
       }
     }
   }
-  if (*abort_flag) let_started_work_end();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -94,5 +94,8 @@ def test_a_ring_that_was_given_up_is_not_used_or_left_at_once():
     (given_up,) = re.findall(r"if \(!mbar_wait_warp\([^{;]*\)(.*?)break;", page_loop, re.S)
     assert "let_started_work_end();" in given_up
     tc = re.sub(r"//[^\n]*", "", (CSRC / "attn_shared_tc.cu").read_text())
-    end = tc.index("tmem_dealloc(")
-    assert re.search(r"if \(\*abort_flag\) let_started_work_end\(\);\s*tc_fence_before\(\);\s*__syncthreads\(\);\s*tc_fence_after\(\);\s*if \(warp == 7\) $", tc[:end])
+    k_loader, v_loader, issuer = (tc[tc.index(a) : tc.index(b)] for a, b in (("if (warp < 4) {", "else if (warp < 7) {"), ("else if (warp < 7) {", "else if (warp == 7) {"),
+                                                                             ("else if (warp == 7) {", "scores = ")))
+    assert k_loader.rstrip("} \n").endswith("drain(ok);") and v_loader.rstrip("} \n").endswith("drain(ok);") and "if (!ok) let_started_work_end();" in issuer
+    (drain,) = re.findall(r"const auto drain = \[&\]\(bool ok\) \{(.*?)\n  \};", tc, re.S)
+    assert "if (!ok) let_started_work_end();" in drain and "if (!ring_wait()) let_started_work_end();" in drain
