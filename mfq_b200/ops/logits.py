@@ -17,6 +17,7 @@ from .lib import check, elsewhere, lib, ptr, stream_ptr
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_BIASES = 1 << 16  # places per row; kMaxBias of the kernel
+MAX_ROWS = 65535  # of logits on a GPU: blocks of a grid in y
 RECORD_WORDS = 8  # a sampling record: temperature f32, top_k i32, top_p f32, presence f32, frequency f32, repetition f32, seed u64
 
 
@@ -34,9 +35,10 @@ def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch
                    bias: tuple[torch.Tensor, torch.Tensor] | None = None, allowed: torch.Tensor | None = None,
                    rows: torch.Tensor | None = None, first: int = 0, fill: float = float("-inf"), out: torch.Tensor | None = None) -> torch.Tensor:
     """``logits [B, V]`` (bf16, fp16 or fp32; the rows may lie apart) with biases, penalties and mask applied in that order, in fp32,
-    rounded once.  Returns ``out``: a new tensor, one given, or ``logits`` itself.
+    rounded once; at most :data:`MAX_ROWS` rows on a GPU.  Returns ``out``: a new tensor, one given, or ``logits`` itself.
 
-    * ``records [R, 8]`` int32: the requests' sampling records; their penalties apply where ``counts`` is given;
+    * ``records [R, 8]`` int32: the requests' sampling records; their penalties apply where ``counts`` is given (16-bit logits on a GPU are multiplied by the
+      reciprocal of the repetition penalty, which is infinite for a factor under 2^-128);
     * ``counts [R, V]`` int16 words of :func:`count_tokens` (a column slice of a wider table will do);
     * ``bias`` = (ids ``[R, K]`` int32, values ``[R, K]`` fp32), at most :data:`MAX_BIASES` places a row; negative ids are unused places,
       an id that occurs twice has the sum;
@@ -81,6 +83,8 @@ def process_logits(logits: torch.Tensor, records: torch.Tensor, *, counts: torch
     if index < 0:
         out.copy_(reference.process_logits(logits, records, counts, bias, allowed, rows, first, fill))
         return out
+    if b > MAX_ROWS:
+        raise ValueError(f"{b} rows of logits, a call takes {MAX_ROWS}")
     if elsewhere(index):
         with torch.cuda.device(index):
             return process_logits(logits, records, counts=counts, bias=bias, allowed=allowed, rows=rows, first=first, fill=fill, out=out)

@@ -184,3 +184,12 @@ def test_plans_of_pages_of_nearly_2_to_the_31_tokens(ps, past, count):
         for got, w in zip(plan_parts(plan), want):
             assert got.tolist() == w
         assert mine.tolist() == after and plan.check() == tuple(want[-1])
+
+
+def test_more_rows_of_logits_than_a_grid_are_refused():
+    require_gpu_lib()
+    logits = torch.zeros((65536, 8), device="cuda")
+    rows = torch.zeros(65536, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="65535"):
+        ops.process_logits(logits, records([(0.0, 0.0, 1.0)], "cuda"), rows=rows)
+    ops.process_logits(logits[:65535], records([(0.0, 0.0, 1.0)], "cuda"), rows=rows[:65535])
