@@ -449,7 +449,7 @@ shared_tail_kernel(const SharedAttnArgs a) {
     return;
   }
   const int front = a.prefix_splits ? min(max(a.prefix_lens[group], 0) >> 4, a.max_pages) : 0;
-  const int all = max(min((max(seq_len, 0) + 15) >> 4, a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
+  const int all = max(min(int((unsigned(max(seq_len, 0)) + 15u) >> 4), a.max_pages) - front, 0), per = (all + ranks - 1) / ranks;
   const int page_lo = front + min(all, rank * per), page_hi = front + min(all, (rank + 1) * per);
   float *mine = reinterpret_cast<float*>(smem), *weights = mine + P::kEnd, *inverse = weights + 16 * (kMostRanks + kMostSlots);
   const auto row_of = [&](int r) -> long long { return r < rows ? (static_cast<long long>(row) * a.q_len + r / G) * a.Hq + kvh * G + r % G : -1; };
@@ -568,7 +568,7 @@ extern "C" int mfq_paged_attn_decode_shared(const void* q, const void* k, const 
                                             float* part_o, float* part_ml, int B, int Hq, int Hk, int D, int max_pages, int pages, int groups, int q_len,
                                             int tile, int prefix_splits, int tail_splits, float sm_scale, int* status, cudaStream_t stream) {
   using namespace mfq;
-  if (B <= 0 || B > 65535 || Hk <= 0 || Hk > 65535 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || pages < 1 || max_pages < 1)
+  if (B <= 0 || B > 65535 || Hk <= 0 || Hk > 65535 || Hq % Hk || q_len < 1 || (Hq / Hk) * q_len > 16 || groups < 1 || groups > B || pages < 1 || max_pages < 1 || max_pages >= 1 << 27)
     return -1;
   if (prefix_splits < 0 || prefix_splits * (tile == 128 ? 2 : 1) > kMostSlots || tail_splits < 1 || tail_splits > kMostRanks) return -1;
   if (prefix_splits && (D > 128 || (tile != 8 && tile != 16 && tile != 128 && tile != 256))) return -1;

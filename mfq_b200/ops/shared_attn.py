@@ -15,6 +15,7 @@ from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
 from .logits import _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
+MAX_ROWS = 65535  # of a batch: blocks of a grid in y
 SMS = 148
 
 
@@ -75,7 +76,8 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
                              max_group: int | None = None, max_prefix: int | None = None, max_tail: int | None = None,
                              out: torch.Tensor | None = None) -> torch.Tensor:
     """``q [B * q_len, Hq, D]`` (bf16) against the paged FP8 cache ``kv`` (a :class:`LayerKV`), ``D`` 64, 128 or 256 and at most 16 query heads
-    times ``q_len`` to a KV head; ``block_table [B, P]`` and ``seq_lens [B]`` int32 as for ``paged_attn_decode`` (the lengths count the query tokens too).
+    times ``q_len`` to a KV head; ``block_table [B, P]`` and ``seq_lens [B]`` int32 as for ``paged_attn_decode`` (the lengths count the query tokens too, and go up to
+    ``16 P``); at most :data:`MAX_ROWS` sequences.
 
     * ``members [B]`` int32: batch rows in the order of the groups, each once (default ``0 .. B - 1``);
     * ``group_starts [n + 1]`` int32, ascending: group ``g`` has the rows ``members[group_starts[g] : group_starts[g + 1]]``; rows behind
@@ -103,11 +105,13 @@ def paged_attn_decode_shared(q: torch.Tensor, kv, block_table: torch.Tensor, seq
     for t in (k, v, kv.k_scale, kv.v_scale):
         if t.get_device() != index or not t.is_contiguous():
             _refuse("kv", "contiguous pages on the device of q are", t)
-    if hq % hk or hq // hk * q_len > 16:
+    if hk < 1 or pages < 1 or hq % hk or hq // hk * q_len > 16:
         raise ValueError(f"{hq} query heads on {hk} KV heads in windows of {q_len}: at most 16 query rows a KV head are taken")
     if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous():
         _refuse("block_table", f"contiguous int32 [{b}, P] on the device of q is", block_table)
     groups, width = prefix_lens.numel(), block_table.shape[1]
+    if not 1 <= width < 1 << 27 or b > MAX_ROWS:
+        raise ValueError(f"{b} sequences of up to {width} pages: at most {MAX_ROWS}, of 1 to 2^27 - 1")
     _index("seq_lens", seq_lens, b, index)
     _index("group_starts", group_starts, groups + 1, index)
     _index("prefix_lens", prefix_lens, groups, index)

@@ -211,3 +211,15 @@ def test_equals_the_attention_of_unshared_rows():
         t.nan_to_num_(0.0)
     want = ops.paged_attn_decode(s.q, s.kv, s.table, s.seq_lens, sm_scale=s.scale, splits=4)
     assert_close(call(ops, s), want, rel=1e-2, what="shared against unshared")
+
+
+def test_lengths_of_nearly_2_to_the_31_see_all_of_their_table():
+    """A length behind the table's end sees what the table has, whatever is added to it on the way."""
+    require_gpu_lib()
+    s = batch(3, [(64, [96, 96, 96])], device="cuda")
+    want = exact(s)
+    s.table = s.table[:, :6].contiguous()
+    s.seq_lens.fill_(2 ** 31 - 1)
+    out = call(ops, s)
+    check_status()
+    assert_attends(s, out, want)

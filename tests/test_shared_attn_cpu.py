@@ -92,3 +92,26 @@ def test_chosen_forms_are_forms_that_the_kernels_have():
         tile, splits, ranks = _shape(b, per_seq, hk, d, groups, pick(1, max(1, b // groups), b), whole, tail)
         assert tile in (8, 16, 128, 256) and ranks in (1, 2, 4, 8) and 0 <= splits * (2 if tile == 128 else 1) <= 64
         assert splits == 0 or (d <= 128 and splits <= max(1, whole)) and (tile != 8 or per_seq <= 8)
+
+
+def test_pools_without_heads_and_tables_without_pages_are_refused():
+    s = batch(1, [(16, [20, 30])])
+    table = s.table
+    s.table = table[:, :0].contiguous()
+    with pytest.raises(ValueError, match="pages"):
+        call(ops, s)
+    s.table = table
+    for name in ("k", "v", "k_scale", "v_scale"):
+        setattr(s.kv, name, getattr(s.kv, name)[:, :0].contiguous())
+    with pytest.raises(ValueError, match="KV heads"):
+        call(ops, s)
+
+
+def test_batches_of_more_sequences_than_a_grid_are_refused():
+    n = 65536
+    s = batch(1, [(16, [20])], hq=1, hk=1, d=64)
+    i32 = torch.int32
+    s.q, s.table, s.seq_lens = s.q.expand(n, 1, 64).contiguous(), s.table.expand(n, -1).contiguous(), s.seq_lens.expand(n).contiguous()
+    s.starts, s.members = torch.tensor([0, n], dtype=i32), None
+    with pytest.raises(ValueError, match="65535"):
+        call(ops, s)
