@@ -8,7 +8,7 @@
 // and one split of the pages, and leaves (m, l, o) in fp32 for the merge.
 // The page layout is that of attn_decode.cu, which says how its fragments are single shared-memory loads.
 //
-// Numbers: a row of q is scaled by a power of two to 2^13 <= max |q| < 2^14, so that fp16 holds its bf16 values exactly unless they are 2^-27 of
+// Numbers: a row of q is scaled by a power of two to 2^13 <= max |q| < 2^14, so that fp16 holds its bf16 values exactly down to 2^-30 of
 // the largest; E4M3 is exact in fp16; a page's multipliers meet the scores in fp32.  P times the V multiplier is rounded to fp16 (2^-12) after a power of
 // two, kept for the rows of a warp, that brings the multipliers near 2^4 and is raised, the sums with it, where a page has larger ones.
 // The reference reads shared prefixes once per row (mfq/kernels/cuda/paged_kv.cu).

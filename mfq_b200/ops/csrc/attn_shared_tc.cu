@@ -354,7 +354,8 @@ shared_attn_tc_kernel(const SharedAttnArgs a) {
   } else {
     // ----- softmax: warps 8 - 15 stream 0, 16 - 23 stream 1; a warp has 32 rows and 64 of a block's keys, a lane parts of four rows -----
     const int t = (warp - 8) >> 3, half = (warp - 8) >> 2 & 1, quarter = warp & 3, c = lane & 3;
-    {  // 16 rows of Q to fp16, D / 8 lanes to a row: as they are where the largest value is between 2^-4 and 2^15 (exact down to 2^-21 of that), else scaled to 2^13
+    {  // 16 rows of Q to fp16, D / 8 lanes to a row: as they are where the largest value is between 2^-4 and 2^15 (bf16 values
+       // are exact in fp16 down to 2^-17, which is 2^-13 of 2^-4; smaller ones are off by at most 2^-25, which is 2^-21 of it), else scaled to 2^13
       constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
       const int row16 = (warp - 8) * 16 + lane / kLanes, piece = lane % kLanes;
       uint4 v[16 / kAtOnce];

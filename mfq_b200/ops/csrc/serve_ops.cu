@@ -235,6 +235,7 @@ mark_tokens_kernel(unsigned short* __restrict__ counts, long long stride, int R,
 // different one goes to the table once.  The common tokens of a text then meet in a few blocks instead of in every warp, and where not even all of the
 // call's tokens would bring a count past its largest value an addition that nothing waits for takes it there; a compare-and-swap does otherwise.
 // 32000 tokens of 24 rows on a B200: 32 us with warps that swapped, 12 with blocks that swapped, 4.5 now; 30000 of one row 595, 37, 6.6; 900 of two 10 with either, 3.3.
+// A call of more than 32767 tokens always swaps: 64000 of 24 rows 13 us, as by blocks that swapped before there were additions, 400000 of 200 rows 20 where those took 16.
 // Blocks of 256 or 1024 pairs are within a tenth.
 constexpr int kCountThreads = 512, kCountPlaces = 2 * kCountThreads;
 __global__ void __launch_bounds__(kCountThreads)
