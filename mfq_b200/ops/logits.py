@@ -99,8 +99,8 @@ def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, rows: torch.Tensor,
     answer, whose counts stay at 32767 once there, or with ``prompt`` as tokens that the prompt has.  A pair outside the table is left
     out, so a batch may be padded with negative rows.  Calls that count in the same rows follow one another: two at once could bring a count
     past 32767 between them."""
-    if counts.dtype is not torch.int16 or counts.ndim != 2 or (counts.shape[1] > 1 and counts.stride(1) != 1):
-        _refuse("counts", "int16 [R, V] with neighbouring columns are", counts)
+    if counts.dtype is not torch.int16 or counts.ndim != 2 or (counts.shape[1] > 1 and counts.stride(1) != 1) or (counts.shape[0] > 1 and counts.stride(0) < counts.shape[1]):
+        _refuse("counts", "int16 [R, V] with neighbouring columns and rows apart are", counts)
     index = counts.get_device()
     _index("tokens", tokens, None, index)
     _index("rows", rows, tokens.numel(), index)

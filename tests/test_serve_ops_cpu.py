@@ -145,3 +145,13 @@ def test_the_c_entry_refuses_short_masks_of_the_last_tokens():
         pytest.skip("the CUDA library is not built")
     for first, v in ((2 ** 31 - 2, 1), (2 ** 31 - 41, 40), (64, 33)):
         assert lib().mfq_process_logits(16, 16, 0, 1, v, v, v, 16, 1, None, 0, None, None, 0, 16, (first + v + 31) // 32 - 1, None, first, 0.0, None) == -1
+
+
+def test_rows_of_counts_that_lie_over_one_another_are_refused():
+    """A token of one row would be another's of the next."""
+    buffer, one = torch.zeros(40, dtype=torch.int16), torch.zeros(1, dtype=torch.int32)
+    for bad in (buffer[:9].expand(3, 9), buffer.as_strided((3, 9), (5, 1))):
+        with pytest.raises(ValueError, match="counts"):
+            ops.count_tokens(bad, one, one)
+    ops.count_tokens(buffer[:9].expand(1, 9), one, one)
+    assert buffer[0] == 1
