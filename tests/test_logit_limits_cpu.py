@@ -124,7 +124,7 @@ def words_of(engine, row, prompt, answer):
     for t in answer:
         want[t] += 1
     want[torch.tensor(prompt, dtype=torch.long)] |= 0x8000
-    return torch.equal(engine.logit_tables.counts[row].int() & 0xFFFF, want)
+    return torch.equal(engine.logit_tables.counts[row].cpu().int() & 0xFFFF, want)
 
 
 def decoded(engine, row, steps):
