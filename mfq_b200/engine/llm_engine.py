@@ -254,10 +254,8 @@ class LLMEngine:
         """Install the row's sampling record (``params``: a :class:`SamplingParams`-like object or None = greedy).  Penalties go by all
         tokens of the row's sequence, those from before the call too: a row advanced by :meth:`decode_step` itself, of whose tokens the engine keeps
         no record, cannot be given any."""
-        self.row_penalized.discard(row)
         if penalized(params):
             self._recount(row)
-            self.row_penalized.add(row)
         rec = torch.zeros(8, dtype=torch.int32)
         stochastic = bool(params is not None and getattr(params, "temperature", 0.0) > 0.0)
         if params is not None:
@@ -269,6 +267,9 @@ class LLMEngine:
             rec[5] = torch.tensor([1.0]).view(torch.int32)[0]
         self.sample_rows[row] = rec.to(self.device)
         self.row_stochastic[row] = stochastic
+        self.row_penalized.discard(row)
+        if penalized(params):
+            self.row_penalized.add(row)
 
     def _count(self, row: int, tokens, prompt: bool) -> None:
         ids = torch.as_tensor(tokens, dtype=torch.int32).to(self.device)

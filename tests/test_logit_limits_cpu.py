@@ -337,3 +337,14 @@ def test_penalties_biases_and_masks_over_vocabulary_shards():
     for _, a, c in ranks:
         assert a == ranks[0][1] and c == ranks[0][2] and a[0] == forced and len(set(a)) == len(a)
         assert sum(x & 0x7FFF for x in c) == len(a) - 1
+
+
+def test_a_refused_set_sampling_leaves_the_row_as_it_was(model):
+    eng = LLMEngine(model, max_batch=2, max_seq_len=160, device="cpu")
+    eng.prefill(0, PROMPTS[0], params(presence_penalty=1.0))
+    eng.grow(0, 60)
+    eng.decode_step(1, constrained=True)
+    kept, counts = eng.sample_rows[0].clone(), eng.logit_tables.counts.clone()
+    with pytest.raises(ValueError, match="penalties"):
+        eng.set_sampling(0, params(presence_penalty=2.0))
+    assert torch.equal(eng.sample_rows[0], kept) and 0 in eng.row_penalized and torch.equal(eng.logit_tables.counts, counts)
