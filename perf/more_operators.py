@@ -259,7 +259,7 @@ def _plain_codes(x):
     lower = torch.nextafter(scale, zero)
     scale = torch.where(scale.double() * 15 < wide, torch.nextafter(scale, far), torch.where(lower.double() * 15 >= wide, lower, scale))
     codes = torch.round((x.double() - least.double()[..., None]) / torch.where(scale > 0, scale, 1.0).double()[..., None])
-    bad = ~(x.abs() <= 2.0 ** 127).all(-1)
+    bad = ~(x.abs() <= 2.0 ** 126).all(-1)
     codes = torch.where(bad[..., None] | (scale == 0)[..., None], 0.0, codes)
     return codes.to(torch.uint8), torch.where(bad, math.nan, scale), torch.where(bad, math.nan, least)
 
