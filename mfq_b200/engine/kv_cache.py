@@ -1,5 +1,5 @@
-"""Paged KV caches: page tables (:class:`PagedTables`) over FP8 pages (:class:`PagedKVCache`) or over unquantized pages whose
-geometry may differ from layer to layer (:class:`PlainPagedKVCache`).
+"""Paged KV caches: page tables (:class:`PagedTables`) over FP8 pages (:class:`PagedKVCache`), over pages held in 4 bits
+(:class:`PagedKV4Cache`) or over unquantized pages whose geometry may differ from layer to layer (:class:`PlainPagedKVCache`).
 
 FP8 pool layout per layer (what the CUDA kernels index), chosen so that the decode-attention kernel can fetch a
 page with one bulk copy and read tensor-core fragments with single shared-memory loads:
@@ -204,3 +204,47 @@ class PagedKVCache(PagedTables):
 
     def bytes_per_token(self) -> int:
         return self.layers * self.kv_heads * (2 * self.head_dim + 8)
+
+
+@dataclass
+class LayerKV4:
+    """One layer's pages held in 4 bits: the record of a page and head has ``18 * head_dim`` bytes, K's codes and parameters, then V's, laid out as the operand
+    fragments of ``ops/csrc/kv4.cuh``; ``ops.kv4_write`` and ``ops.kv4_gather`` say what they stand for."""
+    data: torch.Tensor  # [pages, kv_heads, 18 * head_dim] uint8
+    head_dim: int
+    page_size: int
+
+
+class PagedKV4Cache(PagedTables):
+    """Pages of 16 tokens held in 4 bits, 4.5 with the parameters of every 64 values: ``1.125 * head_dim`` bytes a token and head for keys and values, against
+    ``2 * head_dim + 8`` in FP8 pages.  Written by ``ops.kv4_write``, read by ``ops.paged_attn_decode_kv4`` and ``ops.kv4_gather``."""
+
+    def __init__(self, *, layers: int, kv_heads: int, head_dim: int, num_pages: int, max_seqs: int,
+                 max_pages_per_seq: int, device: torch.device | str, page_size: int = PAGE_SIZE) -> None:
+        dev = torch.device(device)
+        super().__init__(num_pages=num_pages, max_seqs=max_seqs, max_pages_per_seq=max_pages_per_seq, device=dev, page_size=page_size)
+        if page_size != 16 or head_dim not in (64, 128, 256):
+            raise ValueError("the 4-bit page layout needs 16-token pages and heads of 64, 128 or 256")
+        self.head_dim, self.kv_heads, self.layers = head_dim, kv_heads, layers
+        self.data = torch.zeros((layers, num_pages, kv_heads, 18 * head_dim), dtype=torch.uint8, device=dev)
+        self._by_layer = [LayerKV4(self.data[i], head_dim, page_size) for i in range(layers)]
+
+    def layer(self, i: int) -> LayerKV4:
+        return self._by_layer[i]
+
+    def bytes_per_token(self) -> int:
+        return self.layers * self.kv_heads * 18 * self.head_dim // 16
+
+    def page_blob_bytes(self, pages: int) -> int:
+        return pages * self.page_size * self.bytes_per_token()
+
+    def export_pages(self, page_ids: list[int]):
+        """All layers' records of the given pages as one contiguous uint8 numpy array (host)."""
+        idx = torch.tensor(page_ids, dtype=torch.long, device=self.data.device)
+        return self.data.index_select(1, idx).reshape(-1).cpu().numpy()
+
+    def import_pages(self, page_ids: list[int], blob) -> None:
+        """Inverse of :meth:`export_pages` into (possibly different) physical pages."""
+        idx = torch.tensor(page_ids, dtype=torch.long, device=self.data.device)
+        raw = torch.from_numpy(blob).to(self.data.device)
+        self.data.index_copy_(1, idx, raw.view(self.layers, len(page_ids), self.kv_heads, 18 * self.head_dim))

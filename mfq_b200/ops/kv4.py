@@ -1,0 +1,161 @@
+"""A KV cache held in 4 bits: writing tokens into its pages (:func:`kv4_write`), reading them back (:func:`kv4_gather`), and decode attention over the pages
+(:func:`paged_attn_decode_kv4`).  The pool of a layer is a :class:`~mfq_b200.engine.kv_cache.LayerKV4`.
+
+A head's vector is held in groups of 64 values.  A group has a bf16 scale ``s``, a bf16 minimum ``m`` and a code ``c`` of 0 to 15 for each value, which
+stands for ``m + s c``: ``m`` is the largest bf16 that is not above the group's values, ``s`` the least one whose 15-fold reaches the largest value,
+``c`` the integer nearest to ``(x - m) / s``, ties to even, and 0 where ``s`` is 0.  So a value is off by at most ``s / 2``.  A group with a NaN or a magnitude above
+2^126 stands for NaN.  4.5 bits a value, 1.83 times the tokens of the FP8 pages; a value of normally distributed groups is off by 9 % of their deviation.
+
+The reference holds its pages in fp16, bf16 or TurboQuant codes (``cpp_runtime/backends/cuda/kernels/kv_quantization.cu``); this format is this repository's own.
+
+CPU tensors take the restatements in :mod:`mfq_b200.ops.reference`.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import reference
+from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
+from .logits import _DTYPES, _index, _refuse
+
+HEAD_DIMS = (64, 128, 256)
+MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
+
+
+def _pool(kv, index: int) -> tuple[int, int, int]:
+    """(pages, heads, head dim) of a pool that the kernels take."""
+    data = kv.data
+    if kv.page_size != 16 or data.dtype is not torch.uint8 or data.ndim != 3 or data.shape[2] not in (18 * 64, 18 * 128, 18 * 256) or not data.is_contiguous() or \
+            data.get_device() != index or not 1 <= data.shape[0] <= MAX_PAGES or data.shape[1] < 1:
+        _refuse("kv", f"contiguous uint8 [at most {MAX_PAGES} pages of 16 tokens, heads, 18 * (64 | 128 | 256)] on the device of the others are", data)
+    if data.data_ptr() & 15:
+        raise ValueError("kv: the pool has to begin on 16 bytes")
+    return data.shape[0], data.shape[1], data.shape[2] // 18
+
+
+def _rows(name: str, t: torch.Tensor, n: int, heads: int, d: int, index: int, *, written: bool = False) -> tuple[int, int]:
+    """Strides of tokens and heads of ``t [n, heads, d]``, which is read or written 16 bytes at a time."""
+    if t.ndim != 3 or t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1:
+        _refuse(name, f"bf16, fp16 or fp32 [{n}, {heads}, {d}] with neighbouring dims on the device of the others are", t)
+    a, b = (t.stride(0) if n > 1 else 0), (t.stride(1) if heads > 1 else 0)
+    unit = 16 // t.element_size()
+    if a % unit or b % unit or t.data_ptr() & 15:
+        raise ValueError(f"{name}: tokens and heads have to begin on 16 bytes, got strides {t.stride()} of {t.dtype}")
+    if written:  # heads inside a token or tokens inside a head: no two of them over one another
+        (near, count), (far, more) = sorted(((a, n) if n > 1 else (0, 1), (b, heads) if heads > 1 else (0, 1)))
+        if (count > 1 and near < d) or (more > 1 and far < (count - 1) * near + d):
+            raise ValueError(f"{name}: rows lie over one another, strides {t.stride()}")
+    return a, b
+
+
+def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None:
+    """Quantise ``k`` and ``v [T, heads, D]`` (bf16, fp16 or fp32; slices of a fused projection will do: tokens and heads may lie apart, in steps of 16 bytes)
+    into the pages of ``kv`` (a :class:`~mfq_b200.engine.kv_cache.LayerKV4`) at ``slots [T]`` int32: ``page * 16 + place``.  Tokens of negative slots are left out, so a
+    batch may be padded; a slot behind the pool is left out and reported by ``Workspace.check``.  A slot that several tokens of a call name holds codes
+    and parameters of any of them: a step writes a token once."""
+    index = k.get_device()
+    pages, heads, d = _pool(kv, index)
+    n = k.shape[0] if k.ndim == 3 else 0
+    ks, vs = _rows("k", k, n, heads, d, index), _rows("v", v, n, heads, d, index)
+    if v.dtype is not k.dtype:
+        _refuse("v", f"{k.dtype}, as k is,", v)
+    _index("slots", slots, n, index)
+    if n == 0:
+        return
+    if index < 0:
+        reference.kv4_write(kv, k, v, slots)
+        return
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return kv4_write(k, v, slots, kv)
+    check(lib().mfq_kv4_write(k.data_ptr(), v.data_ptr(), slots.data_ptr(), kv.data.data_ptr(), _DTYPES[k.dtype], n, heads, d, pages, *ks, *vs,
+                              Workspace.get(k.device).status.data_ptr(), stream_ptr()), "kv4_write")
+
+
+def _table(block_table: torch.Tensor, b: int, index: int) -> int:
+    if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous() or \
+            not 1 <= block_table.shape[1] < MAX_PAGES:
+        _refuse("block_table", f"contiguous int32 [{b}, 1 to {MAX_PAGES - 1} pages] on the device of the others is", block_table)
+    return block_table.shape[1]
+
+
+def kv4_gather(kv, block_table: torch.Tensor, starts: torch.Tensor, tokens: int | None = None, *, first: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cached keys and values of ragged sequences as packed rows ``[tokens, heads, D]`` of ``dtype`` (bf16, fp16 or fp32), for the attention of a prompt's next chunk.
+
+    * ``block_table [B, P]`` int32: the sequences' pages;
+    * ``starts [B + 1]`` int32, ascending: rows ``starts[i] : starts[i + 1]`` are sequence ``i``'s; rows in front of the first and behind the last are left as they were;
+    * ``first [B]`` int32: the position of each sequence's first row (default 0);
+    * ``k_out`` / ``v_out``: where to, both or neither (tokens and heads may lie apart, in steps of 16 bytes); they say ``tokens`` and ``dtype`` then.
+
+    A row without a page in the table, or whose page is out of range, is left as it was and reported by ``Workspace.check``."""
+    index = block_table.get_device()
+    pages, heads, d = _pool(kv, index)
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out are given together")
+    if k_out is None:
+        if tokens is None or not 0 <= tokens < 1 << 31:
+            raise ValueError(f"tokens: 0 to 2^31 - 1 rows wanted, got {tokens}")
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype: bf16, fp16 or fp32 wanted, got {dtype}")
+        k_out, v_out = (torch.empty((tokens, heads, d), dtype=dtype, device=block_table.device) for _ in range(2))
+    n = k_out.shape[0] if k_out.ndim == 3 else 0
+    if tokens is not None and tokens != n:
+        raise ValueError(f"tokens: {tokens}, but k_out has {n} rows")
+    ks, vs = _rows("k_out", k_out, n, heads, d, index, written=True), _rows("v_out", v_out, n, heads, d, index, written=True)
+    if v_out.dtype is not k_out.dtype:
+        _refuse("v_out", f"{k_out.dtype}, as k_out is,", v_out)
+    b = block_table.shape[0] if block_table.ndim == 2 else -1
+    width = _table(block_table, b, index)
+    _index("starts", starts, b + 1, index)
+    if first is not None:
+        _index("first", first, b, index)
+    if n == 0 or b == 0:
+        return k_out, v_out
+    if index < 0:
+        reference.kv4_gather(kv, block_table, starts, first, k_out, v_out)
+        return k_out, v_out
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return kv4_gather(kv, block_table, starts, tokens, first=first, k_out=k_out, v_out=v_out)
+    check(lib().mfq_kv4_gather(kv.data.data_ptr(), block_table.data_ptr(), starts.data_ptr(), ptr(first), k_out.data_ptr(), v_out.data_ptr(), _DTYPES[k_out.dtype], b, n, heads,
+                               d, width, pages, *ks, *vs, Workspace.get(block_table.device).status.data_ptr(), stream_ptr()), "kv4_gather")
+    return k_out, v_out
+
+
+def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, *, sm_scale: float, q_len: int = 1,
+                          max_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """What ``paged_attn_decode`` computes, over pages held in 4 bits: ``q [B * q_len, Hq, D]`` (bf16 or fp16) against the cache ``kv`` (a
+    :class:`~mfq_b200.engine.kv_cache.LayerKV4`); ``block_table [B, P]`` and ``seq_lens [B]`` int32.  The lengths count the query tokens too and go up to ``16 P``; a
+    window's query sees no later token of it, and one that sees nothing has zeros.  Any number of query heads to a KV head.
+
+    The tables and lengths may change on the device between replays of a graph.  ``max_len``: what the host knows of the longest sequence; it chooses the shape of the
+    launches, a wrong one costs time.  A page out of range that a sequence reads is reported by ``Workspace.check``; ``q`` and ``out`` begin on 16 bytes."""
+    index = q.get_device()
+    pages, hk, d = _pool(kv, index)
+    if q.ndim != 3 or q.dtype not in (torch.bfloat16, torch.float16) or not q.is_contiguous() or q.shape[2] != d or q_len < 1 or q.shape[0] % q_len:
+        _refuse("q", f"contiguous bf16 or fp16 [B * {q_len}, Hq, {d}] are", q)
+    n, hq, _ = q.shape
+    b = n // q_len
+    if hq < 1 or hq % hk:
+        raise ValueError(f"{hq} query heads on {hk} KV heads")
+    width = _table(block_table, b, index)
+    _index("seq_lens", seq_lens, b, index)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
+        _refuse("out", f"contiguous {q.dtype} {tuple(q.shape)} on the device of q is", out)
+    if (q.data_ptr() | out.data_ptr()) & 15:
+        raise ValueError("q and out have to begin on 16 bytes")
+    if b == 0:
+        return out
+    if index < 0:
+        out.copy_(reference.paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale, q_len))
+        return out
+    if elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale=sm_scale, q_len=q_len, max_len=max_len, out=out)
+    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), 0, 0, int(q.dtype is torch.float16), b, hq,
+                                          hk, d, width, pages, q_len, 1, 1, sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4")
+    return out

@@ -161,6 +161,116 @@ def write_kv(kv, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     kv.v_scale[pages, :, off] = vs
 
 
+KV4_GROUP = 64
+
+
+def _bf16_side(x: torch.Tensor, up: bool) -> torch.Tensor:
+    """The bf16 (as fp32) next to the fp32 ``x``: the least that is not below it, or the largest that is not above it."""
+    near = x.to(torch.bfloat16).float()
+    other = torch.nextafter(near.to(torch.bfloat16), torch.full_like(x, math.inf if up else -math.inf, dtype=torch.bfloat16)).float()
+    return torch.where(near < x if up else near > x, other, near)
+
+
+def kv4_quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``[T, H, D]`` -> codes ``[T, H, D]`` uint8, scales and minima ``[T, H, D / 64]`` fp32 (their values are bf16 ones)."""
+    g = x.float().unflatten(-1, (-1, KV4_GROUP))
+    bad = ((g != g) | (g.abs() > 2.0 ** 126)).any(-1)
+    g = torch.where(bad[..., None], torch.zeros_like(g), g).double()
+    m = _bf16_side(g.amin(-1).float(), up=False) + 0.0  # no negative zero
+    span = g.amax(-1) - m.double() + 0.0
+    s = _bf16_side((span / 15).float(), up=True)
+    down = torch.nextafter(s.to(torch.bfloat16), torch.zeros_like(s, dtype=torch.bfloat16)).float()
+    more = torch.nextafter(s.to(torch.bfloat16), torch.full_like(s, math.inf, dtype=torch.bfloat16)).float()
+    s = torch.where(15 * s.double() < span, more, torch.where((s > 0) & (15 * down.double() >= span), down, s))  # span / 15 was rounded
+    codes = ((g - m.double()[..., None]) / torch.where(s > 0, s, torch.ones_like(s)).double()[..., None]).round().clamp_(0, 15)
+    codes = torch.where((s > 0)[..., None], codes, torch.zeros_like(codes)).to(torch.uint8).flatten(-2)
+    nan = torch.full_like(s, math.nan)
+    return codes, torch.where(bad, nan, s), torch.where(bad, nan, m)
+
+
+def kv4_places(d: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Where a record has K's and V's codes: ``[2, 16 tokens, D / 2]`` bytes, in the order of the pairs (dim ``64 g + 16 j + i``, the one eight behind it)
+    by ``g``, ``j``, ``i``; and the first byte of each token's parameters ``[2, 16]``."""
+    t = torch.arange(16)[:, None]
+    n = torch.arange(d // 2)
+    g, j, i = n // 32, n // 8 % 4, n % 8
+    k = 512 * g + 64 * (t % 8) + 16 * (i // 2) + 4 * j + 2 * (i % 2) + t // 8
+    v = 512 * g + 64 * i + 16 * (t % 8 // 2) + 4 * j + 2 * (t % 2) + t // 8
+    params = 8 * d + (t[:, 0] % 8 * 2 + t[:, 0] // 8) * (d // 16)
+    return torch.stack([k, v + 9 * d]), torch.stack([params, params + 9 * d])
+
+
+def kv4_write(kv, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    pages, _, d = kv.data.shape[0], kv.data.shape[1], kv.data.shape[2] // 18
+    ok = (slots >= 0) & (slots < pages * 16)
+    if bool((slots >= pages * 16).any()):
+        raise ValueError("a slot lies behind the pool")
+    page, t = (slots[ok] // 16).long(), (slots[ok] % 16).long()
+    where, params = kv4_places(d)
+    for x, at, par in zip((k, v), where, params):
+        c, s, m = kv4_quantise(x[ok])
+        pair = c.unflatten(-1, (-1, 2, 8))
+        pair = (pair[..., 0, :] | pair[..., 1, :] << 4).flatten(-2)
+        head = torch.arange(kv.data.shape[1])[None, :, None]
+        kv.data[page[:, None, None], head, at[t][:, None]] = pair
+        bits = torch.stack([s, m], -1).to(torch.bfloat16).view(torch.int16)
+        bits = torch.where(torch.isnan(s)[..., None], torch.full_like(bits, 0x7FC0), bits)  # one NaN, whichever the conversion gives
+        both = bits.view(torch.uint8).flatten(-2)
+        kv.data[page[:, None, None], head, (par[t][:, None] + torch.arange(both.shape[-1]))[:, None]] = both
+
+
+def kv4_tokens(kv, pages: torch.Tensor, t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values ``[T, H, D]`` fp32 of the tokens ``t [T]`` of ``pages [T]``."""
+    d = kv.data.shape[2] // 18
+    where, params = kv4_places(d)
+    rec, out = kv.data[pages.long()], []
+    for at, par in zip(where, params):
+        byte = rec.gather(2, at[t.long()][:, None].expand(-1, rec.shape[1], -1)).unflatten(-1, (-1, 8))
+        codes = torch.stack([byte & 15, byte >> 4], -2).flatten(-3)
+        both = rec.gather(2, (par[t.long()][:, None] + torch.arange(d // 16))[:, None].expand(-1, rec.shape[1], -1)).contiguous().view(torch.bfloat16).float()
+        s, m = both[..., 0::2, None], both[..., 1::2, None]
+        out.append((m + s * codes.float().unflatten(-1, (-1, KV4_GROUP))).flatten(-2))
+    return out[0], out[1]
+
+
+def kv4_gather(kv, block_table, starts, first, k_out, v_out) -> None:
+    begin, pages = starts.tolist(), kv.data.shape[0]
+    for i in range(block_table.shape[0]):
+        a, b = max(0, begin[i]), min(begin[i + 1], k_out.shape[0])
+        if a >= b:
+            continue
+        pos = torch.arange(a, b) - begin[i] + (0 if first is None else int(first[i]))
+        if int(pos[0]) < 0 or int(pos[-1]) >= 16 * block_table.shape[1]:
+            raise ValueError(f"sequence {i}: positions {int(pos[0])} to {int(pos[-1])} of a table of {block_table.shape[1]} pages")
+        page = block_table[i][(pos // 16).long()]
+        if bool(((page < 0) | (page >= pages)).any()):
+            raise ValueError(f"sequence {i}: a page is out of range")
+        k, v = kv4_tokens(kv, page, pos % 16)
+        k_out[a:b], v_out[a:b] = k.to(k_out.dtype), v.to(v_out.dtype)
+
+
+def paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale, q_len: int = 1) -> torch.Tensor:
+    (n, hq, d), out = q.shape, torch.zeros_like(q)
+    hk = kv.data.shape[1]
+    for i in range(n // q_len):
+        length = min(int(seq_lens[i]), 16 * block_table.shape[1])
+        if length <= 0:
+            continue
+        pos = torch.arange(length)
+        page = block_table[i][pos // 16]
+        if bool(((page < 0) | (page >= kv.data.shape[0])).any()):
+            raise ValueError(f"sequence {i}: a page is out of range")
+        k, v = kv4_tokens(kv, page, pos % 16)
+        x = q[i * q_len : (i + 1) * q_len].float().view(q_len, hk, hq // hk, d)
+        scores = torch.einsum("qhgd,khd->hgqk", x, k) * sm_scale
+        seen = pos <= torch.arange(length - q_len, length)[:, None]
+        p = torch.softmax(scores.masked_fill(~seen, -math.inf), -1)
+        p = torch.where(seen.any(-1)[:, None], p, torch.zeros_like(p))  # a query in front of the first token sees nothing
+        o = torch.einsum("hgqk,khd->qhgd", p, v)
+        out[i * q_len : (i + 1) * q_len] = o.reshape(q_len, hq, d).to(q.dtype)
+    return out
+
+
 def process_logits(logits, records, counts=None, bias=None, allowed=None, rows=None, first: int = 0, fill: float = float("-inf")) -> torch.Tensor:
     b, v = logits.shape
     rows = torch.arange(b, device=logits.device) if rows is None else rows.long()
