@@ -1,6 +1,24 @@
-// Decode / verify attention over pages held in 4 bits (kv4.cuh has the format).
-// A warp takes one query row and head: token by token, with the running maximum and sum of the softmax; a lane has the dims of one byte of every group.
+// Decode / verify attention over pages held in 4 bits (kv4.cuh has the format and the layout of a page).
+//
+// With k = m + s c and v likewise, per group of 64 dims:
+//   score(q, t) = sum_g (s_tg sum_d q_d c_td + m_tg sum_d q_d)          the sums over d are the products' work, on codes alone
+//   o_d         = sum_t p_t (s_tg c_td + m_tg) / sum_t p_t                p_t s_tg is the products' operand, sum_t p_t m_tg is kept beside
+// so that a code is never turned into a value.  A code becomes an operand by one AND: 0 .. 15 in the low bits of an fp16 is c 2^-24, which tensor cores
+// multiply as any other number; in the next four bits it is 16 times that.  Two registers of a fragment have their codes 16 times as large: the dims
+// d + 8 of K, whose queries are divided by 16, and the rows d + 8 of V's output, which are divided in the end.
+//
+// A CTA has one sequence, one KV head, up to 8 or 16 of its query rows (query token, head of the group) and one split of the pages.  Its warps take
+// two pages at a time, in turn, each through a ring of bulk copies of its own.  A page's tokens are the rows of the products and the query rows their columns:
+//   S^T [16 x 8] = K Q^T,   O^T [D x 8] += V^T (p s),   p s being S^T's accumulator transposed by movmatrix.
+//
+// Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
+// maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum, less a power of two that brings the
+// scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest.  Scales of V between 2^-98 and 2^98.
+#include "attn_shared.cuh"
 #include "kv4.cuh"
+
+#include <cfloat>
+#include <climits>
 
 namespace mfq {
 
@@ -9,92 +27,476 @@ struct Kv4AttnArgs {
   const uint8_t* pool;
   const int *table, *seq_lens;
   void* out;
-  float *part_o, *part_ml;
+  float *part_o, *part_ml;  // [B * q_len * Hq, splits, D], [.., splits, 2]
   int* status;
-  int B, Hq, Hk, width, pages, q_len, splits, chunk;
+  int B, Hq, Hk, width, pages, q_len, splits, chunk, tiles;  // chunk: pages; tiles: of query rows of a KV head
   float scale_log2;
 };
 
-template <int D, bool kHalf>
-__global__ void __launch_bounds__(128) kv4_attn_kernel(Kv4AttnArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int G = D / 64;
-  const int lane = threadIdx.x & 31, j = lane >> 3, i = lane & 7;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (unit >= (long long)a.B * a.q_len * a.Hq) return;
-  const long long row = unit / a.Hq;
-  const int head = int(unit % a.Hq), kvh = head / (a.Hq / a.Hk), seq = int(row / a.q_len);
-  const int len = int(min((long long)a.seq_lens[seq], 16ll * a.width)) - (a.q_len - 1 - int(row % a.q_len));
-  float q[G][2], o[G][2], top = -INFINITY, sum = 0.f;
+template <int D>
+struct Kv4Ring {
+  static constexpr int kRecord = 18 * D, kStage = 2 * kRecord, kStages = D <= 128 ? 3 : 2, kWarps = 4;
+  static constexpr int kWarp = kStages * kStage, kBars = kWarps * kWarp, kSmem = kBars + kWarps * kStages * 8 + 16;
+};
+
+__device__ __forceinline__ float kv4_exp2(float x) {  // results under 2^-126 are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t kv4_transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void kv4_product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  const uint32_t a[4] = {a0, a1, a2, a3};
+  mma_half(d, a, b0, b1);
+}
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+
+template <typename T> __device__ __forceinline__ float2 kv4_pair(uint32_t v);
+template <> __device__ __forceinline__ float2 kv4_pair<__nv_bfloat16>(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 kv4_pair<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+template <typename T> __device__ __forceinline__ T kv4_out(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 kv4_out(float v) { return __float2bfloat16(v); }
+template <> __device__ __forceinline__ __half kv4_out(float v) { return __float2half_rn(v); }
+
+// What a warp has of its query rows: column blocks of 8, a lane has the columns 8 b + 2 c and the one behind it
+template <int D, int NB, typename T>
+struct Kv4Rows {
+  static constexpr int G = D / 64, kSteps = D / 16;
+  uint32_t q[NB][kSteps][2];
+  float sums[NB][G][2], to_log2[NB][2];        // of a group's q; what a score in units of the products is times log2 e
+  float o[NB][kSteps][4], om[NB][G][2], l[NB][2], top[NB][2], ref[NB][2];
+  float up, over;  // log2 of what V's scales are multiplied by, and the scale that would be too large
+  int len[NB][2], low, most;
+
+  __device__ __forceinline__ void load(const Kv4AttnArgs& a, int seq, int kvh, int first, int rows, int length) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3, per = a.Hq / a.Hk;
+    int lo = INT_MAX, hi = 0;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
+    for (int b = 0; b < NB; ++b) {
+      const int r = first + 8 * b + g8;
+      const bool there = r < rows;
+      uint32_t raw[kSteps][2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const size_t at = size_t(unit) * D + 64 * g + 16 * j + i + 8 * e;
-      q[g][e] = (kHalf ? __half2float(static_cast<const __half*>(a.q)[at]) : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at])) * a.scale_log2;
-      o[g][e] = 0.f;
-    }
-  }
-  for (int t = 0; t < len; ++t) {
-    int page = a.table[size_t(seq) * a.width + (t >> 4)];
-    if (page < 0 || page >= a.pages) {
-      if (lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
-      page = 0;
-    }
-    const uint8_t* rec = a.pool + (size_t(page) * a.Hk + kvh) * (18 * D);
-    float part = 0.f, v[G][2];
+      for (int s = 0; s < kSteps; ++s) raw[s][0] = raw[s][1] = 0;
+      if (there) {
+        const T* qp = static_cast<const T*>(a.q) + ((size_t(seq) * a.q_len + r / per) * a.Hq + kvh * per + r % per) * D + 2 * c;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int at = 8 * D + kv4_param_byte<D>(t & 15) + 4 * g;
-      const uint32_t kp = *reinterpret_cast<const uint32_t*>(rec + at), vp = *reinterpret_cast<const uint32_t*>(rec + 9 * D + at);
-      const uint32_t kc = rec[kv4_k_byte(t & 15, g, j, i)], vc = rec[9 * D + kv4_v_byte(t & 15, g, j, i)];
-      const float ks = __uint_as_float(kp << 16), km = __uint_as_float(kp & 0xffff0000u), vs = __uint_as_float(vp << 16), vm = __uint_as_float(vp & 0xffff0000u);
+        for (int s = 0; s < kSteps; ++s) {
+          raw[s][0] = *reinterpret_cast<const uint32_t*>(qp + 16 * s);
+          raw[s][1] = *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8);
+        }
+      }
+      float big = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 v = kv4_pair<T>(raw[s][e]);
+          big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const float scale = power_to(big, 10);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 4 * g; s < 4 * g + 4; ++s) {
+          const float2 v = kv4_pair<T>(raw[s][0]), w = kv4_pair<T>(raw[s][1]);
+          q[b][s][0] = half_pair(v.x * scale, v.y * scale);
+          q[b][s][1] = half_pair(w.x * scale * 0.0625f, w.y * scale * 0.0625f);
+          sum += (v.x * scale + v.y * scale) + (w.x * scale + w.y * scale);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= 0x1p-24f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sums[b][g][e] = __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        part += q[g][e] * fmaf(ks, float(kc >> (4 * e) & 15), km);
-        v[g][e] = fmaf(vs, float(vc >> (4 * e) & 15), vm);
+        to_log2[b][e] = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, scale, (2 * c + e) * 4);
+        const int mine = first + 8 * b + 2 * c + e;
+        // a row that is not there has a zero query and is never stored: unmasked, it leaves `low` to the others
+        len[b][e] = mine < rows ? max(0, length - (a.q_len - 1 - mine / per)) : INT_MAX;
+        lo = min(lo, len[b][e]);
+        if (mine < rows) hi = max(hi, len[b][e]);
+        top[b][e] = ref[b][e] = -FLT_MAX;
+        l[b][e] = 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) o[b][s][0] = o[b][s][1] = o[b][s][2] = o[b][s][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) om[b][g][0] = om[b][g][1] = 0.f;
+    }
+    low = __reduce_min_sync(0xffffffffu, lo);
+    most = __reduce_max_sync(0xffffffffu, hi);
+    up = 0.f;
+    over = 0.f;  // none chosen yet
+  }
+
+  // Two pages whose first token is tok0
+  __device__ __forceinline__ void pages(const uint8_t* rec0, int tok0) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
+    const bool whole = tok0 + 32 <= low;  // all rows see all of both
+    float sc[NB][2][4];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint8_t* rec = rec0 + p * 18 * D;
+      uint32_t par[2][G];  // of tokens g8 and g8 + 8
+      params(par, rec + 8 * D + g8 * (D / 8));
+#pragma unroll
+      for (int b = 0; b < NB; ++b) sc[b][p][0] = sc[b][p][1] = sc[b][p][2] = sc[b][p][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        float acc[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t h = w[j] >> 8;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) kv4_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
+        }
+        const float s0 = __uint_as_float(par[0][g] << 16), m0 = __uint_as_float(par[0][g] & 0xffff0000u);
+        const float s1 = __uint_as_float(par[1][g] << 16), m1 = __uint_as_float(par[1][g] & 0xffff0000u);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sc[b][p][e] = fmaf(s0, acc[b][e], fmaf(m0, sums[b][g][e], sc[b][p][e]));
+            sc[b][p][2 + e] = fmaf(s1, acc[b][2 + e], fmaf(m1, sums[b][g][e], sc[b][p][2 + e]));
+          }
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[b][p][x] *= to_log2[b][x & 1];
       }
     }
+    if (!whole) {
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) part += __shfl_xor_sync(0xffffffffu, part, x);
-    const float next = fmaxf(top, part), keep = exp2f(top - next), p = exp2f(part - next);
-    top = next;
-    sum = sum * keep + p;
+      for (int b = 0; b < NB; ++b) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      o[g][0] = o[g][0] * keep + p * v[g][0];
-      o[g][1] = o[g][1] * keep + p * v[g][1];
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (tok0 + 16 * p + g8 + 8 * (x >> 1) >= len[b][x & 1]) sc[b][p][x] = -INFINITY;
+        }
+      }
+    }
+    // parameters of V, none where nobody sees the token: what is there may be anything
+    uint32_t par[2][2][G];
+    float widest = 0.f;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      params(par[p], rec0 + p * 18 * D + 17 * D + g8 * (D / 8));
+      if (!whole) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            if (tok0 + 16 * p + g8 + 8 * h >= most) par[p][h][g] = 0;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) widest = fmaxf(widest, __uint_as_float(par[p][h][g] << 16));
+      }
+    }
+    float mx[NB][2];
+    bool moves = widest > over;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[b][e] = fmaxf(fmaxf(sc[b][0][e], sc[b][0][2 + e]), fmaxf(sc[b][1][e], sc[b][1][2 + e]));
+        moves |= mx[b][e] - 6.f > top[b][e];
+      }
+    }
+    if (__any_sync(0xffffffffu, moves)) move(mx, widest);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint8_t* rec = rec0 + p * 18 * D + 9 * D;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[b][p][x] = kv4_exp2(sc[b][p][x] - ref[b][x & 1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[b][e] += sc[b][p][e] + sc[b][p][2 + e];
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float s0 = __uint_as_float(par[p][0][g] << 16), m0 = __uint_as_float(par[p][0][g] & 0xffff0000u);
+        const float s1 = __uint_as_float(par[p][1][g] << 16), m1 = __uint_as_float(par[p][1][g] & 0xffff0000u);
+        uint32_t pb[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          float* t = sc[b][p];
+          float ps[4] = {t[0] * s0, t[1] * s0, t[2] * s1, t[3] * s1};
+          float pm[2] = {fmaf(t[0], m0, t[2] * m1), fmaf(t[1], m0, t[3] * m1)};
+          if (!whole) {  // a NaN stays with the rows that see it
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (tok0 + 16 * p + g8 + 8 * (x >> 1) >= len[b][x & 1]) ps[x] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              pm[e] = tok0 + 16 * p + g8 + 8 < len[b][e] ? pm[e] : (tok0 + 16 * p + g8 < len[b][e] ? t[e] * m0 : 0.f);
+            }
+          }
+          om[b][g][0] += pm[0];
+          om[b][g][1] += pm[1];
+          pb[b][0] = kv4_transposed(half_pair(ps[0], ps[1]));
+          pb[b][1] = kv4_transposed(half_pair(ps[2], ps[3]));
+        }
+        const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t h = w[j] >> 8;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, pb[b][0], pb[b][1]);
+        }
+      }
     }
   }
+
+  static __device__ __forceinline__ void params(uint32_t (&par)[2][G], const uint8_t* at) {  // [half][group] in a row
+    if constexpr (G == 1) {
+      const uint2 v = *reinterpret_cast<const uint2*>(at);
+      par[0][0] = v.x; par[1][0] = v.y;
+    } else {
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
+      for (int i = 0; i < 2 * G; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at + 4 * i);
+        par[i / G][i % G] = v.x; par[(i + 1) / G][(i + 1) % G] = v.y; par[(i + 2) / G][(i + 2) % G] = v.z; par[(i + 3) / G][(i + 3) % G] = v.w;
+      }
+    }
+  }
+
+  // New references: the running maxima and the power of two of V's scales
+  __device__ __forceinline__ void move(const float (&mx)[NB][2], float widest);
+};
+
+template <int D, int NB, typename T>
+__device__ __forceinline__ void Kv4Rows<D, NB, T>::move(const float (&mx)[NB][2], float widest) {
+  widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)));
+  if (widest > over) {
+    const int e = int(__float_as_uint(widest) >> 23) - 127;  // of a denormal one: -127
+    up = fminf(7.f - float(e), 104.f);
+    over = kv4_exp2(9.f - up);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float corr[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const size_t at = size_t(unit) * D + 64 * g + 16 * j + i + 8 * e;
-      const float y = len > 0 ? o[g][e] / sum : 0.f;
-      if (kHalf) static_cast<__half*>(a.out)[at] = __float2half_rn(y);
-      else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(y);
+      float m = mx[b][e];
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      top[b][e] = fmaxf(top[b][e], m);
+      const float next = top[b][e] - up;
+      corr[e] = kv4_exp2(ref[b][e] - next);
+      ref[b][e] = next;
+      l[b][e] *= corr[e];
+#pragma unroll
+      for (int g = 0; g < G; ++g) om[b][g][e] *= corr[e];
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) { o[b][s][0] *= corr[0]; o[b][s][1] *= corr[1]; o[b][s][2] *= corr[0]; o[b][s][3] *= corr[1]; }
+  }
+}
+
+template <int D, int NB, typename T, int kMinBlocks>
+__global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a) {
+  pdl_trigger();
+  using L = Kv4Ring<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l)
+  static_assert(kPart * 4 <= L::kWarp, "the ring is where a warp leaves its sums");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * L::kWarp;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars) + warp * L::kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBars + L::kWarps * L::kStages * 8);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int s = 0; s < L::kStages; ++s) mbar_init(&full[s], 2);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  pdl_wait();
+
+  const int seq = blockIdx.x, kvh = blockIdx.y / a.tiles, first = blockIdx.y % a.tiles * 8 * NB, split = blockIdx.z;
+  const int rows = a.Hq / a.Hk * a.q_len;
+  const int length = int(max(0ll, min((long long)a.seq_lens[seq], 16ll * a.width)));
+  const int total = (length + 15) >> 4, per = a.chunk / (2 * L::kWarps);  // pages; pairs of a chunk that a warp has
+  // chunks split, split + splits, ...; a warp's pairs in them
+  int mine = 0;
+  {
+    const int whole = total / a.chunk, left = total - whole * a.chunk;
+    mine = (whole > split ? (whole - split + a.splits - 1) / a.splits : 0) * per;
+    if (left > 2 * warp && whole >= split && (whole - split) % a.splits == 0) mine += (left - 2 * warp + 2 * L::kWarps - 1) / (2 * L::kWarps);
+  }
+  if (a.splits > 1 && (long long)split * a.chunk >= total) return;  // nothing here, and nobody looks
+  const int* bt = a.table + size_t(seq) * a.width;
+  const auto page_of = [&](int i) { return (split + i / per * a.splits) * a.chunk + 2 * (warp + L::kWarps * (i % per)) + lane; };
+  const auto id_of = [&](int i) {  // of lanes 0 and 1, their page of pair i; -1: there is none
+    const int at = page_of(i);
+    return i < mine && at < total ? bt[at] : -1;
+  };
+  const auto issue = [&](int i, int id, bool there) {
+    const int s = i % L::kStages;
+    if (!there) {
+      mbar_arrive(&full[s]);
+      return;
+    }
+    if (id < 0 || id >= a.pages) {
+      atomicCAS(a.status, 0, kStatusBadArgument);
+      id = 0;
+    }
+    mbar_expect_tx(&full[s], L::kRecord);
+    shared_bulk_load(ring + s * L::kStage + lane * L::kRecord, a.pool + (size_t(id) * a.Hk + kvh) * L::kRecord, L::kRecord, &full[s]);
+  };
+  int next = -1;
+  if (lane < 2) {
+    for (int i = 0; i < min(mine, L::kStages); ++i) issue(i, id_of(i), page_of(i) < total);
+    next = id_of(L::kStages);
+  }
+  Kv4Rows<D, NB, T> t;
+  t.load(a, seq, kvh, first, rows, length);
+  for (int i = 0; i < mine; ++i) {
+    const int s = i % L::kStages;
+    if (!mbar_wait_warp(&full[s], (i / L::kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) {
+      let_started_work_end();
+      break;
+    }
+    t.pages(ring + s * L::kStage, ((split + i / per * a.splits) * a.chunk + 2 * (warp + L::kWarps * (i % per))) << 4);
+    __syncwarp();
+    if (lane < 2 && i + L::kStages < mine) {
+      issue(i + L::kStages, next, page_of(i + L::kStages) < total);
+      next = id_of(i + 1 + L::kStages);
+    }
+  }
+
+  // ---- the lanes of a column, then the warps ----
+  float* part = reinterpret_cast<float*>(ring);
+  float* ml = part + 8 * NB * kStride;
+  __syncwarp();
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * b + 2 * c + e;
+      float sum = t.l[b][e];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (g8 == 0) { ml[2 * r] = t.ref[b][e]; ml[2 * r + 1] = sum; }
+#pragma unroll
+      for (int g = 0; g < D / 64; ++g) {
+        float om = t.om[b][g][e];
+        om += __shfl_xor_sync(0xffffffffu, om, 4);
+        om += __shfl_xor_sync(0xffffffffu, om, 8);
+        om += __shfl_xor_sync(0xffffffffu, om, 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          part[r * kStride + 64 * g + 16 * j + g8] = fmaf(t.o[b][4 * g + j][e], 0x1p24f, om);
+          part[r * kStride + 64 * g + 16 * j + 8 + g8] = fmaf(t.o[b][4 * g + j][2 + e], 0x1p20f, om);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag) return;
+  const int here = min(rows - first, 8 * NB), per_head = a.Hq / a.Hk;
+  for (int i = threadIdx.x; i < here * D; i += 128) {
+    const int r = i / D, d = i % D;
+    float ref = -FLT_MAX, l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < L::kWarps; ++w) ref = fmaxf(ref, reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
+#pragma unroll
+    for (int w = 0; w < L::kWarps; ++w) {
+      const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
+      const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref);
+      l += from[8 * NB * kStride + 2 * r + 1] * weight;
+      o += from[r * kStride + d] * weight;
+    }
+    const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
+    if (a.splits == 1) {
+      static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
+    } else {
+      a.part_o[(row * a.splits + split) * D + d] = o;
+      if (d == 0) { a.part_ml[(row * a.splits + split) * 2] = ref; a.part_ml[(row * a.splits + split) * 2 + 1] = l; }
     }
   }
 }
 
+// Joins the splits of a query row and head; those behind the sequence's last chunk left nothing.
+template <int D, typename T>
+__global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const size_t row = blockIdx.x;
+  const int d = threadIdx.x;
+  const int length = int(max(0ll, min((long long)a.seq_lens[row / a.Hq / a.q_len], 16ll * a.width)));
+  const int n = min(a.splits, (((length + 15) >> 4) + a.chunk - 1) / a.chunk);
+  const float* ml = a.part_ml + row * a.splits * 2;
+  const float* po = a.part_o + row * a.splits * D + d;
+  float ref = -FLT_MAX, l = 0.f, o = 0.f;
+  for (int i = 0; i < n; ++i) ref = fmaxf(ref, ml[2 * i]);
+  for (int i = 0; i < n; ++i) {
+    const float weight = kv4_exp2(ml[2 * i] - ref);
+    l += ml[2 * i + 1] * weight;
+    o += po[size_t(i) * D] * weight;
+  }
+  static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
+}
+
+template <int D, int NB, typename T>
+static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
+  using L = Kv4Ring<D>;
+  constexpr int kMinBlocks = D == 256 ? (NB == 1 ? 2 : 1) : (NB == 1 ? 4 : 3);
+  auto kernel = &kv4_attn_kernel<D, NB, T, kMinBlocks>;
+  static bool attr[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
+  if (!attr[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return -6;
+    attr[dev] = true;
+  }
+  const long long rows = (long long)a.Hq / a.Hk * a.q_len, tiles = (rows + 8 * NB - 1) / (8 * NB);
+  if (a.Hk * tiles > 65535 || a.splits > 65535 || (long long)a.B * a.q_len * a.Hq > 0x7fffffffll || a.chunk % (2 * L::kWarps)) return -2;
+  a.tiles = int(tiles);
+  if (launch_kernel(kernel, dim3(a.B, unsigned(a.Hk * tiles), a.splits), dim3(128), L::kSmem, stream, a) != cudaSuccess) return -7;
+  if (a.splits > 1 && launch_kernel(&kv4_merge_kernel<D, T>, dim3(unsigned(a.B * a.q_len * a.Hq)), dim3(D), 0, stream, a) != cudaSuccess) return -7;
+  return 0;
+}
 template <int D>
 static int launch_kv4_attn(const Kv4AttnArgs& a, bool half, cudaStream_t stream) {
-  const long long blocks = ((long long)a.B * a.q_len * a.Hq + 3) / 4;
-  if (blocks > 0x7fffffffll) return -2;
-  return launch_kernel(half ? kv4_attn_kernel<D, true> : kv4_attn_kernel<D, false>, dim3(unsigned(blocks)), dim3(128), 0, stream, a) == cudaSuccess ? 0 : -7;
+  if ((long long)a.Hq / a.Hk * a.q_len <= 8) return half ? launch_kv4_attn_of<D, 1, __half>(a, stream) : launch_kv4_attn_of<D, 1, __nv_bfloat16>(a, stream);
+  return half ? launch_kv4_attn_of<D, 2, __half>(a, stream) : launch_kv4_attn_of<D, 2, __nv_bfloat16>(a, stream);
 }
 
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16 or fp16 (`half`); pool: [pages, Hk, 18 D]; table: [B, width]; seq_lens count every token visible to the last query row.
-// The tokens of a sequence are taken in chunks of `chunk` pages by `splits` blocks in turn; part_o, part_ml: [B * q_len * Hq, splits, D], [.., 2] fp32.
+// The tokens of a sequence are taken in chunks of `chunk` pages (a multiple of 8) by `splits` blocks in turn; part_o, part_ml: [B * q_len * Hq, splits, D],
+// [.., 2] fp32 where there are several.
 extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, float* part_o, float* part_ml, int half,
                                          int B, int Hq, int Hk, int D, int width, int pages, int q_len, int splits, int chunk, float sm_scale, int* status,
                                          cudaStream_t stream) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || splits < 1 || chunk < 1) return -1;
-  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, part_ml, status, B, Hq, Hk, width, pages, q_len, splits, chunk, sm_scale * 1.4426950408889634f};
+  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, part_ml, status, B, Hq, Hk, width, pages, q_len, splits, chunk, 0, sm_scale * 1.4426950408889634f};
   if (D == 64) return mfq::launch_kv4_attn<64>(a, half != 0, stream);
   if (D == 128) return mfq::launch_kv4_attn<128>(a, half != 0, stream);
   if (D == 256) return mfq::launch_kv4_attn<256>(a, half != 0, stream);

@@ -13,6 +13,8 @@ CPU tensors take the restatements in :mod:`mfq_b200.ops.reference`.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import reference
@@ -20,6 +22,8 @@ from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
 from .logits import _DTYPES, _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
+SMS = 148
+MAX_SPLITS = 64
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
 
 
@@ -71,6 +75,17 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None
             return kv4_write(k, v, slots, kv)
     check(lib().mfq_kv4_write(k.data_ptr(), v.data_ptr(), slots.data_ptr(), kv.data.data_ptr(), _DTYPES[k.dtype], n, heads, d, pages, *ks, *vs,
                               Workspace.get(k.device).status.data_ptr(), stream_ptr()), "kv4_write")
+
+
+@lru_cache(maxsize=4096)
+def _shape(units: int, rows: int, d: int, pages: int) -> tuple[int, int]:
+    """(splits, pages of a chunk) for ``units`` sequences and KV heads with ``rows`` query rows each and up to ``pages`` pages."""
+    wide = rows > 8
+    units *= -(-rows // (16 if wide else 8))
+    slots = SMS * ((1 if wide else 2) if d == 256 else (3 if wide else 4))
+    splits = max(1, min(slots // units, -(-pages // 8), MAX_SPLITS))
+    chunk = max(8, -(-pages // (8 * splits)) * 8)
+    return max(1, -(-pages // chunk)), chunk
 
 
 def _table(block_table: torch.Tensor, b: int, index: int) -> int:
@@ -156,6 +171,11 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     if elsewhere(index):
         with torch.cuda.device(index):
             return paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale=sm_scale, q_len=q_len, max_len=max_len, out=out)
-    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), 0, 0, int(q.dtype is torch.float16), b, hq,
-                                          hk, d, width, pages, q_len, 1, 1, sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4")
+    splits, chunk = _shape(b * hk, hq // hk * q_len, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)))
+    parts = n * hq * splits if splits > 1 else 0
+    scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device) if parts else None  # of this call: a workspace would tie streams and graphs together
+    at = scratch.data_ptr() if parts else 0
+    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), at, at + 4 * parts * d,
+                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, splits, chunk, sm_scale, Workspace.get(q.device).status.data_ptr(),
+                                          stream_ptr()), "paged_attn_decode_kv4", 2 if parts else 1)
     return out
