@@ -53,6 +53,15 @@ __device__ __forceinline__ void kv4_product(float (&d)[4], uint32_t a0, uint32_t
   const uint32_t a[4] = {a0, a1, a2, a3};
   mma_half(d, a, b0, b1);
 }
+__device__ __forceinline__ void kv4_first_product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {  // d was nothing
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 template <typename T> __device__ __forceinline__ float2 kv4_pair(uint32_t v);
@@ -151,19 +160,18 @@ struct Kv4Rows {
       uint32_t par[2][G];  // of tokens g8 and g8 + 8
       params(par, rec + 8 * D + g8 * (D / 8));
 #pragma unroll
-      for (int b = 0; b < NB; ++b) sc[b][p][0] = sc[b][p][1] = sc[b][p][2] = sc[b][p][3] = 0.f;
-#pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         float acc[NB][4];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.f;
-#pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t h = w[j] >> 8;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) kv4_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
+          for (int b = 0; b < NB; ++b) {
+            if (j == 0) kv4_first_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
+            else kv4_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
+          }
         }
         const float s0 = __uint_as_float(par[0][g] << 16), m0 = __uint_as_float(par[0][g] & 0xffff0000u);
         const float s1 = __uint_as_float(par[1][g] << 16), m1 = __uint_as_float(par[1][g] & 0xffff0000u);
@@ -171,8 +179,8 @@ struct Kv4Rows {
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            sc[b][p][e] = fmaf(s0, acc[b][e], fmaf(m0, sums[b][g][e], sc[b][p][e]));
-            sc[b][p][2 + e] = fmaf(s1, acc[b][2 + e], fmaf(m1, sums[b][g][e], sc[b][p][2 + e]));
+            sc[b][p][e] = fmaf(s0, acc[b][e], g == 0 ? m0 * sums[b][g][e] : fmaf(m0, sums[b][g][e], sc[b][p][e]));
+            sc[b][p][2 + e] = fmaf(s1, acc[b][2 + e], g == 0 ? m1 * sums[b][g][e] : fmaf(m1, sums[b][g][e], sc[b][p][2 + e]));
           }
         }
       }
@@ -208,10 +216,7 @@ struct Kv4Rows {
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int g = 0; g < G; ++g) widest = fmaxf(widest, __uint_as_float(par[p][h][g] << 16));
-      }
+      for (int g = 0; g < G; ++g) widest = max3(widest, __uint_as_float(par[p][0][g] << 16), __uint_as_float(par[p][1][g] << 16));
     }
     float mx[NB][2];
     bool moves = widest > over;
@@ -219,7 +224,7 @@ struct Kv4Rows {
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mx[b][e] = fmaxf(fmaxf(sc[b][0][e], sc[b][0][2 + e]), fmaxf(sc[b][1][e], sc[b][1][2 + e]));
+        mx[b][e] = max3(fmaxf(sc[b][0][e], sc[b][0][2 + e]), sc[b][1][e], sc[b][1][2 + e]);
         moves |= mx[b][e] - 6.f > top[b][e];
       }
     }
@@ -349,42 +354,57 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   }
   if (a.splits > 1 && (long long)split * a.chunk >= total) return;  // nothing here, and nobody looks
   const int* bt = a.table + size_t(seq) * a.width;
-  const auto page_of = [&](int i) { return (split + i / per * a.splits) * a.chunk + 2 * (warp + L::kWarps * (i % per)) + lane; };
-  const auto id_of = [&](int i) {  // of lanes 0 and 1, their page of pair i; -1: there is none
-    const int at = page_of(i);
-    return i < mine && at < total ? bt[at] : -1;
+  // The pairs in order, twice: as they are requested, ids a pair ahead, and as they are used
+  struct Walk {
+    int page, left;
   };
-  const auto issue = [&](int i, int id, bool there) {
-    const int s = i % L::kStages;
+  const auto step = [&](Walk& x) {
+    x.page += 2 * L::kWarps;
+    if (--x.left == 0) {
+      x.page += (a.splits - 1) * a.chunk;
+      x.left = per;
+    }
+  };
+  Walk asked{split * a.chunk + 2 * warp + lane, per}, used{split * a.chunk + 2 * warp, per};
+  const auto issue = [&](int s, int id, bool there) {
     if (!there) {
       mbar_arrive(&full[s]);
       return;
     }
-    if (id < 0 || id >= a.pages) {
+    if (uint32_t(id) >= uint32_t(a.pages)) {
       atomicCAS(a.status, 0, kStatusBadArgument);
       id = 0;
     }
     mbar_expect_tx(&full[s], L::kRecord);
     shared_bulk_load(ring + s * L::kStage + lane * L::kRecord, a.pool + (size_t(id) * a.Hk + kvh) * L::kRecord, L::kRecord, &full[s]);
   };
-  int next = -1;
+  int next = 0;
   if (lane < 2) {
-    for (int i = 0; i < min(mine, L::kStages); ++i) issue(i, id_of(i), page_of(i) < total);
-    next = id_of(L::kStages);
+    for (int i = 0; i < min(mine, L::kStages); ++i) {
+      issue(i, asked.page < total ? bt[asked.page] : 0, asked.page < total);
+      step(asked);
+    }
+    if (L::kStages < mine && asked.page < total) next = bt[asked.page];
   }
   Kv4Rows<D, NB, T> t;
   t.load(a, seq, kvh, first, rows, length);
+  int s = 0, parity = 0;
   for (int i = 0; i < mine; ++i) {
-    const int s = i % L::kStages;
-    if (!mbar_wait_warp(&full[s], (i / L::kStages) & 1, abort_flag, a.status, kStatusTimeoutEpilogue)) {
+    if (!mbar_wait_warp(&full[s], parity, abort_flag, a.status, kStatusTimeoutEpilogue)) {
       let_started_work_end();
       break;
     }
-    t.pages(ring + s * L::kStage, ((split + i / per * a.splits) * a.chunk + 2 * (warp + L::kWarps * (i % per))) << 4);
+    t.pages(ring + s * L::kStage, used.page << 4);
+    step(used);
     __syncwarp();
     if (lane < 2 && i + L::kStages < mine) {
-      issue(i + L::kStages, next, page_of(i + L::kStages) < total);
-      next = id_of(i + 1 + L::kStages);
+      issue(s, next, asked.page < total);
+      step(asked);
+      if (i + 1 + L::kStages < mine && asked.page < total) next = bt[asked.page];
+    }
+    if (++s == L::kStages) {
+      s = 0;
+      parity ^= 1;
     }
   }
 
