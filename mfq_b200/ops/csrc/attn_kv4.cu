@@ -57,6 +57,10 @@ __device__ __forceinline__ void kv4_first_product(float (&d)[4], uint32_t a0, ui
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+__device__ __forceinline__ float2 add_f2(float2 a, float2 b) {
+  add2(a.x, a.y, __float_as_uint(b.x), __float_as_uint(b.y));
+  return a;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -76,8 +80,9 @@ template <int D, int NB, typename T>
 struct Kv4Rows {
   static constexpr int G = D / 64, kSteps = D / 16;
   uint32_t q[NB][kSteps][2];
-  float sums[NB][G][2], to_log2[NB][2];        // of a group's q; what a score in units of the products is times log2 e
-  float o[NB][kSteps][4], om[NB][G][2], l[NB][2], top[NB][2], ref[NB][2];
+  float sums[NB][G][2], top[NB][2], lim[NB][2];  // of a group's q; the running maximum; the score, in units of the products, that is too far above it
+  float2 to_log2[NB], less[NB], om[NB][G], l[NB];   // what such a score is times log2 e; -ref
+  float o[NB][kSteps][4];
   float up, over;  // log2 of what V's scales are multiplied by, and the scale that would be too large
   int len[NB][2], low, most;
 
@@ -110,7 +115,7 @@ struct Kv4Rows {
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      const float scale = power_to(big, 10);
+      const float scale = a.scale_log2 < 0.f ? -power_to(big, 10) : power_to(big, 10);  // scores have the sign of their units
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         float sum = 0.f;
@@ -129,19 +134,22 @@ struct Kv4Rows {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        to_log2[b][e] = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, scale, (2 * c + e) * 4);
+        const float f = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, scale, (2 * c + e) * 4);
+        (e == 0 ? to_log2[b].x : to_log2[b].y) = f;
         const int mine = first + 8 * b + 2 * c + e;
         // a row that is not there has a zero query and is never stored: unmasked, it leaves `low` to the others
         len[b][e] = mine < rows ? max(0, length - (a.q_len - 1 - mine / per)) : INT_MAX;
         lo = min(lo, len[b][e]);
         if (mine < rows) hi = max(hi, len[b][e]);
-        top[b][e] = ref[b][e] = -FLT_MAX;
-        l[b][e] = 0.f;
+        top[b][e] = -FLT_MAX;
+        lim[b][e] = -FLT_MAX;
       }
+      less[b] = both(FLT_MAX);
+      l[b] = both(0.f);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) o[b][s][0] = o[b][s][1] = o[b][s][2] = o[b][s][3] = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; ++g) om[b][g][0] = om[b][g][1] = 0.f;
+      for (int g = 0; g < G; ++g) om[b][g] = both(0.f);
     }
     low = __reduce_min_sync(0xffffffffu, lo);
     most = __reduce_max_sync(0xffffffffu, hi);
@@ -149,11 +157,11 @@ struct Kv4Rows {
     over = 0.f;  // none chosen yet
   }
 
-  // Two pages whose first token is tok0
+  // Two pages whose first token is tok0; kWhole: all rows see all of both
+  template <bool kWhole>
   __device__ __forceinline__ void pages(const uint8_t* rec0, int tok0) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
-    const bool whole = tok0 + 32 <= low;  // all rows see all of both
-    float sc[NB][2][4];
+    float2 sc[NB][2][2];  // [page][token g8, g8 + 8], of two columns
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const uint8_t* rec = rec0 + p * 18 * D;
@@ -173,31 +181,29 @@ struct Kv4Rows {
             else kv4_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
           }
         }
-        const float s0 = __uint_as_float(par[0][g] << 16), m0 = __uint_as_float(par[0][g] & 0xffff0000u);
-        const float s1 = __uint_as_float(par[1][g] << 16), m1 = __uint_as_float(par[1][g] & 0xffff0000u);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int h = 0; h < 2; ++h) {
+          const float ps = __uint_as_float(par[h][g] << 16), pm = __uint_as_float(par[h][g] & 0xffff0000u);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            sc[b][p][e] = fmaf(s0, acc[b][e], g == 0 ? m0 * sums[b][g][e] : fmaf(m0, sums[b][g][e], sc[b][p][e]));
-            sc[b][p][2 + e] = fmaf(s1, acc[b][2 + e], g == 0 ? m1 * sums[b][g][e] : fmaf(m1, sums[b][g][e], sc[b][p][2 + e]));
+          for (int b = 0; b < NB; ++b) {
+            float2& x = sc[b][p][h];
+            x.x = fmaf(ps, acc[b][2 * h], g == 0 ? pm * sums[b][g][0] : fmaf(pm, sums[b][g][0], x.x));
+            x.y = fmaf(ps, acc[b][2 * h + 1], g == 0 ? pm * sums[b][g][1] : fmaf(pm, sums[b][g][1], x.y));
           }
         }
       }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sc[b][p][x] *= to_log2[b][x & 1];
-      }
     }
-    if (!whole) {
+    const auto sees = [&](int b, int e, int p, int h) { return tok0 + 16 * p + 8 * h + g8 < len[b][e]; };
+    if constexpr (!kWhole) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (tok0 + 16 * p + g8 + 8 * (x >> 1) >= len[b][x & 1]) sc[b][p][x] = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            if (!sees(b, 0, p, h)) sc[b][p][h].x = -INFINITY;
+            if (!sees(b, 1, p, h)) sc[b][p][h].y = -INFINITY;
+          }
         }
       }
     }
@@ -207,7 +213,7 @@ struct Kv4Rows {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       params(par[p], rec0 + p * 18 * D + 17 * D + g8 * (D / 8));
-      if (!whole) {
+      if constexpr (!kWhole) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -222,11 +228,9 @@ struct Kv4Rows {
     bool moves = widest > over;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mx[b][e] = max3(fmaxf(sc[b][0][e], sc[b][0][2 + e]), sc[b][1][e], sc[b][1][2 + e]);
-        moves |= mx[b][e] - 6.f > top[b][e];
-      }
+      mx[b][0] = max3(fmaxf(sc[b][0][0].x, sc[b][0][1].x), sc[b][1][0].x, sc[b][1][1].x);
+      mx[b][1] = max3(fmaxf(sc[b][0][0].y, sc[b][0][1].y), sc[b][1][0].y, sc[b][1][1].y);
+      moves |= mx[b][0] > lim[b][0] || mx[b][1] > lim[b][1];
     }
     if (__any_sync(0xffffffffu, moves)) move(mx, widest);
 #pragma unroll
@@ -235,33 +239,34 @@ struct Kv4Rows {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[b][p][x] = kv4_exp2(sc[b][p][x] - ref[b][x & 1]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[b][e] += sc[b][p][e] + sc[b][p][2 + e];
+        for (int h = 0; h < 2; ++h) {
+          float2 x = fma_f2(sc[b][p][h], to_log2[b], less[b]);
+          if constexpr (!kWhole) {  // with a scale of 0 the products made it a NaN
+            if (!sees(b, 0, p, h)) x.x = -INFINITY;
+            if (!sees(b, 1, p, h)) x.y = -INFINITY;
+          }
+          sc[b][p][h] = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
+          l[b] = add_f2(l[b], sc[b][p][h]);
+        }
       }
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float s0 = __uint_as_float(par[p][0][g] << 16), m0 = __uint_as_float(par[p][0][g] & 0xffff0000u);
-        const float s1 = __uint_as_float(par[p][1][g] << 16), m1 = __uint_as_float(par[p][1][g] & 0xffff0000u);
         uint32_t pb[NB][2];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          float* t = sc[b][p];
-          float ps[4] = {t[0] * s0, t[1] * s0, t[2] * s1, t[3] * s1};
-          float pm[2] = {fmaf(t[0], m0, t[2] * m1), fmaf(t[1], m0, t[3] * m1)};
-          if (!whole) {  // a NaN stays with the rows that see it
+        for (int h = 0; h < 2; ++h) {
+          const float ps = __uint_as_float(par[p][h][g] << 16), pm = __uint_as_float(par[p][h][g] & 0xffff0000u);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (tok0 + 16 * p + g8 + 8 * (x >> 1) >= len[b][x & 1]) ps[x] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              pm[e] = tok0 + 16 * p + g8 + 8 < len[b][e] ? pm[e] : (tok0 + 16 * p + g8 < len[b][e] ? t[e] * m0 : 0.f);
+          for (int b = 0; b < NB; ++b) {
+            float2 v = make_float2(sc[b][p][h].x * ps, sc[b][p][h].y * ps);
+            if constexpr (!kWhole) {  // a NaN stays with the rows that see it
+              const bool s0 = sees(b, 0, p, h), s1 = sees(b, 1, p, h);
+              v = make_float2(s0 ? v.x : 0.f, s1 ? v.y : 0.f);
+              om[b][g] = make_float2(s0 ? fmaf(sc[b][p][h].x, pm, om[b][g].x) : om[b][g].x, s1 ? fmaf(sc[b][p][h].y, pm, om[b][g].y) : om[b][g].y);
+            } else {
+              om[b][g] = make_float2(fmaf(sc[b][p][h].x, pm, om[b][g].x), fmaf(sc[b][p][h].y, pm, om[b][g].y));
             }
+            pb[b][h] = kv4_transposed(half_pair(v.x, v.y));
           }
-          om[b][g][0] += pm[0];
-          om[b][g][1] += pm[1];
-          pb[b][0] = kv4_transposed(half_pair(ps[0], ps[1]));
-          pb[b][1] = kv4_transposed(half_pair(ps[2], ps[3]));
         }
         const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -305,18 +310,21 @@ __device__ __forceinline__ void Kv4Rows<D, NB, T>::move(const float (&mx)[NB][2]
     float corr[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
+      const float f = e == 0 ? to_log2[b].x : to_log2[b].y;
+      float& now = e == 0 ? less[b].x : less[b].y;
       float m = mx[b][e];
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      top[b][e] = fmaxf(top[b][e], m);
-      const float next = top[b][e] - up;
-      corr[e] = kv4_exp2(ref[b][e] - next);
-      ref[b][e] = next;
-      l[b][e] *= corr[e];
-#pragma unroll
-      for (int g = 0; g < G; ++g) om[b][g][e] *= corr[e];
+      if (m > -INFINITY) top[b][e] = fmaxf(top[b][e], m * f);
+      lim[b][e] = top[b][e] > -FLT_MAX ? (top[b][e] + 6.f) / f : -FLT_MAX;
+      const float next = up - top[b][e];
+      corr[e] = kv4_exp2(next - now);
+      now = next;
     }
+    l[b] = make_float2(l[b].x * corr[0], l[b].y * corr[1]);
+#pragma unroll
+    for (int g = 0; g < G; ++g) om[b][g] = make_float2(om[b][g].x * corr[0], om[b][g].y * corr[1]);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) { o[b][s][0] *= corr[0]; o[b][s][1] *= corr[1]; o[b][s][2] *= corr[0]; o[b][s][3] *= corr[1]; }
   }
@@ -394,7 +402,8 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       let_started_work_end();
       break;
     }
-    t.pages(ring + s * L::kStage, used.page << 4);
+    if ((used.page << 4) + 32 <= t.low) t.template pages<true>(ring + s * L::kStage, used.page << 4);
+    else t.template pages<false>(ring + s * L::kStage, used.page << 4);
     step(used);
     __syncwarp();
     if (lane < 2 && i + L::kStages < mine) {
@@ -417,14 +426,14 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = 8 * b + 2 * c + e;
-      float sum = t.l[b][e];
+      float sum = e == 0 ? t.l[b].x : t.l[b].y;
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      if (g8 == 0) { ml[2 * r] = t.ref[b][e]; ml[2 * r + 1] = sum; }
+      if (g8 == 0) { ml[2 * r] = -(e == 0 ? t.less[b].x : t.less[b].y); ml[2 * r + 1] = sum; }
 #pragma unroll
       for (int g = 0; g < D / 64; ++g) {
-        float om = t.om[b][g][e];
+        float om = e == 0 ? t.om[b][g].x : t.om[b][g].y;
         om += __shfl_xor_sync(0xffffffffu, om, 4);
         om += __shfl_xor_sync(0xffffffffu, om, 8);
         om += __shfl_xor_sync(0xffffffffu, om, 16);
@@ -485,7 +494,7 @@ __global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a) {
 template <int D, int NB, typename T>
 static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
   using L = Kv4Ring<D>;
-  constexpr int kMinBlocks = D == 256 ? (NB == 1 ? 2 : 1) : (NB == 1 ? 4 : 3);
+  constexpr int kMinBlocks = D == 256 ? 2 : (NB == 1 ? 4 : 2);
   auto kernel = &kv4_attn_kernel<D, NB, T, kMinBlocks>;
   static bool attr[64] = {};
   int dev = 0;
@@ -503,8 +512,9 @@ static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
 }
 template <int D>
 static int launch_kv4_attn(const Kv4AttnArgs& a, bool half, cudaStream_t stream) {
-  if ((long long)a.Hq / a.Hk * a.q_len <= 8) return half ? launch_kv4_attn_of<D, 1, __half>(a, stream) : launch_kv4_attn_of<D, 1, __nv_bfloat16>(a, stream);
-  return half ? launch_kv4_attn_of<D, 2, __half>(a, stream) : launch_kv4_attn_of<D, 2, __nv_bfloat16>(a, stream);
+  if (D == 256 || (long long)a.Hq / a.Hk * a.q_len <= 8) return half ? launch_kv4_attn_of<D, 1, __half>(a, stream) : launch_kv4_attn_of<D, 1, __nv_bfloat16>(a, stream);
+  if constexpr (D < 256) return half ? launch_kv4_attn_of<D, 2, __half>(a, stream) : launch_kv4_attn_of<D, 2, __nv_bfloat16>(a, stream);
+  return -1;
 }
 
 }  // namespace mfq

@@ -80,9 +80,9 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None
 @lru_cache(maxsize=4096)
 def _shape(units: int, rows: int, d: int, pages: int) -> tuple[int, int]:
     """(splits, pages of a chunk) for ``units`` sequences and KV heads with ``rows`` query rows each and up to ``pages`` pages."""
-    wide = rows > 8
+    wide = rows > 8 and d < 256
     units *= -(-rows // (16 if wide else 8))
-    slots = SMS * ((1 if wide else 2) if d == 256 else (3 if wide else 4))
+    slots = SMS * (2 if wide or d == 256 else 4)
     splits = max(1, min(slots // units, -(-pages // 8), MAX_SPLITS))
     chunk = max(8, -(-pages // (8 * splits)) * 8)
     return max(1, -(-pages // chunk)), chunk
