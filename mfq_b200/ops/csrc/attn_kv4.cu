@@ -7,9 +7,12 @@
 // multiply as any other number; in the next four bits it is 16 times that.  Two registers of a fragment have their codes 16 times as large: the dims
 // d + 8 of K, whose queries are divided by 16, and the rows d + 8 of V's output, which are divided in the end.
 //
-// A CTA has one sequence, one KV head, up to 8 or 16 of its query rows (query token, head of the group) and one split of the pages.  Its warps take
-// two pages at a time, in turn, each through a ring of bulk copies of its own.  A page's tokens are the rows of the products and the query rows their columns:
+// A CTA has one sequence, one KV head, up to 4, 8 or 16 of its query rows (query token, head of the group) and one split of the pages.  Its warps take
+// two pages at a time, in turn, each through a ring of its own that its lanes fill by 16-byte asynchronous copies; a lane reads the codes that it copied.
+// A page's tokens are the rows of the products and the query rows their columns:
 //   S^T [16 x 8] = K Q^T,   O^T [D x 8] += V^T (p s),   p s being S^T's accumulator transposed by movmatrix.
+// Up to 4 query rows have the two pages side by side: the first page is multiplied by [Q 0], the second by [0 Q], into the same accumulator, so that no
+// lane computes the softmax of columns that nobody has; O^T's halves are added in the end.
 //
 // Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
 // maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum, less a power of two that brings the
@@ -36,9 +39,17 @@ struct Kv4AttnArgs {
 template <int D>
 struct Kv4Ring {
   static constexpr int kRecord = 18 * D, kStage = 2 * kRecord, kStages = D <= 128 ? 3 : 2, kWarps = 4;
-  static constexpr int kWarp = kStages * kStage, kBars = kWarps * kWarp, kSmem = kBars + kWarps * kStages * 8 + 16;
+  static constexpr int kWarp = kStages * kStage, kSmem = kWarps * kWarp;
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
+}
+__device__ __forceinline__ void copies_end_here() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_but_the_last() {  // all groups of this thread's copies but the last kLeft are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
 __device__ __forceinline__ float kv4_exp2(float x) {  // results under 2^-126 are 0
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -75,13 +86,15 @@ template <typename T> __device__ __forceinline__ T kv4_out(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 kv4_out(float v) { return __float2bfloat16(v); }
 template <> __device__ __forceinline__ __half kv4_out(float v) { return __float2half_rn(v); }
 
-// What a warp has of its query rows: column blocks of 8, a lane has the columns 8 b + 2 c and the one behind it
-template <int D, int NB, typename T>
+// What a warp has of its query rows: column blocks of 8, a lane has the columns 8 b + 2 c and the one behind it.  kCols 4: the columns n and n + 4 are row n,
+// of the first and the second page of a pair.
+template <int D, int kCols, typename T>
 struct Kv4Rows {
-  static constexpr int G = D / 64, kSteps = D / 16;
-  uint32_t q[NB][kSteps][2];
-  float sums[NB][G][2], top[NB][2], lim[NB][2];  // of a group's q; the running maximum; the score, in units of the products, that is too far above it
-  float2 to_log2[NB], less[NB], om[NB][G], l[NB];   // what such a score is times log2 e; -ref
+  static constexpr bool kSide = kCols == 4;
+  static constexpr int G = D / 64, kSteps = D / 16, NB = kSide ? 1 : kCols / 8, P = kSide ? 1 : 2;  // P: pages of a pair whose scores a lane has
+  uint32_t q[kSide ? 2 : NB][kSteps][2];              // by column block; kSide: [Q 0] and [0 Q]
+  float sums[NB][G][2], top[NB][2], lim[NB][2];       // of a group's q; the running maximum; the score, in units of the products, that is too far above it
+  float2 to_log2[NB], less[NB], om[NB][G], l[NB];     // what such a score is times log2 e; -ref
   float o[NB][kSteps][4];
   float up, over;  // log2 of what V's scales are multiplied by, and the scale that would be too large
   int len[NB][2], low, most;
@@ -91,7 +104,7 @@ struct Kv4Rows {
     int lo = INT_MAX, hi = 0;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int r = first + 8 * b + g8;
+      const int r = first + 8 * b + (kSide ? g8 & 3 : g8);
       const bool there = r < rows;
       uint32_t raw[kSteps][2];
 #pragma unroll
@@ -122,8 +135,13 @@ struct Kv4Rows {
 #pragma unroll
         for (int s = 4 * g; s < 4 * g + 4; ++s) {
           const float2 v = kv4_pair<T>(raw[s][0]), w = kv4_pair<T>(raw[s][1]);
-          q[b][s][0] = half_pair(v.x * scale, v.y * scale);
-          q[b][s][1] = half_pair(w.x * scale * 0.0625f, w.y * scale * 0.0625f);
+          const uint32_t x = half_pair(v.x * scale, v.y * scale), y = half_pair(w.x * scale * 0.0625f, w.y * scale * 0.0625f);
+          if constexpr (kSide) {
+            q[0][s][0] = g8 < 4 ? x : 0u; q[0][s][1] = g8 < 4 ? y : 0u;
+            q[1][s][0] = g8 < 4 ? 0u : x; q[1][s][1] = g8 < 4 ? 0u : y;
+          } else {
+            q[b][s][0] = x; q[b][s][1] = y;
+          }
           sum += (v.x * scale + v.y * scale) + (w.x * scale + w.y * scale);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -136,7 +154,7 @@ struct Kv4Rows {
       for (int e = 0; e < 2; ++e) {
         const float f = a.scale_log2 * 0x1p24f / __shfl_sync(0xffffffffu, scale, (2 * c + e) * 4);
         (e == 0 ? to_log2[b].x : to_log2[b].y) = f;
-        const int mine = first + 8 * b + 2 * c + e;
+        const int mine = first + 8 * b + (kSide ? 2 * (c & 1) : 2 * c) + e;
         // a row that is not there has a zero query and is never stored: unmasked, it leaves `low` to the others
         len[b][e] = mine < rows ? max(0, length - (a.q_len - 1 - mine / per)) : INT_MAX;
         lo = min(lo, len[b][e]);
@@ -161,44 +179,50 @@ struct Kv4Rows {
   template <bool kWhole>
   __device__ __forceinline__ void pages(const uint8_t* rec0, int tok0) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
-    float2 sc[NB][2][2];  // [page][token g8, g8 + 8], of two columns
+    const int side = kSide ? c >> 1 : 0;  // the page whose scores this lane has
+    const auto sees = [&](int b, int e, int p, int h) { return tok0 + 16 * (p + side) + 8 * h + g8 < len[b][e]; };
+    float2 sc[NB][P][2];  // [page][token g8, g8 + 8], of two columns
+    float acc[NB][G][4];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const uint8_t* rec = rec0 + p * 18 * D;
-      uint32_t par[2][G];  // of tokens g8 and g8 + 8
-      params(par, rec + 8 * D + g8 * (D / 8));
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        float acc[NB][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t h = w[j] >> 8;
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            if (j == 0) kv4_first_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
-            else kv4_product(acc[b], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, q[b][4 * g + j][0], q[b][4 * g + j][1]);
+            const uint32_t(&qb)[2] = q[kSide ? p : b][4 * g + j];
+            if (j == 0 && (p == 0 || !kSide)) kv4_first_product(acc[b][g], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, qb[0], qb[1]);
+            else kv4_product(acc[b][g], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, qb[0], qb[1]);
           }
         }
+      }
+      if (kSide && p == 0) continue;
+      uint32_t par[2][G];  // of tokens g8 and g8 + 8
+      params(par, rec0 + (kSide ? side : p) * 18 * D + 8 * D + g8 * (D / 8));
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float ps = __uint_as_float(par[h][g] << 16), pm = __uint_as_float(par[h][g] & 0xffff0000u);
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            float2& x = sc[b][p][h];
-            x.x = fmaf(ps, acc[b][2 * h], g == 0 ? pm * sums[b][g][0] : fmaf(pm, sums[b][g][0], x.x));
-            x.y = fmaf(ps, acc[b][2 * h + 1], g == 0 ? pm * sums[b][g][1] : fmaf(pm, sums[b][g][1], x.y));
+            float2& x = sc[b][kSide ? 0 : p][h];
+            x.x = fmaf(ps, acc[b][g][2 * h], g == 0 ? pm * sums[b][g][0] : fmaf(pm, sums[b][g][0], x.x));
+            x.y = fmaf(ps, acc[b][g][2 * h + 1], g == 0 ? pm * sums[b][g][1] : fmaf(pm, sums[b][g][1], x.y));
           }
         }
       }
     }
-    const auto sees = [&](int b, int e, int p, int h) { return tok0 + 16 * p + 8 * h + g8 < len[b][e]; };
     if constexpr (!kWhole) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+        for (int p = 0; p < P; ++p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (!sees(b, 0, p, h)) sc[b][p][h].x = -INFINITY;
@@ -208,17 +232,17 @@ struct Kv4Rows {
       }
     }
     // parameters of V, none where nobody sees the token: what is there may be anything
-    uint32_t par[2][2][G];
+    uint32_t par[P][2][G];
     float widest = 0.f;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      params(par[p], rec0 + p * 18 * D + 17 * D + g8 * (D / 8));
+    for (int p = 0; p < P; ++p) {
+      params(par[p], rec0 + (p + side) * 18 * D + 17 * D + g8 * (D / 8));
       if constexpr (!kWhole) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            if (tok0 + 16 * p + g8 + 8 * h >= most) par[p][h][g] = 0;
+            if (tok0 + 16 * (p + side) + g8 + 8 * h >= most) par[p][h][g] = 0;
         }
       }
 #pragma unroll
@@ -228,14 +252,18 @@ struct Kv4Rows {
     bool moves = widest > over;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      mx[b][0] = max3(fmaxf(sc[b][0][0].x, sc[b][0][1].x), sc[b][1][0].x, sc[b][1][1].x);
-      mx[b][1] = max3(fmaxf(sc[b][0][0].y, sc[b][0][1].y), sc[b][1][0].y, sc[b][1][1].y);
+      mx[b][0] = fmaxf(sc[b][0][0].x, sc[b][0][1].x);
+      mx[b][1] = fmaxf(sc[b][0][0].y, sc[b][0][1].y);
+      if constexpr (P == 2) {
+        mx[b][0] = max3(mx[b][0], sc[b][P - 1][0].x, sc[b][P - 1][1].x);
+        mx[b][1] = max3(mx[b][1], sc[b][P - 1][0].y, sc[b][P - 1][1].y);
+      }
       moves |= mx[b][0] > lim[b][0] || mx[b][1] > lim[b][1];
     }
     if (__any_sync(0xffffffffu, moves)) move(mx, widest);
+    uint32_t pb[NB][P][G][2];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint8_t* rec = rec0 + p * 18 * D + 9 * D;
+    for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -251,7 +279,6 @@ struct Kv4Rows {
       }
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint32_t pb[NB][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float ps = __uint_as_float(par[p][h][g] << 16), pm = __uint_as_float(par[p][h][g] & 0xffff0000u);
@@ -265,16 +292,27 @@ struct Kv4Rows {
             } else {
               om[b][g] = make_float2(fmaf(sc[b][p][h].x, pm, om[b][g].x), fmaf(sc[b][p][h].y, pm, om[b][g].y));
             }
-            pb[b][h] = kv4_transposed(half_pair(v.x, v.y));
+            pb[b][p][g][h] = kv4_transposed(half_pair(v.x, v.y));
           }
         }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint8_t* rec = rec0 + p * 18 * D + 9 * D;
+      const uint32_t keep = !kSide || (g8 < 4) == (p == 0) ? 0xffffffffu : 0u;  // this page's columns
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
         const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t b0[NB], b1[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) { b0[b] = pb[b][kSide ? 0 : p][g][0] & keep; b1[b] = pb[b][kSide ? 0 : p][g][1] & keep; }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t h = w[j] >> 8;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, pb[b][0], pb[b][1]);
+          for (int b = 0; b < NB; ++b) kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, b0[b], b1[b]);
         }
       }
     }
@@ -294,65 +332,57 @@ struct Kv4Rows {
   }
 
   // New references: the running maxima and the power of two of V's scales
-  __device__ __forceinline__ void move(const float (&mx)[NB][2], float widest);
+  __device__ __forceinline__ void move(const float (&mx)[NB][2], float widest) {
+    widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)));
+    if (widest > over) {
+      const int e = int(__float_as_uint(widest) >> 23) - 127;  // of a denormal one: -127
+      up = fminf(7.f - float(e), 104.f);
+      over = kv4_exp2(9.f - up);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float corr[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f = e == 0 ? to_log2[b].x : to_log2[b].y;
+        float& now = e == 0 ? less[b].x : less[b].y;
+        float m = mx[b][e];
+        if constexpr (kSide) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (m > -INFINITY) top[b][e] = fmaxf(top[b][e], m * f);
+        lim[b][e] = top[b][e] > -FLT_MAX ? (top[b][e] + 6.f) / f : -FLT_MAX;
+        const float next = up - top[b][e];
+        corr[e] = kv4_exp2(next - now);
+        now = next;
+      }
+      l[b] = make_float2(l[b].x * corr[0], l[b].y * corr[1]);
+#pragma unroll
+      for (int g = 0; g < G; ++g) om[b][g] = make_float2(om[b][g].x * corr[0], om[b][g].y * corr[1]);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) { o[b][s][0] *= corr[0]; o[b][s][1] *= corr[1]; o[b][s][2] *= corr[0]; o[b][s][3] *= corr[1]; }
+    }
+  }
 };
 
-template <int D, int NB, typename T>
-__device__ __forceinline__ void Kv4Rows<D, NB, T>::move(const float (&mx)[NB][2], float widest) {
-  widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)));
-  if (widest > over) {
-    const int e = int(__float_as_uint(widest) >> 23) - 127;  // of a denormal one: -127
-    up = fminf(7.f - float(e), 104.f);
-    over = kv4_exp2(9.f - up);
-  }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    float corr[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float f = e == 0 ? to_log2[b].x : to_log2[b].y;
-      float& now = e == 0 ? less[b].x : less[b].y;
-      float m = mx[b][e];
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      if (m > -INFINITY) top[b][e] = fmaxf(top[b][e], m * f);
-      lim[b][e] = top[b][e] > -FLT_MAX ? (top[b][e] + 6.f) / f : -FLT_MAX;
-      const float next = up - top[b][e];
-      corr[e] = kv4_exp2(next - now);
-      now = next;
-    }
-    l[b] = make_float2(l[b].x * corr[0], l[b].y * corr[1]);
-#pragma unroll
-    for (int g = 0; g < G; ++g) om[b][g] = make_float2(om[b][g].x * corr[0], om[b][g].y * corr[1]);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) { o[b][s][0] *= corr[0]; o[b][s][1] *= corr[1]; o[b][s][2] *= corr[0]; o[b][s][3] *= corr[1]; }
-  }
-}
-
-template <int D, int NB, typename T, int kMinBlocks>
+template <int D, int kCols, typename T, int kMinBlocks>
 __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a) {
   pdl_trigger();
   using L = Kv4Ring<D>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l)
+  using R = Kv4Rows<D, kCols, T>;
+  constexpr int NB = R::NB, kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l)
   static_assert(kPart * 4 <= L::kWarp, "the ring is where a warp leaves its sums");
+  extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * L::kWarp;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars) + warp * L::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBars + L::kWarps * L::kStages * 8);
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) {
-    for (int s = 0; s < L::kStages; ++s) mbar_init(&full[s], 2);
-    mbar_fence_init();
-  }
-  __syncthreads();
   pdl_wait();
 
-  const int seq = blockIdx.x, kvh = blockIdx.y / a.tiles, first = blockIdx.y % a.tiles * 8 * NB, split = blockIdx.z;
+  const int seq = blockIdx.x, kvh = blockIdx.y / a.tiles, first = blockIdx.y % a.tiles * kCols, split = blockIdx.z;
   const int rows = a.Hq / a.Hk * a.q_len;
   const int length = int(max(0ll, min((long long)a.seq_lens[seq], 16ll * a.width)));
   const int total = (length + 15) >> 4, per = a.chunk / (2 * L::kWarps);  // pages; pairs of a chunk that a warp has
+  if (a.splits > 1 && (long long)split * a.chunk >= total) return;  // nothing here, and nobody looks
   // chunks split, split + splits, ...; a warp's pairs in them
   int mine = 0;
   {
@@ -360,7 +390,6 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     mine = (whole > split ? (whole - split + a.splits - 1) / a.splits : 0) * per;
     if (left > 2 * warp && whole >= split && (whole - split) % a.splits == 0) mine += (left - 2 * warp + 2 * L::kWarps - 1) / (2 * L::kWarps);
   }
-  if (a.splits > 1 && (long long)split * a.chunk >= total) return;  // nothing here, and nobody looks
   const int* bt = a.table + size_t(seq) * a.width;
   // The pairs in order, twice: as they are requested, ids a pair ahead, and as they are used
   struct Walk {
@@ -373,48 +402,71 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       x.left = per;
     }
   };
-  Walk asked{split * a.chunk + 2 * warp + lane, per}, used{split * a.chunk + 2 * warp, per};
-  const auto issue = [&](int s, int id, bool there) {
-    if (!there) {
-      mbar_arrive(&full[s]);
-      return;
-    }
-    if (uint32_t(id) >= uint32_t(a.pages)) {
-      atomicCAS(a.status, 0, kStatusBadArgument);
-      id = 0;
-    }
-    mbar_expect_tx(&full[s], L::kRecord);
-    shared_bulk_load(ring + s * L::kStage + lane * L::kRecord, a.pool + (size_t(id) * a.Hk + kvh) * L::kRecord, L::kRecord, &full[s]);
+  Walk asked{split * a.chunk + 2 * warp, per}, used = asked;
+  int id[2] = {0, 0};
+  const auto look = [&] {  // the ids of the pair that is asked for next
+    id[0] = bt[asked.page];
+    id[1] = asked.page + 1 < total ? bt[asked.page + 1] : id[0];
   };
-  int next = 0;
-  if (lane < 2) {
-    for (int i = 0; i < min(mine, L::kStages); ++i) {
-      issue(i, asked.page < total ? bt[asked.page] : 0, asked.page < total);
+  const uint32_t to = smem_u32(ring) + 16 * lane;
+  constexpr int kParts = D / 8;  // pieces of 16 bytes of a page's parameters: K's, then V's
+  const int piece = lane % (kParts < 32 ? kParts : 32);
+  const uint32_t piece_at = piece < kParts / 2 ? 8 * D + 16 * piece : 17 * D + 16 * (piece - kParts / 2);
+  const auto request = [&](int s) {
+    const uint8_t* rec[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (uint32_t(id[p]) >= uint32_t(a.pages)) {
+        if (lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
+        id[p] = 0;
+      }
+      rec[p] = a.pool + (size_t(id[p]) * a.Hk + kvh) * L::kRecord;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {  // a second page that is not there: the first again
+      const uint8_t* from = rec[p] + 16 * lane;
+      const uint32_t at = to + s * L::kStage + p * L::kRecord;
+#pragma unroll
+      for (int g = 0; g < D / 64; ++g) copy16(at + 512 * g, from + 512 * g);
+#pragma unroll
+      for (int g = 0; g < D / 64; ++g) copy16(at + 9 * D + 512 * g, from + 9 * D + 512 * g);
+    }
+    const uint32_t at = smem_u32(ring) + s * L::kStage + piece_at;
+    if constexpr (kParts == 32) {
+      copy16(at, rec[0] + piece_at);
+      copy16(at + L::kRecord, rec[1] + piece_at);
+    } else {
+      const int p = lane / kParts;
+      if (p < 2) copy16(at + p * L::kRecord, (p == 0 ? rec[0] : rec[1]) + piece_at);
+    }
+  };
+  if (mine > 0) look();
+#pragma unroll
+  for (int i = 0; i < L::kStages; ++i) {
+    if (i < mine) {
+      request(i);
       step(asked);
+      if (i + 1 < mine) look();
     }
-    if (L::kStages < mine && asked.page < total) next = bt[asked.page];
+    copies_end_here();
   }
-  Kv4Rows<D, NB, T> t;
+  R t;
   t.load(a, seq, kvh, first, rows, length);
-  int s = 0, parity = 0;
+  int s = 0;
   for (int i = 0; i < mine; ++i) {
-    if (!mbar_wait_warp(&full[s], parity, abort_flag, a.status, kStatusTimeoutEpilogue)) {
-      let_started_work_end();
-      break;
-    }
+    copies_but_the_last<L::kStages - 1>();
+    __syncwarp();
     if ((used.page << 4) + 32 <= t.low) t.template pages<true>(ring + s * L::kStage, used.page << 4);
     else t.template pages<false>(ring + s * L::kStage, used.page << 4);
     step(used);
     __syncwarp();
-    if (lane < 2 && i + L::kStages < mine) {
-      issue(s, next, asked.page < total);
+    if (i + L::kStages < mine) {
+      request(s);
       step(asked);
-      if (i + 1 + L::kStages < mine && asked.page < total) next = bt[asked.page];
+      if (i + 1 + L::kStages < mine) look();
     }
-    if (++s == L::kStages) {
-      s = 0;
-      parity ^= 1;
-    }
+    copies_end_here();
+    if (++s == L::kStages) s = 0;
   }
 
   // ---- the lanes of a column, then the warps ----
@@ -446,8 +498,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     }
   }
   __syncthreads();
-  if (*abort_flag) return;
-  const int here = min(rows - first, 8 * NB), per_head = a.Hq / a.Hk;
+  const int here = min(rows - first, kCols), per_head = a.Hq / a.Hk;
   for (int i = threadIdx.x; i < here * D; i += 128) {
     const int r = i / D, d = i % D;
     float ref = -FLT_MAX, l = 0.f, o = 0.f;
@@ -457,8 +508,10 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     for (int w = 0; w < L::kWarps; ++w) {
       const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
       const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref);
-      l += from[8 * NB * kStride + 2 * r + 1] * weight;
-      o += from[r * kStride + d] * weight;
+      float lw = from[8 * NB * kStride + 2 * r + 1], ow = from[r * kStride + d];
+      if constexpr (R::kSide) { lw += from[8 * NB * kStride + 2 * r + 9]; ow += from[(r + 4) * kStride + d]; }
+      l += lw * weight;
+      o += ow * weight;
     }
     const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
     if (a.splits == 1) {
@@ -491,11 +544,11 @@ __global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a) {
   static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
 }
 
-template <int D, int NB, typename T>
+template <int D, int kCols, typename T>
 static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
   using L = Kv4Ring<D>;
-  constexpr int kMinBlocks = D == 256 ? 2 : (NB == 1 ? 4 : 2);
-  auto kernel = &kv4_attn_kernel<D, NB, T, kMinBlocks>;
+  constexpr int kMinBlocks = D == 256 || kCols == 16 ? 2 : 4;
+  auto kernel = &kv4_attn_kernel<D, kCols, T, kMinBlocks>;
   static bool attr[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
@@ -503,18 +556,24 @@ static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return -6;
     attr[dev] = true;
   }
-  const long long rows = (long long)a.Hq / a.Hk * a.q_len, tiles = (rows + 8 * NB - 1) / (8 * NB);
+  const long long rows = (long long)a.Hq / a.Hk * a.q_len, tiles = (rows + kCols - 1) / kCols;
   if (a.Hk * tiles > 65535 || a.splits > 65535 || (long long)a.B * a.q_len * a.Hq > 0x7fffffffll || a.chunk % (2 * L::kWarps)) return -2;
   a.tiles = int(tiles);
   if (launch_kernel(kernel, dim3(a.B, unsigned(a.Hk * tiles), a.splits), dim3(128), L::kSmem, stream, a) != cudaSuccess) return -7;
   if (a.splits > 1 && launch_kernel(&kv4_merge_kernel<D, T>, dim3(unsigned(a.B * a.q_len * a.Hq)), dim3(D), 0, stream, a) != cudaSuccess) return -7;
   return 0;
 }
+template <int D, typename T>
+static int launch_kv4_attn_for(const Kv4AttnArgs& a, cudaStream_t stream) {
+  const long long rows = (long long)a.Hq / a.Hk * a.q_len;
+  if (rows <= 4) return launch_kv4_attn_of<D, 4, T>(a, stream);
+  if (D == 256 || rows <= 8) return launch_kv4_attn_of<D, 8, T>(a, stream);
+  if constexpr (D < 256) return launch_kv4_attn_of<D, 16, T>(a, stream);
+  return -1;
+}
 template <int D>
 static int launch_kv4_attn(const Kv4AttnArgs& a, bool half, cudaStream_t stream) {
-  if (D == 256 || (long long)a.Hq / a.Hk * a.q_len <= 8) return half ? launch_kv4_attn_of<D, 1, __half>(a, stream) : launch_kv4_attn_of<D, 1, __nv_bfloat16>(a, stream);
-  if constexpr (D < 256) return half ? launch_kv4_attn_of<D, 2, __half>(a, stream) : launch_kv4_attn_of<D, 2, __nv_bfloat16>(a, stream);
-  return -1;
+  return half ? launch_kv4_attn_for<D, __half>(a, stream) : launch_kv4_attn_for<D, __nv_bfloat16>(a, stream);
 }
 
 }  // namespace mfq
