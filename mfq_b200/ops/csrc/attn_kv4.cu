@@ -7,8 +7,10 @@
 // multiply as any other number; in the next four bits it is 16 times that.  Two registers of a fragment have their codes 16 times as large: the dims
 // d + 8 of K, whose queries are divided by 16, and the rows d + 8 of V's output, which are divided in the end.
 //
-// A CTA has one sequence, one KV head, up to 4, 8 or 16 of its query rows (query token, head of the group) and one split of the pages.  Its warps take
-// two pages at a time, in turn, each through a ring of its own that its lanes fill by 16-byte asynchronous copies; a lane reads the codes that it copied.
+// A unit is one sequence, one KV head and up to 4, 8 or 16 of its query rows (query token, head of the group), with all pairs of pages of the sequence.
+// The pairs of all units in a row are cut into equal shares, one a CTA, as many as the GPU holds at once, whatever the lengths are: a CTA has the end of
+// one unit, whole ones, and the beginning of another.  What it has of a unit that others have too it leaves in fp32 for the merge.
+// The warps of a CTA take pairs in turn, each through a ring of its own that its lanes fill by 16-byte asynchronous copies; a lane reads the codes that it copied.
 // A page's tokens are the rows of the products and the query rows their columns:
 //   S^T [16 x 8] = K Q^T,   O^T [D x 8] += V^T (p s),   p s being S^T's accumulator transposed by movmatrix.
 // Up to 4 query rows have the two pages side by side: the first page is multiplied by [Q 0], the second by [0 Q], into the same accumulator, so that no
@@ -30,9 +32,9 @@ struct Kv4AttnArgs {
   const uint8_t* pool;
   const int *table, *seq_lens;
   void* out;
-  float *part_o, *part_ml;  // [B * q_len * Hq, splits, D], [.., splits, 2]
+  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if a unit goes on in it, and of its last one; null: a CTA has a unit
   int* status;
-  int B, Hq, Hk, width, pages, q_len, splits, chunk, tiles;  // chunk: pages; tiles: of query rows of a KV head
+  int B, Hq, Hk, width, pages, q_len, least, tiles;  // least: pairs of a share at least; tiles: of query rows of a KV head
   float scale_log2;
 };
 
@@ -77,6 +79,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+constexpr int kAtOnce = 8;  // pieces of the merge
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 template <typename T> __device__ __forceinline__ float2 kv4_pair(uint32_t v);
@@ -366,6 +369,45 @@ struct Kv4Rows {
   }
 };
 
+// The units' pairs in a row, found by a whole warp
+struct Kv4Shares {
+  long long total, share;
+  int per_seq;  // units of a sequence
+  __device__ __forceinline__ static int pairs(const Kv4AttnArgs& a, int seq) {
+    return seq < a.B ? int((max(0ll, min((long long)a.seq_lens[seq], 16ll * a.width)) + 31) >> 5) : 0;
+  }
+  __device__ __forceinline__ Kv4Shares(const Kv4AttnArgs& a, int ctas) : total(0), per_seq(a.Hk * a.tiles) {
+    for (int b = 0; b < a.B; b += 32) total += __reduce_add_sync(0xffffffffu, unsigned(pairs(a, b + int(lane_id()))));  // 32 * 2^26 at most
+    total *= per_seq;
+    share = max((long long)a.least, (total + ctas - 1) / ctas);
+  }
+  // The sequence that has the x-th pair, and the pairs in front of it
+  __device__ __forceinline__ int find(const Kv4AttnArgs& a, long long x, long long& before) const {
+    before = 0;
+    for (int b = 0;; b += 32) {
+      const unsigned n = unsigned(pairs(a, b + int(lane_id())));
+      unsigned upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (int(lane_id()) >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * per_seq > x);
+      if (past || b + 32 >= a.B) {
+        const int at = past ? __ffs(past) - 1 : 31;
+        before += __shfl_sync(0xffffffffu, upto - n, at);
+        return b + at;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  __device__ __forceinline__ long long in_front_of(const Kv4AttnArgs& a, int seq) const {  // pairs
+    long long before = 0;
+    for (int b = 0; b < seq; b += 32) before += __reduce_add_sync(0xffffffffu, b + int(lane_id()) < seq ? unsigned(pairs(a, b + int(lane_id()))) : 0u);
+    return before;
+  }
+};
+
 template <int D, int kCols, typename T, int kMinBlocks>
 __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a) {
   pdl_trigger();
@@ -378,174 +420,233 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   uint8_t* ring = smem + warp * L::kWarp;
   pdl_wait();
 
-  const int seq = blockIdx.x, kvh = blockIdx.y / a.tiles, first = blockIdx.y % a.tiles * kCols, split = blockIdx.z;
-  const int rows = a.Hq / a.Hk * a.q_len;
-  const int length = int(max(0ll, min((long long)a.seq_lens[seq], 16ll * a.width)));
-  const int total = (length + 15) >> 4, per = a.chunk / (2 * L::kWarps);  // pages; pairs of a chunk that a warp has
-  if (a.splits > 1 && (long long)split * a.chunk >= total) return;  // nothing here, and nobody looks
-  // chunks split, split + splits, ...; a warp's pairs in them
-  int mine = 0;
-  {
-    const int whole = total / a.chunk, left = total - whole * a.chunk;
-    mine = (whole > split ? (whole - split + a.splits - 1) / a.splits : 0) * per;
-    if (left > 2 * warp && whole >= split && (whole - split) % a.splits == 0) mine += (left - 2 * warp + 2 * L::kWarps - 1) / (2 * L::kWarps);
+  const int rows = a.Hq / a.Hk * a.q_len, per_head = a.Hq / a.Hk;
+  // sequences without a token: zeros
+  for (int seq = blockIdx.x; seq < a.B; seq += gridDim.x) {
+    if (a.seq_lens[seq] > 0) continue;
+    uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + size_t(seq) * a.q_len * a.Hq * D);
+    for (long long i = threadIdx.x; i < (long long)a.q_len * a.Hq * D / 8; i += 128) y[i] = make_uint4(0, 0, 0, 0);
   }
-  const int* bt = a.table + size_t(seq) * a.width;
-  // The pairs in order, twice: as they are requested, ids a pair ahead, and as they are used
-  struct Walk {
-    int page, left;
-  };
-  const auto step = [&](Walk& x) {
-    x.page += 2 * L::kWarps;
-    if (--x.left == 0) {
-      x.page += (a.splits - 1) * a.chunk;
-      x.left = per;
-    }
-  };
-  Walk asked{split * a.chunk + 2 * warp, per}, used = asked;
-  int id[2] = {0, 0};
-  const auto look = [&] {  // the ids of the pair that is asked for next
-    id[0] = bt[asked.page];
-    id[1] = asked.page + 1 < total ? bt[asked.page + 1] : id[0];
-  };
-  const uint32_t to = smem_u32(ring) + 16 * lane;
+  int seq, unit, off, pairs;  // where this CTA is: unit of the sequence, pair of the unit
+  long long left;
+  if (a.part_o == nullptr) {
+    seq = blockIdx.x / (a.Hk * a.tiles);
+    unit = blockIdx.x % (a.Hk * a.tiles);
+    off = 0;
+    left = pairs = Kv4Shares::pairs(a, seq);
+  } else {
+    const Kv4Shares all(a, gridDim.x);
+    const long long x = blockIdx.x * all.share;
+    if (x >= all.total) return;
+    left = min(all.share, all.total - x);
+    long long before;
+    seq = all.find(a, x, before);
+    pairs = Kv4Shares::pairs(a, seq);
+    const long long in = x - before * all.per_seq;
+    unit = int(in / pairs);
+    off = int(in - (long long)unit * pairs);
+  }
   constexpr int kParts = D / 8;  // pieces of 16 bytes of a page's parameters: K's, then V's
   const int piece = lane % (kParts < 32 ? kParts : 32);
   const uint32_t piece_at = piece < kParts / 2 ? 8 * D + 16 * piece : 17 * D + 16 * (piece - kParts / 2);
-  const auto request = [&](int s) {
-    const uint8_t* rec[2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      if (uint32_t(id[p]) >= uint32_t(a.pages)) {
-        if (lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
-        id[p] = 0;
-      }
-      rec[p] = a.pool + (size_t(id[p]) * a.Hk + kvh) * L::kRecord;
-    }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {  // a second page that is not there: the first again
-      const uint8_t* from = rec[p] + 16 * lane;
-      const uint32_t at = to + s * L::kStage + p * L::kRecord;
-#pragma unroll
-      for (int g = 0; g < D / 64; ++g) copy16(at + 512 * g, from + 512 * g);
-#pragma unroll
-      for (int g = 0; g < D / 64; ++g) copy16(at + 9 * D + 512 * g, from + 9 * D + 512 * g);
-    }
-    const uint32_t at = smem_u32(ring) + s * L::kStage + piece_at;
-    if constexpr (kParts == 32) {
-      copy16(at, rec[0] + piece_at);
-      copy16(at + L::kRecord, rec[1] + piece_at);
-    } else {
-      const int p = lane / kParts;
-      if (p < 2) copy16(at + p * L::kRecord, (p == 0 ? rec[0] : rec[1]) + piece_at);
-    }
-  };
-  if (mine > 0) look();
-#pragma unroll
-  for (int i = 0; i < L::kStages; ++i) {
-    if (i < mine) {
-      request(i);
-      step(asked);
-      if (i + 1 < mine) look();
-    }
-    copies_end_here();
-  }
-  R t;
-  t.load(a, seq, kvh, first, rows, length);
-  int s = 0;
-  for (int i = 0; i < mine; ++i) {
-    copies_but_the_last<L::kStages - 1>();
-    __syncwarp();
-    if ((used.page << 4) + 32 <= t.low) t.template pages<true>(ring + s * L::kStage, used.page << 4);
-    else t.template pages<false>(ring + s * L::kStage, used.page << 4);
-    step(used);
-    __syncwarp();
-    if (i + L::kStages < mine) {
-      request(s);
-      step(asked);
-      if (i + 1 + L::kStages < mine) look();
-    }
-    copies_end_here();
-    if (++s == L::kStages) s = 0;
-  }
+  bool begins = true;  // the share's first piece
+  uint32_t strays = 0;  // not 0: a page out of range, the last one was read in its place
 
-  // ---- the lanes of a column, then the warps ----
-  float* part = reinterpret_cast<float*>(ring);
-  float* ml = part + 8 * NB * kStride;
-  __syncwarp();
+  while (left > 0) {
+    const int here = int(min(left, (long long)(pairs - off)));
+    const int kvh = unit / a.tiles, first = unit % a.tiles * kCols;
+    const int length = int(min((long long)a.seq_lens[seq], 16ll * a.width)), total = (length + 15) >> 4;  // pages
+    const int mine = here > warp ? (here - warp + L::kWarps - 1) / L::kWarps : 0;
+    const int* bt = a.table + size_t(seq) * a.width;
+    int asked = 2 * (off + warp), used = asked, id[2];  // pages
+    const auto look = [&] {  // the ids of the pair that is asked for next; a second page that is not there: the first again
+      const int at = min(asked, total - 1);
+      id[0] = bt[at];
+      id[1] = bt[min(at + 1, total - 1)];
+      asked += 2 * L::kWarps;
+    };
+    const auto request = [&](uint32_t stage) {
+      const uint8_t* rec[2];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t page = min(uint32_t(id[p]), uint32_t(a.pages - 1));
+        strays |= page ^ uint32_t(id[p]);
+        rec[p] = a.pool + (size_t(page) * a.Hk + kvh) * L::kRecord;
+      }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = 8 * b + 2 * c + e;
-      float sum = e == 0 ? t.l[b].x : t.l[b].y;
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      if (g8 == 0) { ml[2 * r] = -(e == 0 ? t.less[b].x : t.less[b].y); ml[2 * r + 1] = sum; }
+      for (int p = 0; p < 2; ++p) {
+        const uint8_t* from = rec[p] + 16 * lane;
+        const uint32_t at = stage + 16 * lane + p * L::kRecord;
 #pragma unroll
-      for (int g = 0; g < D / 64; ++g) {
-        float om = e == 0 ? t.om[b][g].x : t.om[b][g].y;
-        om += __shfl_xor_sync(0xffffffffu, om, 4);
-        om += __shfl_xor_sync(0xffffffffu, om, 8);
-        om += __shfl_xor_sync(0xffffffffu, om, 16);
+        for (int g = 0; g < D / 64; ++g) copy16(at + 512 * g, from + 512 * g);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          part[r * kStride + 64 * g + 16 * j + g8] = fmaf(t.o[b][4 * g + j][e], 0x1p24f, om);
-          part[r * kStride + 64 * g + 16 * j + 8 + g8] = fmaf(t.o[b][4 * g + j][2 + e], 0x1p20f, om);
+        for (int g = 0; g < D / 64; ++g) copy16(at + 9 * D + 512 * g, from + 9 * D + 512 * g);
+      }
+      if constexpr (kParts == 32) {
+        copy16(stage + piece_at, rec[0] + piece_at);
+        copy16(stage + piece_at + L::kRecord, rec[1] + piece_at);
+      } else if constexpr (kParts == 16) {
+        copy16(stage + piece_at + (lane < 16 ? 0 : L::kRecord), (lane < 16 ? rec[0] : rec[1]) + piece_at);
+      } else {
+        if (lane < 2 * kParts) copy16(stage + piece_at + (lane < kParts ? 0 : L::kRecord), (lane < kParts ? rec[0] : rec[1]) + piece_at);
+      }
+    };
+    const uint32_t ring_at = smem_u32(ring);
+    look();
+#pragma unroll
+    for (int i = 0; i < L::kStages; ++i) {
+      if (i < mine) {
+        request(ring_at + i * L::kStage);
+        look();
+      }
+      copies_end_here();
+    }
+    R t;
+    t.load(a, seq, kvh, first, rows, length);
+    // pairs that all rows see whole come first, the masked ones of a sequence's end behind them
+    int stage = 0, more = mine - L::kStages;
+    const auto next = [&] {
+      used += 2 * L::kWarps;
+      __syncwarp();
+      if (more > 0) {
+        request(ring_at + stage);
+        look();
+      }
+      copies_end_here();
+      --more;
+      stage = stage == (L::kStages - 1) * L::kStage ? 0 : stage + L::kStage;
+    };
+    const int end = used + 2 * L::kWarps * mine, seen = min(end, (t.low >> 4) - 1);
+    while (used < seen) {
+      copies_but_the_last<L::kStages - 1>();
+      __syncwarp();
+      t.template pages<true>(ring + stage, used << 4);
+      next();
+    }
+    while (used < end) {
+      copies_but_the_last<L::kStages - 1>();
+      __syncwarp();
+      t.template pages<false>(ring + stage, used << 4);
+      next();
+    }
+
+    // ---- the lanes of a column, then the warps ----
+    float* part = reinterpret_cast<float*>(ring);
+    float* ml = part + 8 * NB * kStride;
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * b + 2 * c + e;
+        float sum = e == 0 ? t.l[b].x : t.l[b].y;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g8 == 0) { ml[2 * r] = -(e == 0 ? t.less[b].x : t.less[b].y); ml[2 * r + 1] = sum; }
+#pragma unroll
+        for (int g = 0; g < D / 64; ++g) {
+          float om = e == 0 ? t.om[b][g].x : t.om[b][g].y;
+          om += __shfl_xor_sync(0xffffffffu, om, 4);
+          om += __shfl_xor_sync(0xffffffffu, om, 8);
+          om += __shfl_xor_sync(0xffffffffu, om, 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            part[r * kStride + 64 * g + 16 * j + g8] = fmaf(t.o[b][4 * g + j][e], 0x1p24f, om);
+            part[r * kStride + 64 * g + 16 * j + 8 + g8] = fmaf(t.o[b][4 * g + j][2 + e], 0x1p20f, om);
+          }
         }
       }
     }
-  }
-  __syncthreads();
-  const int here = min(rows - first, kCols), per_head = a.Hq / a.Hk;
-  for (int i = threadIdx.x; i < here * D; i += 128) {
-    const int r = i / D, d = i % D;
-    float ref = -FLT_MAX, l = 0.f, o = 0.f;
+    __syncthreads();
+    const bool whole = here == pairs;
+    const size_t slot = (2 * size_t(blockIdx.x) + (begins ? 0 : 1)) * kCols;
+    const int live = min(rows - first, kCols);
+    for (int i = threadIdx.x; i < live * D; i += 128) {
+      const int r = i / D, d = i % D;
+      float ref = -FLT_MAX, l = 0.f, o = 0.f;
 #pragma unroll
-    for (int w = 0; w < L::kWarps; ++w) ref = fmaxf(ref, reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
+      for (int w = 0; w < L::kWarps; ++w) ref = fmaxf(ref, reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
 #pragma unroll
-    for (int w = 0; w < L::kWarps; ++w) {
-      const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
-      const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref);
-      float lw = from[8 * NB * kStride + 2 * r + 1], ow = from[r * kStride + d];
-      if constexpr (R::kSide) { lw += from[8 * NB * kStride + 2 * r + 9]; ow += from[(r + 4) * kStride + d]; }
-      l += lw * weight;
-      o += ow * weight;
+      for (int w = 0; w < L::kWarps; ++w) {
+        const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
+        const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref);
+        float lw = from[8 * NB * kStride + 2 * r + 1], ow = from[r * kStride + d];
+        if constexpr (R::kSide) { lw += from[8 * NB * kStride + 2 * r + 9]; ow += from[(r + 4) * kStride + d]; }
+        l += lw * weight;
+        o += ow * weight;
+      }
+      if (whole) {
+        const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
+        static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
+      } else {
+        a.part_o[(slot + r) * D + d] = o;
+        if (d == 0) { a.part_ml[(slot + r) * 2] = ref; a.part_ml[(slot + r) * 2 + 1] = l; }
+      }
     }
-    const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
-    if (a.splits == 1) {
-      static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
-    } else {
-      a.part_o[(row * a.splits + split) * D + d] = o;
-      if (d == 0) { a.part_ml[(row * a.splits + split) * 2] = ref; a.part_ml[(row * a.splits + split) * 2 + 1] = l; }
+    left -= here;
+    begins = false;
+    off = 0;
+    if (left > 0) {
+      __syncthreads();  // the rings are rings again
+      if (++unit == a.Hk * a.tiles) {
+        unit = 0;
+        do pairs = Kv4Shares::pairs(a, ++seq);
+        while (pairs == 0 && seq < a.B);
+        if (seq >= a.B) break;  // lengths that changed under the kernel
+      }
     }
   }
+  if (strays && lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
 }
 
-// Joins the splits of a query row and head; those behind the sequence's last chunk left nothing.
-template <int D, typename T>
-__global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a) {
+// Joins the pieces of a unit that several CTAs have, a block a query row and head.  `ctas`: of the kernel before
+template <int D, int kCols, typename T>
+__global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a, int ctas) {
   pdl_trigger();
   pdl_wait();
+  const int per_head = a.Hq / a.Hk, d = threadIdx.x;
   const size_t row = blockIdx.x;
-  const int d = threadIdx.x;
-  const int length = int(max(0ll, min((long long)a.seq_lens[row / a.Hq / a.q_len], 16ll * a.width)));
-  const int n = min(a.splits, (((length + 15) >> 4) + a.chunk - 1) / a.chunk);
-  const float* ml = a.part_ml + row * a.splits * 2;
-  const float* po = a.part_o + row * a.splits * D + d;
+  const int seq = int(row / a.Hq / a.q_len), head = int(row % a.Hq), kvh = head / per_head, r = int(row / a.Hq % a.q_len) * per_head + head % per_head;
+  const int pairs = Kv4Shares::pairs(a, seq);
+  if (pairs == 0) return;
+  const Kv4Shares all(a, ctas);
+  const long long from = all.in_front_of(a, seq) * all.per_seq + (long long)(kvh * a.tiles + r / kCols) * pairs;
+  const int c0 = int(from / all.share), n = int((from + pairs - 1) / all.share) - c0 + 1;
+  if (n == 1) return;
+  // the unit's pieces are the first ones of their CTAs, but for its beginning, where something may be in front of it
+  const auto slot = [&](int k) { return (2 * size_t(c0 + k) + (k > 0 || from == c0 * all.share ? 0 : 1)) * kCols + r % kCols; };
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   float ref = -FLT_MAX, l = 0.f, o = 0.f;
-  for (int i = 0; i < n; ++i) ref = fmaxf(ref, ml[2 * i]);
-  for (int i = 0; i < n; ++i) {
-    const float weight = kv4_exp2(ml[2 * i] - ref);
-    l += ml[2 * i + 1] * weight;
-    o += po[size_t(i) * D] * weight;
+  for (int k = 0; k < n; k += kAtOnce) {
+    float2 of[kAtOnce];
+    float part[kAtOnce];
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {  // all requested before the first is used
+      of[e] = k + e < n ? ml[slot(k + e)] : make_float2(-FLT_MAX, 0.f);
+      part[e] = k + e < n ? a.part_o[slot(k + e) * D + d] : 0.f;
+    }
+    float next = ref;
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) next = fmaxf(next, of[e].x);
+    const float keep = kv4_exp2(ref - next);
+    l *= keep;
+    o *= keep;
+    ref = next;
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      if (k + e < n) {
+        const float weight = kv4_exp2(of[e].x - ref);
+        l += of[e].y * weight;
+        o += part[e] * weight;
+      }
+    }
   }
   static_cast<T*>(a.out)[row * D + d] = kv4_out<T>(l == 0.f ? 0.f : o / l);
 }
 
 template <int D, int kCols, typename T>
-static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
+static int launch_kv4_attn_of(Kv4AttnArgs a, int ctas, cudaStream_t stream) {
   using L = Kv4Ring<D>;
   constexpr int kMinBlocks = D == 256 || kCols == 16 ? 2 : 4;
   auto kernel = &kv4_attn_kernel<D, kCols, T, kMinBlocks>;
@@ -556,38 +657,38 @@ static int launch_kv4_attn_of(Kv4AttnArgs a, cudaStream_t stream) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return -6;
     attr[dev] = true;
   }
-  const long long rows = (long long)a.Hq / a.Hk * a.q_len, tiles = (rows + kCols - 1) / kCols;
-  if (a.Hk * tiles > 65535 || a.splits > 65535 || (long long)a.B * a.q_len * a.Hq > 0x7fffffffll || a.chunk % (2 * L::kWarps)) return -2;
+  const long long tiles = ((long long)a.Hq / a.Hk * a.q_len + kCols - 1) / kCols, units = (long long)a.B * a.Hk * tiles;
+  if (units > 0x7fffffffll || (long long)a.B * a.q_len * a.Hq > 0x7fffffffll) return -2;
   a.tiles = int(tiles);
-  if (launch_kernel(kernel, dim3(a.B, unsigned(a.Hk * tiles), a.splits), dim3(128), L::kSmem, stream, a) != cudaSuccess) return -7;
-  if (a.splits > 1 && launch_kernel(&kv4_merge_kernel<D, T>, dim3(unsigned(a.B * a.q_len * a.Hq)), dim3(D), 0, stream, a) != cudaSuccess) return -7;
+  if (launch_kernel(kernel, dim3(unsigned(a.part_o ? ctas : units)), dim3(128), L::kSmem, stream, a) != cudaSuccess) return -7;
+  if (a.part_o && launch_kernel(&kv4_merge_kernel<D, kCols, T>, dim3(unsigned(a.B * a.q_len * a.Hq)), dim3(D), 0, stream, a, ctas) != cudaSuccess) return -7;
   return 0;
 }
 template <int D, typename T>
-static int launch_kv4_attn_for(const Kv4AttnArgs& a, cudaStream_t stream) {
+static int launch_kv4_attn_for(const Kv4AttnArgs& a, int ctas, cudaStream_t stream) {
   const long long rows = (long long)a.Hq / a.Hk * a.q_len;
-  if (rows <= 4) return launch_kv4_attn_of<D, 4, T>(a, stream);
-  if (D == 256 || rows <= 8) return launch_kv4_attn_of<D, 8, T>(a, stream);
-  if constexpr (D < 256) return launch_kv4_attn_of<D, 16, T>(a, stream);
+  if (rows <= 4) return launch_kv4_attn_of<D, 4, T>(a, ctas, stream);
+  if (D == 256 || rows <= 8) return launch_kv4_attn_of<D, 8, T>(a, ctas, stream);
+  if constexpr (D < 256) return launch_kv4_attn_of<D, 16, T>(a, ctas, stream);
   return -1;
 }
 template <int D>
-static int launch_kv4_attn(const Kv4AttnArgs& a, bool half, cudaStream_t stream) {
-  return half ? launch_kv4_attn_for<D, __half>(a, stream) : launch_kv4_attn_for<D, __nv_bfloat16>(a, stream);
+static int launch_kv4_attn(const Kv4AttnArgs& a, int ctas, bool half, cudaStream_t stream) {
+  return half ? launch_kv4_attn_for<D, __half>(a, ctas, stream) : launch_kv4_attn_for<D, __nv_bfloat16>(a, ctas, stream);
 }
 
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16 or fp16 (`half`); pool: [pages, Hk, 18 D]; table: [B, width]; seq_lens count every token visible to the last query row.
-// The tokens of a sequence are taken in chunks of `chunk` pages (a multiple of 8) by `splits` blocks in turn; part_o, part_ml: [B * q_len * Hq, splits, D],
-// [.., 2] fp32 where there are several.
+// part_o: null, and every unit has a CTA of its own, or scratch for `ctas` equal shares of at least `least` pairs of pages: [2 * ctas, cols, D] fp32,
+// with part_ml [2 * ctas, cols, 2], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
 extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, float* part_o, float* part_ml, int half,
-                                         int B, int Hq, int Hk, int D, int width, int pages, int q_len, int splits, int chunk, float sm_scale, int* status,
+                                         int B, int Hq, int Hk, int D, int width, int pages, int q_len, int ctas, int least, float sm_scale, int* status,
                                          cudaStream_t stream) {
-  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || splits < 1 || chunk < 1) return -1;
-  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, part_ml, status, B, Hq, Hk, width, pages, q_len, splits, chunk, 0, sm_scale * 1.4426950408889634f};
-  if (D == 64) return mfq::launch_kv4_attn<64>(a, half != 0, stream);
-  if (D == 128) return mfq::launch_kv4_attn<128>(a, half != 0, stream);
-  if (D == 256) return mfq::launch_kv4_attn<256>(a, half != 0, stream);
+  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || (part_o == nullptr) != (part_ml == nullptr)) return -1;
+  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, part_ml, status, B, Hq, Hk, width, pages, q_len, least, 0, sm_scale * 1.4426950408889634f};
+  if (D == 64) return mfq::launch_kv4_attn<64>(a, ctas, half != 0, stream);
+  if (D == 128) return mfq::launch_kv4_attn<128>(a, ctas, half != 0, stream);
+  if (D == 256) return mfq::launch_kv4_attn<256>(a, ctas, half != 0, stream);
   return -1;
 }

@@ -23,7 +23,8 @@ from .logits import _DTYPES, _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
 SMS = 148
-MAX_SPLITS = 64
+ALONE = 8  # pairs of pages of a unit that has a CTA of its own
+LEAST = 4  # pairs of pages of a share: one a warp
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
 
 
@@ -78,14 +79,15 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None
 
 
 @lru_cache(maxsize=4096)
-def _shape(units: int, rows: int, d: int, pages: int) -> tuple[int, int]:
-    """(splits, pages of a chunk) for ``units`` sequences and KV heads with ``rows`` query rows each and up to ``pages`` pages."""
-    wide = rows > 8 and d < 256
-    units *= -(-rows // (16 if wide else 8))
-    slots = SMS * (2 if wide or d == 256 else 4)
-    splits = max(1, min(slots // units, -(-pages // 8), MAX_SPLITS))
-    chunk = max(8, -(-pages // (8 * splits)) * 8)
-    return max(1, -(-pages // chunk)), chunk
+def _shape(b: int, hk: int, rows: int, d: int, pages: int, width: int) -> tuple[int, int, int]:
+    """(columns of a unit, CTAs that share all pairs of pages or 0 for a CTA a unit, pairs of a share at least) for ``b`` sequences of up to ``pages`` pages,
+    ``width`` in the table, and ``rows`` query rows a KV head."""
+    cols = 4 if rows <= 4 else (8 if rows <= 8 or d == 256 else 16)
+    units = b * hk * -(-rows // cols)
+    if (width + 1) // 2 <= ALONE:
+        return cols, 0, 1
+    slots = SMS * (2 if d == 256 or cols == 16 else 4)
+    return cols, max(1, min(slots, units * -(-((pages + 1) // 2) // LEAST))), LEAST
 
 
 def _table(block_table: torch.Tensor, b: int, index: int) -> int:
@@ -171,11 +173,11 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     if elsewhere(index):
         with torch.cuda.device(index):
             return paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale=sm_scale, q_len=q_len, max_len=max_len, out=out)
-    splits, chunk = _shape(b * hk, hq // hk * q_len, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)))
-    parts = n * hq * splits if splits > 1 else 0
+    cols, ctas, least = _shape(b, hk, hq // hk * q_len, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)), width)
+    parts = 2 * ctas * cols
     scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device) if parts else None  # of this call: a workspace would tie streams and graphs together
     at = scratch.data_ptr() if parts else 0
     check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), at, at + 4 * parts * d,
-                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, splits, chunk, sm_scale, Workspace.get(q.device).status.data_ptr(),
-                                          stream_ptr()), "paged_attn_decode_kv4", 2 if parts else 1)
+                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, max(1, ctas), least, sm_scale,
+                                          Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if parts else 1)
     return out
