@@ -27,12 +27,16 @@
 
 namespace mfq {
 
+struct Kv4Join {  // the unit that ends in a CTA's first piece: how many CTAs have pieces of it (0: there is none), and whether the first of these has something in front
+  int seq, unit, n, behind;
+};
 struct Kv4AttnArgs {
   const void* q;
   const uint8_t* pool;
   const int *table, *seq_lens;
   void* out;
-  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if a unit goes on in it, and of its last one; null: a CTA has a unit
+  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if others have the rest of the unit, and of its last one; null: a CTA has a unit
+  Kv4Join* joins;           // [CTAs]
   int* status;
   int B, Hq, Hk, width, pages, q_len, least, tiles;  // least: pairs of a share at least; tiles: of query rows of a KV head
   float scale_log2;
@@ -40,7 +44,7 @@ struct Kv4AttnArgs {
 
 template <int D>
 struct Kv4Ring {
-  static constexpr int kRecord = 18 * D, kStage = 2 * kRecord, kStages = D <= 128 ? 3 : 2, kWarps = 4;
+  static constexpr int kRecord = 18 * D, kStage = 2 * kRecord, kStages = D == 64 ? 3 : 2, kWarps = 4;
   static constexpr int kWarp = kStages * kStage, kSmem = kWarps * kWarp;
 };
 
@@ -94,16 +98,16 @@ template <> __device__ __forceinline__ __half kv4_out(float v) { return __float2
 template <int D, int kCols, typename T>
 struct Kv4Rows {
   static constexpr bool kSide = kCols == 4;
+  static constexpr int kQ = kCols == 8 ? 2 : 4;  // words of a lane's q of a step: of a column block, or of two; kSide: of [Q 0] and [0 Q]
   static constexpr int G = D / 64, kSteps = D / 16, NB = kSide ? 1 : kCols / 8, P = kSide ? 1 : 2;  // P: pages of a pair whose scores a lane has
-  uint32_t q[kSide ? 2 : NB][kSteps][2];              // by column block; kSide: [Q 0] and [0 Q]
   float sums[NB][G][2], top[NB][2], lim[NB][2];       // of a group's q; the running maximum; the score, in units of the products, that is too far above it
   float2 to_log2[NB], less[NB], om[NB][G], l[NB];     // what such a score is times log2 e; -ref
   float o[NB][kSteps][4];
   float up, over;  // log2 of what V's scales are multiplied by, and the scale that would be too large
   int len[NB][2], low, most;
 
-  __device__ __forceinline__ void load(const Kv4AttnArgs& a, int seq, int kvh, int first, int rows, int length) {
-    const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3, per = a.Hq / a.Hk;
+  __device__ __forceinline__ void load(const Kv4AttnArgs& a, int seq, int kvh, int first, int rows, int length, uint32_t* q) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, c = lane & 3, per = a.Hq / a.Hk;
     int lo = INT_MAX, hi = 0;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -139,11 +143,10 @@ struct Kv4Rows {
         for (int s = 4 * g; s < 4 * g + 4; ++s) {
           const float2 v = kv4_pair<T>(raw[s][0]), w = kv4_pair<T>(raw[s][1]);
           const uint32_t x = half_pair(v.x * scale, v.y * scale), y = half_pair(w.x * scale * 0.0625f, w.y * scale * 0.0625f);
-          if constexpr (kSide) {
-            q[0][s][0] = g8 < 4 ? x : 0u; q[0][s][1] = g8 < 4 ? y : 0u;
-            q[1][s][0] = g8 < 4 ? 0u : x; q[1][s][1] = g8 < 4 ? 0u : y;
-          } else {
-            q[b][s][0] = x; q[b][s][1] = y;
+          if (s % 4 == warp) {  // the block's, for all of its warps
+            uint32_t* mine = q + (32 * s + lane) * kQ;
+            if constexpr (kSide) *reinterpret_cast<uint4*>(mine) = g8 < 4 ? make_uint4(x, y, 0u, 0u) : make_uint4(0u, 0u, x, y);
+            else *reinterpret_cast<uint2*>(mine + 2 * b) = make_uint2(x, y);
           }
           sum += (v.x * scale + v.y * scale) + (w.x * scale + w.y * scale);
         }
@@ -180,43 +183,57 @@ struct Kv4Rows {
 
   // Two pages whose first token is tok0; kWhole: all rows see all of both
   template <bool kWhole>
-  __device__ __forceinline__ void pages(const uint8_t* rec0, int tok0) {
+  __device__ __forceinline__ void pages(const uint8_t* rec0, const uint32_t* q, int tok0) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
     const int side = kSide ? c >> 1 : 0;  // the page whose scores this lane has
     const auto sees = [&](int b, int e, int p, int h) { return tok0 + 16 * (p + side) + 8 * h + g8 < len[b][e]; };
     float2 sc[NB][P][2];  // [page][token g8, g8 + 8], of two columns
-    float acc[NB][G][4];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint8_t* rec = rec0 + p * 18 * D;
+    for (int g = 0; g < G; ++g) {
+      float acc[NB][P][4];
+      uint32_t w[2][4];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      for (int p = 0; p < 2; ++p) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(rec0 + p * 18 * D + 512 * g + 16 * lane);
+        w[p][0] = raw.x; w[p][1] = raw.y; w[p][2] = raw.z; w[p][3] = raw.w;
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t h = w[j] >> 8;
+      for (int j = 0; j < 4; ++j) {
+        uint32_t qw[kQ];
+        const uint32_t* from = q + (32 * (4 * g + j) + lane) * kQ;
+        if constexpr (kQ == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(from);
+          qw[0] = v.x; qw[1] = v.y; qw[2] = v.z; qw[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(from);
+          qw[0] = v.x; qw[1] = v.y;
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t h = w[p][j] >> 8;
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            const uint32_t(&qb)[2] = q[kSide ? p : b][4 * g + j];
-            if (j == 0 && (p == 0 || !kSide)) kv4_first_product(acc[b][g], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, qb[0], qb[1]);
-            else kv4_product(acc[b][g], w[j] & kLow, h & kLow, w[j] & kHigh, h & kHigh, qb[0], qb[1]);
+            const int of = 2 * (kSide ? p : b);
+            float(&x)[4] = acc[b][kSide ? 0 : p];
+            if (j == 0 && (p == 0 || !kSide)) kv4_first_product(x, w[p][j] & kLow, h & kLow, w[p][j] & kHigh, h & kHigh, qw[of], qw[of + 1]);
+            else kv4_product(x, w[p][j] & kLow, h & kLow, w[p][j] & kHigh, h & kHigh, qw[of], qw[of + 1]);
           }
         }
       }
-      if (kSide && p == 0) continue;
-      uint32_t par[2][G];  // of tokens g8 and g8 + 8
-      params(par, rec0 + (kSide ? side : p) * 18 * D + 8 * D + g8 * (D / 8));
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
+      for (int p = 0; p < P; ++p) {
+        uint32_t par[2];  // of tokens g8 and g8 + 8
+        const uint8_t* at = rec0 + (p + side) * 18 * D + 8 * D + g8 * (D / 8) + 4 * g;
+        par[0] = *reinterpret_cast<const uint32_t*>(at);
+        par[1] = *reinterpret_cast<const uint32_t*>(at + 4 * G);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float ps = __uint_as_float(par[h][g] << 16), pm = __uint_as_float(par[h][g] & 0xffff0000u);
+          const float ps = __uint_as_float(par[h] << 16), pm = __uint_as_float(par[h] & 0xffff0000u);
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            float2& x = sc[b][kSide ? 0 : p][h];
-            x.x = fmaf(ps, acc[b][g][2 * h], g == 0 ? pm * sums[b][g][0] : fmaf(pm, sums[b][g][0], x.x));
-            x.y = fmaf(ps, acc[b][g][2 * h + 1], g == 0 ? pm * sums[b][g][1] : fmaf(pm, sums[b][g][1], x.y));
+            float2& x = sc[b][p][h];
+            x.x = fmaf(ps, acc[b][p][2 * h], g == 0 ? pm * sums[b][g][0] : fmaf(pm, sums[b][g][0], x.x));
+            x.y = fmaf(ps, acc[b][p][2 * h + 1], g == 0 ? pm * sums[b][g][1] : fmaf(pm, sums[b][g][1], x.y));
           }
         }
       }
@@ -369,42 +386,52 @@ struct Kv4Rows {
   }
 };
 
+__device__ __forceinline__ long long kv4_quotient(long long a, long long b) {  // of numbers that are not negative; 64 bits take ten times as long
+  return (a | b) >> 32 ? a / b : (long long)(uint32_t(a) / uint32_t(b));
+}
 // The units' pairs in a row, found by a whole warp
 struct Kv4Shares {
+  static constexpr int kHeld = 4;  // lengths that a lane keeps: of 128 sequences
+  unsigned held[kHeld];
   long long total, share;
   int per_seq;  // units of a sequence
   __device__ __forceinline__ static int pairs(const Kv4AttnArgs& a, int seq) {
     return seq < a.B ? int((max(0ll, min((long long)a.seq_lens[seq], 16ll * a.width)) + 31) >> 5) : 0;
   }
   __device__ __forceinline__ Kv4Shares(const Kv4AttnArgs& a, int ctas) : total(0), per_seq(a.Hk * a.tiles) {
-    for (int b = 0; b < a.B; b += 32) total += __reduce_add_sync(0xffffffffu, unsigned(pairs(a, b + int(lane_id()))));  // 32 * 2^26 at most
-    total *= per_seq;
-    share = max((long long)a.least, (total + ctas - 1) / ctas);
-  }
-  // The sequence that has the x-th pair, and the pairs in front of it
-  __device__ __forceinline__ int find(const Kv4AttnArgs& a, long long x, long long& before) const {
-    before = 0;
-    for (int b = 0;; b += 32) {
-      const unsigned n = unsigned(pairs(a, b + int(lane_id())));
-      unsigned upto = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (int(lane_id()) >= o) upto += v;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * per_seq > x);
-      if (past || b + 32 >= a.B) {
-        const int at = past ? __ffs(past) - 1 : 31;
-        before += __shfl_sync(0xffffffffu, upto - n, at);
-        return b + at;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
+    for (int k = 0; k < kHeld; ++k) held[k] = unsigned(pairs(a, 32 * k + int(lane_id())));
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) total += __reduce_add_sync(0xffffffffu, held[k]);  // 32 * 2^26 at most
+    for (int b = 32 * kHeld; b < a.B; b += 32) total += __reduce_add_sync(0xffffffffu, unsigned(pairs(a, b + int(lane_id()))));
+    total *= per_seq;
+    share = max((long long)a.least, kv4_quotient(total + ctas - 1, ctas));
   }
-  __device__ __forceinline__ long long in_front_of(const Kv4AttnArgs& a, int seq) const {  // pairs
-    long long before = 0;
-    for (int b = 0; b < seq; b += 32) before += __reduce_add_sync(0xffffffffu, b + int(lane_id()) < seq ? unsigned(pairs(a, b + int(lane_id()))) : 0u);
-    return before;
+  // Among 32 sequences with n pairs each: the one that has the x-th pair, -1: it is behind them; `before`: the pairs in front of it (of them all)
+  __device__ __forceinline__ int among(unsigned n, long long x, long long& before) const {
+    unsigned upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (int(lane_id()) >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * per_seq > x);
+    const int at = past ? __ffs(past) - 1 : 31;
+    before += __shfl_sync(0xffffffffu, past ? upto - n : upto, at);
+    return past ? at : -1;
+  }
+  __device__ __forceinline__ int find(const Kv4AttnArgs& a, long long x, long long& before) const {  // of all sequences, x < total
+    before = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int at = among(held[k], x, before);
+      if (at >= 0) return 32 * k + at;
+    }
+    for (int b = 32 * kHeld; b < a.B; b += 32) {
+      const int at = among(unsigned(pairs(a, b + int(lane_id()))), x, before);
+      if (at >= 0) return b + at;
+    }
+    return a.B;
   }
 };
 
@@ -418,6 +445,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * L::kWarp;
+  uint32_t* block_q = reinterpret_cast<uint32_t*>(smem + L::kSmem);
   pdl_wait();
 
   const int rows = a.Hq / a.Hk * a.q_len, per_head = a.Hq / a.Hk;
@@ -428,7 +456,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     for (long long i = threadIdx.x; i < (long long)a.q_len * a.Hq * D / 8; i += 128) y[i] = make_uint4(0, 0, 0, 0);
   }
   int seq, unit, off, pairs;  // where this CTA is: unit of the sequence, pair of the unit
-  long long left;
+  long long left, x = 0, share = 1;
   if (a.part_o == nullptr) {
     seq = blockIdx.x / (a.Hk * a.tiles);
     unit = blockIdx.x % (a.Hk * a.tiles);
@@ -436,15 +464,28 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     left = pairs = Kv4Shares::pairs(a, seq);
   } else {
     const Kv4Shares all(a, gridDim.x);
-    const long long x = blockIdx.x * all.share;
-    if (x >= all.total) return;
-    left = min(all.share, all.total - x);
+    share = all.share;
+    x = blockIdx.x * share;
+    left = min(share, all.total - x);
+    if (left <= 0) {
+      if (threadIdx.x == 0) a.joins[blockIdx.x].n = 0;
+      return;
+    }
     long long before;
     seq = all.find(a, x, before);
     pairs = Kv4Shares::pairs(a, seq);
     const long long in = x - before * all.per_seq;
-    unit = int(in / pairs);
+    unit = int(kv4_quotient(in, pairs));
     off = int(in - (long long)unit * pairs);
+    if (threadIdx.x == 0) {  // the last one of a unit's pieces says where the others are
+      Kv4Join join{seq, unit, 0, 0};
+      if (off > 0 && off + left >= pairs) {
+        const long long first = kv4_quotient(x - off, share);
+        join.n = int(blockIdx.x - first) + 1;
+        join.behind = x - off != first * share;
+      }
+      a.joins[blockIdx.x] = join;
+    }
   }
   constexpr int kParts = D / 8;  // pieces of 16 bytes of a page's parameters: K's, then V's
   const int piece = lane % (kParts < 32 ? kParts : 32);
@@ -502,7 +543,8 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       copies_end_here();
     }
     R t;
-    t.load(a, seq, kvh, first, rows, length);
+    t.load(a, seq, kvh, first, rows, length, block_q);
+    __syncthreads();
     // pairs that all rows see whole come first, the masked ones of a sequence's end behind them
     int stage = 0, more = mine - L::kStages;
     const auto next = [&] {
@@ -520,13 +562,13 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     while (used < seen) {
       copies_but_the_last<L::kStages - 1>();
       __syncwarp();
-      t.template pages<true>(ring + stage, used << 4);
+      t.template pages<true>(ring + stage, block_q, used << 4);
       next();
     }
     while (used < end) {
       copies_but_the_last<L::kStages - 1>();
       __syncwarp();
-      t.template pages<false>(ring + stage, used << 4);
+      t.template pages<false>(ring + stage, block_q, used << 4);
       next();
     }
 
@@ -600,22 +642,17 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   if (strays && lane == 0) atomicCAS(a.status, 0, kStatusBadArgument);
 }
 
-// Joins the pieces of a unit that several CTAs have, a block a query row and head.  `ctas`: of the kernel before
+// Joins the pieces of the unit that ends in a CTA's first one, a block a query row of it
 template <int D, int kCols, typename T>
-__global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(D) kv4_merge_kernel(Kv4AttnArgs a) {
   pdl_trigger();
   pdl_wait();
-  const int per_head = a.Hq / a.Hk, d = threadIdx.x;
-  const size_t row = blockIdx.x;
-  const int seq = int(row / a.Hq / a.q_len), head = int(row % a.Hq), kvh = head / per_head, r = int(row / a.Hq % a.q_len) * per_head + head % per_head;
-  const int pairs = Kv4Shares::pairs(a, seq);
-  if (pairs == 0) return;
-  const Kv4Shares all(a, ctas);
-  const long long from = all.in_front_of(a, seq) * all.per_seq + (long long)(kvh * a.tiles + r / kCols) * pairs;
-  const int c0 = int(from / all.share), n = int((from + pairs - 1) / all.share) - c0 + 1;
-  if (n == 1) return;
-  // the unit's pieces are the first ones of their CTAs, but for its beginning, where something may be in front of it
-  const auto slot = [&](int k) { return (2 * size_t(c0 + k) + (k > 0 || from == c0 * all.share ? 0 : 1)) * kCols + r % kCols; };
+  const int cta = blockIdx.x / kCols, r = blockIdx.x % kCols, d = threadIdx.x, per_head = a.Hq / a.Hk;
+  const Kv4Join join = a.joins[cta];
+  const int n = join.n, kvh = join.unit / a.tiles, q_row = join.unit % a.tiles * kCols + r;
+  if (n == 0 || q_row >= per_head * a.q_len) return;
+  const size_t row = (size_t(join.seq) * a.q_len + q_row / per_head) * a.Hq + kvh * per_head + q_row % per_head;
+  const auto slot = [&](int k) { return (2 * size_t(cta - n + 1 + k) + (k == 0 ? join.behind : 0)) * kCols + r; };
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
   float ref = -FLT_MAX, l = 0.f, o = 0.f;
   for (int k = 0; k < n; k += kAtOnce) {
@@ -649,19 +686,20 @@ template <int D, int kCols, typename T>
 static int launch_kv4_attn_of(Kv4AttnArgs a, int ctas, cudaStream_t stream) {
   using L = Kv4Ring<D>;
   constexpr int kMinBlocks = D == 256 || kCols == 16 ? 2 : 4;
+  constexpr int kSmem = L::kSmem + Kv4Rows<D, kCols, T>::kSteps * 128 * Kv4Rows<D, kCols, T>::kQ;
   auto kernel = &kv4_attn_kernel<D, kCols, T, kMinBlocks>;
   static bool attr[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
   if (!attr[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return -6;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return -6;
     attr[dev] = true;
   }
   const long long tiles = ((long long)a.Hq / a.Hk * a.q_len + kCols - 1) / kCols, units = (long long)a.B * a.Hk * tiles;
-  if (units > 0x7fffffffll || (long long)a.B * a.q_len * a.Hq > 0x7fffffffll) return -2;
+  if (units > 0x7fffffffll || ctas > 1 << 20) return -2;
   a.tiles = int(tiles);
-  if (launch_kernel(kernel, dim3(unsigned(a.part_o ? ctas : units)), dim3(128), L::kSmem, stream, a) != cudaSuccess) return -7;
-  if (a.part_o && launch_kernel(&kv4_merge_kernel<D, kCols, T>, dim3(unsigned(a.B * a.q_len * a.Hq)), dim3(D), 0, stream, a, ctas) != cudaSuccess) return -7;
+  if (launch_kernel(kernel, dim3(unsigned(a.part_o ? ctas : units)), dim3(128), kSmem, stream, a) != cudaSuccess) return -7;
+  if (a.part_o && launch_kernel(&kv4_merge_kernel<D, kCols, T>, dim3(unsigned(ctas * kCols)), dim3(D), 0, stream, a) != cudaSuccess) return -7;
   return 0;
 }
 template <int D, typename T>
@@ -680,13 +718,16 @@ static int launch_kv4_attn(const Kv4AttnArgs& a, int ctas, bool half, cudaStream
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16 or fp16 (`half`); pool: [pages, Hk, 18 D]; table: [B, width]; seq_lens count every token visible to the last query row.
-// part_o: null, and every unit has a CTA of its own, or scratch for `ctas` equal shares of at least `least` pairs of pages: [2 * ctas, cols, D] fp32,
-// with part_ml [2 * ctas, cols, 2], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
-extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, float* part_o, float* part_ml, int half,
+// scratch: null, and every unit has a CTA of its own, or for `ctas` equal shares of at least `least` pairs of pages, beginning on 16 bytes: 4 words a share, then
+// fp32 [2 * ctas, cols, D] and [2 * ctas, cols, 2], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
+extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, void* scratch, int half,
                                          int B, int Hq, int Hk, int D, int width, int pages, int q_len, int ctas, int least, float sm_scale, int* status,
                                          cudaStream_t stream) {
-  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || (part_o == nullptr) != (part_ml == nullptr)) return -1;
-  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, part_ml, status, B, Hq, Hk, width, pages, q_len, least, 0, sm_scale * 1.4426950408889634f};
+  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || ctas > 1 << 20) return -1;
+  const long long cols = Hq / Hk * (long long)q_len <= 4 ? 4 : (D == 256 || Hq / Hk * (long long)q_len <= 8 ? 8 : 16);
+  mfq::Kv4Join* joins = static_cast<mfq::Kv4Join*>(scratch);
+  float* part_o = scratch ? reinterpret_cast<float*>(joins + ctas) : nullptr;
+  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, scratch ? part_o + 2 * ctas * cols * D : nullptr, joins, status, B, Hq, Hk, width, pages, q_len, least, 0, sm_scale * 1.4426950408889634f};
   if (D == 64) return mfq::launch_kv4_attn<64>(a, ctas, half != 0, stream);
   if (D == 128) return mfq::launch_kv4_attn<128>(a, ctas, half != 0, stream);
   if (D == 256) return mfq::launch_kv4_attn<256>(a, ctas, half != 0, stream);

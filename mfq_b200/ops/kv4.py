@@ -174,10 +174,8 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
         with torch.cuda.device(index):
             return paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale=sm_scale, q_len=q_len, max_len=max_len, out=out)
     cols, ctas, least = _shape(b, hk, hq // hk * q_len, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)), width)
-    parts = 2 * ctas * cols
-    scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device) if parts else None  # of this call: a workspace would tie streams and graphs together
-    at = scratch.data_ptr() if parts else 0
-    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), at, at + 4 * parts * d,
+    scratch = torch.empty(ctas * (4 + 2 * cols * (d + 2)), dtype=torch.float32, device=q.device) if ctas else None  # of this call: a workspace would tie streams and graphs together
+    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ptr(scratch),
                                           int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, max(1, ctas), least, sm_scale,
-                                          Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if parts else 1)
+                                          Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if ctas else 1)
     return out

@@ -44,7 +44,7 @@ _SIGNATURES = {
     "mfq_paged_attn_decode_shared": [_vp] * 13 + [_i] * 11 + [_f, _vp, _vp],
     "mfq_kv4_write": [_vp] * 4 + [_i] * 5 + [_ll] * 4 + [_vp, _vp],
     "mfq_kv4_gather": [_vp] * 6 + [_i] * 7 + [_ll] * 4 + [_vp, _vp],
-    "mfq_paged_attn_decode_kv4": [_vp] * 7 + [_i] * 10 + [_f, _vp, _vp],
+    "mfq_paged_attn_decode_kv4": [_vp] * 6 + [_i] * 10 + [_f, _vp, _vp],
     "mfq_process_logits": [_vp, _vp, _i, _i, _i, _ll, _ll, _vp, _i, _vp, _ll, _vp, _vp, _i, _vp, _i, _vp, _i, _f, _vp],
     "mfq_count_tokens": [_vp, _ll, _i, _i, _vp, _vp, _i, _i, _vp],
     "mfq_plan_batch": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp],
