@@ -500,6 +500,8 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     const int mine = here > warp ? (here - warp + L::kWarps - 1) / L::kWarps : 0;
     const int* bt = a.table + size_t(seq) * a.width;
     int asked = 2 * (off + warp), used = asked, id[2];  // pages
+    const uint32_t page_bytes = uint32_t(a.Hk) * L::kRecord;
+    const uint8_t *codes_at = a.pool + size_t(kvh) * L::kRecord + 16 * lane, *pieces_at = a.pool + size_t(kvh) * L::kRecord + piece_at;
     const auto look = [&] {  // the ids of the pair that is asked for next; a second page that is not there: the first again
       const int at = min(asked, total - 1);
       id[0] = bt[at];
@@ -507,16 +509,15 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       asked += 2 * L::kWarps;
     };
     const auto request = [&](uint32_t stage) {
-      const uint8_t* rec[2];
+      uint32_t page[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint32_t page = min(uint32_t(id[p]), uint32_t(a.pages - 1));
-        strays |= page ^ uint32_t(id[p]);
-        rec[p] = a.pool + (size_t(page) * a.Hk + kvh) * L::kRecord;
+        page[p] = min(uint32_t(id[p]), uint32_t(a.pages - 1));
+        strays |= page[p] ^ uint32_t(id[p]);
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint8_t* from = rec[p] + 16 * lane;
+        const uint8_t* from = codes_at + (unsigned long long)page[p] * page_bytes;  // one multiplication and addition
         const uint32_t at = stage + 16 * lane + p * L::kRecord;
 #pragma unroll
         for (int g = 0; g < D / 64; ++g) copy16(at + 512 * g, from + 512 * g);
@@ -524,12 +525,11 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
         for (int g = 0; g < D / 64; ++g) copy16(at + 9 * D + 512 * g, from + 9 * D + 512 * g);
       }
       if constexpr (kParts == 32) {
-        copy16(stage + piece_at, rec[0] + piece_at);
-        copy16(stage + piece_at + L::kRecord, rec[1] + piece_at);
-      } else if constexpr (kParts == 16) {
-        copy16(stage + piece_at + (lane < 16 ? 0 : L::kRecord), (lane < 16 ? rec[0] : rec[1]) + piece_at);
+        copy16(stage + piece_at, pieces_at + (unsigned long long)page[0] * page_bytes);
+        copy16(stage + piece_at + L::kRecord, pieces_at + (unsigned long long)page[1] * page_bytes);
       } else {
-        if (lane < 2 * kParts) copy16(stage + piece_at + (lane < kParts ? 0 : L::kRecord), (lane < kParts ? rec[0] : rec[1]) + piece_at);
+        const uint8_t* from = pieces_at + (unsigned long long)(lane < kParts ? page[0] : page[1]) * page_bytes;
+        if (kParts == 16 || lane < 2 * kParts) copy16(stage + piece_at + (lane < kParts ? 0 : L::kRecord), from);
       }
     };
     const uint32_t ring_at = smem_u32(ring);
