@@ -31,14 +31,16 @@ __device__ __forceinline__ float bf16_down(float x) {  // the largest bf16 <= x
   if (int(b) < 0) b += 0xffffu;
   return __uint_as_float(b & 0xffff0000u);
 }
-__device__ __forceinline__ float bf16_up(float x) {  // the least bf16 >= x, for x >= 0
-  return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u);
-}
-// From the least and the greatest value, both NaN if one value is.  15 s has 12 bits, so s reaches max - m if it reaches that rounded up to 24.
+// From the least and the greatest value, both NaN if one value is.  s is the least bf16 that reaches d = max - m fifteenfold: 15 s has 12 bits and is exact, so
+// it reaches d if it reaches d rounded up to 24.  The search begins at d / 15 or less and ends after two steps at most.
 __device__ __forceinline__ Kv4Group kv4_group(float least, float most) {
   if (!(least >= -kKv4Most && most <= kKv4Most)) return {__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)};
   const float m = bf16_down(least) + 0.f;  // no negative zeros
-  return {bf16_up(__fdiv_ru(__fsub_ru(most, m) + 0.f, 15.f)), m};
+  const float d = __fsub_ru(most, m) + 0.f;
+  uint32_t s = __float_as_uint(__fmul_rd(d, 0.06666666f)) & 0xffff0000u;  // 1 / 15 rounded down
+#pragma unroll
+  for (int i = 0; i < 2; ++i) s += 15.f * __uint_as_float(s) < d ? 0x10000u : 0u;
+  return {__uint_as_float(s), m};
 }
 __device__ __forceinline__ uint32_t kv4_params(Kv4Group g) { return __float_as_uint(g.s) >> 16 | __float_as_uint(g.m); }
 
@@ -50,7 +52,7 @@ __device__ __forceinline__ int kv4_side(float x, float m, float t) {
   return lost > 0.f ? 1 : (lost < 0.f ? -1 : 0);
 }
 // The nearest code; s (c +- 1/2) has 13 bits and is exact.
-__device__ __forceinline__ uint32_t kv4_code(float x, Kv4Group g) {
+static __device__ __noinline__ uint32_t kv4_code(float x, Kv4Group g) {
   if (!(g.s > 0.f)) return 0;
   int c = int(fminf(rintf((x - g.m) / g.s), 15.f));
   const int down = kv4_side(x, g.m, g.s * (float(c) - 0.5f));

@@ -94,26 +94,45 @@ struct Kv4Sixteen {
   }
 };
 
+// fma.rm of two numbers, and the plain forms of common.cuh
+__device__ __forceinline__ float2 fma_down_f2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rm.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 plus_f2(float2 a, float b) {
+  add2(a.x, a.y, __float_as_uint(b), __float_as_uint(b));
+  return a;
+}
+
 // Codes of 16 values, value i in the lowest 4 bits of code[i] (what is above them is anything).
-// floor((x - m) / s) is found by the rounded reciprocal, one too large or small at worst where the quotient is next to an integer, and what is left of x - m
-// is exact: it says whether the value is nearer to the next code.  x - m may be rounded itself, which matters where that is a tie, s (c + 1/2) with its 13 bits.
-// In 32 bits a tie is looked at again; in 16 bits, where 0.3 % of normal values are ties, a rounded difference has as few bits only where all of the smaller
-// number was lost in the larger one, 2^-23 of it or less.
+// floor((x - m) / s) is found by a reciprocal 2^-10 too small: it may be one too small, never too large.  What is left of x - m then is exact and not
+// negative, and says whether the next code is nearer, or as near and even.  x - m may be rounded itself, which matters where that makes a tie, s (c + 1/2)
+// with its 13 bits.  In 32 bits ties are looked at again.  In 16 bits, where 0.3 % of normal values are ties, a rounded difference has as few bits only where all of
+// the smaller number was lost in the larger one: a small x where -m by itself is a tie, or any x where m is as small.
 template <typename T>
 __device__ __forceinline__ void kv4_codes(uint32_t (&code)[16], const Kv4Sixteen<T>& x, Kv4Group g) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: integers in the lowest bits
-  const float inv = g.s != 0.f ? 1.f / g.s : 0.f, half = 0.5f * g.s;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(g.s));
+  inv = g.s != 0.f ? inv * 0.9990234375f : 0.f;
+  const float half = 0.5f * g.s, less_m = 0.f - g.m;  // no negative zeros: what is left has to be none
   bool slow = !(g.s >= 0x1p-120f) && g.s != 0.f;
-  if constexpr (sizeof(T) < 4) {
-    const float big = fmaxf(fabsf(g.m), 15.f * g.s), small = fminf(x.least_magnitude(), g.m != 0.f ? fabsf(g.m) : big);
-    slow |= small < big * 0x1p-20f;
-  }
+  const auto both_codes = [&](float2 v, uint32_t& c0, uint32_t& c1) {
+    const float2 h = plus_f2(v, less_m), f = fma_down_f2(h, both(inv), both(kMagic)), left = fma_f2(plus_f2(f, -kMagic), both(-g.s), h);
+    const uint32_t b0 = __float_as_uint(f.x), b1 = __float_as_uint(f.y);
+    if constexpr (sizeof(T) == 4) slow |= left.x == half || left.y == half;
+    // left > half, or left = half and the code is odd: the sign of half - left - odd, as integers
+    c0 = b0 + ((__float_as_uint(half) - __float_as_uint(left.x) - (b0 & 1u)) >> 31);
+    c1 = b1 + ((__float_as_uint(half) - __float_as_uint(left.y) - (b1 & 1u)) >> 31);
+  };
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float h = x.at(i) - g.m, v = __fmaf_rd(h, inv, kMagic), left = fmaf(-g.s, v - kMagic, h);
-    const uint32_t bits = __float_as_uint(v);
-    if constexpr (sizeof(T) == 4) slow |= left == half;
-    code[i] = bits + (left > __uint_as_float(__float_as_uint(half) - (bits & 1u)) ? 1u : 0u);  // half a step from an odd code: to the even one
+  for (int i = 0; i < 16; i += 2) both_codes(make_float2(x.at(i), x.at(i + 1)), code[i], code[i + 1]);
+  if constexpr (sizeof(T) < 4) {
+    const float f = __fmaf_rd(less_m, inv, kMagic), left = fmaf(f - kMagic, -g.s, less_m);
+    slow |= (left == half || left == half + g.s) && x.least_magnitude() < fabsf(g.m) * 0x1p-20f;
+    slow |= g.m != 0.f && fabsf(g.m) < g.s * 0x1p-16f;
   }
   if (slow) {
 #pragma unroll
@@ -121,92 +140,101 @@ __device__ __forceinline__ void kv4_codes(uint32_t (&code)[16], const Kv4Sixteen
   }
 }
 
-// A run of n tokens from `x` (`stride` elements apart) at places p0 .. p0 + n - 1 of the record `rec`
-template <int D, typename T, bool kV>
-__device__ __forceinline__ void kv4_write_run(const T* x, long long stride, int p0, int n, uint8_t* rec) {
-  constexpr int G = D / 64, kAhead = G * int(sizeof(T)) <= 4 ? G : 4 / int(sizeof(T));  // groups whose values are requested at once
+// A run of n tokens from `x` (`stride` elements apart) at places p0 .. p0 + n - 1 of the record `rec`: group g
+template <int D, typename T>
+__device__ __forceinline__ void kv4_write_run(const T* x, long long stride, int p0, int n, uint8_t* rec, int g, bool is_v) {
+  constexpr int G = D / 64;
   const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   const bool there[2] = {g8 >= p0 && g8 < p0 + n, g8 + 8 >= p0 && g8 + 8 < p0 + n};
-  const T* from[2] = {x + (long long)(g8 - p0) * stride + 16 * c, x + (long long)(g8 + 8 - p0) * stride + 16 * c};
-  uint32_t params[2][G];
+  Kv4Sixteen<T> v[2];
 #pragma unroll
-  for (int g0 = 0; g0 < G; g0 += kAhead) {
-    Kv4Sixteen<T> v[kAhead][2];
+  for (int h = 0; h < 2; ++h) {
+    if (there[h]) v[h].load(x + (long long)(g8 + 8 * h - p0) * stride + 64 * g + 16 * c);
+    else v[h].none();
+  }
+  uint32_t w[4], bytes[2][8], params[2];
 #pragma unroll
-    for (int g = 0; g < kAhead; ++g) {
+  for (int h = 0; h < 2; ++h) {
+    float least = v[h].at(0), most = least;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (there[h]) v[g][h].load(from[h] + 64 * (g0 + g));
-        else v[g][h].none();
-      }
+    for (int i = 1; i < 15; i += 2) {
+      least = min3_nan(least, v[h].at(i), v[h].at(i + 1));
+      most = max3_nan(most, v[h].at(i), v[h].at(i + 1));
     }
+    least = min_nan(least, v[h].at(15));
+    most = max_nan(most, v[h].at(15));
 #pragma unroll
-    for (int g = 0; g < kAhead; ++g) {
-      uint32_t w[4], bytes[2][8];
+    for (int o = 1; o < 4; o <<= 1) {
+      least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, o));
+      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    const Kv4Group grp = kv4_group(least, most);
+    params[h] = kv4_params(grp);
+    uint32_t code[16];
+    kv4_codes(code, v[h], grp);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float least = v[g][h].at(0), most = least;
+    for (int i = 0; i < 8; ++i) bytes[h][i] = (code[i] & 15u) + code[i + 8] * 16u;  // in the lowest 8 bits
+  }
 #pragma unroll
-        for (int i = 1; i < 15; i += 2) {
-          least = min3_nan(least, v[g][h].at(i), v[g][h].at(i + 1));
-          most = max3_nan(most, v[g][h].at(i), v[g][h].at(i + 1));
-        }
-        least = min_nan(least, v[g][h].at(15));
-        most = max_nan(most, v[g][h].at(15));
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t even = __byte_perm(bytes[0][2 * k], bytes[1][2 * k], 0x0040), odd = __byte_perm(bytes[0][2 * k + 1], bytes[1][2 * k + 1], 0x0040);
+    w[k] = __byte_perm(even, odd, 0x5410);
+  }
+  transpose4(w, c);
+  if (is_v) {
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, o));
-          most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
-        const Kv4Group grp = kv4_group(least, most);
-        params[h][g0 + g] = kv4_params(grp);
-        uint32_t code[16];
-        kv4_codes(code, v[g][h], grp);
+    for (int k = 0; k < 4; ++k) w[k] = transposed8(w[k]);
+  }
+  uint8_t* at = rec + 512 * g + 16 * lane;
+  if (n == 16) {
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bytes[h][i] = (code[i] & 15u) + code[i + 8] * 16u;  // in the lowest 8 bits
-      }
+    for (int b = 0; b < 4; ++b) {  // the token that has this byte of each word
+      const int place = is_v ? 2 * c + (b >> 1) + 8 * (b & 1) : g8 + 8 * (b & 1);
+      if (place >= p0 && place < p0 + n) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t even = __byte_perm(bytes[0][2 * k], bytes[1][2 * k], 0x0040), odd = __byte_perm(bytes[0][2 * k + 1], bytes[1][2 * k + 1], 0x0040);
-        w[k] = __byte_perm(even, odd, 0x5410);
-      }
-      transpose4(w, c);
-      if constexpr (kV) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = transposed8(w[k]);
-      }
-      uint8_t* at = rec + 512 * (g0 + g) + 16 * lane;
-      if (n == 16) {
-        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {  // the token that has this byte of each word
-          const int place = kV ? 2 * c + (b >> 1) + 8 * (b & 1) : g8 + 8 * (b & 1);
-          if (place >= p0 && place < p0 + n) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) at[4 * k + b] = uint8_t(w[k] >> (8 * b));
-          }
-        }
+        for (int k = 0; k < 4; ++k) at[4 * k + b] = uint8_t(w[k] >> (8 * b));
       }
     }
   }
-  uint32_t* to = reinterpret_cast<uint32_t*>(rec + 8 * D) + g8 * 2 * G;  // [place g8, g8 + 8][group]
-#pragma unroll
-  for (int i = 0; i < 2 * G; ++i) {
-    if (i % 4 == c && there[i / G]) to[i] = params[i / G][i % G];
-  }
+  if (c < 2 && there[c]) reinterpret_cast<uint32_t*>(rec + 8 * D)[(g8 * 2 + c) * G + g] = params[c];
 }
 
+// One token, group g: a lane has the pair of dims of one byte
 template <int D, typename T>
-__global__ void __launch_bounds__(128) kv4_write_kernel(Kv4WriteArgs a) {
+__device__ __forceinline__ void kv4_write_token(const T* x, int place, uint8_t* rec, int g, bool is_v) {
+  const int lane = threadIdx.x & 31, j = lane >> 3, i = lane & 7;
+  const T* at = x + 64 * g + 16 * j + i;
+  float lo, hi;
+  if constexpr (sizeof(T) == 4) { lo = at[0]; hi = at[8]; }
+  else if constexpr (__is_same(T, __half)) { lo = __half2float(at[0]); hi = __half2float(at[8]); }
+  else { lo = __bfloat162float(at[0]); hi = __bfloat162float(at[8]); }
+  float least = min_nan(lo, hi), most = max_nan(lo, hi);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, o));
+    most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  const Kv4Group grp = kv4_group(least, most);
+  rec[is_v ? kv4_v_byte(place, g, j, i) : kv4_k_byte(place, g, j, i)] = uint8_t(kv4_code(lo, grp) | kv4_code(hi, grp) << 4);
+  if (lane == 0) *reinterpret_cast<uint32_t*>(rec + 8 * D + kv4_param_byte<D>(place) + 4 * g) = kv4_params(grp);
+}
+
+// A warp has one group of 64 dims: with all groups of a head 4096 tokens of 8 heads of 128 took 9.7 us instead of 8.2 (16384: 25.7 instead of 28.4), single
+// tokens of a batch of 64 5.2 instead of 3.8.  Eight blocks an SM in 16 bits, six in 32: 49 -> 28 us for 16384 tokens, together with a path that fits the
+// instruction cache (the exact choice of a code is a call).
+template <int D, typename T>
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 6 : 8) kv4_write_kernel(Kv4WriteArgs a) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const long long of = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long first = of / (2 * a.Hk) * a.window;
+  constexpr int G = D / 64;
+  const long long first = of / (2 * G * a.Hk) * a.window;
   if (first >= a.T) return;
-  const int head = int(of % (2 * a.Hk)) >> 1;
-  const bool is_v = of & 1;
+  const int head = int(of % (2 * G * a.Hk)) / (2 * G), g = int(of % G);
+  const bool is_v = of / G & 1;
   // lane i: token first - 1 + i.  A run begins in the window and ends 15 tokens behind it at most
   const long long token = first - 1 + lane;
   int slot = token >= 0 && token < a.T ? a.slots[token] : -1;
@@ -225,8 +253,9 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Kv4WriteArgs a) {
     const int at = __shfl_sync(0xffffffffu, slot, i);
     uint8_t* rec = a.pool + (size_t(at >> 4) * a.Hk + head) * (18 * D) + (is_v ? 9 * D : 0);
     const long long t = first - 1 + i;
-    if (is_v) kv4_write_run<D, T, true>(static_cast<const T*>(a.v) + t * a.v_token + head * a.v_head, a.v_token, at & 15, n, rec);
-    else kv4_write_run<D, T, false>(static_cast<const T*>(a.k) + t * a.k_token + head * a.k_head, a.k_token, at & 15, n, rec);
+    const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (is_v ? t * a.v_token + head * a.v_head : t * a.k_token + head * a.k_head);
+    if (n == 1) kv4_write_token<D, T>(x, at & 15, rec, g, is_v);
+    else kv4_write_run<D, T>(x, is_v ? a.v_token : a.k_token, at & 15, n, rec, g, is_v);
   }
 }
 
@@ -238,17 +267,6 @@ struct Kv4GatherArgs {
   long long k_token, k_head, v_token, v_head;
   int B, N, Hk, width, pages, window;
 };
-
-// The sequence whose rows have row r: the last one that starts at r or before
-__device__ __forceinline__ int kv4_sequence(const int* starts, int B, int r) {
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo + 1) / 2;
-    if (starts[mid] <= r) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
 
 template <typename T>
 __device__ __forceinline__ void kv4_store16(T* to, const float (&y)[16]) {
@@ -271,20 +289,31 @@ __device__ __forceinline__ void kv4_store16(T* to, const float (&y)[16]) {
   }
 }
 
-// n tokens at places p0 .. p0 + n - 1 of the record `rec` to `y` (`stride` elements apart)
-template <int D, typename T, bool kV>
-__device__ __forceinline__ void kv4_read_run(const uint8_t* rec, int p0, int n, T* y, long long stride) {
-  constexpr int G = D / 64;
-  const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
+// K or V of a record as a lane has them: requested first, used behind all that was requested
+template <int D>
+struct Kv4Raw {
+  static constexpr int G = D / 64;
   uint4 raw[G];
   uint32_t params[2 * G];  // [place g8, g8 + 8][group]
+  __device__ __forceinline__ void load(const uint8_t* rec) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int g = 0; g < G; ++g) raw[g] = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
+    for (int g = 0; g < G; ++g) raw[g] = *reinterpret_cast<const uint4*>(rec + 512 * g + 16 * lane);
 #pragma unroll
-  for (int i = 0; i < 2 * G; i += 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(rec + 8 * D + 8 * G * g8 + 4 * i);
-    params[i] = v.x; params[i + 1] = v.y;
+    for (int i = 0; i < 2 * G; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(rec + 8 * D + 8 * G * (lane >> 2) + 4 * i);
+      params[i] = v.x; params[i + 1] = v.y;
+    }
   }
+};
+
+// The tokens at places p0 .. p0 + n - 1 to `y` (`stride` elements apart)
+template <int D, typename T, bool kV>
+__device__ __forceinline__ void kv4_read_run(const Kv4Raw<D>& rec, int p0, int n, T* y, long long stride) {
+  constexpr int G = D / 64;
+  const int lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
+  const auto& raw = rec.raw;
+  const auto& params = rec.params;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
@@ -292,22 +321,51 @@ __device__ __forceinline__ void kv4_read_run(const uint8_t* rec, int p0, int n, 
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = transposed8(w[k]);
     }
-    transpose4(w, c);
+    // 16 bits: a lane gets 16 neighbouring dims.  32 bits: the four lanes of a row have 8 neighbouring ones as they are, a sector
+    if constexpr (sizeof(T) < 4) transpose4(w, c);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float s = __uint_as_float(params[h * G + g] << 16), m = __uint_as_float(params[h * G + g] & 0xffff0000u);
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t byte = w[i >> 1] >> (16 * (i & 1) + 8 * h);
-        v[i] = fmaf(s, __uint_as_float((byte & 15u) | 0x4b000000u) - 8388608.f, m);  // 2^23 + c, exactly
-        v[i + 8] = fmaf(s, __uint_as_float((byte >> 4 & 15u) | 0x4b000000u) - 8388608.f, m);
-      }
       const int place = g8 + 8 * h;
-      if (place >= p0 && place < p0 + n) kv4_store16(y + (long long)(place - p0) * stride + 64 * g + 16 * c, v);
+      const bool there = place >= p0 && place < p0 + n;
+      T* to = y + (long long)(place - p0) * stride + 64 * g;
+      const float s = __uint_as_float(params[h * G + g] << 16), m = __uint_as_float(params[h * G + g] & 0xffff0000u);
+      const auto value = [&](uint32_t code) { return fmaf(s, __uint_as_float((code & 15u) | 0x4b000000u) - 8388608.f, m); };  // 2^23 + c, exactly
+      if constexpr (sizeof(T) < 4) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t byte = w[i >> 1] >> (16 * (i & 1) + 8 * h);
+          v[i] = value(byte);
+          v[i + 8] = value(byte >> 4);
+        }
+        if (there) kv4_store16(to + 16 * c, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t code = w[k] >> (8 * h + 4 * e);
+            if (there) *reinterpret_cast<float2*>(to + 16 * k + 8 * e + 2 * c) = make_float2(value(code), value(code >> 16));
+          }
+        }
+      }
     }
   }
 }
+
+// The sequence whose rows have row r: the last one that starts at r or before, by a whole warp, in steps of a 32nd
+__device__ __forceinline__ int kv4_sequence(const int* starts, int B, int r) {
+  int lo = 0;
+  for (int span = B; span > 1;) {
+    const int part = (span + 31) >> 5, at = int(lane_id()) * part;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, at == 0 || (at < span && starts[lo + at] <= r)));
+    lo += last * part;
+    span = min(part, span - last * part);
+  }
+  return lo;
+}
+
+__host__ __device__ constexpr int kv4_gather_heads(int d) { return d == 64 ? 2 : 1; }
 
 template <int D, typename T>
 __global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4GatherArgs a) {
@@ -315,15 +373,17 @@ __global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4GatherArgs a) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const long long of = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long first = of / (2 * a.Hk) * a.window;
+  constexpr int kEach = D == 256 ? 1 : 2, kHeads = kv4_gather_heads(D);  // a warp has K or V of a head of 256, both of one of 128, of two of 64
+  const int jobs = (a.Hk + kHeads - 1) / kHeads * (2 / kEach);
+  const long long first = of / jobs * a.window;
   if (first >= a.N) return;
-  const int head = int(of % (2 * a.Hk)) >> 1;
-  const bool is_v = of & 1;
+  const int head = int(of % jobs) / (2 / kEach) * kHeads;
+  const bool is_v = kEach == 1 && (of & 1);
   // lane i: row first - 1 + i, as in the kernel above; a run is one of rows whose tokens follow one another in a page, whoever's they are
   const long long row = first - 1 + lane;
-  int slot = -1;
+  int slot = -1, seq = kv4_sequence(a.starts, a.B, int(max(first - 1, 0ll)));
   if (row >= 0 && row < a.N && row >= a.starts[0] && row < a.starts[a.B]) {
-    const int seq = kv4_sequence(a.starts, a.B, int(row));
+    while (seq + 1 < a.B && a.starts[seq + 1] <= row) ++seq;
     const long long pos = (long long)(a.first ? a.first[seq] : 0) + row - a.starts[seq];
     const int page = pos >= 0 && (pos >> 4) < a.width ? a.table[size_t(seq) * a.width + (pos >> 4)] : -1;
     if (page < 0 || page >= a.pages) atomicCAS(a.status, 0, kStatusBadArgument);
@@ -338,10 +398,21 @@ __global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4GatherArgs a) {
     begins &= begins - 1;
     const int n = __ffs(~(on >> (i + 1)));  // 1 and the ones behind bit i, which is 16 at most
     const int at = __shfl_sync(0xffffffffu, slot, i);
-    const uint8_t* rec = a.pool + (size_t(at >> 4) * a.Hk + head) * (18 * D) + (is_v ? 9 * D : 0);
     const long long to = first - 1 + i;
-    if (is_v) kv4_read_run<D, T, true>(rec, at & 15, n, static_cast<T*>(a.v) + to * a.v_token + head * a.v_head, a.v_token);
-    else kv4_read_run<D, T, false>(rec, at & 15, n, static_cast<T*>(a.k) + to * a.k_token + head * a.k_head, a.k_token);
+    Kv4Raw<D> raw[kHeads][kEach];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      const uint8_t* rec = a.pool + (size_t(at >> 4) * a.Hk + min(head + k, a.Hk - 1)) * (18 * D);
+      raw[k][0].load(rec + (is_v ? 9 * D : 0));
+      if constexpr (kEach == 2) raw[k][kEach - 1].load(rec + 9 * D);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      if (head + k >= a.Hk) break;
+      T *ky = static_cast<T*>(a.k) + to * a.k_token + (head + k) * a.k_head, *vy = static_cast<T*>(a.v) + to * a.v_token + (head + k) * a.v_head;
+      if (!is_v) kv4_read_run<D, T, false>(raw[k][0], at & 15, n, ky, a.k_token);
+      if (kEach == 2 || is_v) kv4_read_run<D, T, true>(raw[k][kEach - 1], at & 15, n, vy, a.v_token);
+    }
   }
 }
 
@@ -356,7 +427,7 @@ static int kv4_window(long long units) {
 template <int D>
 static int launch_write(Kv4WriteArgs a, int dtype, cudaStream_t stream) {
   a.window = kv4_window(2ll * a.T * a.Hk);
-  const long long blocks = ((a.T + a.window - 1ll) / a.window * 2 * a.Hk + 3) / 4;
+  const long long blocks = ((a.T + a.window - 1ll) / a.window * 2 * a.Hk * (D / 64) + 3) / 4;
   if (blocks > 0x7fffffffll) return -2;
   auto kernel = dtype == 0 ? kv4_write_kernel<D, __nv_bfloat16> : (dtype == 1 ? kv4_write_kernel<D, __half> : kv4_write_kernel<D, float>);
   return launch_kernel(kernel, dim3(unsigned(blocks)), dim3(128), 0, stream, a) == cudaSuccess ? 0 : -7;
@@ -364,7 +435,8 @@ static int launch_write(Kv4WriteArgs a, int dtype, cudaStream_t stream) {
 template <int D>
 static int launch_gather(Kv4GatherArgs a, int dtype, cudaStream_t stream) {
   a.window = kv4_window(2ll * a.N * a.Hk);
-  const long long blocks = ((a.N + a.window - 1ll) / a.window * 2 * a.Hk + 3) / 4;
+  const int heads = kv4_gather_heads(D);
+  const long long blocks = ((a.N + a.window - 1ll) / a.window * ((a.Hk + heads - 1) / heads * (D == 256 ? 2 : 1)) + 3) / 4;
   if (blocks > 0x7fffffffll) return -2;
   auto kernel = dtype == 0 ? kv4_gather_kernel<D, __nv_bfloat16> : (dtype == 1 ? kv4_gather_kernel<D, __half> : kv4_gather_kernel<D, float>);
   return launch_kernel(kernel, dim3(unsigned(blocks)), dim3(128), 0, stream, a) == cudaSuccess ? 0 : -7;
