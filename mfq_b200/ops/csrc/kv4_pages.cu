@@ -16,6 +16,7 @@ struct Kv4WriteArgs {
   int* status;
   long long k_token, k_head, v_token, v_head;  // strides in elements
   int T, Hk, pages, window;  // window: tokens in which the runs of a warp begin, 1 .. 16
+  unsigned blocks;           // of a window
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -229,12 +230,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 6 : 8) kv4_write_kernel(
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long of = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   constexpr int G = D / 64;
-  const long long first = of / (2 * G * a.Hk) * a.window;
-  if (first >= a.T) return;
-  const int head = int(of % (2 * G * a.Hk)) / (2 * G), g = int(of % G);
-  const bool is_v = of / G & 1;
+  const unsigned at_window = blockIdx.x / a.blocks, job = blockIdx.x % a.blocks * 4 + (threadIdx.x >> 5);  // of a window's (head, K or V, group)
+  const long long first = (long long)at_window * a.window;
+  if (job >= unsigned(2 * G * a.Hk)) return;
+  const int head = job / (2 * G), g = job % G;
+  const bool is_v = job / G & 1;
   // lane i: token first - 1 + i.  A run begins in the window and ends 15 tokens behind it at most
   const long long token = first - 1 + lane;
   int slot = token >= 0 && token < a.T ? a.slots[token] : -1;
@@ -266,6 +267,7 @@ struct Kv4GatherArgs {
   int* status;
   long long k_token, k_head, v_token, v_head;
   int B, N, Hk, width, pages, window;
+  unsigned blocks;
 };
 
 template <typename T>
@@ -372,13 +374,12 @@ __global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4GatherArgs a) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long of = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   constexpr int kEach = D == 256 ? 1 : 2, kHeads = kv4_gather_heads(D);  // a warp has K or V of a head of 256, both of one of 128, of two of 64
-  const int jobs = (a.Hk + kHeads - 1) / kHeads * (2 / kEach);
-  const long long first = of / jobs * a.window;
-  if (first >= a.N) return;
-  const int head = int(of % jobs) / (2 / kEach) * kHeads;
-  const bool is_v = kEach == 1 && (of & 1);
+  const unsigned at_window = blockIdx.x / a.blocks, job = blockIdx.x % a.blocks * 4 + (threadIdx.x >> 5);
+  const long long first = (long long)at_window * a.window;
+  const int head = job / (2 / kEach) * kHeads;
+  if (head >= a.Hk) return;
+  const bool is_v = kEach == 1 && (job & 1);
   // lane i: row first - 1 + i, as in the kernel above; a run is one of rows whose tokens follow one another in a page, whoever's they are
   const long long row = first - 1 + lane;
   int slot = -1, seq = kv4_sequence(a.starts, a.B, int(max(first - 1, 0ll)));
@@ -427,7 +428,8 @@ static int kv4_window(long long units) {
 template <int D>
 static int launch_write(Kv4WriteArgs a, int dtype, cudaStream_t stream) {
   a.window = kv4_window(2ll * a.T * a.Hk);
-  const long long blocks = ((a.T + a.window - 1ll) / a.window * 2 * a.Hk * (D / 64) + 3) / 4;
+  a.blocks = (2 * a.Hk * (D / 64) + 3) / 4;
+  const long long blocks = (a.T + a.window - 1ll) / a.window * a.blocks;
   if (blocks > 0x7fffffffll) return -2;
   auto kernel = dtype == 0 ? kv4_write_kernel<D, __nv_bfloat16> : (dtype == 1 ? kv4_write_kernel<D, __half> : kv4_write_kernel<D, float>);
   return launch_kernel(kernel, dim3(unsigned(blocks)), dim3(128), 0, stream, a) == cudaSuccess ? 0 : -7;
@@ -436,7 +438,8 @@ template <int D>
 static int launch_gather(Kv4GatherArgs a, int dtype, cudaStream_t stream) {
   a.window = kv4_window(2ll * a.N * a.Hk);
   const int heads = kv4_gather_heads(D);
-  const long long blocks = ((a.N + a.window - 1ll) / a.window * ((a.Hk + heads - 1) / heads * (D == 256 ? 2 : 1)) + 3) / 4;
+  a.blocks = ((a.Hk + heads - 1) / heads * (D == 256 ? 2 : 1) + 3) / 4;
+  const long long blocks = (a.N + a.window - 1ll) / a.window * a.blocks;
   if (blocks > 0x7fffffffll) return -2;
   auto kernel = dtype == 0 ? kv4_gather_kernel<D, __nv_bfloat16> : (dtype == 1 ? kv4_gather_kernel<D, __half> : kv4_gather_kernel<D, float>);
   return launch_kernel(kernel, dim3(unsigned(blocks)), dim3(128), 0, stream, a) == cudaSuccess ? 0 : -7;
@@ -448,7 +451,7 @@ static int launch_gather(Kv4GatherArgs a, int dtype, cudaStream_t stream) {
 extern "C" int mfq_kv4_write(const void* k, const void* v, const int* slots, uint8_t* pool, int dtype, int T, int Hk, int D, int pages, long long k_token,
                              long long k_head, long long v_token, long long v_head, int* status, cudaStream_t stream) {
   if (T <= 0 || Hk <= 0 || pages <= 0 || dtype < 0 || dtype > 2) return -1;
-  const mfq::Kv4WriteArgs a{k, v, slots, pool, status, k_token, k_head, v_token, v_head, T, Hk, pages, 1};
+  const mfq::Kv4WriteArgs a{k, v, slots, pool, status, k_token, k_head, v_token, v_head, T, Hk, pages, 1, 1};
   if (D == 64) return mfq::launch_write<64>(a, dtype, stream);
   if (D == 128) return mfq::launch_write<128>(a, dtype, stream);
   if (D == 256) return mfq::launch_write<256>(a, dtype, stream);
@@ -459,7 +462,7 @@ extern "C" int mfq_kv4_write(const void* k, const void* v, const int* slots, uin
 extern "C" int mfq_kv4_gather(const uint8_t* pool, const int* table, const int* starts, const int* first, void* k, void* v, int dtype, int B, int N, int Hk, int D,
                               int width, int pages, long long k_token, long long k_head, long long v_token, long long v_head, int* status, cudaStream_t stream) {
   if (B <= 0 || N <= 0 || Hk <= 0 || width <= 0 || pages <= 0 || dtype < 0 || dtype > 2) return -1;
-  const mfq::Kv4GatherArgs a{pool, table, starts, first, k, v, status, k_token, k_head, v_token, v_head, B, N, Hk, width, pages, 1};
+  const mfq::Kv4GatherArgs a{pool, table, starts, first, k, v, status, k_token, k_head, v_token, v_head, B, N, Hk, width, pages, 1, 1};
   if (D == 64) return mfq::launch_gather<64>(a, dtype, stream);
   if (D == 128) return mfq::launch_gather<128>(a, dtype, stream);
   if (D == 256) return mfq::launch_gather<256>(a, dtype, stream);
