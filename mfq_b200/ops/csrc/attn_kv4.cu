@@ -9,7 +9,8 @@
 //
 // A unit is one sequence, one KV head and up to 4, 8 or 16 of its query rows (query token, head of the group), with all pairs of pages of the sequence.
 // The pairs of all units in a row are cut into equal shares, one a CTA, as many as the GPU holds at once, whatever the lengths are: a CTA has the end of
-// one unit, whole ones, and the beginning of another.  What it has of a unit that others have too it leaves in fp32 for the merge.
+// one unit, whole ones, and the beginning of another.  What it has of a unit that others have too it leaves in fp32 for the merge.  Where there are few
+// units, or short ones, a cluster of 1 to 8 CTAs has a unit instead, cut into as many equal pieces, which meet in their shared memory: one kernel.
 // The warps of a CTA take pairs in turn, each through a ring of its own that its lanes fill by 16-byte asynchronous copies; a lane reads the codes that it copied.
 // A page's tokens are the rows of the products and the query rows their columns:
 //   S^T [16 x 8] = K Q^T,   O^T [D x 8] += V^T (p s),   p s being S^T's accumulator transposed by movmatrix.
@@ -35,10 +36,10 @@ struct Kv4AttnArgs {
   const uint8_t* pool;
   const int *table, *seq_lens;
   void* out;
-  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if others have the rest of the unit, and of its last one; null: a CTA has a unit
+  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if others have the rest of the unit, and of its last one; null: a cluster has a unit
   Kv4Join* joins;           // [CTAs]
   int* status;
-  int B, Hq, Hk, width, pages, q_len, least, tiles;  // least: pairs of a share at least; tiles: of query rows of a KV head
+  int B, Hq, Hk, width, pages, q_len, least, tiles, cluster;  // least: pairs of a share at least; tiles: of query rows of a KV head; cluster: CTAs of a unit
   float scale_log2;
 };
 
@@ -155,6 +156,25 @@ template <typename T> __device__ __forceinline__ T kv4_out(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 kv4_out(float v) { return __float2bfloat16(v); }
 template <> __device__ __forceinline__ __half kv4_out(float v) { return __float2half_rn(v); }
 
+// Barrier of all threads of the cluster, in the form that asks nothing of the lanes of a warp; what was written before is seen behind it
+__device__ __forceinline__ void cluster_meets() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_peer(const float* mine, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(mine)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 of_peer4(const float* mine, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at_peer(mine, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 of_peer2(const float* mine, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at_peer(mine, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ void kv4_add4(float4& o, float4 v, float weight) {
   o = make_float4(fmaf(v.x, weight, o.x), fmaf(v.y, weight, o.y), fmaf(v.z, weight, o.z), fmaf(v.w, weight, o.w));
 }
@@ -470,7 +490,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   using L = Kv4Ring<D>;
   using R = Kv4Rows<D, kCols, T>;
   constexpr int NB = R::NB, kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l)
-  static_assert(kPart * 4 <= L::kWarp, "the ring is where a warp leaves its sums");
+  static_assert(kPart * 4 <= L::kWarp && kCols * (D + 2) * 4 <= L::kSmem, "the rings are where the sums are left");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * L::kWarp;
@@ -486,11 +506,18 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   }
   int seq, unit, off, pairs;  // where this CTA is: unit of the sequence, pair of the unit
   long long left, x = 0, share = 1;
+  int rank = 0;  // in the cluster
+  bool none = false;
   if (a.part_o == nullptr) {
-    seq = blockIdx.x / (a.Hk * a.tiles);
-    unit = blockIdx.x % (a.Hk * a.tiles);
-    off = 0;
-    left = pairs = Kv4Shares::pairs(a, seq);
+    const int of = blockIdx.x / a.cluster;
+    rank = blockIdx.x % a.cluster;
+    seq = of / (a.Hk * a.tiles);
+    unit = of % (a.Hk * a.tiles);
+    pairs = Kv4Shares::pairs(a, seq);
+    const int each = (pairs + a.cluster - 1) / a.cluster;
+    off = min(rank * each, pairs);
+    none = off == pairs;
+    left = none ? (a.cluster > 1 ? 1 : 0) : min(each, pairs - off);  // an empty piece of a cluster takes part, whatever the lengths are
   } else {
     const Kv4Shares all(a, gridDim.x);
     share = all.share;
@@ -523,7 +550,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   uint32_t strays = 0;  // not 0: a page out of range, the last one was read in its place
 
   while (left > 0) {
-    const int here = int(min(left, (long long)(pairs - off)));
+    const int here = none ? 0 : int(min(left, (long long)(pairs - off)));
     const int kvh = unit / a.tiles, first = unit % a.tiles * kCols;
     const int length = int(min((long long)a.seq_lens[seq], 16ll * a.width)), total = (length + 15) >> 4;  // pages
     const int mine = here > warp ? (here - warp + L::kWarps - 1) / L::kWarps : 0;
@@ -562,7 +589,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       }
     };
     const uint32_t ring_at = smem_u32(ring);
-    look();
+    if (mine > 0) look();
 #pragma unroll
     for (int i = 0; i < L::kStages; ++i) {
       if (i < mine) {
@@ -631,35 +658,83 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
       }
     }
     __syncthreads();
-    const bool whole = here == pairs;
+    const bool whole = here == pairs || a.part_o == nullptr;
     const size_t slot = (2 * size_t(blockIdx.x) + (begins ? 0 : 1)) * kCols;
     const int live = min(rows - first, kCols);
-    for (int i = threadIdx.x; i < live * (D / 4); i += 128) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float ref = -FLT_MAX, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kEach = (kCols * (D / 4) + 127) / 128;  // four values each of a thread
+    float4 o[kEach];
+    float ref[kEach], l[kEach];
 #pragma unroll
-      for (int w = 0; w < L::kWarps; ++w) ref = fmaxf(ref, reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
+    for (int k = 0; k < kEach; ++k) {
+      const int i = threadIdx.x + 128 * k, r = i / (D / 4), d = i % (D / 4) * 4;
+      if (r >= live) break;
+      ref[k] = -FLT_MAX;
+      l[k] = 0.f;
+      o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < L::kWarps; ++w) ref[k] = fmaxf(ref[k], reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
 #pragma unroll
       for (int w = 0; w < L::kWarps; ++w) {
         const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
-        const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref);
-        l += from[8 * NB * kStride + 2 * r + 1] * weight;
-        kv4_add4(o, *reinterpret_cast<const float4*>(from + r * kStride + d), weight);
+        const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref[k]);
+        l[k] += from[8 * NB * kStride + 2 * r + 1] * weight;
+        kv4_add4(o[k], *reinterpret_cast<const float4*>(from + r * kStride + d), weight);
         if constexpr (R::kSide) {
-          l += from[8 * NB * kStride + 2 * r + 9] * weight;
-          kv4_add4(o, *reinterpret_cast<const float4*>(from + (r + 4) * kStride + d), weight);
+          l[k] += from[8 * NB * kStride + 2 * r + 9] * weight;
+          kv4_add4(o[k], *reinterpret_cast<const float4*>(from + (r + 4) * kStride + d), weight);
         }
       }
-      if (whole) {
-        const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
-        kv4_store4(static_cast<T*>(a.out) + row * D + d, o, l);
-      } else {
-        *reinterpret_cast<float4*>(a.part_o + (slot + r) * D + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot + r) * 2) = make_float2(ref, l);
+      if (a.cluster == 1) {
+        if (whole) {
+          const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
+          kv4_store4(static_cast<T*>(a.out) + row * D + d, o[k], l[k]);
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + (slot + r) * D + d) = o[k];
+          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot + r) * 2) = make_float2(ref[k], l[k]);
+        }
       }
     }
-    left -= here;
+    if (a.cluster > 1) {  // every CTA of the cluster comes here once: its sums where the rings were, then a part of the rows of all
+      float* mine = reinterpret_cast<float*>(smem);
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int i = threadIdx.x + 128 * k, r = i / (D / 4), d = i % (D / 4) * 4;
+        if (r >= live) break;
+        *reinterpret_cast<float4*>(mine + r * D + d) = o[k];
+        if (d == 0) *reinterpret_cast<float2*>(mine + kCols * D + 2 * r) = make_float2(ref[k], l[k]);
+      }
+      cluster_meets();
+      for (int i = threadIdx.x + 128 * rank; i < live * (D / 4); i += 128 * a.cluster) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float2 of[8];
+        float4 part[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // all requested before the first is used
+          of[k] = make_float2(-FLT_MAX, 0.f);
+          part[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k < a.cluster) {
+            of[k] = of_peer2(mine + kCols * D + 2 * r, k);
+            part[k] = of_peer4(mine + r * D + d, k);
+          }
+        }
+        float most = -FLT_MAX, sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = fmaxf(most, of[k].x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float weight = kv4_exp2(of[k].x - most);
+          sum += of[k].y * weight;
+          kv4_add4(y, part[k], weight);
+        }
+        const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
+        kv4_store4(static_cast<T*>(a.out) + row * D + d, y, sum);
+      }
+      cluster_meets();  // nobody leaves while its sums are read
+      break;
+    }
+    left -= none ? left : here;
     begins = false;
     off = 0;
     if (left > 0) {
@@ -730,8 +805,10 @@ static int launch_kv4_attn_of(Kv4AttnArgs a, int ctas, cudaStream_t stream) {
     attr[dev] = true;
   }
   const long long tiles = ((long long)a.Hq / a.Hk * a.q_len + kCols - 1) / kCols, units = (long long)a.B * a.Hk * tiles;
-  if (units > 0x7fffffffll || ctas > 1 << 20) return -2;
+  if (units * 8 > 0x7fffffffll || ctas > 1 << 20) return -2;
   a.tiles = int(tiles);
+  if (a.part_o) a.cluster = 1;
+  if (a.cluster > 1) return launch_kernel_clustered(kernel, dim3(unsigned(units * a.cluster)), dim3(128), dim3(a.cluster), kSmem, stream, a) == cudaSuccess ? 0 : -7;
   if (launch_kernel(kernel, dim3(unsigned(a.part_o ? ctas : units)), dim3(128), kSmem, stream, a) != cudaSuccess) return -7;
   if (a.part_o && launch_kernel(&kv4_merge_kernel<D, kCols, T>, dim3(unsigned(ctas)), dim3(D * kCols / 4 < 256 ? D * kCols / 4 : 256), 0, stream, a) != cudaSuccess) return -7;
   return 0;
@@ -752,16 +829,17 @@ static int launch_kv4_attn(const Kv4AttnArgs& a, int ctas, bool half, cudaStream
 }  // namespace mfq
 
 // q, out: [B * q_len, Hq, D] bf16 or fp16 (`half`); pool: [pages, Hk, 18 D]; table: [B, width]; seq_lens count every token visible to the last query row.
-// scratch: null, and every unit has a CTA of its own, or for `ctas` equal shares of at least `least` pairs of pages, beginning on 16 bytes: 4 words a share, then
+// scratch: null, and every unit has a cluster of `ctas` (1, 2, 4 or 8) CTAs, or for `ctas` equal shares of at least `least` pairs of pages, beginning on 16 bytes: 4 words a share, then
 // fp32 [2 * ctas, cols, D] and [2 * ctas, cols, 2], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
 extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, void* scratch, int half,
                                          int B, int Hq, int Hk, int D, int width, int pages, int q_len, int ctas, int least, float sm_scale, int* status,
                                          cudaStream_t stream) {
   if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || ctas > 1 << 20) return -1;
+  if (scratch == nullptr && ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) return -1;
   const long long cols = Hq / Hk * (long long)q_len <= 4 ? 4 : (D == 256 || Hq / Hk * (long long)q_len <= 8 ? 8 : 16);
   mfq::Kv4Join* joins = static_cast<mfq::Kv4Join*>(scratch);
   float* part_o = scratch ? reinterpret_cast<float*>(joins + ctas) : nullptr;
-  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, scratch ? part_o + 2 * ctas * cols * D : nullptr, joins, status, B, Hq, Hk, width, pages, q_len, least, 0, sm_scale * 1.4426950408889634f};
+  const mfq::Kv4AttnArgs a{q, pool, table, seq_lens, out, part_o, scratch ? part_o + 2 * ctas * cols * D : nullptr, joins, status, B, Hq, Hk, width, pages, q_len, least, 0, scratch ? 1 : ctas, sm_scale * 1.4426950408889634f};
   if (D == 64) return mfq::launch_kv4_attn<64>(a, ctas, half != 0, stream);
   if (D == 128) return mfq::launch_kv4_attn<128>(a, ctas, half != 0, stream);
   if (D == 256) return mfq::launch_kv4_attn<256>(a, ctas, half != 0, stream);

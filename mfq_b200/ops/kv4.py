@@ -13,6 +13,7 @@ CPU tensors take the restatements in :mod:`mfq_b200.ops.reference`.
 
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 
 import torch
@@ -23,7 +24,6 @@ from .logits import _DTYPES, _index, _refuse
 
 HEAD_DIMS = (64, 128, 256)
 SMS = 148
-ALONE = 8  # pairs of pages of a unit that has a CTA of its own
 LEAST = 4  # pairs of pages of a share: one a warp
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
 
@@ -79,15 +79,26 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None
 
 
 @lru_cache(maxsize=4096)
-def _shape(b: int, hk: int, rows: int, d: int, pages: int, width: int) -> tuple[int, int, int]:
-    """(columns of a unit, CTAs that share all pairs of pages or 0 for a CTA a unit, pairs of a share at least) for ``b`` sequences of up to ``pages`` pages,
-    ``width`` in the table, and ``rows`` query rows a KV head."""
-    cols = 4 if rows <= 4 else (8 if rows <= 8 or d == 256 else 16)
-    units = b * hk * -(-rows // cols)
-    if (width + 1) // 2 <= ALONE:
-        return cols, 0, 1
-    slots = SMS * (2 if d == 256 or cols == 16 else 4)
-    return cols, max(1, min(slots, units * -(-((pages + 1) // 2) // LEAST))), LEAST
+def _shape(units: int, cols: int, d: int, pages: int) -> tuple[int, int]:
+    """(CTAs of a unit's cluster, 0) or (0, CTAs that share all pairs of pages) for ``units`` units of ``cols`` columns and up to ``pages`` pages.
+
+    The fastest by a model in microseconds, its numbers fitted on a B200 to 1 to 200 sequences of 48 to 32000 tokens (8 KV heads of 128), in eight forms each.
+    Four warps take four pairs in a round.  With n CTAs an SM a round takes 0.33 + 0.31 n, what is before and behind the rounds 1.4 for each of them; shares need a second
+    kernel, 3 for every unit or piece of one, and a sum over a unit's pieces.  64 rows of 4096 tokens: 63.5 in single CTAs | 67.6 in pairs | 64.5 in shares; of 16384:
+    213 | 197 | 200; 3 of 2000: 20.6 | 16.4 | 19.5, in clusters of eight 12.3; 1 of 32000: 201 | 107 | 33.8, in 296 shares 27.6, in clusters 36.9."""
+    each = 2 if d == 256 or cols == 16 else 4  # CTAs that an SM holds
+    work = {64: 0.6, 128: 1.0, 256: 2.0}[d] * {4: 1.0, 8: 1.2, 16: 2.0}[cols]
+    pairs = max(1, (pages + 1) // 2)
+
+    def rounds(n: float, r: float) -> float:
+        n = n if n > each else math.ceil(n)
+        return n * (0.31 * work * r + 1.4) + 0.33 * work * r * math.ceil(n / each)
+
+    forms = [(9 + rounds(units * c / SMS, -(-pairs // (4 * c))), c, 0) for c in (1, 2, 4, 8) if c == 1 or 2 * c <= pairs]
+    for k in range(1, each + 1):
+        ctas = min(SMS * k, units * -(-pairs // LEAST))
+        forms.append((15 + rounds(ctas / SMS, units * pairs / (4 * ctas)) + 3 * units / ctas + 0.15 * ctas / units, 0, ctas))
+    return min(forms)[1:]
 
 
 def _table(block_table: torch.Tensor, b: int, index: int) -> int:
@@ -173,9 +184,11 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     if elsewhere(index):
         with torch.cuda.device(index):
             return paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale=sm_scale, q_len=q_len, max_len=max_len, out=out)
-    cols, ctas, least = _shape(b, hk, hq // hk * q_len, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)), width)
+    rows = hq // hk * q_len
+    cols = 4 if rows <= 4 else (8 if rows <= 8 or d == 256 else 16)
+    cluster, ctas = _shape(b * hk * -(-rows // cols), cols, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)))
     scratch = torch.empty(ctas * (4 + 2 * cols * (d + 2)), dtype=torch.float32, device=q.device) if ctas else None  # of this call: a workspace would tie streams and graphs together
     check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ptr(scratch),
-                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, max(1, ctas), least, sm_scale,
+                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, ctas or cluster, LEAST, sm_scale,
                                           Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if ctas else 1)
     return out
