@@ -43,9 +43,9 @@ def _rows(name: str, t: torch.Tensor, n: int, heads: int, d: int, index: int, *,
     """Strides of tokens and heads of ``t [n, heads, d]``, which is read or written 16 bytes at a time."""
     if t.ndim != 3 or t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1:
         _refuse(name, f"bf16, fp16 or fp32 [{n}, {heads}, {d}] with neighbouring dims on the device of the others are", t)
-    a, b = (t.stride(0) if n > 1 else 0), (t.stride(1) if heads > 1 else 0)
-    unit = 16 // t.element_size()
-    if a % unit or b % unit or t.data_ptr() & 15:
+    a, b, _ = t.stride()
+    a, b, unit = a if n > 1 else 0, b if heads > 1 else 0, 16 // t.element_size()
+    if (a | b) & (unit - 1) or t.data_ptr() & 15:
         raise ValueError(f"{name}: tokens and heads have to begin on 16 bytes, got strides {t.stride()} of {t.dtype}")
     if written:  # heads inside a token or tokens inside a head: no two of them over one another
         (near, count), (far, more) = sorted(((a, n) if n > 1 else (0, 1), (b, heads) if heads > 1 else (0, 1)))
@@ -83,21 +83,22 @@ def _shape(units: int, cols: int, d: int, pages: int) -> tuple[int, int]:
     """(CTAs of a unit's cluster, 0) or (0, CTAs that share all pairs of pages) for ``units`` units of ``cols`` columns and up to ``pages`` pages.
 
     The fastest by a model in microseconds, its numbers fitted on a B200 to 1 to 200 sequences of 48 to 32000 tokens (8 KV heads of 128), in eight forms each.
-    Four warps take four pairs in a round.  With n CTAs an SM a round takes 0.33 + 0.31 n, what is before and behind the rounds 1.4 for each of them; shares need a second
-    kernel, 3 for every unit or piece of one, and a sum over a unit's pieces.  64 rows of 4096 tokens: 63.5 in single CTAs | 67.6 in pairs | 64.5 in shares; of 16384:
+    Four warps take four pairs in a round.  With n CTAs an SM a round takes 0.45 + 0.29 n, what is before and behind the rounds 1.4 for each of them, a further wave 1.5; shares need a
+    second kernel, 3 for every unit or piece of one, and a sum over a unit's pieces.  64 rows of 4096 tokens: 63.5 in single CTAs | 67.6 in pairs | 64.5 in shares; of 16384:
     213 | 197 | 200; 3 of 2000: 20.6 | 16.4 | 19.5, in clusters of eight 12.3; 1 of 32000: 201 | 107 | 33.8, in 296 shares 27.6, in clusters 36.9."""
     each = 2 if d == 256 or cols == 16 else 4  # CTAs that an SM holds
     work = {64: 0.6, 128: 1.0, 256: 2.0}[d] * {4: 1.0, 8: 1.2, 16: 2.0}[cols]
     pairs = max(1, (pages + 1) // 2)
 
     def rounds(n: float, r: float) -> float:
-        n = n if n > each else math.ceil(n)
-        return n * (0.31 * work * r + 1.4) + 0.33 * work * r * math.ceil(n / each)
+        waves = math.ceil(n / each)
+        n = math.ceil(n) if 2 < n <= each else max(1.0, n)
+        return n * (0.29 * work * r + 1.4) + (0.45 * work * r + 1.5) * waves
 
-    forms = [(9 + rounds(units * c / SMS, -(-pairs // (4 * c))), c, 0) for c in (1, 2, 4, 8) if c == 1 or 2 * c <= pairs]
+    forms = [(7.5 + rounds(units * c / SMS, -(-pairs // (4 * c))), c, 0) for c in (1, 2, 4, 8) if c == 1 or 2 * c <= pairs]
     for k in range(1, each + 1):
         ctas = min(SMS * k, units * -(-pairs // LEAST))
-        forms.append((15 + rounds(ctas / SMS, units * pairs / (4 * ctas)) + 3 * units / ctas + 0.15 * ctas / units, 0, ctas))
+        forms.append((13.5 + rounds(ctas / SMS, units * pairs / (4 * ctas)) + 3 * units / ctas + 0.15 * ctas / units, 0, ctas))
     return min(forms)[1:]
 
 
@@ -115,25 +116,29 @@ def kv4_gather(kv, block_table: torch.Tensor, starts: torch.Tensor, tokens: int 
     * ``block_table [B, P]`` int32: the sequences' pages;
     * ``starts [B + 1]`` int32, ascending: rows ``starts[i] : starts[i + 1]`` are sequence ``i``'s; rows in front of the first and behind the last are left as they were;
     * ``first [B]`` int32: the position of each sequence's first row (default 0);
-    * ``k_out`` / ``v_out``: where to, both or neither (tokens and heads may lie apart, in steps of 16 bytes); they say ``tokens`` and ``dtype`` then.
+    * ``k_out`` / ``v_out``: where to, both or neither (tokens and heads may lie apart, in steps of 16 bytes, not over one another); they say ``tokens`` and ``dtype`` then.
 
     A row without a page in the table, or whose page is out of range, is left as it was and reported by ``Workspace.check``."""
     index = block_table.get_device()
     pages, heads, d = _pool(kv, index)
-    if (k_out is None) != (v_out is None):
-        raise ValueError("k_out and v_out are given together")
-    if k_out is None:
+    if k_out is None and v_out is None:
         if tokens is None or not 0 <= tokens < 1 << 31:
             raise ValueError(f"tokens: 0 to 2^31 - 1 rows wanted, got {tokens}")
         if dtype not in _DTYPES:
             raise ValueError(f"dtype: bf16, fp16 or fp32 wanted, got {dtype}")
-        k_out, v_out = (torch.empty((tokens, heads, d), dtype=dtype, device=block_table.device) for _ in range(2))
-    n = k_out.shape[0] if k_out.ndim == 3 else 0
-    if tokens is not None and tokens != n:
-        raise ValueError(f"tokens: {tokens}, but k_out has {n} rows")
-    ks, vs = _rows("k_out", k_out, n, heads, d, index, written=True), _rows("v_out", v_out, n, heads, d, index, written=True)
-    if v_out.dtype is not k_out.dtype:
-        _refuse("v_out", f"{k_out.dtype}, as k_out is,", v_out)
+        n, ks = tokens, (heads * d, d)
+        vs = ks
+        k_out = torch.empty((n, heads, d), dtype=dtype, device=block_table.device)
+        v_out = torch.empty_like(k_out)
+    elif k_out is None or v_out is None:
+        raise ValueError("k_out and v_out are given together")
+    else:
+        n = k_out.shape[0] if k_out.ndim == 3 else 0
+        if tokens is not None and tokens != n:
+            raise ValueError(f"tokens: {tokens}, but k_out has {n} rows")
+        ks, vs = _rows("k_out", k_out, n, heads, d, index, written=True), _rows("v_out", v_out, n, heads, d, index, written=True)
+        if v_out.dtype is not k_out.dtype:
+            _refuse("v_out", f"{k_out.dtype}, as k_out is,", v_out)
     b = block_table.shape[0] if block_table.ndim == 2 else -1
     width = _table(block_table, b, index)
     _index("starts", starts, b + 1, index)

@@ -145,6 +145,18 @@ def test_attention_against_the_definition(lens, how):
         run(s, want, max_len=most)
 
 
+@pytest.mark.parametrize("form", [(1, 0), (2, 0), (4, 0), (8, 0), (0, 1), (0, 3), (0, 50), (0, 592)])
+@pytest.mark.parametrize("lens,how", BATCHES + [([40 * (i % 9) for i in range(150)], {"hq": 4, "hk": 2})])
+def test_every_form_takes_every_batch(lens, how, form, monkeypatch):
+    """Clusters of a unit and shares of all units differ in time alone."""
+    require_gpu_lib()
+    monkeypatch.setattr(kv4, "_shape", lambda *a: form)
+    s = batch(len(lens), lens, device="cuda", **how)
+    want = exact(s)
+    one = run(s, want)
+    assert torch.equal(one, run(s, want)), "the same inputs, the same bits"
+
+
 @pytest.mark.parametrize("hq,hk,d,q_len", [(32, 8, 128, 1), (16, 8, 64, 1), (32, 8, 128, 4), (16, 2, 256, 2), (8, 8, 128, 1), (16, 1, 128, 1), (40, 8, 128, 1), (14, 2, 64, 2),
                                            (24, 1, 128, 3)])
 @pytest.mark.parametrize("rows,length", [(1, 9001), (3, 2500), (17, 777), (70, 140)])
