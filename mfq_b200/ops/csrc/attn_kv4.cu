@@ -19,7 +19,8 @@
 //
 // Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
 // maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum, less a power of two that brings the
-// scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest.  Scales of V between 2^-98 and 2^98.
+// scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest; that is 1/8 of a bf16 output's
+// rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  Scales of V between 2^-98 and 2^98.
 #include "attn_shared.cuh"
 #include "kv4.cuh"
 
@@ -188,7 +189,7 @@ __device__ __forceinline__ void kv4_store4(T* to, float4 o, float l) {  // o / l
 // of the first and the second page of a pair.
 template <int D, int kCols, typename T>
 struct Kv4Rows {
-  static constexpr bool kSide = kCols == 4;
+  static constexpr bool kSide = kCols == 4, kSplit = __is_same(T, __half);  // kSplit: p s as two fp16 numbers
   static constexpr int kQ = Kv4Queries<D, kCols, T>::kQ;
   static constexpr int G = D / 64, kSteps = D / 16, NB = kSide ? 1 : kCols / 8, P = kSide ? 1 : 2;  // P: pages of a pair whose scores a lane has
   float sums[NB][G][2], top[NB][2], lim[NB][2];       // of a group's q; the running maximum; the score, in units of the products, that is too far above it
@@ -330,7 +331,7 @@ struct Kv4Rows {
       moves |= mx[b][0] > lim[b][0] || mx[b][1] > lim[b][1];
     }
     if (__any_sync(0xffffffffu, moves)) move(mx, widest);
-    uint32_t pb[NB][P][G][2];
+    uint32_t pb[NB][P][G][2], rest[kSplit ? NB : 1][P][G][2];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
@@ -361,7 +362,12 @@ struct Kv4Rows {
             } else {
               om[b][g] = make_float2(fmaf(sc[b][p][h].x, pm, om[b][g].x), fmaf(sc[b][p][h].y, pm, om[b][g].y));
             }
-            pb[b][p][g][h] = kv4_transposed(half_pair(v.x, v.y));
+            const uint32_t near = half_pair(v.x, v.y);
+            pb[b][p][g][h] = kv4_transposed(near);
+            if constexpr (kSplit) {
+              const float2 as = __half22float2(*reinterpret_cast<const __half2*>(&near));
+              rest[b][p][g][h] = kv4_transposed(half_pair(v.x - as.x, v.y - as.y));
+            }
           }
         }
       }
@@ -381,7 +387,11 @@ struct Kv4Rows {
         for (int j = 0; j < 4; ++j) {
           const uint32_t h = w[j] >> 8;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, b0[b], b1[b]);
+          for (int b = 0; b < NB; ++b) {
+            kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, b0[b], b1[b]);
+            if constexpr (kSplit)
+              kv4_product(o[b][4 * g + j], w[j] & kLow, w[j] & kHigh, h & kLow, h & kHigh, rest[b][kSide ? 0 : p][g][0] & keep, rest[b][kSide ? 0 : p][g][1] & keep);
+          }
         }
       }
     }

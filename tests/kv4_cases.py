@@ -115,12 +115,13 @@ def exact(s):
 def assert_attends(s, got, want):
     """Roundings on the way to ``o = sum p (m + s c) / l``: a score is a sum of ``d`` products and a few more, on tensor cores, whose additions may cut off
     (2^-23 each of at most ``size``, and a query's values 2^-31 of its largest one); a score off by e puts p off by e, and l too; p times the scale to fp16 (2^-11
-    each, or 2^-25 where the largest is 2^7 at least, times up to 15); exponentials and sums over the keys in fp32 (a key in eight counts as one addition); and the result to its type."""
+    each for bf16 queries, 2^-22 for fp16 ones, or 2^-25 where the largest is 2^7 at least, times up to 15); exponentials and sums over the keys in fp32 (a key in eight counts as one addition); and the result to its type."""
     last = torch.finfo(s.q.dtype).eps / 2
+    each = 2.0 ** -11 if s.q.dtype is torch.bfloat16 else 2.0 ** -22
     got = got.cpu().double().view(-1, s.hk, s.hq // s.hk, s.d)
     for r, (o, weight, size, n, top) in want.items():
         score = (s.d + 16) * 2.0 ** -23 * size
-        limit = last * o.abs() + (1 + last) * (weight * (2.0 ** -11 + 2 * score + (16 + n / 8) * 2.0 ** -23) + n * 2.0 ** -32 * top) + 1e-37
+        limit = last * o.abs() + (1 + last) * (weight * (each + 2 * score + (16 + n / 8) * 2.0 ** -23) + n * 2.0 ** -32 * top) + 1e-37
         if s.q.dtype is torch.float16:
             limit = limit + 2.0 ** -25
         off = (got[r] - o).abs() - limit
