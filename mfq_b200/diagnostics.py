@@ -403,6 +403,30 @@ def check_mla_latent_cache() -> dict:
     return {"ok": err < 2e-2, "max_rel_err": err, "bytes_per_token": cache.bytes_per_token()}
 
 
+def check_kv4_cache() -> dict:
+    """The cache held in 4 bits: a ragged batch written, read back and attended against the restatements, codes and values bit for bit."""
+    from . import ops
+    from .engine.kv_cache import LayerKV4, PagedKV4Cache
+    from .ops import reference as ref
+    g = torch.Generator().manual_seed(3)
+    lens, hq, hk, d = [1, 33, 150], 8, 2, 128
+    cache = PagedKV4Cache(layers=1, kv_heads=hk, head_dim=d, num_pages=32, max_seqs=3, max_pages_per_seq=12, device="cuda")
+    kv, host = cache.layer(0), LayerKV4(torch.zeros((32, hk, 18 * d), dtype=torch.uint8), d, 16)
+    for r, n in enumerate(lens):
+        cache.assign(r, 700 + r, n)
+        rows, slots = torch.randn((n, 2 * hk, d), generator=g).to(torch.bfloat16), cache.slots(700 + r, 0, n)
+        ops.kv4_write(rows[:, :hk].cuda(), rows[:, hk:].cuda(), slots.cuda(), kv)
+        ref.kv4_write(host, rows[:, :hk], rows[:, hk:], slots)
+    starts = torch.tensor([0, 1, 34, 184], dtype=torch.int32)
+    read = ops.kv4_gather(kv, cache.block_table, starts.cuda(), 184)
+    table = cache.block_table.cpu()
+    same = torch.equal(kv.data.cpu(), host.data) and all(torch.equal(a.cpu(), b) for a, b in zip(read, ops.kv4_gather(host, table, starts, 184)))
+    q, seq_lens = torch.randn((3, hq, d), generator=g).to(torch.bfloat16), torch.tensor(lens, dtype=torch.int32)
+    got = ops.paged_attn_decode_kv4(q.cuda(), kv, cache.block_table, seq_lens.cuda(), sm_scale=d ** -0.5).float().cpu()
+    err = _rel(got, ref.paged_attn_decode_kv4(q, host, table, seq_lens, d ** -0.5).float())
+    return {"ok": same and err < 1e-2, "same_bits": same, "max_rel_err": err, "bytes_per_token": cache.bytes_per_token()}
+
+
 def check_moe_grouped() -> dict:
     """Router top-k, route plan, grouped FP8 expert GEMMs and combine against a per-expert fp32 loop."""
     from .ops import moe as moe_ops
@@ -440,7 +464,7 @@ CPU_CHECKS = {"nint": check_nint_roundtrip, "fp8-block": check_fp8_block_roundtr
               "native": check_native_helpers, "natscale": check_natscale, "tensor-schema": check_tensor_schema,
               "mtp-policy": check_mtp_policy}
 GPU_CHECKS = {"fp8-gemm": check_fp8_gemm, "attention": check_attention, "engine": check_engine_greedy, "gdn-chunked": check_gdn_chunked,
-              "packed-experts": check_packed_experts, "mla-latent-cache": check_mla_latent_cache, "moe-grouped": check_moe_grouped}
+              "packed-experts": check_packed_experts, "mla-latent-cache": check_mla_latent_cache, "moe-grouped": check_moe_grouped, "kv4-cache": check_kv4_cache}
 
 
 def run(names: list[str] | None = None, tmp_dir: str | None = None) -> dict:

@@ -20,7 +20,7 @@
 // Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
 // maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum, less a power of two that brings the
 // scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest; that is 1/8 of a bf16 output's
-// rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  Scales of V between 2^-98 and 2^98.
+// rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
 #include "attn_shared.cuh"
 #include "kv4.cuh"
 
@@ -561,6 +561,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
 
   while (left > 0) {
     const int here = none ? 0 : int(min(left, (long long)(pairs - off)));
+    if (here <= 0 && !none) break;  // lengths that changed under the kernel
     const int kvh = unit / a.tiles, first = unit % a.tiles * kCols;
     const int length = int(min((long long)a.seq_lens[seq], 16ll * a.width)), total = (length + 15) >> 4;  // pages
     const int mine = here > warp ? (here - warp + L::kWarps - 1) / L::kWarps : 0;
@@ -844,7 +845,7 @@ static int launch_kv4_attn(const Kv4AttnArgs& a, int ctas, bool half, cudaStream
 extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, void* scratch, int half,
                                          int B, int Hq, int Hk, int D, int width, int pages, int q_len, int ctas, int least, float sm_scale, int* status,
                                          cudaStream_t stream) {
-  if (B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || ctas > 1 << 20) return -1;
+  if (B <= 0 || Hk <= 0 || Hk > 65536 || Hq <= 0 || Hq % Hk || q_len < 1 || width <= 0 || pages <= 0 || ctas < 1 || least < 1 || ctas > 1 << 20) return -1;
   if (scratch == nullptr && ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) return -1;
   const long long cols = Hq / Hk * (long long)q_len <= 4 ? 4 : (D == 256 || Hq / Hk * (long long)q_len <= 8 ? 8 : 16);
   mfq::Kv4Join* joins = static_cast<mfq::Kv4Join*>(scratch);

@@ -26,14 +26,15 @@ HEAD_DIMS = (64, 128, 256)
 SMS = 148
 LEAST = 4  # pairs of pages of a share: one a warp
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
+MAX_HEADS = 65536
 
 
 def _pool(kv, index: int) -> tuple[int, int, int]:
     """(pages, heads, head dim) of a pool that the kernels take."""
     data = kv.data
     if kv.page_size != 16 or data.dtype is not torch.uint8 or data.ndim != 3 or data.shape[2] not in (18 * 64, 18 * 128, 18 * 256) or not data.is_contiguous() or \
-            data.get_device() != index or not 1 <= data.shape[0] <= MAX_PAGES or data.shape[1] < 1:
-        _refuse("kv", f"contiguous uint8 [at most {MAX_PAGES} pages of 16 tokens, heads, 18 * (64 | 128 | 256)] on the device of the others are", data)
+            data.get_device() != index or not 1 <= data.shape[0] <= MAX_PAGES or not 1 <= data.shape[1] <= MAX_HEADS:
+        _refuse("kv", f"contiguous uint8 [at most {MAX_PAGES} pages of 16 tokens, at most {MAX_HEADS} heads, 18 * (64 | 128 | 256)] on the device of the others are", data)
     if data.data_ptr() & 15:
         raise ValueError("kv: the pool has to begin on 16 bytes")
     return data.shape[0], data.shape[1], data.shape[2] // 18

@@ -394,3 +394,10 @@ def test_a_group_of_nan_is_seen_by_those_who_see_it():
     ops.kv4_write(k, torch.randn_like(k), torch.tensor([page * 16 + 3], dtype=torch.int32, device="cuda"), s.kv)
     out = call(ops, s)
     assert torch.equal(out[0], clean[0]) and out[1, 2:].isnan().all() and torch.isfinite(out[1, :2]).all()
+
+
+def test_the_self_check():
+    require_gpu_lib()
+    from mfq_b200 import diagnostics
+    report = diagnostics.run(["kv4-cache"])
+    assert report["ok"] and report["checks"]["kv4-cache"]["same_bits"], report
