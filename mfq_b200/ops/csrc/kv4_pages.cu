@@ -95,43 +95,40 @@ struct Kv4Sixteen {
   }
 };
 
-// fma.rm of two numbers, and the plain forms of common.cuh
-__device__ __forceinline__ float2 fma_down_f2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rm.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 plus_f2(float2 a, float b) {
-  add2(a.x, a.y, __float_as_uint(b), __float_as_uint(b));
-  return a;
-}
-
-// Codes of 16 values, value i in the lowest 4 bits of code[i] (what is above them is anything).
-// floor((x - m) / s) is found by a reciprocal 2^-10 too small: it may be one too small, never too large.  What is left of x - m then is exact and not
-// negative, and says whether the next code is nearer, or as near and even.  x - m may be rounded itself, which matters where that makes a tie, s (c + 1/2)
-// with its 13 bits.  In 32 bits ties are looked at again.  In 16 bits, where 0.3 % of normal values are ties, a rounded difference has as few bits only where all of
-// the smaller number was lost in the larger one: a small x where -m by itself is a tie, or any x where m is as small.
+// Codes of 16 values, value i in the lowest 8 bits of code[i] (what is above them is anything).
+// (x - m) / s by a reciprocal and one step that leaves it off by 2^-45 before it is rounded, so that a tie, c + 1/2 with its few bits, comes out as one and goes to the
+// even code when 1.5 * 2^23 is added.  What is left of x - m then is exact; more than half a step would say that the quotient was rounded to a tie.
+// x - m may be rounded itself, which matters where that makes a tie, s (c + 1/2) with its 13 bits.  In 32 bits ties are looked at again.  In 16 bits, where 0.3 % of
+// normal values are ties, a rounded difference has as few bits only where all of the smaller number was lost in the larger one: a small x where -m by itself is a
+// tie, or any x where m is as small.
 template <typename T>
 __device__ __forceinline__ void kv4_codes(uint32_t (&code)[16], const Kv4Sixteen<T>& x, Kv4Group g) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: integers in the lowest bits
+  constexpr float kMagic = 12582912.f;
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(g.s));
-  inv = g.s != 0.f ? inv * 0.9990234375f : 0.f;
-  const float half = 0.5f * g.s, less_m = 0.f - g.m;  // no negative zeros: what is left has to be none
-  bool slow = !(g.s >= 0x1p-120f) && g.s != 0.f;
-  const auto both_codes = [&](float2 v, uint32_t& c0, uint32_t& c1) {
-    const float2 h = plus_f2(v, less_m), f = fma_down_f2(h, both(inv), both(kMagic)), left = fma_f2(plus_f2(f, -kMagic), both(-g.s), h);
-    const uint32_t b0 = __float_as_uint(f.x), b1 = __float_as_uint(f.y);
-    if constexpr (sizeof(T) == 4) slow |= left.x == half || left.y == half;
-    // left > half, or left = half and the code is odd: the sign of half - left - odd, as integers
-    c0 = b0 + ((__float_as_uint(half) - __float_as_uint(left.x) - (b0 & 1u)) >> 31);
-    c1 = b1 + ((__float_as_uint(half) - __float_as_uint(left.y) - (b1 & 1u)) >> 31);
-  };
+  if (g.s == 0.f) inv = 0.f;
+  const float half = 0.5f * g.s, less_m = 0.f - g.m, less_s = -g.s;
+  bool slow = !(g.s >= 0x1p-100f) && g.s != 0.f;
+  float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) both_codes(make_float2(x.at(i), x.at(i + 1)), code[i], code[i + 1]);
+  for (int i = 0; i < 16; i += 2) {
+    float2 h = make_float2(x.at(i), x.at(i + 1));
+    add2(h.x, h.y, __float_as_uint(less_m), __float_as_uint(less_m));
+    float2 q = h;
+    scale2(q.x, q.y, inv);
+    q = fma_f2(fma_f2(q, both(less_s), h), both(inv), q);
+    add2(q.x, q.y, __float_as_uint(kMagic), __float_as_uint(kMagic));
+    code[i] = __float_as_uint(q.x);
+    code[i + 1] = __float_as_uint(q.y);
+    add2(q.x, q.y, __float_as_uint(-kMagic), __float_as_uint(-kMagic));
+    const float2 left = fma_f2(q, both(less_s), h);
+    if constexpr (sizeof(T) == 4) slow |= fabsf(left.x) == half || fabsf(left.y) == half;
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(far) : "f"(fabsf(left.x)), "f"(fabsf(left.y)));
+  }
+  if constexpr (sizeof(T) == 4) slow &= g.s != 0.f;
+  slow |= far > half;
   if constexpr (sizeof(T) < 4) {
-    const float f = __fmaf_rd(less_m, inv, kMagic), left = fmaf(f - kMagic, -g.s, less_m);
+    const float f = __fmaf_rd(less_m, inv * 0.9990234375f, kMagic), left = fmaf(f - kMagic, less_s, less_m);
     slow |= (left == half || left == half + g.s) && x.least_magnitude() < fabsf(g.m) * 0x1p-20f;
     slow |= g.m != 0.f && fabsf(g.m) < g.s * 0x1p-16f;
   }
@@ -174,7 +171,7 @@ __device__ __forceinline__ void kv4_write_run(const T* x, long long stride, int 
     uint32_t code[16];
     kv4_codes(code, v[h], grp);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bytes[h][i] = (code[i] & 15u) + code[i + 8] * 16u;  // in the lowest 8 bits
+    for (int i = 0; i < 8; ++i) bytes[h][i] = code[i] + code[i + 8] * 16u;  // in the lowest 8 bits
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
