@@ -22,7 +22,7 @@ from . import reference
 from .lib import Workspace, check, elsewhere, lib, ptr, stream_ptr
 from .logits import _DTYPES, _index, _refuse
 
-HEAD_DIMS = (64, 128, 256)
+RECORDS = {18 * 64: 64, 18 * 128: 128, 18 * 256: 256}  # bytes of a page and head: head dim
 SMS = 148
 LEAST = 4  # pairs of pages of a share: one a warp
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
@@ -32,17 +32,18 @@ MAX_HEADS = 65536
 def _pool(kv, index: int) -> tuple[int, int, int]:
     """(pages, heads, head dim) of a pool that the kernels take."""
     data = kv.data
-    if kv.page_size != 16 or data.dtype is not torch.uint8 or data.ndim != 3 or data.shape[2] not in (18 * 64, 18 * 128, 18 * 256) or not data.is_contiguous() or \
-            data.get_device() != index or not 1 <= data.shape[0] <= MAX_PAGES or not 1 <= data.shape[1] <= MAX_HEADS:
+    shape = data.shape
+    if kv.page_size != 16 or data.dtype is not torch.uint8 or len(shape) != 3 or shape[2] not in RECORDS or not data.is_contiguous() or data.get_device() != index or \
+            not 1 <= shape[0] <= MAX_PAGES or not 1 <= shape[1] <= MAX_HEADS:
         _refuse("kv", f"contiguous uint8 [at most {MAX_PAGES} pages of 16 tokens, at most {MAX_HEADS} heads, 18 * (64 | 128 | 256)] on the device of the others are", data)
     if data.data_ptr() & 15:
         raise ValueError("kv: the pool has to begin on 16 bytes")
-    return data.shape[0], data.shape[1], data.shape[2] // 18
+    return shape[0], shape[1], RECORDS[shape[2]]
 
 
 def _rows(name: str, t: torch.Tensor, n: int, heads: int, d: int, index: int, *, written: bool = False) -> tuple[int, int]:
     """Strides of tokens and heads of ``t [n, heads, d]``, which is read or written 16 bytes at a time."""
-    if t.ndim != 3 or t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1:
+    if t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1:
         _refuse(name, f"bf16, fp16 or fp32 [{n}, {heads}, {d}] with neighbouring dims on the device of the others are", t)
     a, b, _ = t.stride()
     a, b, unit = a if n > 1 else 0, b if heads > 1 else 0, 16 // t.element_size()
@@ -104,10 +105,11 @@ def _shape(units: int, cols: int, d: int, pages: int) -> tuple[int, int]:
 
 
 def _table(block_table: torch.Tensor, b: int, index: int) -> int:
-    if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous() or \
-            not 1 <= block_table.shape[1] < MAX_PAGES:
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous() or \
+            not 1 <= shape[1] < MAX_PAGES:
         _refuse("block_table", f"contiguous int32 [{b}, 1 to {MAX_PAGES - 1} pages] on the device of the others is", block_table)
-    return block_table.shape[1]
+    return shape[1]
 
 
 def kv4_gather(kv, block_table: torch.Tensor, starts: torch.Tensor, tokens: int | None = None, *, first: torch.Tensor | None = None,
@@ -168,9 +170,10 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     launches, a wrong one costs time.  A page out of range that a sequence reads is reported by ``Workspace.check``; ``q`` and ``out`` begin on 16 bytes."""
     index = q.get_device()
     pages, hk, d = _pool(kv, index)
-    if q.ndim != 3 or q.dtype not in (torch.bfloat16, torch.float16) or not q.is_contiguous() or q.shape[2] != d or q_len < 1 or q.shape[0] % q_len:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or (dtype is not torch.bfloat16 and dtype is not torch.float16) or not q.is_contiguous() or shape[2] != d or q_len < 1 or shape[0] % q_len:
         _refuse("q", f"contiguous bf16 or fp16 [B * {q_len}, Hq, {d}] are", q)
-    n, hq, _ = q.shape
+    n, hq, _ = shape
     b = n // q_len
     if hq < 1 or hq % hk:
         raise ValueError(f"{hq} query heads on {hk} KV heads")
@@ -178,9 +181,10 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     _index("seq_lens", seq_lens, b, index)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
-        _refuse("out", f"contiguous {q.dtype} {tuple(q.shape)} on the device of q is", out)
-    if (q.data_ptr() | out.data_ptr()) & 15:
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous():
+        _refuse("out", f"contiguous {dtype} {tuple(shape)} on the device of q is", out)
+    at, to = q.data_ptr(), out.data_ptr()
+    if (at | to) & 15:
         raise ValueError("q and out have to begin on 16 bytes")
     if b == 0:
         return out
@@ -194,7 +198,6 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     cols = 4 if rows <= 4 else (8 if rows <= 8 or d == 256 else 16)
     cluster, ctas = _shape(b * hk * -(-rows // cols), cols, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)))
     scratch = torch.empty(ctas * (4 + 2 * cols * (d + 2)), dtype=torch.float32, device=q.device) if ctas else None  # of this call: a workspace would tie streams and graphs together
-    check(lib().mfq_paged_attn_decode_kv4(q.data_ptr(), kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ptr(scratch),
-                                          int(q.dtype is torch.float16), b, hq, hk, d, width, pages, q_len, ctas or cluster, LEAST, sm_scale,
-                                          Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if ctas else 1)
+    check(lib().mfq_paged_attn_decode_kv4(at, kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), to, ptr(scratch), int(dtype is torch.float16), b, hq, hk, d, width,
+                                          pages, q_len, ctas or cluster, LEAST, sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if ctas else 1)
     return out
