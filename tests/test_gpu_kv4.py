@@ -396,6 +396,87 @@ def test_a_group_of_nan_is_seen_by_those_who_see_it():
     assert torch.equal(out[0], clean[0]) and out[1, 2:].isnan().all() and torch.isfinite(out[1, :2]).all()
 
 
+@pytest.mark.parametrize("d,hk,dtype", [(64, 3, torch.bfloat16), (128, 2, torch.float32), (256, 2, torch.float16)])
+def test_many_tokens_in_runs_of_every_kind(d, hk, dtype):
+    """Enough of them that a warp has windows of 8 or 16 tokens: whole pages, parts, single tokens and padding beside one another."""
+    require_gpu_lib()
+    g = torch.Generator().manual_seed(d)
+    pages, parts = 3000, []
+    for page in torch.randperm(pages, generator=g).tolist():
+        kind = int(torch.randint(0, 6, (1,), generator=g))
+        lo = int(torch.randint(0, 16, (1,), generator=g))
+        hi = int(torch.randint(lo, 17, (1,), generator=g))
+        at = list(range(16 * page, 16 * page + 16))
+        parts += [at, at, at[lo:hi], at[hi:] + [-1] * 3 + at[:lo], at[::-1], at[lo : lo + 1]][kind]
+    slots = torch.tensor(parts, dtype=torch.int32, device="cuda")
+    assert 2 * len(parts) * hk > 148 * 64 * 8
+    wide = torch.randn((len(parts), 2 * hk, d), generator=g).mul_(2).to(dtype).cuda()
+    kv = empty_pool(pages, hk, d)
+    want = write_both(wide[:, :hk], wide[:, hk:], slots, kv)
+    assert_bytes(kv.data, want)
+
+
+@pytest.mark.parametrize("d,hk,dtype", [(64, 3, torch.bfloat16), (128, 2, torch.float32), (256, 2, torch.float16)])
+def test_many_sequences_read_back(d, hk, dtype):
+    require_gpu_lib()
+    g = torch.Generator().manual_seed(d)
+    b, width, pages = 1500, 12, 700
+    lens = (torch.rand(b, generator=g) * 90).int() * (torch.rand(b, generator=g) < 0.7)
+    first = (torch.rand(b, generator=g) * 90).int()
+    table = torch.randint(0, pages, (b, width), generator=g, dtype=torch.int32)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int32), lens.cumsum(0).int()])
+    data, n = pool(d, pages, hk, d), int(starts[-1])
+    want = ops.kv4_gather(LayerKV4(data, d, 16), table, starts, n, first=first, dtype=dtype)
+    got = ops.kv4_gather(LayerKV4(data.cuda(), d, 16), table.cuda(), starts.cuda(), n, first=first.cuda(), dtype=dtype)
+    check_status()
+    for x, y in zip(got, want):
+        assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("form", [(1, 0), (0, 592)])
+def test_more_sequences_than_a_grid_has_rows(form, monkeypatch):
+    """70000 sequences of one or two tokens; of one token the output is its value."""
+    require_gpu_lib()
+    monkeypatch.setattr(kv4, "_shape", lambda *a: form)
+    b = 70000
+    data = pool(1, b + 1, 1, 64)
+    kv = LayerKV4(data.cuda(), 64, 16)
+    table = (torch.randperm(b) + 1).int().view(b, 1).cuda()
+    lens = torch.ones(b, dtype=torch.int32, device="cuda")
+    lens[::7] = 0
+    q = torch.randn(b, 4, 64, device="cuda").to(torch.bfloat16)
+    out = ops.paged_attn_decode_kv4(q, kv, table, lens, sm_scale=0.1)
+    check_status()
+    _, v = ops.kv4_gather(kv, table, torch.arange(b + 1, dtype=torch.int32, device="cuda"), b, dtype=torch.float32)
+    assert (out[::7] == 0).all()
+    some = lens.bool()
+    off = (out[some].float() - v[some]).abs() - (2.0 ** -8 * v[some].abs() + 2.0 ** -10 * 15 * 0.36)  # the output's rounding, and p s to fp16 of up to 15 scales
+    assert (off <= 0).all()
+
+
+@pytest.mark.parametrize("hq,hk,d,q_len,dtype", [(64, 1, 128, 3, torch.bfloat16), (128, 2, 64, 2, torch.float16), (48, 1, 256, 2, torch.bfloat16), (8, 8, 128, 40, torch.bfloat16)])
+def test_many_query_rows(hq, hk, d, q_len, dtype):
+    require_gpu_lib()
+    s = batch(4, [100, 30, 700], hq=hq, hk=hk, d=d, q_len=q_len, dtype=dtype, device="cuda")
+    run(s, exact(s))
+
+
+@pytest.mark.parametrize("hq,d", [(2, 128), (4, 128), (8, 128), (2, 64), (4, 256)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_a_later_token_of_a_window_is_not_seen_through_its_nan(what, hq, d):
+    require_gpu_lib()
+    s = batch(2, [64, 90, 33], hq=hq, hk=2, d=d, q_len=4, device="cuda")
+    clean = call(ops, s)
+    assert torch.isfinite(clean).all()
+    k, v = torch.randn(1, 2, d, device="cuda"), torch.randn(1, 2, d, device="cuda")
+    (k if what == "k" else v)[:] = math.nan
+    for n in (64, 90, 33):
+        row, last = (64, 90, 33).index(n), n - 1
+        ops.kv4_write(k, v, (s.table[row, last // 16 : last // 16 + 1] * 16 + last % 16).int(), s.kv)
+    out = call(ops, s).view(3, 4, hq, d)
+    assert torch.equal(out[:, :3], clean.view(3, 4, hq, d)[:, :3]) and out[:, 3].isnan().all()
+
+
 def test_the_self_check():
     require_gpu_lib()
     from mfq_b200 import diagnostics
