@@ -262,12 +262,11 @@ def paged_attn_decode_kv4(q, kv, block_table, seq_lens, sm_scale, q_len: int = 1
             raise ValueError(f"sequence {i}: a page is out of range")
         k, v = kv4_tokens(kv, page, pos % 16)
         x = q[i * q_len : (i + 1) * q_len].float().view(q_len, hk, hq // hk, d)
-        scores = torch.einsum("qhgd,khd->hgqk", x, k) * sm_scale
-        seen = pos <= torch.arange(length - q_len, length)[:, None]
-        p = torch.softmax(scores.masked_fill(~seen, -math.inf), -1)
-        p = torch.where(seen.any(-1)[:, None], p, torch.zeros_like(p))  # a query in front of the first token sees nothing
-        o = torch.einsum("hgqk,khd->qhgd", p, v)
-        out[i * q_len : (i + 1) * q_len] = o.reshape(q_len, hq, d).to(q.dtype)
+        for j in range(q_len):
+            sees = length - (q_len - 1 - j)
+            if sees > 0:  # a query's products are with the tokens it sees alone: a weight of 0 times a NaN behind them would be one
+                p = torch.softmax(torch.einsum("hgd,khd->hgk", x[j], k[:sees]) * sm_scale, -1)
+                out[i * q_len + j] = torch.einsum("hgk,khd->hgd", p, v[:sees]).reshape(hq, d).to(q.dtype)
     return out
 
 
