@@ -16,6 +16,7 @@ from __future__ import annotations
 import math
 from functools import lru_cache
 
+import numpy as np
 import torch
 
 from . import reference
@@ -54,6 +55,24 @@ def _rows(name: str, t: torch.Tensor, n: int, heads: int, d: int, index: int, *,
         if (count > 1 and near < d) or (more > 1 and far < (count - 1) * near + d):
             raise ValueError(f"{name}: rows lie over one another, strides {t.stride()}")
     return a, b
+
+
+def _meet(gap: int, n: int, heads: int, d: int, ks: tuple[int, int], vs: tuple[int, int]) -> bool:
+    """Whether a row of ``v_out`` lies over one of ``k_out``: ``[n, heads]`` rows of ``d`` elements each, strides ``vs`` and ``ks``, ``gap`` elements from k's first to v's.
+    Rows of one output are known not to lie over one another."""
+    if gap >= (n - 1) * ks[0] + (heads - 1) * ks[1] + d or -gap >= (n - 1) * vs[0] + (heads - 1) * vs[1] + d:
+        return False
+    if ks == vs:  # a row of v is i near strides, j far ones and the gap from one of k
+        (near, count), (far, more) = sorted(((ks[0], n), (ks[1], heads)))
+        for j in range(-(gap // far) - 2, -(gap // far) + 3) if far else (0,):
+            if -more < j < more:
+                rest = -gap - j * far
+                i = rest // near if near else 0
+                if any(-count < e < count and abs(e * near - rest) < d for e in (i, i + 1)):
+                    return True
+        return False
+    at = [(np.arange(n, dtype=np.int64)[:, None] * a + np.arange(heads, dtype=np.int64) * b).ravel() for a, b in (ks, vs)]
+    return bool((np.diff(np.sort(np.concatenate([at[0], at[1] + gap]))) < d).any())
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None:
@@ -119,7 +138,7 @@ def kv4_gather(kv, block_table: torch.Tensor, starts: torch.Tensor, tokens: int 
     * ``block_table [B, P]`` int32: the sequences' pages;
     * ``starts [B + 1]`` int32, ascending: rows ``starts[i] : starts[i + 1]`` are sequence ``i``'s; rows in front of the first and behind the last are left as they were;
     * ``first [B]`` int32: the position of each sequence's first row (default 0);
-    * ``k_out`` / ``v_out``: where to, both or neither (tokens and heads may lie apart, in steps of 16 bytes, not over one another); they say ``tokens`` and ``dtype`` then.
+    * ``k_out`` / ``v_out``: where to, both or neither (tokens and heads may lie apart, in steps of 16 bytes, neither's rows over others of it or of the other); they say ``tokens`` and ``dtype`` then.
 
     A row without a page in the table, or whose page is out of range, is left as it was and reported by ``Workspace.check``."""
     index = block_table.get_device()
@@ -142,6 +161,8 @@ def kv4_gather(kv, block_table: torch.Tensor, starts: torch.Tensor, tokens: int 
         ks, vs = _rows("k_out", k_out, n, heads, d, index, written=True), _rows("v_out", v_out, n, heads, d, index, written=True)
         if v_out.dtype is not k_out.dtype:
             _refuse("v_out", f"{k_out.dtype}, as k_out is,", v_out)
+        if n and _meet((v_out.data_ptr() - k_out.data_ptr()) // k_out.element_size(), n, heads, d, ks, vs):
+            raise ValueError("v_out: lies over k_out")
     b = block_table.shape[0] if block_table.ndim == 2 else -1
     width = _table(block_table, b, index)
     _index("starts", starts, b + 1, index)
