@@ -28,6 +28,7 @@ SMS = 148
 LEAST = 4  # pairs of pages of a share: one a warp
 MAX_PAGES = 1 << 27  # of a pool, and of a table's row: slots and lengths are int32
 MAX_HEADS = 65536
+MAX_SEQS = 1 << 30  # of a table: they are counted in 32 bits, as tokens are
 
 
 def _pool(kv, index: int) -> tuple[int, int, int]:
@@ -44,8 +45,8 @@ def _pool(kv, index: int) -> tuple[int, int, int]:
 
 def _rows(name: str, t: torch.Tensor, n: int, heads: int, d: int, index: int, *, written: bool = False) -> tuple[int, int]:
     """Strides of tokens and heads of ``t [n, heads, d]``, which is read or written 16 bytes at a time."""
-    if t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1:
-        _refuse(name, f"bf16, fp16 or fp32 [{n}, {heads}, {d}] with neighbouring dims on the device of the others are", t)
+    if t.shape != (n, heads, d) or t.dtype not in _DTYPES or t.get_device() != index or t.stride(2) != 1 or n >= 1 << 31:
+        _refuse(name, f"bf16, fp16 or fp32 [{n} below 2^31, {heads}, {d}] with neighbouring dims on the device of the others are", t)
     a, b, _ = t.stride()
     a, b, unit = a if n > 1 else 0, b if heads > 1 else 0, 16 // t.element_size()
     if (a | b) & (unit - 1) or t.data_ptr() & 15:
@@ -126,8 +127,8 @@ def _shape(units: int, cols: int, d: int, pages: int) -> tuple[int, int]:
 def _table(block_table: torch.Tensor, b: int, index: int) -> int:
     shape = block_table.shape
     if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != b or block_table.get_device() != index or not block_table.is_contiguous() or \
-            not 1 <= shape[1] < MAX_PAGES:
-        _refuse("block_table", f"contiguous int32 [{b}, 1 to {MAX_PAGES - 1} pages] on the device of the others is", block_table)
+            not 1 <= shape[1] < MAX_PAGES or b > MAX_SEQS:
+        _refuse("block_table", f"contiguous int32 [{b}, at most {MAX_SEQS}; 1 to {MAX_PAGES - 1} pages] on the device of the others is", block_table)
     return shape[1]
 
 

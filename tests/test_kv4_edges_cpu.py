@@ -59,3 +59,13 @@ def test_one_row_of_neighbouring_outputs():
     assert (row != 0).any(-1).all()
     with pytest.raises(ValueError, match="lies over"):
         ops.kv4_gather(kv, i32(1)[None], i32(0, 1), k_out=row[:, :2], v_out=row[:, 1:3])
+
+
+def test_more_than_32_bits_count_is_refused():
+    """Memory that is asked for and never touched; a token's row may be one for all."""
+    kv, n = LayerKV4(pool(1, 2, 1, 64), 64, 16), 2 ** 32 + 3
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        ops.kv4_write(torch.zeros(1, 1, 64).expand(n, 1, 64), torch.zeros(1, 1, 64).expand(n, 1, 64), i32[:1].expand(n), kv)
+    with pytest.raises(ValueError, match="block_table: .*at most 1073741824"):
+        ops.kv4_gather(kv, torch.empty(2 ** 30 + 1, 1, dtype=torch.int32, device="meta"), i32, 1)
