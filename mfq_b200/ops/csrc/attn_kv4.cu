@@ -18,9 +18,11 @@
 // lane computes the softmax of columns that nobody has; O^T's halves are added in the end.
 //
 // Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
-// maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum, less a power of two that brings the
-// scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest; that is 1/8 of a bf16 output's
-// rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
+// maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum.  p s and p m are multiplied by a power of two that
+// brings the largest scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest p times the largest scale that
+// the warp has met; that is 1/8 of a bf16 output's rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  The sum of p has
+// no such factor: warps, CTAs and pieces are joined by ref for p and by both for the rest, so that scales of V may lie apart as far as their type lets
+// them and the softmax is the same wherever they are.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
 //
 // Measured, 8 KV heads of 128, bf16: 64 rows of 16384 tokens (1.2 GB) 195 to 204 us, 0.91 to 0.95 of the measured copy rate, 217 to 233 where the power limit holds
 // the clock at 1.64 GHz; 64 of 4096 59 us; 3 of up to 2000 8.3.  A pair of pages costs a warp 400 instructions, 225 of them on the half-rate integer
@@ -43,7 +45,7 @@ struct Kv4AttnArgs {
   const uint8_t* pool;
   const int *table, *seq_lens;
   void* out;
-  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 2]: of a CTA's first piece, if others have the rest of the unit, and of its last one; null: a cluster has a unit
+  float *part_o, *part_ml;  // [2 * CTAs, kCols, D], [.., 4]: of a CTA's first piece, if others have the rest of the unit, and of its last one; null: a cluster has a unit
   Kv4Join* joins;           // [CTAs]
   int* status;
   int B, Hq, Hk, width, pages, q_len, least, tiles, cluster;  // least: pairs of a share at least; tiles: of query rows of a KV head; cluster: CTAs of a unit
@@ -177,18 +179,13 @@ __device__ __forceinline__ float4 of_peer4(const float* mine, int rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at_peer(mine, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 of_peer2(const float* mine, int rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at_peer(mine, rank)) : "memory");
-  return v;
-}
 __device__ __forceinline__ void kv4_add4(float4& o, float4 v, float weight) {
   o = make_float4(fmaf(v.x, weight, o.x), fmaf(v.y, weight, o.y), fmaf(v.z, weight, o.z), fmaf(v.w, weight, o.w));
 }
 template <typename T>
-__device__ __forceinline__ void kv4_store4(T* to, float4 o, float l) {  // o / l; nothing seen: zeros
-  const float by = l == 0.f ? 0.f : 1.f / l;
-  T y[4] = {kv4_out<T>(o.x * by), kv4_out<T>(o.y * by), kv4_out<T>(o.z * by), kv4_out<T>(o.w * by)};
+__device__ __forceinline__ void kv4_store4(T* to, float4 o, float l, float power) {  // o 2^power / l; nothing seen: zeros
+  const float by = l == 0.f ? 0.f : 1.f / l, times = l == 0.f ? 0.f : kv4_exp2(power);
+  T y[4] = {kv4_out<T>(o.x * by * times), kv4_out<T>(o.y * by * times), kv4_out<T>(o.z * by * times), kv4_out<T>(o.w * by * times)};
   *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(y);
 }
 // What a warp has of its query rows: column blocks of 8, a lane has the columns 8 b + 2 c and the one behind it.  kCols 4: the columns n and n + 4 are row n,
@@ -201,7 +198,7 @@ struct Kv4Rows {
   float sums[NB][G][2], top[NB][2], lim[NB][2];       // of a group's q; the running maximum; the score, in units of the products, that is too far above it
   float2 to_log2[NB], less[NB], om[NB][G], l[NB];     // what such a score is times log2 e; -ref
   float o[NB][kSteps][4];
-  float up, over;  // log2 of what V's scales are multiplied by, and the scale that would be too large
+  float lift;  // the power of two by which o and om are multiplied, l is not
   int len[NB][2], low, most;
 
   __device__ __forceinline__ void load(const Kv4AttnArgs& a, int first, int rows, int length, const uint32_t* q) {
@@ -233,8 +230,7 @@ struct Kv4Rows {
     }
     low = __reduce_min_sync(0xffffffffu, lo);
     most = __reduce_max_sync(0xffffffffu, hi);
-    up = 0.f;
-    over = 0.f;  // none chosen yet
+    lift = 0x1p104f;
   }
 
   // Two pages whose first token is tok0; kWhole: all rows see all of both
@@ -309,7 +305,7 @@ struct Kv4Rows {
     }
     // parameters of V, none where nobody sees the token: what is there may be anything
     uint32_t par[P][2][G];
-    float widest = 0.f;
+    float widest = 0.f, largest = 0.f;  // scale, minimum
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       params(par[p], rec0 + (p + side) * 18 * D + 17 * D + g8 * (D / 8));
@@ -322,10 +318,13 @@ struct Kv4Rows {
         }
       }
 #pragma unroll
-      for (int g = 0; g < G; ++g) widest = max3(widest, __uint_as_float(par[p][0][g] << 16), __uint_as_float(par[p][1][g] << 16));
+      for (int g = 0; g < G; ++g) {
+        widest = max3(widest, __uint_as_float(par[p][0][g] << 16), __uint_as_float(par[p][1][g] << 16));
+        largest = max3(largest, fabsf(__uint_as_float(par[p][0][g] & 0xffff0000u)), fabsf(__uint_as_float(par[p][1][g] & 0xffff0000u)));
+      }
     }
     float mx[NB][2];
-    bool moves = widest > over;
+    bool moves = fmaxf(widest, largest * 0x1p-77f) * lift > 0x1p9f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       mx[b][0] = fmaxf(sc[b][0][0].x, sc[b][0][1].x);
@@ -336,7 +335,7 @@ struct Kv4Rows {
       }
       moves |= mx[b][0] > lim[b][0] || mx[b][1] > lim[b][1];
     }
-    if (__any_sync(0xffffffffu, moves)) move(mx, widest);
+    if (__any_sync(0xffffffffu, moves)) move(mx, widest, largest);
     uint32_t pb[NB][P][G][2], rest[kSplit ? NB : 1][P][G][2];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -351,6 +350,7 @@ struct Kv4Rows {
           }
           sc[b][p][h] = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
           l[b] = add_f2(l[b], sc[b][p][h]);
+          scale2(sc[b][p][h].x, sc[b][p][h].y, lift);
         }
       }
 #pragma unroll
@@ -416,14 +416,12 @@ struct Kv4Rows {
     }
   }
 
-  // New references: the running maxima and the power of two of V's scales
-  __device__ __forceinline__ void move(const float (&mx)[NB][2], float widest) {
-    widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)));
-    if (widest > over) {
-      const int e = int(__float_as_uint(widest) >> 23) - 127;  // of a denormal one: -127
-      up = fminf(7.f - float(e), 104.f);
-      over = kv4_exp2(9.f - up);
-    }
+  // New references: the running maxima, and the power of two of V's sums.  It brings the scales to 2^7 .. 2^9 and leaves the minima below 2^87, which
+  // matters where a group of one value (scale 0) stands beside values of 2^-77 of it.
+  __device__ __forceinline__ void move(const float (&mx)[NB][2], float widest, float largest) {
+    const auto exponent = [](float x) { return int(__reduce_max_sync(0xffffffffu, __float_as_uint(x)) >> 23) - 127; };  // of the warp's largest; a denormal one: -127
+    const int before = int(__float_as_uint(lift) >> 23) - 127, up = min(before, min(7 - exponent(widest), 84 - exponent(largest)));
+    lift = __uint_as_float(uint32_t(up + 127) << 23);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float corr[2];
@@ -438,11 +436,11 @@ struct Kv4Rows {
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (m > -INFINITY) top[b][e] = fmaxf(top[b][e], m * f);
         lim[b][e] = top[b][e] > -FLT_MAX ? (top[b][e] + 6.f) / f : -FLT_MAX;
-        const float next = up - top[b][e];
-        corr[e] = kv4_exp2(next - now);
+        const float next = -top[b][e], by = next - now;
+        corr[e] = kv4_exp2(by + float(up - before));
+        (e == 0 ? l[b].x : l[b].y) *= kv4_exp2(by);
         now = next;
       }
-      l[b] = make_float2(l[b].x * corr[0], l[b].y * corr[1]);
 #pragma unroll
       for (int g = 0; g < G; ++g) om[b][g] = make_float2(om[b][g].x * corr[0], om[b][g].y * corr[1]);
 #pragma unroll
@@ -505,8 +503,8 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
   pdl_trigger();
   using L = Kv4Ring<D>;
   using R = Kv4Rows<D, kCols, T>;
-  constexpr int NB = R::NB, kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l)
-  static_assert(kPart * 4 <= L::kWarp && kCols * (D + 2) * 4 <= L::kSmem, "the rings are where the sums are left");
+  constexpr int NB = R::NB, kStride = D + 4, kPart = 8 * NB * kStride + 16 * NB + 1;  // what a warp leaves, in floats: rows of columns on different banks, then (ref, l), log2 of what its sums are in units of
+  static_assert(kPart * 4 <= L::kWarp && kCols * (D + 4) * 4 <= L::kSmem, "the rings are where the sums are left");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * L::kWarp;
@@ -650,6 +648,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     float* part = reinterpret_cast<float*>(ring);
     float* ml = part + 8 * NB * kStride;
     __syncwarp();
+    if (lane == 0) ml[16 * NB] = float(127 - int(__float_as_uint(t.lift) >> 23));
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -680,34 +679,39 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     const int live = min(rows - first, kCols);
     constexpr int kEach = (kCols * (D / 4) + 127) / 128;  // four values each of a thread
     float4 o[kEach];
-    float ref[kEach], l[kEach];
+    float ref[kEach], l[kEach], power[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       const int i = threadIdx.x + 128 * k, r = i / (D / 4), d = i % (D / 4) * 4;
       if (r >= live) break;
+      const auto left_by = [&](int w) { return reinterpret_cast<const float*>(smem + w * L::kWarp); };
+      const auto ref_of = [&](int w) { return left_by(w)[8 * NB * kStride + 2 * r]; };
       ref[k] = -FLT_MAX;
+      power[k] = -FLT_MAX;
       l[k] = 0.f;
       o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < L::kWarps; ++w) ref[k] = fmaxf(ref[k], reinterpret_cast<const float*>(smem + w * L::kWarp)[8 * NB * kStride + 2 * r]);
+      for (int w = 0; w < L::kWarps; ++w) ref[k] = fmaxf(ref[k], ref_of(w));
+#pragma unroll
+      for (int w = 0; w < L::kWarps; ++w) power[k] = fmaxf(power[k], ref_of(w) - ref[k] + left_by(w)[8 * NB * kStride + 16 * NB]);
 #pragma unroll
       for (int w = 0; w < L::kWarps; ++w) {
-        const float* from = reinterpret_cast<const float*>(smem + w * L::kWarp);
-        const float weight = kv4_exp2(from[8 * NB * kStride + 2 * r] - ref[k]);
+        const float* from = left_by(w);
+        const float weight = kv4_exp2(ref_of(w) - ref[k]), of_o = kv4_exp2(ref_of(w) - ref[k] + from[8 * NB * kStride + 16 * NB] - power[k]);
         l[k] += from[8 * NB * kStride + 2 * r + 1] * weight;
-        kv4_add4(o[k], *reinterpret_cast<const float4*>(from + r * kStride + d), weight);
+        kv4_add4(o[k], *reinterpret_cast<const float4*>(from + r * kStride + d), of_o);
         if constexpr (R::kSide) {
           l[k] += from[8 * NB * kStride + 2 * r + 9] * weight;
-          kv4_add4(o[k], *reinterpret_cast<const float4*>(from + (r + 4) * kStride + d), weight);
+          kv4_add4(o[k], *reinterpret_cast<const float4*>(from + (r + 4) * kStride + d), of_o);
         }
       }
       if (a.cluster == 1) {
         if (whole) {
           const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
-          kv4_store4(static_cast<T*>(a.out) + row * D + d, o[k], l[k]);
+          kv4_store4(static_cast<T*>(a.out) + row * D + d, o[k], l[k], power[k]);
         } else {
           *reinterpret_cast<float4*>(a.part_o + (slot + r) * D + d) = o[k];
-          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot + r) * 2) = make_float2(ref[k], l[k]);
+          if (d == 0) *reinterpret_cast<float4*>(a.part_ml + (slot + r) * 4) = make_float4(ref[k], l[k], power[k], 0.f);
         }
       }
     }
@@ -719,34 +723,34 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
         const int i = threadIdx.x + 128 * k, r = i / (D / 4), d = i % (D / 4) * 4;
         if (r >= live) break;
         *reinterpret_cast<float4*>(mine + r * D + d) = o[k];
-        if (d == 0) *reinterpret_cast<float2*>(mine + kCols * D + 2 * r) = make_float2(ref[k], l[k]);
+        if (d == 0) *reinterpret_cast<float4*>(mine + kCols * D + 4 * r) = make_float4(ref[k], l[k], power[k], 0.f);
       }
       cluster_meets();
       for (int i = threadIdx.x + 128 * rank; i < live * (D / 4); i += 128 * a.cluster) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float2 of[8];
-        float4 part[8];
+        float4 of[8], part[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // all requested before the first is used
-          of[k] = make_float2(-FLT_MAX, 0.f);
+          of[k] = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
           part[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (k < a.cluster) {
-            of[k] = of_peer2(mine + kCols * D + 2 * r, k);
+            of[k] = of_peer4(mine + kCols * D + 4 * r, k);
             part[k] = of_peer4(mine + r * D + d, k);
           }
         }
-        float most = -FLT_MAX, sum = 0.f;
+        float most = -FLT_MAX, power = -FLT_MAX, sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) most = fmaxf(most, of[k].x);
 #pragma unroll
+        for (int k = 0; k < 8; ++k) power = fmaxf(power, of[k].x - most + of[k].z);
+#pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float weight = kv4_exp2(of[k].x - most);
-          sum += of[k].y * weight;
-          kv4_add4(y, part[k], weight);
+          sum += of[k].y * kv4_exp2(of[k].x - most);
+          kv4_add4(y, part[k], kv4_exp2(of[k].x - most + of[k].z - power));
         }
         const size_t row = (size_t(seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
-        kv4_store4(static_cast<T*>(a.out) + row * D + d, y, sum);
+        kv4_store4(static_cast<T*>(a.out) + row * D + d, y, sum, power);
       }
       cluster_meets();  // nobody leaves while its sums are read
       break;
@@ -775,36 +779,39 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
   const int cta = blockIdx.x, per_head = a.Hq / a.Hk;
   const Kv4Join join = a.joins[cta];
   const int n = join.n, kvh = join.unit / a.tiles, first = join.unit % a.tiles * kCols, live = n == 0 ? 0 : min(per_head * a.q_len - first, kCols);
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  const float4* ml = reinterpret_cast<const float4*>(a.part_ml);
   for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     const auto slot = [&](int k) { return (2 * size_t(cta - n + 1 + k) + (k == 0 ? join.behind : 0)) * kCols + r; };
-    float ref = -FLT_MAX, l = 0.f;
+    float ref = -FLT_MAX, l = 0.f, power = -FLT_MAX;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < n; k += kAtOnce) {
-      float2 of[kAtOnce];
-      float4 part[kAtOnce];
+      float4 of[kAtOnce], part[kAtOnce];
 #pragma unroll
       for (int e = 0; e < kAtOnce; ++e) {  // all requested before the first is used
-        of[e] = k + e < n ? ml[slot(k + e)] : make_float2(-FLT_MAX, 0.f);
+        of[e] = k + e < n ? ml[slot(k + e)] : make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
         part[e] = k + e < n ? *reinterpret_cast<const float4*>(a.part_o + slot(k + e) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      float next = ref;
+      float most = ref;
 #pragma unroll
-      for (int e = 0; e < kAtOnce; ++e) next = fmaxf(next, of[e].x);
-      const float keep = kv4_exp2(ref - next);
-      l *= keep;
+      for (int e = 0; e < kAtOnce; ++e) most = fmaxf(most, of[e].x);
+      const float had = ref - most + power;
+      float next = had;
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) next = fmaxf(next, of[e].x - most + of[e].z);
+      l *= kv4_exp2(ref - most);
+      const float keep = kv4_exp2(had - next);
       o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-      ref = next;
+      ref = most;
+      power = next;
 #pragma unroll
       for (int e = 0; e < kAtOnce; ++e) {
-        const float weight = kv4_exp2(of[e].x - ref);
-        l += of[e].y * weight;
-        kv4_add4(o, part[e], weight);
+        l += of[e].y * kv4_exp2(of[e].x - ref);
+        kv4_add4(o, part[e], kv4_exp2(of[e].x - ref + of[e].z - power));
       }
     }
     const size_t row = (size_t(join.seq) * a.q_len + (first + r) / per_head) * a.Hq + kvh * per_head + (first + r) % per_head;
-    kv4_store4(static_cast<T*>(a.out) + row * D + d, o, l);
+    kv4_store4(static_cast<T*>(a.out) + row * D + d, o, l, power);
   }
 }
 
@@ -847,7 +854,7 @@ static int launch_kv4_attn(const Kv4AttnArgs& a, int ctas, bool half, cudaStream
 
 // q, out: [B * q_len, Hq, D] bf16 or fp16 (`half`); pool: [pages, Hk, 18 D]; table: [B, width]; seq_lens count every token visible to the last query row.
 // scratch: null, and every unit has a cluster of `ctas` (1, 2, 4 or 8) CTAs, or for `ctas` equal shares of at least `least` pairs of pages, beginning on 16 bytes: 4 words a share, then
-// fp32 [2 * ctas, cols, D] and [2 * ctas, cols, 2], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
+// fp32 [2 * ctas, cols, D] and [2 * ctas, cols, 4], cols being 4 for up to 4 query rows of a KV head, 8 for up to 8 or heads of 256, else 16.
 extern "C" int mfq_paged_attn_decode_kv4(const void* q, const uint8_t* pool, const int* table, const int* seq_lens, void* out, void* scratch, int half,
                                          int B, int Hq, int Hk, int D, int width, int pages, int q_len, int ctas, int least, float sm_scale, int* status,
                                          cudaStream_t stream) {

@@ -219,7 +219,7 @@ def paged_attn_decode_kv4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_le
     rows = hq // hk * q_len
     cols = 4 if rows <= 4 else (8 if rows <= 8 or d == 256 else 16)
     cluster, ctas = _shape(b * hk * -(-rows // cols), cols, d, width if max_len is None else max(1, min(width, (max_len + 15) // 16)))
-    scratch = torch.empty(ctas * (4 + 2 * cols * (d + 2)), dtype=torch.float32, device=q.device) if ctas else None  # of this call: a workspace would tie streams and graphs together
+    scratch = torch.empty(ctas * (4 + 2 * cols * (d + 4)), dtype=torch.float32, device=q.device) if ctas else None  # of this call: a workspace would tie streams and graphs together
     check(lib().mfq_paged_attn_decode_kv4(at, kv.data.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), to, ptr(scratch), int(dtype is torch.float16), b, hq, hk, d, width,
                                           pages, q_len, ctas or cluster, LEAST, sm_scale, Workspace.get(q.device).status.data_ptr(), stream_ptr()), "paged_attn_decode_kv4", 2 if ctas else 1)
     return out
