@@ -193,10 +193,11 @@ __device__ __forceinline__ void kv4_store4(T* to, float4 o, float l, float power
 template <int D, int kCols, typename T>
 struct Kv4Rows {
   static constexpr bool kSide = kCols == 4, kSplit = __is_same(T, __half);  // kSplit: p s as two fp16 numbers
+  static constexpr int kApart = kSplit ? 4 : 32;  // pairs of pages after which o and om meet
   static constexpr int kQ = Kv4Queries<D, kCols, T>::kQ;
   static constexpr int G = D / 64, kSteps = D / 16, NB = kSide ? 1 : kCols / 8, P = kSide ? 1 : 2;  // P: pages of a pair whose scores a lane has
-  float sums[NB][G][2], top[NB][2], lim[NB][2];       // of a group's q; the running maximum; the score, in units of the products, that is too far above it
-  float2 to_log2[NB], less[NB], om[NB][G], l[NB];     // what such a score is times log2 e; -ref
+  float sums[NB][G][2];                            // of a group's q
+  float2 to_log2[NB], less[NB], om[NB][G], l[NB];  // what a score in units of the products is times log2 e; -ref
   float o[NB][kSteps][4];
   float lift;  // the power of two by which o and om are multiplied, l is not
   int len[NB][2], low, most;
@@ -218,8 +219,6 @@ struct Kv4Rows {
         len[b][e] = mine < rows ? max(0, length - (a.q_len - 1 - mine / per)) : INT_MAX;
         lo = min(lo, len[b][e]);
         if (mine < rows) hi = max(hi, len[b][e]);
-        top[b][e] = -FLT_MAX;
-        lim[b][e] = -FLT_MAX;
       }
       less[b] = both(FLT_MAX);
       l[b] = both(0.f);
@@ -333,7 +332,7 @@ struct Kv4Rows {
         mx[b][0] = max3(mx[b][0], sc[b][P - 1][0].x, sc[b][P - 1][1].x);
         mx[b][1] = max3(mx[b][1], sc[b][P - 1][0].y, sc[b][P - 1][1].y);
       }
-      moves |= mx[b][0] > lim[b][0] || mx[b][1] > lim[b][1];
+      moves |= fmaf(mx[b][0], to_log2[b].x, less[b].x) > 6.f || fmaf(mx[b][1], to_log2[b].y, less[b].y) > 6.f;
     }
     if (__any_sync(0xffffffffu, moves)) move(mx, widest, largest);
     uint32_t pb[NB][P][G][2], rest[kSplit ? NB : 1][P][G][2];
@@ -403,6 +402,27 @@ struct Kv4Rows {
     }
   }
 
+  // o, a sum of codes that are 0 or more, and om, a sum of minima that mostly are 0 or less, are many times their difference: an average over n tokens falls with sqrt(n).
+  // What tensor cores cut off at an addition (2^-24 of the sum, always towards 0) then is an error of the average.  So they meet before either is large.
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float2 m = om[b][g];
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) m = add_f2(m, make_float2(__shfl_xor_sync(0xffffffffu, m.x, x), __shfl_xor_sync(0xffffffffu, m.y, x)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float(&y)[4] = o[b][4 * g + j];
+          y[0] = fmaf(m.x, 0x1p-24f, y[0]); y[1] = fmaf(m.y, 0x1p-24f, y[1]);
+          y[2] = fmaf(m.x, 0x1p-20f, y[2]); y[3] = fmaf(m.y, 0x1p-20f, y[3]);
+        }
+        om[b][g] = both(0.f);
+      }
+    }
+  }
+
   static __device__ __forceinline__ void params(uint32_t (&par)[2][G], const uint8_t* at) {  // [half][group] in a row
     if constexpr (G == 1) {
       const uint2 v = *reinterpret_cast<const uint2*>(at);
@@ -434,9 +454,7 @@ struct Kv4Rows {
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if (m > -INFINITY) top[b][e] = fmaxf(top[b][e], m * f);
-        lim[b][e] = top[b][e] > -FLT_MAX ? (top[b][e] + 6.f) / f : -FLT_MAX;
-        const float next = -top[b][e], by = next - now;
+        const float next = m > -INFINITY ? fminf(now, -(m * f)) : now, by = next - now;
         corr[e] = kv4_exp2(by + float(up - before));
         (e == 0 ? l[b].x : l[b].y) *= kv4_exp2(by);
         now = next;
@@ -632,10 +650,14 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
     };
     const int end = used + 2 * L::kWarps * mine, seen = min(end, (t.low >> 4) - 1);
     while (used < seen) {
-      copies_but_the_last<L::kStages - 1>();
-      __syncwarp();
-      t.template pages<true>(ring + stage, block_q, used << 4);
-      next();
+      const int stop = min(seen, used + 2 * L::kWarps * R::kApart);
+      do {
+        copies_but_the_last<L::kStages - 1>();
+        __syncwarp();
+        t.template pages<true>(ring + stage, block_q, used << 4);
+        next();
+      } while (used < stop);
+      t.settle();
     }
     while (used < end) {
       copies_but_the_last<L::kStages - 1>();

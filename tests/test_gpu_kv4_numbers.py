@@ -10,6 +10,7 @@ from mfq_b200.engine.kv_cache import LayerKV4
 from mfq_b200.ops import kv4
 from gpu_common import check_status, require_gpu_lib
 from kv4_cases import assert_attends, batch, call, exact
+from kv4_rms import assert_close_on_average, exact_and_weights, skewed
 
 pytestmark = pytest.mark.gpu
 FORMS = [None, (1, 0), (2, 0), (8, 0), (0, 1), (0, 3), (0, 50)]
@@ -98,3 +99,33 @@ def test_many_keys_above_the_first_ones_and_tiny_values(form, monkeypatch):
     want, size = p @ kept_v[:, 0].double(), p @ kept_v[:, 0].double().abs()
     # the output's rounding; p s to fp16 of up to 15 scales, of which the groups have 7.5 on average and |v| 2.7 or more: 2^-11 * 15 / 2.7
     assert ((out[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * size).all(), (out[0, 0, :4], want[:4])
+
+
+LONG = [  # lengths, form, what else: chains of thousands of tokens a warp in every kind of columns
+    ([16384, 12345], (1, 0), {}),
+    ([16384, 12345], (0, 1), {"hq": 32, "hk": 2}),
+    ([16384, 9000], (1, 0), {"hq": 16, "hk": 2}),
+    ([16384, 12345], (1, 0), {"hq": 4, "hk": 1, "q_len": 3}),
+    ([16384], (1, 0), {"hq": 8, "hk": 2, "d": 64}),
+    ([16384, 700], (1, 0), {"hq": 32, "hk": 2, "d": 64}),
+    ([9000, 16384], (1, 0), {"hq": 8, "hk": 1, "d": 256}),
+    ([60000], (1, 0), {"hq": 8, "hk": 1}),
+    ([60000], (8, 0), {"hq": 16, "hk": 1}),
+    ([60000, 300, 16384], None, {"hq": 32, "hk": 2}),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["even", "skewed"])
+@pytest.mark.parametrize("lens,form,how", LONG)
+def test_averages_over_long_contexts_keep_their_precision(lens, form, how, kind, dtype, monkeypatch):
+    """Queries that see all keys nearly alike: outputs a hundredth of the values, and of what is added up for them."""
+    require_gpu_lib()
+    if form is not None:
+        monkeypatch.setattr(kv4, "_shape", lambda *a: form)
+    s = batch(len(lens), lens, dtype=dtype, device="cuda", q_std=0.15, **how)
+    if kind == "skewed":
+        skewed(s)
+    out = call(ops, s)
+    check_status()
+    assert_close_on_average(s, out, exact_and_weights(s))
