@@ -20,8 +20,8 @@
 // Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
 // maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum.  p s and p m are multiplied by a power of two that
 // brings the largest scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest p times the largest scale that
-// the warp has met; that is 1/8 of a bf16 output's rounding.  For fp16 outputs p s is a sum of two fp16 numbers (2^-22), each multiplied by itself.  The sum of p has
-// no such factor: warps, CTAs and pieces are joined by ref for p and by both for the rest, so that scales of V may lie apart as far as their type lets
+// the warp has met; that is 1/8 of a bf16 output's rounding.  For fp16 outputs p s is a sum of two fp16 numbers (off by 2^-22, or 2^-27
+// of the largest where that is more), each multiplied by itself.  The sum of p has no such factor: warps, CTAs and pieces are joined by ref for p and by both for the rest, so that scales of V may lie apart as far as their type lets
 // them and the softmax is the same wherever they are.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
 //
 // Measured, 8 KV heads of 128, bf16: 64 rows of 16384 tokens (1.2 GB) 195 to 204 us, 0.91 to 0.95 of the measured copy rate, 217 to 233 where the power limit holds
@@ -193,6 +193,11 @@ __device__ __forceinline__ void kv4_store4(T* to, float4 o, float l, float power
 template <int D, int kCols, typename T>
 struct Kv4Rows {
   static constexpr bool kSide = kCols == 4, kSplit = __is_same(T, __half);  // kSplit: p s as two fp16 numbers
+  // Products of an instruction are lined up by their operands' exponents, which of a code as a denormal number is 2^-14, ten bits above the code: of a p s, bits some 2^-15
+  // of the 16 tokens' largest are cut off, always towards 0.  So the first of the two numbers has no bits below 2^-8, where the largest have 2^7 to 2^9 and more, and
+  // the second, multiplied by itself, has them.  5000 keys, scores 2.3 powers of two apart: errors beside the output's rounding from 0.37 of it to 0.13; without bits below
+  // 2^-4 0.04, but then p s of 2^-18 of the largest would be one number of 11 bits.
+  static constexpr float kGrid = 6.f;  // 2^-8 is the step of fp16 between 4 and 8
   static constexpr int kApart = kSplit ? 4 : 32;  // pairs of pages after which o and om meet
   static constexpr int kQ = Kv4Queries<D, kCols, T>::kQ;
   static constexpr int G = D / 64, kSteps = D / 16, NB = kSide ? 1 : kCols / 8, P = kSide ? 1 : 2;  // P: pages of a pair whose scores a lane has
@@ -367,11 +372,13 @@ struct Kv4Rows {
             } else {
               om[b][g] = make_float2(fmaf(sc[b][p][h].x, pm, om[b][g].x), fmaf(sc[b][p][h].y, pm, om[b][g].y));
             }
-            const uint32_t near = half_pair(v.x, v.y);
-            pb[b][p][g][h] = kv4_transposed(near);
             if constexpr (kSplit) {
-              const float2 as = __half22float2(*reinterpret_cast<const __half2*>(&near));
+              const __half2 near = __hsub2(__floats2half2_rn(v.x + kGrid, v.y + kGrid), __float2half2_rn(kGrid));
+              const float2 as = __half22float2(near);
+              pb[b][p][g][h] = kv4_transposed(*reinterpret_cast<const uint32_t*>(&near));
               rest[b][p][g][h] = kv4_transposed(half_pair(v.x - as.x, v.y - as.y));
+            } else {
+              pb[b][p][g][h] = kv4_transposed(half_pair(v.x, v.y));
             }
           }
         }

@@ -9,7 +9,7 @@ from mfq_b200 import ops
 from mfq_b200.engine.kv_cache import LayerKV4
 from mfq_b200.ops import kv4
 from gpu_common import check_status, require_gpu_lib
-from kv4_cases import assert_attends, batch, call, exact
+from kv4_cases import BATCHES, assert_attends, batch, call, exact
 from kv4_rms import assert_close_on_average, exact_and_weights, skewed
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +129,13 @@ def test_averages_over_long_contexts_keep_their_precision(lens, form, how, kind,
     out = call(ops, s)
     check_status()
     assert_close_on_average(s, out, exact_and_weights(s))
+
+
+@pytest.mark.parametrize("lens,how", [x for x in BATCHES if sum(x[0]) > 700 and "spread" not in x[1]])
+def test_batches_are_off_by_little_more_than_their_rounding(lens, how):
+    require_gpu_lib()
+    for dtype in (torch.float16, torch.bfloat16):
+        s = batch(len(lens), lens, device="cuda", **{**how, "dtype": dtype})
+        out = call(ops, s)
+        check_status()
+        assert_close_on_average(s, out, exact_and_weights(s))
