@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(128, kMinBlocks) kv4_attn_kernel(Kv4AttnArgs a
         t.template pages<true>(ring + stage, block_q, used << 4);
         next();
       } while (used < stop);
-      t.settle();
+      if (used < seen) t.settle();
     }
     while (used < end) {
       copies_but_the_last<L::kStages - 1>();
