@@ -17,18 +17,19 @@
 // Up to 4 query rows have the two pages side by side: the first page is multiplied by [Q 0], the second by [0 Q], into the same accumulator, so that no
 // lane computes the softmax of columns that nobody has; O^T's halves are added in the end.
 //
-// Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest.  Scores,
-// maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below the row's running maximum.  p s and p m are multiplied by a power of two that
-// brings the largest scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a normal number (2^-11) down to 2^-21 of the largest p times the largest scale that
-// the warp has met; that is 1/8 of a bf16 output's rounding.  For fp16 outputs p s is a sum of two fp16 numbers (off by 2^-22, or 2^-27
-// of the largest where that is more), each multiplied by itself.  The sum of p has no such factor: warps, CTAs and pieces are joined by ref for p and by both for the rest, so that scales of V may lie apart as far as their type lets
-// them and the softmax is the same wherever they are.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
+// Numbers: a row of q is scaled by a power of two to 2^10 <= max |q| < 2^11, so that fp16 holds its values exactly down to 2^-24 of the largest; in a product with
+// codes, bits some 2^-15 below the largest of 16 dims are cut off.  Scores, maxima, sums and outputs are fp32.  p is exp2(score - ref): ref is at most 6 below
+// the row's running maximum.  p s and p m are multiplied by a power of two that brings the largest scales of V to 2^7 .. 2^9, so that p s is rounded to fp16 as a
+// normal number (2^-11) down to 2^-21 of the largest p times the largest scale that the warp has met; that is 1/8 of a bf16 output's rounding.  For fp16 outputs
+// p s is a sum of two fp16 numbers (off by 2^-22, or 2^-27 of the largest where that is more), each multiplied by itself.  The sum of p has no such factor: warps,
+// CTAs and pieces are joined by ref for p and by both for the rest, so that scales of V may lie apart as far as their type lets them and the softmax is the same
+// wherever they are.  Scales of V between 2^-98 and 2^98, queries up to 2^100.
 //
-// Measured, 8 KV heads of 128, bf16: 64 rows of 16384 tokens (1.2 GB) 195 to 204 us, 0.91 to 0.95 of the measured copy rate, 217 to 233 where the power limit holds
-// the clock at 1.64 GHz; 64 of 4096 59 us; 3 of up to 2000 8.3.  A pair of pages costs a warp 400 instructions, 225 of them on the half-rate integer
+// Measured, 8 KV heads of 128, bf16: 64 rows of 16384 tokens (1.2 GB) 201 to 206 us, 0.90 to 0.92 of the measured copy rate, 213 to 230 where the power limit holds
+// the clock at 1.64 GHz; 64 of 4096 60 us; 3 of up to 2000 8.4.  A pair of pages costs a warp 392 instructions, 223 of them on the half-rate integer
 // pipe (160 to unpack codes, five for eight), where memory at its full rate leaves 780 issue slots: latency between dependent instructions with four warps a
 // scheduler is what keeps it from hiding all of the arithmetic.  Queries in shared memory instead of registers: 214 -> 205 us; five CTAs an SM of 96
-// registers took 217, a shift of the upper codes on the multiplier 251 instead of 214.
+// registers took 217, a shift of the upper codes on the multiplier 251 instead of 214 (before V's sums met in between, which takes 1 %).
 #include "attn_shared.cuh"
 #include "kv4.cuh"
 

@@ -104,10 +104,12 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kv) -> None
 def _shape(units: int, cols: int, d: int, pages: int) -> tuple[int, int]:
     """(CTAs of a unit's cluster, 0) or (0, CTAs that share all pairs of pages) for ``units`` units of ``cols`` columns and up to ``pages`` pages.
 
-    The fastest by a model in microseconds, its numbers fitted on a B200 to 1 to 200 sequences of 48 to 32000 tokens (8 KV heads of 128), in eight forms each.
+    The fastest by a model in microseconds, its numbers fitted on a B200 to 1 to 200 sequences of 48 to 32000 tokens (8 KV heads of 128, 4 columns, bf16), in eight forms each.
     Four warps take four pairs in a round.  With n CTAs an SM a round takes 0.45 + 0.29 n, what is before and behind the rounds 1.4 for each of them, a further wave 1.5; shares need a
-    second kernel, 3 for every unit or piece of one, and a sum over a unit's pieces.  64 rows of 4096 tokens: 63.5 in single CTAs | 67.6 in pairs | 64.5 in shares; of 16384:
-    213 | 197 | 200; 3 of 2000: 20.6 | 16.4 | 19.5, in clusters of eight 12.3; 1 of 32000: 201 | 107 | 33.8, in 296 shares 27.6, in clusters 36.9."""
+    second kernel, 3 for every unit or piece of one, and a sum over a unit's pieces.  Replayed, in single CTAs | in pairs | in 592 shares: 64 rows of 4096 tokens 60 | 66 | 63; of 16384
+    218 | 200 | 201; 3 of 2000: 16 | 12 | 14, in clusters of eight 10; 1 of 32000: 188 | 98 | 25, in 296 shares 21, in 148, as is chosen, 23 to 25, in clusters of eight 31.
+    Other heads and columns enter by ``work``, types not at all: of 30 shapes with heads of 64 to 256, 2 to 16 rows a head and both types the choice was within 4 % of the fastest
+    form in 28; 8 of 8000 with heads of 64 took 16.4 instead of 14.4, and 1 of 32000."""
     each = 2 if d == 256 or cols == 16 else 4  # CTAs that an SM holds
     work = {64: 0.6, 128: 1.0, 256: 2.0}[d] * {4: 1.0, 8: 1.2, 16: 2.0}[cols]
     pairs = max(1, (pages + 1) // 2)
